@@ -28,6 +28,11 @@ BM_DEVERR_BAD_ID = 0x1
 BM_DEVERR_BAD_POSITION = 0x2
 BM_DEVERR_BAD_SEQUENCE = 0x4
 BM_DEVERR_TIMEOUT = 0x8
+BM_DEVERR_BAD_PAGE = 0x10
+BM_DEVERR_BAD_PARAMETER = 0x20
+
+BM_ROPE_SCALING = {"none": 0, "linear": 1, "ntk": 2, "bands": 3, "yarn": 4}
+
 
 class LayerStepC(ctypes.Structure):
     """Mirror of bm_layer_step_t (include/bm_layer_ops.h): one layer step's sizes
@@ -43,6 +48,21 @@ class LayerStepC(ctypes.Structure):
         ("rope_table_len", c_int32), ("ffn_out", c_void_p), ("w_ffn", c_void_p), ("y_ffn", c_void_p),
         ("gate", c_void_p), ("up", c_void_p), ("act", c_void_p),
     ]
+
+
+class RopeScalingC(ctypes.Structure):
+    """Mirror of bm_rope_scaling_t."""
+
+    _fields_ = [("kind", c_int32), ("original_max_pos", c_int32), ("factor", c_double), ("low", c_double),
+                ("high", c_double), ("mscale", c_double)]
+
+
+class PagedKVC(ctypes.Structure):
+    """Mirror of bm_paged_kv_t."""
+
+    _fields_ = [("k_pages", c_void_p), ("v_pages", c_void_p), ("page_table", c_void_p), ("num_pages", c_int32),
+                ("page_size", c_int32), ("max_pages", c_int32), ("num_seqs", c_int32), ("num_kv_heads", c_int32),
+                ("head_dim", c_int32)]
 
 
 # name -> (restype, argtypes). Every symbol include/bm_layer_ops.h declares.
@@ -98,6 +118,20 @@ SIGNATURES = {
     "bm_kv_cache_append": (c_int, [c_void_p, c_void_p, c_int64, ctypes.POINTER(c_void_p), ctypes.POINTER(c_void_p),
                                    c_void_p]),
     "bm_selftest_bounded_wait": (c_int, [c_int64, c_void_p, c_void_p, c_void_p]),
+    "bm_rotary_table_fill": (c_int, [c_void_p, c_int32, c_int32, c_double, ctypes.POINTER(RopeScalingC), c_void_p]),
+    "bm_rotary": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_void_p, c_int32, c_int32, c_int32,
+                          c_int64, c_int32, c_int32, c_int32, c_int64, c_int64, c_int64, c_int64, c_int, c_void_p,
+                          c_void_p]),
+    "bm_paged_kv_append": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                                   ctypes.POINTER(PagedKVC), c_void_p, c_int32, c_int32, c_int32, c_int64, c_int32,
+                                   c_int64, c_int64, c_int64, c_int64, c_int, c_void_p, c_void_p]),
+    "bm_paged_tree_attention_workspace_size": (c_int, [c_int64, c_int64, c_int32, c_int32, c_int32, c_int32, c_int32,
+                                                       ctypes.POINTER(ctypes.c_size_t)]),
+    "bm_paged_tree_attention": (c_int, [c_void_p, c_void_p, ctypes.POINTER(PagedKVC), c_void_p, c_void_p, c_void_p,
+                                        c_void_p, c_int32, c_int64, c_int64, c_int32, c_int32, c_int32, c_float,
+                                        c_void_p, ctypes.c_size_t, c_int, c_void_p, c_void_p]),
+    "bm_sample": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64,
+                          c_int64, c_int, c_void_p, c_void_p]),
     "bm_layer_step": (c_int, [ctypes.POINTER(LayerStepC), c_int, c_void_p, c_void_p]),
 }
 

@@ -83,6 +83,9 @@ inline bool valid_dtype(int dt) { return dt == BM_F32 || dt == BM_BF16; }
 
 inline cudaStream_t as_stream(void* s) { return reinterpret_cast<cudaStream_t>(s); }
 
+// Host checks of a paged cache's description, shared by its entry points.
+int check_paged_kv(const char* what, const bm_paged_kv_t* cache);
+
 // bm_decode_attention with a host-side length for every query (lens == NULL:
 // len0), as the reference's single-token launch_attention needs.
 int decode_attention(void* out, const void* q, const void* k_cache, const void* v_cache, const int32_t* seq_ids,

@@ -106,10 +106,13 @@ int bm_status_read(int32_t* d_status, int32_t* flags_out, void* stream) {
   }
   *flags_out = host;
   if (host != 0) {
-    return bm::fail(BM_ERR_DEVICE, "device status bits 0x%x%s%s%s", host,
+    return bm::fail(BM_ERR_DEVICE, "device status bits 0x%x%s%s%s%s%s%s", host,
                     (host & BM_DEVERR_BAD_ID) ? " bad-token-id" : "",
                     (host & BM_DEVERR_BAD_POSITION) ? " bad-position" : "",
-                    (host & BM_DEVERR_BAD_SEQUENCE) ? " bad-sequence" : "");
+                    (host & BM_DEVERR_BAD_SEQUENCE) ? " bad-sequence" : "",
+                    (host & BM_DEVERR_TIMEOUT) ? " timeout" : "",
+                    (host & BM_DEVERR_BAD_PAGE) ? " bad-page" : "",
+                    (host & BM_DEVERR_BAD_PARAMETER) ? " bad-parameter" : "");
   }
   bm::clear_error();
   return BM_OK;

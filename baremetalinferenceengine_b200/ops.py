@@ -14,6 +14,7 @@ Two layers, mirroring the reference:
 from __future__ import annotations
 
 import ctypes
+import dataclasses
 from typing import Optional
 
 import torch
@@ -87,16 +88,51 @@ class DeviceStatus:
         return int(flags.value)
 
 
+@dataclasses.dataclass(frozen=True)
+class RopeScaling:
+    """How a :class:`RopeTable` stretches its frequencies for contexts past the trained
+    one (the formulas stand at bm_rotary_table_fill): ``kind`` none, linear, ntk, bands
+    (low_freq_factor, high_freq_factor) or yarn (beta_fast, beta_slow). ``mscale``
+    multiplies cos and sin; None is the kind's own (0.1 ln(factor) + 1 for yarn)."""
+
+    kind: str = "none"
+    factor: float = 1.0
+    original_max_pos: int = 0
+    low_freq_factor: float = 1.0
+    high_freq_factor: float = 4.0
+    beta_fast: float = 32.0
+    beta_slow: float = 1.0
+    mscale: Optional[float] = None
+
+    def c_struct(self) -> "_lib.RopeScalingC":
+        if self.kind not in _lib.BM_ROPE_SCALING:
+            raise BMError(_lib.BM_ERR_INVALID_ARGUMENT, f"unknown rope scaling {self.kind!r}")
+        if self.mscale is not None and not self.mscale > 0:
+            raise BMError(_lib.BM_ERR_INVALID_ARGUMENT, "mscale must be > 0")
+        yarn = self.kind == "yarn"
+        return _lib.RopeScalingC(_lib.BM_ROPE_SCALING[self.kind], int(self.original_max_pos), float(self.factor),
+                                 float(self.beta_fast if yarn else self.low_freq_factor),
+                                 float(self.beta_slow if yarn else self.high_freq_factor),
+                                 0.0 if self.mscale is None else float(self.mscale))
+
+
 class RopeTable:
-    """Device (cos, sin) table [max_pos][head_dim/2] of fp32 pairs, filled in fp64."""
+    """Device (cos, sin) table [max_pos][head_dim/2] of fp32 pairs, filled in fp64; with
+    ``scaling`` (a :class:`RopeScaling`) its frequencies stretched. For heads that are
+    rotated in part, ``head_dim`` is the rotated part (rotary, paged_kv_append)."""
 
     def __init__(self, max_pos: int, head_dim: int, theta: float, device: torch.device | str | int = "cuda",
-                 stream: Optional[torch.cuda.Stream] = None):
+                 stream: Optional[torch.cuda.Stream] = None, scaling: Optional[RopeScaling] = None):
         self.max_pos, self.head_dim, self.theta = int(max_pos), int(head_dim), float(theta)
+        self.scaling = scaling
         self.data = torch.empty(self.max_pos, self.head_dim // 2, 2, dtype=torch.float32, device=device)
         with torch.cuda.device(self.data.device):
-            check(load().bm_rope_table_fill(self.data.data_ptr(), self.max_pos, self.head_dim, self.theta,
-                                            _stream(self.data.device, stream)))
+            s = _stream(self.data.device, stream)
+            if scaling is None:
+                check(load().bm_rope_table_fill(self.data.data_ptr(), self.max_pos, self.head_dim, self.theta, s))
+            else:
+                check(load().bm_rotary_table_fill(self.data.data_ptr(), self.max_pos, self.head_dim, self.theta,
+                                                  ctypes.byref(scaling.c_struct()), s))
 
     @property
     def ptr(self) -> int:
@@ -397,6 +433,255 @@ def kv_store(cache: torch.Tensor, src: torch.Tensor, positions, seq_ids: Optiona
         check(load().bm_kv_store(_ptr(cache), _ptr(src), _ptr(pos_t), pos0, _ptr(seq_ids), rows, h, hd,
                                  cache.shape[2], cache.shape[0], bm_dtype(src), status.ptr if status else None,
                                  _stream(src.device, stream)))
+
+
+# --------------------------------------------------------------------------
+# Rotary forms, the paged KV cache, tree attention and sampling
+# --------------------------------------------------------------------------
+
+def _invalid(message: str) -> BMError:
+    return BMError(_lib.BM_ERR_INVALID_ARGUMENT, message)
+
+
+def _empty(shape, dtype: torch.dtype, device: torch.device, stream) -> torch.Tensor:
+    """Uninitialised memory that belongs to the stream that will write it."""
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    with torch.cuda.stream(stream):
+        return torch.empty(shape, dtype=dtype, device=device)
+
+
+def _head_rows(t: torch.Tensor, name: str, ref: torch.Tensor) -> None:
+    """[rows, heads, head_dim] of ref's device and dtype with dense heads (rows may be
+    slices of wider ones)."""
+    if t.dim() != 3 or t.dtype != ref.dtype or t.device != ref.device or t.shape[2] != ref.shape[2]:
+        raise _invalid(f"{name} must be [rows, heads, head_dim] of the other tensors' device, dtype and head_dim")
+    if t.numel() > 0 and ((t.shape[2] > 1 and t.stride(2) != 1) or (t.shape[1] > 1 and t.stride(1) != t.shape[2])):
+        raise _invalid(f"{name} must have dense heads")
+
+
+def _row_stride(t: torch.Tensor) -> int:
+    """Elements between rows (a single row's or an empty tensor's stride means nothing)."""
+    return t.stride(0) if t.shape[0] > 1 and t.numel() > 0 else t.shape[1] * t.shape[2]
+
+
+def _same_device_i32(t: Optional[torch.Tensor], name: str, device: torch.device, numel: Optional[int] = None) -> None:
+    if t is None:
+        return
+    if t.dtype != torch.int32 or not t.is_contiguous() or t.device != device:
+        raise _invalid(f"{name} must be a contiguous int32 tensor on {device}")
+    if numel is not None and t.numel() != numel:
+        raise _invalid(f"{name} must have {numel} entries")
+
+
+def _table_device(table: Optional[RopeTable], device: torch.device) -> None:
+    if table is not None and table.data.device != device:
+        raise _invalid("the rope table is on another device")
+
+
+def _status_ptr(status: Optional[DeviceStatus], device: torch.device) -> Optional[int]:
+    if status is None:
+        return None
+    if status.word.device != device:
+        raise _invalid("the status word is on another device")
+    return status.ptr
+
+
+def rotary(q: Optional[torch.Tensor], k: Optional[torch.Tensor], positions, table: RopeTable,
+           interleaved: bool = False, q_out: Optional[torch.Tensor] = None, k_out: Optional[torch.Tensor] = None,
+           status: Optional[DeviceStatus] = None, stream=None):
+    """Rotates the first ``table.head_dim`` elements of every head of q [rows, Hq, hd] and
+    k [rows, Hkv, hd] (either may be None) and copies the rest; returns (q_out, k_out),
+    made when not given; ``q_out=q`` rotates in place. Pairs are (i, i + rotary_dim/2),
+    or (2i, 2i + 1) with ``interleaved``. q and k may be slices of a fused projection's
+    rows. ``positions``: int32 tensor, or an int pos0 (row r at pos0 + r). A position
+    outside the table leaves its row unwritten and sets BAD_POSITION."""
+    ref = q if q is not None else k
+    if ref is None:
+        raise _invalid("neither q nor k given")
+    if ref.dim() != 3:
+        raise _invalid("q and k must be [rows, heads, head_dim]")
+    dev, rows = _dev(ref), ref.shape[0]
+    outs = []
+    for name, x, out in (("q", q, q_out), ("k", k, k_out)):
+        if x is None:
+            if out is not None:
+                raise _invalid(f"{name}_out without {name}")
+            outs.append(None)
+            continue
+        _head_rows(x, name, ref)
+        if out is None:
+            out = _empty(x.shape, x.dtype, dev, stream)
+        _head_rows(out, name + "_out", ref)
+        if x.shape[0] != rows or out.shape != x.shape:
+            raise _invalid("q, k and their outputs must have the same rows, and an output its input's shape")
+        outs.append(out)
+    pos_t, pos0 = (None, positions) if isinstance(positions, int) else (positions, 0)
+    _same_device_i32(pos_t, "positions", dev, rows)
+    _table_device(table, dev)
+    q_out, k_out = outs
+    none = torch.empty(0, 0, 0)
+    qs, ks, qo, ko = (none if t is None else t for t in (q, k, q_out, k_out))
+    with torch.cuda.device(dev):
+        check(load().bm_rotary(_ptr(q_out), _ptr(k_out), _ptr(q), _ptr(k), _ptr(pos_t), pos0, table.ptr, table.max_pos,
+                               table.head_dim, int(interleaved), rows, qs.shape[1], ks.shape[1], ref.shape[2],
+                               _row_stride(qs), _row_stride(ks), _row_stride(qo), _row_stride(ko), bm_dtype(ref),
+                               _status_ptr(status, dev), _stream(dev, stream)))
+    return q_out, k_out
+
+
+class PagedKV:
+    """A paged KV cache over the caller's tensors: k_pages and v_pages [num_pages, Hkv,
+    page_size, hd] (contiguous, one dtype and device) and page_table int32 [num_seqs,
+    max_pages]: slot t of sequence s is in page page_table[s, t // page_size] at
+    t % page_size. The tensors are read by every call, so page_table may be rewritten
+    between calls (on the calls' stream)."""
+
+    def __init__(self, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor):
+        if k_pages.dim() != 4 or k_pages.shape != v_pages.shape:
+            raise _invalid("k_pages and v_pages must be [num_pages, kv_heads, page_size, head_dim]")
+        _dense(k_pages, "k_pages")
+        _dense(v_pages, "v_pages")
+        bm_dtype(k_pages)
+        _same(k_pages, v_pages)
+        if page_table.dim() != 2:
+            raise _invalid("page_table must be [num_seqs, max_pages]")
+        _same_device_i32(page_table, "page_table", _dev(k_pages))
+        self.k_pages, self.v_pages, self.page_table = k_pages, v_pages, page_table
+        self.num_pages, self.num_kv_heads, self.page_size, self.head_dim = k_pages.shape
+        self.num_seqs, self.max_pages = page_table.shape
+        self.device, self.dtype = k_pages.device, k_pages.dtype
+        self.c = _lib.PagedKVC(k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr(), self.num_pages,
+                               self.page_size, self.max_pages, self.num_seqs, self.num_kv_heads, self.head_dim)
+
+
+def paged_kv_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, positions: Optional[torch.Tensor],
+                    cache: PagedKV, table: Optional[RopeTable] = None, seq_ids: Optional[torch.Tensor] = None,
+                    slots: Optional[torch.Tensor] = None, interleaved: bool = False,
+                    q_out: Optional[torch.Tensor] = None, status: Optional[DeviceStatus] = None,
+                    stream=None) -> Optional[torch.Tensor]:
+    """rope_kv_store for a paged cache: writes rotated k and raw v [rows, Hkv, hd] into
+    slot ``slots[r]`` (positions[r] without slots; -1: a padding row) of sequence
+    ``seq_ids[r]`` (0 without) and returns q [rows, Hq, hd] rotated (``q_out``, made when
+    not given; ``q_out=q`` in place; None without q). Without a table nothing is
+    rotated."""
+    dev, rows = _dev(k), k.shape[0]
+    if k.dim() != 3:
+        raise _invalid("k and v must be [rows, kv_heads, head_dim]")
+    for name, t in (("k", k), ("v", v), ("q", q)):
+        if t is not None:
+            _head_rows(t, name, k)
+    if v.shape != k.shape or k.shape[1] != cache.num_kv_heads or k.shape[2] != cache.head_dim:
+        raise _invalid("k and v do not match the cache")
+    if cache.dtype != k.dtype or cache.device != dev:
+        raise _invalid("the cache has another dtype or device")
+    if q is None:
+        if q_out is not None:
+            raise _invalid("q_out without q")
+    else:
+        if q_out is None:
+            q_out = _empty(q.shape, q.dtype, dev, stream)
+        _head_rows(q_out, "q_out", k)
+        if q.shape[0] != rows or q_out.shape != q.shape:
+            raise _invalid("q must have k's rows, and q_out q's shape")
+    for name, t in (("positions", positions), ("seq_ids", seq_ids), ("slots", slots)):
+        _same_device_i32(t, name, dev, rows)
+    _table_device(table, dev)
+    with torch.cuda.device(dev):
+        check(load().bm_paged_kv_append(_ptr(q_out), _ptr(q), _ptr(k), _ptr(v), _ptr(positions), _ptr(slots),
+                                        _ptr(seq_ids), ctypes.byref(cache.c), None if table is None else table.ptr,
+                                        0 if table is None else table.max_pos, 0 if table is None else table.head_dim,
+                                        int(interleaved), rows, 0 if q is None else q.shape[1],
+                                        0 if q is None else _row_stride(q), _row_stride(k), _row_stride(v),
+                                        0 if q is None else _row_stride(q_out), bm_dtype(k), _status_ptr(status, dev),
+                                        _stream(dev, stream)))
+    return q_out
+
+
+def paged_tree_attention_workspace(q: torch.Tensor, cache: PagedKV, batch: int, max_ctx: int, max_tree: int,
+                                   stream=None) -> torch.Tensor:
+    """Device scratch for paged_tree_attention calls of these sizes (q's rows, batch and
+    bounds). Calls that overlap on the GPU need one each."""
+    if q.dim() != 3:
+        raise _invalid("q must be [rows, heads, head_dim]")
+    n = ctypes.c_size_t()
+    with torch.cuda.device(cache.device):
+        check(load().bm_paged_tree_attention_workspace_size(q.shape[0], batch, q.shape[1], cache.num_kv_heads,
+                                                            cache.head_dim, max_ctx, max_tree, ctypes.byref(n)))
+    return _empty((n.value,), torch.uint8, cache.device, stream)
+
+
+def paged_tree_attention(q: torch.Tensor, cache: PagedKV, ctx_lens: torch.Tensor, q_starts: torch.Tensor,
+                         max_ctx: int, max_tree: int, tree_mask: Optional[torch.Tensor] = None,
+                         seq_ids: Optional[torch.Tensor] = None, scale: float = 0.0,
+                         out: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None,
+                         status: Optional[DeviceStatus] = None, stream=None) -> torch.Tensor:
+    """Attention of each sequence's drafted tokens over its cached context and over the
+    drafted tokens that they see. q [rows, Hq, hd] holds sequence b's rows
+    q_starts[b]:q_starts[b + 1]; its context is the cache slots before ctx_lens[b], its
+    drafted tokens' K and V are in the slots behind (paged_kv_append). Bit j % 64 of
+    ``tree_mask`` (int64 [rows, words])[row, j // 64] lets the row see drafted token j;
+    without a mask row i sees j <= i (a prompt's chunk; with one row, decode attention).
+    max_ctx and max_tree bound ctx_lens and a sequence's rows. Rows outside every
+    sequence are left as they were in ``out``. ``workspace``:
+    paged_tree_attention_workspace's, made for the call when None."""
+    dev = _dev(q)
+    if q.dim() != 3 or not q.is_contiguous() or q.shape[2] != cache.head_dim:
+        raise _invalid("q must be contiguous [rows, heads, head_dim] with the cache's head_dim")
+    if cache.dtype != q.dtype or cache.device != dev:
+        raise _invalid("the cache has another dtype or device")
+    batch = ctx_lens.numel()
+    _same_device_i32(ctx_lens, "ctx_lens", dev)
+    _same_device_i32(q_starts, "q_starts", dev, batch + 1)
+    _same_device_i32(seq_ids, "seq_ids", dev, batch)
+    words = 0
+    if tree_mask is not None:
+        if (tree_mask.dtype != torch.int64 or tree_mask.dim() != 2 or tree_mask.shape[0] != q.shape[0]
+                or not tree_mask.is_contiguous() or tree_mask.device != dev):
+            raise _invalid("tree_mask must be contiguous int64 [rows, words] on q's device")
+        words = tree_mask.shape[1]
+    if out is None:
+        out = _empty(q.shape, q.dtype, dev, stream)
+    if out.shape != q.shape or out.dtype != q.dtype or out.device != dev or not out.is_contiguous():
+        raise _invalid("out must be contiguous and like q")
+    if workspace is None:
+        workspace = paged_tree_attention_workspace(q, cache, batch, max_ctx, max_tree, stream)
+    if workspace.device != dev or not workspace.is_contiguous():
+        raise _invalid("workspace must be contiguous on q's device")
+    with torch.cuda.device(dev):
+        check(load().bm_paged_tree_attention(_ptr(out), _ptr(q), ctypes.byref(cache.c), _ptr(seq_ids), _ptr(ctx_lens),
+                                             _ptr(q_starts), _ptr(tree_mask), words, q.shape[0], batch, q.shape[1],
+                                             max_ctx, max_tree, scale, workspace.data_ptr(),
+                                             workspace.numel() * workspace.element_size(), bm_dtype(q),
+                                             _status_ptr(status, dev), _stream(dev, stream)))
+    return out
+
+
+def sample(logits: torch.Tensor, uniforms: torch.Tensor, temperature: Optional[torch.Tensor] = None,
+           top_k: Optional[torch.Tensor] = None, top_p: Optional[torch.Tensor] = None,
+           min_p: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
+           status: Optional[DeviceStatus] = None, stream=None) -> torch.Tensor:
+    """One token per row of logits [rows, vocab] from uniforms [rows] in [0, 1):
+    temperature, then top-k, top-p and min-p (each a tensor of one entry per row, or None:
+    off), then the first index whose running weight exceeds its uniform's share. Ties
+    go to the lowest index; temperature 0 takes the largest logit; a row without any
+    weight gives -1. Returns int32 [rows]."""
+    dev = _dev(logits)
+    if logits.dim() != 2 or logits.shape[1] == 0 or (logits.shape[1] > 1 and logits.stride(1) != 1):
+        raise _invalid("logits must be [rows, vocab] with unit inner stride")
+    rows, vocab = logits.shape
+    for name, t in (("uniforms", uniforms), ("temperature", temperature), ("top_p", top_p), ("min_p", min_p)):
+        if t is not None and (t.dtype != torch.float32 or t.numel() != rows or not t.is_contiguous() or t.device != dev):
+            raise _invalid(f"{name} must be a contiguous float32 tensor of one entry per row on the logits' device")
+    _same_device_i32(top_k, "top_k", dev, rows)
+    if out is None:
+        out = _empty((rows,), torch.int32, dev, stream)
+    _same_device_i32(out, "out", dev, rows)
+    with torch.cuda.device(dev):
+        check(load().bm_sample(_ptr(out), _ptr(logits), _ptr(uniforms), _ptr(temperature), _ptr(top_k), _ptr(top_p),
+                               _ptr(min_p), rows, vocab, logits.stride(0) if rows > 1 else vocab, bm_dtype(logits),
+                               _status_ptr(status, dev), _stream(dev, stream)))
+    return out
 
 
 # --------------------------------------------------------------------------

@@ -57,6 +57,8 @@ typedef enum bm_status {
 #define BM_DEVERR_BAD_POSITION 0x2 /* position outside [0, max_seq) or beyond the RoPE table */
 #define BM_DEVERR_BAD_SEQUENCE 0x4 /* sequence id outside [0, num_seqs) */
 #define BM_DEVERR_TIMEOUT 0x8      /* a tensor-core pipeline wait passed its time limit; outputs incomplete */
+#define BM_DEVERR_BAD_PAGE 0x10    /* page id of a page table outside [0, num_pages) */
+#define BM_DEVERR_BAD_PARAMETER 0x20 /* a sampling setting or uniform number of a row outside its range */
 
 /* Human-readable name of a bm_status_t. Never NULL. */
 const char* bm_status_string(int status);
@@ -404,6 +406,149 @@ int bm_kv_cache_seq_len(const bm_kv_cache_t* cache, int32_t seq, int32_t* len_ou
 int bm_kv_cache_reset(bm_kv_cache_t* cache, int32_t seq);
 int bm_kv_cache_append(bm_kv_cache_t* cache, const int32_t* seq_ids, int64_t rows,
                        const int32_t** positions_dev, const int32_t** seq_ids_dev, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Rotary positions in their other forms. No counterpart in the reference, whose
+ * launch_rope (src/kernels.cu:126-140) rotates whole heads, half-split, unscaled.
+ *
+ * Scaled tables. A table is fp32 (cos, sin) pairs [max_pos][rotary_dim/2], the
+ * layout of bm_rope_table_fill, entry (p, i) = mscale * (cos, sin)(p * f_i), angles in
+ * fp64, with f_i = theta^(-2i/rotary_dim) changed by `kind`:
+ *   NONE    f_i (bm_rope_table_fill's table, bit for bit, when mscale is 1)
+ *   LINEAR  f_i / factor
+ *   NTK     theta replaced by theta * factor^(rotary_dim / (rotary_dim - 2))
+ *   BANDS   with t = original_max_pos * f_i / 2pi turns in the original context and
+ *           k = clamp((t - low) / (high - low), 0, 1):  k f_i + (1 - k) f_i / factor
+ *           (low, high: the low and high frequency factors, low < high)
+ *   YARN    r = clamp((i - a) / max(b - a, 0.001), 0, 1):  (1 - r) f_i + r f_i / factor,
+ *           a = max(floor(e(low)), 0), b = min(ceil(e(high)), rotary_dim - 1),
+ *           e(n) = rotary_dim ln(original_max_pos / (2pi n)) / (2 ln theta)
+ *           (low, high: beta_fast and beta_slow, low >= high > 0; theta > 1)
+ * factor >= 1. mscale <= 0 means the kind's own: 0.1 ln(factor) + 1 for YARN, else 1.
+ * Such a table serves every entry point that takes a rope_table, too. */
+typedef enum bm_rope_scaling_kind {
+  BM_ROPE_SCALING_NONE = 0,
+  BM_ROPE_SCALING_LINEAR = 1,
+  BM_ROPE_SCALING_NTK = 2,
+  BM_ROPE_SCALING_BANDS = 3,
+  BM_ROPE_SCALING_YARN = 4
+} bm_rope_scaling_kind_t;
+
+typedef struct bm_rope_scaling {
+  int32_t kind; /* bm_rope_scaling_kind_t */
+  int32_t original_max_pos;
+  double factor, low, high, mscale;
+} bm_rope_scaling_t;
+
+/* scaling NULL: NONE. */
+int bm_rotary_table_fill(void* table, int32_t max_pos, int32_t rotary_dim, double theta,
+                         const bm_rope_scaling_t* scaling, void* stream);
+
+/* Rotates the first rotary_dim elements of every head and copies the rest:
+ * q_out [rows][num_q_heads][head_dim] from q, k_out [rows][num_kv_heads][head_dim]
+ * from k (either pair may be NULL with its head count 0). The heads of a row are
+ * dense; rows are *_stride elements apart (a slice of a fused Q/K/V projection), so
+ * every stride is at least heads * head_dim. Outputs may be their inputs (same pointer
+ * and stride: in place) and must not overlap them otherwise.
+ * interleaved 0: pairs (i, i + rotary_dim/2), as bm_rope; 1: pairs (2i, 2i + 1).
+ * positions int32[rows] or NULL (pos0 + r); the table is required. With
+ * rotary_dim = head_dim and interleaved 0 the results equal bm_rope's bit for bit. A
+ * position outside [0, table_len) flags BM_DEVERR_BAD_POSITION and leaves its row
+ * unwritten. rotary_dim even, <= head_dim <= 1024. */
+int bm_rotary(void* q_out, void* k_out, const void* q, const void* k, const int32_t* positions, int32_t pos0,
+              const void* table, int32_t table_len, int32_t rotary_dim, int32_t interleaved, int64_t rows,
+              int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, int64_t q_stride, int64_t k_stride,
+              int64_t q_out_stride, int64_t k_out_stride, bm_dtype_t dtype, int32_t* d_status, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Paged KV cache. No counterpart in the reference, whose cache is one static run of
+ * max_seq positions (include/kv_cache.h:37-40).
+ * k_pages and v_pages are [num_pages][num_kv_heads][page_size][head_dim] (the static
+ * cache's layout with a page in a sequence's place); slot t of sequence s lives in page
+ * page_table[s][t / page_size] at t % page_size. page_table is a device array
+ * int32 [num_seqs][max_pages], read by every call: entries behind a sequence's last
+ * slot are never read and may hold anything. */
+typedef struct bm_paged_kv {
+  void* k_pages;
+  void* v_pages;
+  const int32_t* page_table;
+  int32_t num_pages, page_size, max_pages, num_seqs, num_kv_heads, head_dim;
+} bm_paged_kv_t;
+
+/* RoPE + K/V store into a paged cache (bm_rope_kv_store for pages), for `rows` tokens:
+ *   q_out[r] = q[r] rotated (q_out may be q);
+ *   slot slots[r] of sequence seq_ids[r]: K = k[r] rotated, V = v[r].
+ * slots NULL: slot = positions[r]. A drafted tree's tokens share rotary positions and
+ * have slots of their own. seq_ids NULL: all 0. table NULL: nothing is rotated (q_out
+ * and K are copies; positions may be NULL when slots is given). q, k, v and q_out rows are *_stride elements apart;
+ * num_q_heads may be 0 (q and q_out NULL). Rows whose slot is -1 are padding: nothing of
+ * theirs is read or written. Bad positions (outside the table), slots (negative or
+ * outside max_pages pages), sequences and page ids flag *d_status; such a row is
+ * skipped. The rows of one call name distinct slots: with two rows on one slot either
+ * row's values may be kept, chunk by chunk. */
+int bm_paged_kv_append(void* q_out, const void* q, const void* k, const void* v, const int32_t* positions,
+                       const int32_t* slots, const int32_t* seq_ids, const bm_paged_kv_t* cache, const void* table,
+                       int32_t table_len, int32_t rotary_dim, int32_t interleaved, int64_t rows, int32_t num_q_heads,
+                       int64_t q_stride, int64_t k_stride, int64_t v_stride, int64_t q_out_stride, bm_dtype_t dtype,
+                       int32_t* d_status, void* stream);
+
+/* Attention of a tree of drafted tokens per sequence over a paged cache (of one token:
+ * decode attention; without a mask: a chunk of a prompt behind its cached beginning).
+ * Sequence b (cache sequence seq_ids[b], b when NULL) has the query rows
+ * [q_starts[b], q_starts[b+1]) of q and out, [total_q][num_q_heads][head_dim], and
+ * n_b of them. Its context is the cache slots [0, ctx_lens[b]); its drafted tokens'
+ * K and V sit in slots ctx_lens[b] + j, j < n_b (bm_paged_kv_append). Row i of it gets
+ *   out[i][h] = softmax_t(q[i][h] . K[t][h/G] * scale) . V[t][h/G]
+ * over the context and the drafted slots j that it sees: bit j%64 of
+ * tree_mask[row][j/64] (uint64 [total_q][mask_words], bits past n_b ignored), or j <= i
+ * when tree_mask is NULL. G = num_q_heads / num_kv_heads <= 64, scale <= 0 means
+ * 1/sqrt(head_dim), head_dim <= 256 with whole 16-byte rows. A row that sees nothing
+ * gets zeros. Rows outside [q_starts[0], q_starts[batch]) are left as they were.
+ * max_ctx and max_tree are host-side upper bounds of ctx_lens and n_b that size the
+ * work split; with a mask max_tree <= 64 * mask_words. K and V of the ctx + n_b slots
+ * must be finite; slots behind them may hold anything. Softmax statistics and sums are
+ * fp32; bf16 caches with head_dim 64 or 128 and page sizes that divide 128 or are multiples of it
+ * (at least 8) run on the tensor cores with weights rounded to bf16, as
+ * bm_decode_attention does.
+ * A sequence with n_b or ctx outside [0, bound], slots outside its max_pages pages or
+ * rows outside [0, total_q) flags BM_DEVERR_BAD_POSITION, one with a bad sequence id
+ * BM_DEVERR_BAD_SEQUENCE: it is skipped, its rows unwritten. A bad page id flags
+ * BM_DEVERR_BAD_PAGE and its slots count as unseen.
+ * workspace: bm_paged_tree_attention_workspace_size() bytes of device scratch (16-byte aligned),
+ * contents of no matter, for calls of the same sizes; calls that overlap on the GPU
+ * need their own. */
+int bm_paged_tree_attention_workspace_size(int64_t total_q, int64_t batch, int32_t num_q_heads, int32_t num_kv_heads,
+                                           int32_t head_dim, int32_t max_ctx, int32_t max_tree, size_t* bytes_out);
+int bm_paged_tree_attention(void* out, const void* q, const bm_paged_kv_t* cache, const int32_t* seq_ids,
+                            const int32_t* ctx_lens, const int32_t* q_starts, const uint64_t* tree_mask,
+                            int32_t mask_words, int64_t total_q, int64_t batch, int32_t num_q_heads, int32_t max_ctx,
+                            int32_t max_tree, float scale, void* workspace, size_t workspace_bytes, bm_dtype_t dtype,
+                            int32_t* d_status, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Sampling: one token per row of logits [rows][vocab], rows row_stride elements apart,
+ * from given uniform numbers in [0, 1). The reference leaves this to its callers (an
+ * argmax on the host, src/benchmark.cpp). For each row, in this order:
+ *   weights w_i = exp((x_i - max x) / temperature[r])
+ *   top_k[r] = k > 0: only the k largest stay
+ *   top_p[r] = p < 1: in descending order, a token stays while the weights before it
+ *     sum to less than p times what is left after top-k (the first always stays)
+ *   min_p[r] = m > 0: w_i >= m stay (the largest always stay)
+ *   token: the lowest index whose running sum of staying weights, in index order,
+ *     exceeds uniforms[r] times their total.
+ * Equal logits are ordered by index, the lowest first. temperature 0: the largest
+ * logit's lowest index. temperature, top_k, top_p and min_p are device arrays of one
+ * entry per row, or NULL (1, off, off, off); k <= 0 or >= vocab, p >= 1 and m <= 0 are
+ * off, p <= 0 leaves the largest alone. A NaN logit counts as -inf; -inf has no weight;
+ * with +inf logits only these have one, all alike. A row without any weight gets token
+ * -1. Weights are held in 64-bit fixed point (2^min(52, 62 - ceil(log2 vocab)) for the
+ * largest, from fp64 exponentials) and summed as integers, so a result does not depend
+ * on the order of any sum. A row whose temperature, top_p, min_p or uniform number is
+ * NaN, or whose temperature is negative or uniform outside [0, 1), gets -1 and flags
+ * BM_DEVERR_BAD_PARAMETER. vocab <= 2^24. */
+int bm_sample(int32_t* tokens, const void* logits, const float* uniforms, const float* temperature,
+              const int32_t* top_k, const float* top_p, const float* min_p, int64_t rows, int64_t vocab,
+              int64_t row_stride, bm_dtype_t dtype, int32_t* d_status, void* stream);
 
 /* Self-test of the bounded waits behind BM_DEVERR_TIMEOUT (the tensor-core
  * kernels' mbarrier waits): one CTA waits on a barrier that nothing completes,
