@@ -18,4 +18,8 @@ int make_tensor_map_bf16(CUtensorMap* map, const void* base, uint64_t inner, uin
 int make_tensor_map_2d(CUtensorMap* map, const void* base, bm_dtype_t dtype, uint64_t inner, uint64_t outer,
                        uint32_t box_inner, uint32_t box_outer, const char* what);
 
+// A 3-D bf16 tensor map over dense [outer][middle][inner] with 128-byte swizzle.
+int make_tensor_map_3d_bf16(CUtensorMap* map, const void* base, uint64_t inner, uint64_t middle, uint64_t outer,
+                            uint32_t box_inner, uint32_t box_middle, uint32_t box_outer, const char* what);
+
 }  // namespace bm

@@ -379,7 +379,7 @@ extern "C" int bm_paged_tree_attention_workspace_size(int64_t total_q, int64_t b
   if (int st = paged::check_sizes(what, total_q, batch, num_q_heads, num_kv_heads, head_dim, max_ctx, max_tree)) return st;
   if (batch == 0 || max_tree == 0) return BM_OK;
   *bytes_out = std::max(paged::simt_workspace_bytes(total_q, batch, num_q_heads, num_kv_heads, head_dim, max_ctx, max_tree),
-                        paged::tc_workspace_bytes(total_q, batch, num_kv_heads, head_dim, num_q_heads / num_kv_heads,
+                        paged::tc_workspace_bytes(batch, num_kv_heads, head_dim, num_q_heads / num_kv_heads,
                                                   max_ctx, max_tree));
   return BM_OK;
 }
@@ -412,8 +412,8 @@ extern "C" int bm_paged_tree_attention(void* out, const void* q, const bm_paged_
   const uintptr_t bytes = static_cast<uintptr_t>(total_q) * num_q_heads * c.head_dim * dtype_size(dtype);
   if (o < i + bytes && i < o + bytes) return fail(BM_ERR_INVALID_ARGUMENT, "%s: out overlaps q", what);
   const size_t simt = paged::simt_workspace_bytes(total_q, batch, num_q_heads, c.num_kv_heads, c.head_dim, max_ctx, max_tree);
-  const size_t tc = paged::tc_workspace_bytes(total_q, batch, c.num_kv_heads, c.head_dim, num_q_heads / c.num_kv_heads,
-                                              max_ctx, max_tree);
+  const size_t tc = paged::tc_workspace_bytes(batch, c.num_kv_heads, c.head_dim, num_q_heads / c.num_kv_heads, max_ctx,
+                                              max_tree);
   if (std::max(simt, tc) > 0 && (!workspace || workspace_bytes < std::max(simt, tc))) {
     return fail(BM_ERR_INVALID_ARGUMENT, "%s: workspace of %zu bytes is smaller than %zu", what, workspace_bytes,
                 std::max(simt, tc));
@@ -445,7 +445,7 @@ extern "C" int bm_paged_tree_attention(void* out, const void* q, const bm_paged_
   const float s = scale > 0.f ? scale : 1.f / std::sqrt(static_cast<float>(c.head_dim));
   a.qscale = s * 1.4426950408889634f;
   a.status = d_status;
-  if (paged::tc_takes(a.hd, a.group, a.page_size, dtype)) return paged::launch_tc(a, as_stream(stream), what);
+  if (paged::tc_takes(a, dtype)) return paged::launch_tc(a, as_stream(stream), what);
   paged::plan(batch, a.hkv, a.group, max_ctx, max_tree, &a.row_tiles, &a.splits, &a.split_len);
   return dtype == BM_F32 ? paged::launch<float>(a, as_stream(stream), what) : paged::launch<bf16>(a, as_stream(stream), what);
 }

@@ -64,8 +64,8 @@ __device__ __forceinline__ bool sees(const TreeArgs& a, int64_t row0, int i, int
 
 // The tensor-core form (paged_attention_tc.cu): whether it takes these arguments, the
 // scratch it needs, and its launches.
-bool tc_takes(int hd, int group, int page_size, bm_dtype_t dtype);
-size_t tc_workspace_bytes(int64_t total_q, int64_t batch, int hkv, int hd, int group, int max_ctx, int max_tree);
+bool tc_takes(const TreeArgs& a, bm_dtype_t dtype);
+size_t tc_workspace_bytes(int64_t batch, int hkv, int hd, int group, int max_ctx, int max_tree);
 int launch_tc(const TreeArgs& a, cudaStream_t stream, const char* what);
 
 }  // namespace paged

@@ -1,11 +1,830 @@
+// Tree attention over a paged KV cache on the tensor cores (tcgen05, TMA, TMEM), for
+// bf16 caches with head_dim 64 or 128. Same contract as paged_attention.cu.
+//
+// Mathematics: the running softmax of paged_attention.cu on tiles of 128 slots, with
+// both products as tcgen05.mma:
+//   scores  S[row][slot] = Q[row][:] . K[slot][:]    M = 128 rows, N = 128 slots
+//   mix     O[row][:]   += P[row][slot] V[slot][:]   M = 128 rows, N = head_dim
+// A row is (token, head of the group), token-major: 128 / group tokens share a tile of
+// K and V. Each softmax thread owns one row (one TMEM lane), so maxima and sums need no
+// exchange between threads; P overwrites S in TMEM as bf16 and is the A operand of the
+// mix from there. O stays in TMEM; a row whose maximum rises by more than 2^8 (in the
+// exponent's base) is rescaled there, smaller rises leave its weights up to 2^8 (fp32
+// sums, bf16's exponent range: nothing is lost by it). Weights are rounded to bf16 for
+// the mix, the row sums take them before rounding.
+//
+// Bound: memory while group * tokens is below about 200 (two operations per K and V
+// element and row against 2.25 bytes per ns and SM), the tensor cores above. Padding
+// to M = 128 costs nothing that bounds: a tile's two products take 1024 cycles, its
+// 64 KB of K and V 2800 at the SM's share of HBM.
+//
+// Split: the host does not see the lengths, so one CTA per SM takes an equal share of
+// all tiles of the batch, counted on the device: items (sequence, kv head, row tile) laid
+// end to end, CTA c walking tiles [c T / nc, (c + 1) T / nc). An item cut at a CTA border
+// leaves partials in the workspace (at most two per CTA), which tree_merge_kernel adds
+// up; a whole one is written directly.
+//
+// Twelve warps:
+//   warp 0     TMA of K and V, pages looked up by its lanes, one box of page_size rows
+//              (128 at most) x 64 dims each, into separate rings;
+//   warp 1     owns TMEM; one thread issues every MMA;
+//   warp 2     TMA of the queries, once per segment (an item's part in this CTA);
+//   warps 4-7, 8-11  two softmax groups. Unit u of the CTA's sequence goes to group
+//              u & 1 with TMEM buffers S[u & 1] and O[u & 1]: with one row tile per
+//              item (kDual = false) units are its tiles in turn, and both groups' sums
+//              meet at the segment's end; with more rows (kDual = true) a tile is two
+//              units, one per row tile, so K and V are read once for 256 rows.
+// Every mbarrier wait is bounded in time: past the limit the CTA raises
+// BM_DEVERR_TIMEOUT, lets its copies and MMAs land, frees TMEM and returns.
+#include <cuda.h>
+
+#include <algorithm>
+
+#include "bm_tc.cuh"
+#include "bm_tma.h"
 #include "paged_attention.cuh"
 
 namespace bm {
 namespace paged {
 
-bool tc_takes(int, int, int, bm_dtype_t) { return false; }
-size_t tc_workspace_bytes(int64_t, int64_t, int, int, int, int, int) { return 0; }
-int launch_tc(const TreeArgs&, cudaStream_t, const char*) { return BM_OK; }
+using namespace bm::tc;
+
+namespace {
+
+constexpr int kTile = 128;      // slots per tile, rows per row tile
+constexpr int kThreadsTc = 384;
+constexpr int kMinTiles = 2;    // tiles that make a CTA worth starting
+constexpr int kBadRing = 16;    // tiles whose bad-page bits are kept
+constexpr uint64_t kWaitNs = 2000000000ull;
+constexpr uint64_t kDrainNs = 200000000ull;
+constexpr float kRescaleAt = 8.f;
+
+template <int HD, bool DUAL>
+struct Layout {
+  static constexpr int kTiles = DUAL ? 2 : 1;               // row tiles of an item
+  static constexpr int kBox = kTile * 128;                  // 128 rows x 64 dims of bf16
+  static constexpr int kOperand = HD / 64 * kBox;           // a tile of Q, K or V
+  static constexpr int kKS = HD == 128 ? 2 : 4;             // K ring: freed by the scores
+  static constexpr int kVS = HD == 128 ? 3 : 6;             // V ring: freed by the mix
+  static constexpr int kOffK = kTiles * kOperand;
+  static constexpr int kOffV = kOffK + kKS * kOperand;
+  static constexpr int kOffMl = kOffV + kVS * kOperand;     // [2][2][128] (maximum, sum), kDual = false
+  static constexpr int kOffBar = kOffMl + (DUAL ? 0 : 2 * 2 * kTile * 8);
+  static constexpr int kBars = 2 * kKS + 2 * kVS + 6 + 4;
+  static constexpr int kOffPlan = kOffBar + kBars * 8;      // Plan, scan, bad-page ring
+  static constexpr int kBytes = kOffPlan + 64 + 16 * 8 + kBadRing * 4 + 16 + 1024 /* alignment slack */;
+  static constexpr uint32_t kColO = 256;                    // TMEM: S0, S1 (128 each), O0, O1 (HD each)
+  static constexpr uint32_t kCols = 512;
+  static constexpr int kRows = kTiles * kTile;
+  static constexpr int kSlotFloats = kRows * (HD + 2);      // a partial: sums, then maxima, then weight sums
+};
+
+// What a CTA left of its first segment, for the merge.
+struct Record {
+  int64_t lo, total;   // its first tile, and all tiles
+  int32_t b, kvh, p;   // the item
+  int32_t t0, tiles;   // the segment's first tile in it (-1: no segment), the item's tiles
+  int32_t nc;          // CTAs with tiles
+};
+static_assert(sizeof(Record) == 40, "record layout");
+
+__host__ __device__ constexpr size_t records_bytes(int nc) { return (static_cast<size_t>(nc) * sizeof(Record) + 255) / 256 * 256; }
+
+__device__ __forceinline__ int tokens_per_tile(const TreeArgs& a) { return kTile / a.group; }
+
+// Tiles of item p (its row tiles hold `per` tokens) of a sequence.
+__device__ __forceinline__ int item_tiles(const TreeArgs& a, const Seq& s, int p, int per) {
+  const int seen = s.ctx + (a.mask ? s.n : min(s.n, (p + 1) * per));
+  return (seen + kTile - 1) / kTile;
+}
+// All tiles of one kv head of a sequence, and its items.
+__device__ __forceinline__ int64_t head_tiles(const TreeArgs& a, const Seq& s, int per, int* items) {
+  *items = (s.n + per - 1) / per;
+  if (a.mask) return static_cast<int64_t>(*items) * item_tiles(a, s, 0, per);
+  int64_t t = 0;
+  for (int p = 0; p < *items; ++p) t += item_tiles(a, s, p, per);
+  return t;
+}
+
+// The walk over a CTA's segments: every role runs its own, with the same results.
+struct Walk {
+  int64_t b, left;
+  int items, kvh, p, t, tiles;
+  Seq s;
+
+  // Tile `off` of sequence b is the CTA's first, and `n` tiles are its own.
+  __device__ void start(const TreeArgs& a, int64_t b0, int64_t off, int64_t n, int per) {
+    b = b0;
+    left = n;
+    read_seq(a, b, &s);
+    const int64_t head = head_tiles(a, s, per, &items);
+    kvh = static_cast<int>(off / head);
+    off -= kvh * head;
+    p = 0;
+    while (off >= (tiles = item_tiles(a, s, p, per))) {
+      off -= tiles;
+      ++p;
+    }
+    t = static_cast<int>(off);
+  }
+  // Tiles of the current segment (0 when the walk is over).
+  __device__ int segment() const { return static_cast<int>(left < tiles - t ? left : tiles - t); }
+  __device__ void next(const TreeArgs& a, int per) {
+    left -= segment();
+    if (left == 0) return;
+    t = 0;
+    if (++p == items) {
+      p = 0;
+      if (++kvh == a.hkv) {
+        kvh = 0;
+        do {
+          ++b;  // a later sequence has tiles: the plan counted them
+          read_seq(a, b, &s);
+        } while (s.n == 0);
+        items = (s.n + per - 1) / per;
+      }
+    }
+    tiles = item_tiles(a, s, p, per);
+  }
+};
+
+struct Plan {
+  int64_t lo, n, total, b, off;
+  int nc;
+};
+
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int32_t* status) {
+  int ok = 1;
+  if ((threadIdx.x & 31) == 0) ok = wait_phase(bar, parity, abort_flag, status, kWaitNs, true);
+  return __shfl_sync(0xffffffffu, ok, 0) != 0;
+}
+
+// D[tmem] (+)= A[tmem] * B[smem], kind::f16: A's rows are TMEM lanes, two bf16 a column.
+__device__ __forceinline__ void mma_bf16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
+                                            uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// 16 or 32 consecutive 32-bit columns of this thread's TMEM lane.
+__device__ __forceinline__ void tmem_store16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};" ::"r"(r[0]),
+      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_store32(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};" ::"r"(r[0]),
+      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]),
+      "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]),
+      "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+      ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
+
+__device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
+
+// Which of the 32 slots from slot0 on row i of the sequence sees.
+__device__ __forceinline__ uint32_t seen32(const TreeArgs& a, const Seq& s, int i, int slot0) {
+  const int lead = min(max(s.ctx - slot0, 0), 32);
+  uint32_t v = low_bits(lead);
+  const int j0 = slot0 + lead - s.ctx;  // the first drafted slot among them
+  if (lead < 32 && j0 < s.n) {
+    uint32_t tree;
+    if (a.mask == nullptr) {
+      tree = low_bits(min(i + 1, s.n) - j0);
+    } else {
+      const uint64_t* m = a.mask + (s.row0 + i) * a.words;
+      uint64_t bits = __ldg(m + (j0 >> 6)) >> (j0 & 63);
+      if ((j0 & 63) > 32 && (j0 >> 6) + 1 < a.words) bits |= __ldg(m + (j0 >> 6) + 1) << (64 - (j0 & 63));
+      tree = static_cast<uint32_t>(bits) & low_bits(s.n - j0);
+    }
+    v |= tree << lead;
+  }
+  return v;
+}
+
+// Which of the 32 slots at column 32c of a tile have a sound page (bit b of bad: the
+// tile's page b is not). Boxes hold at least 8 slots.
+__device__ __forceinline__ uint32_t sound32(uint32_t bad, int c, int box_rows) {
+  uint32_t v = 0xffffffffu;
+  for (int e = 0; e < 32; e += 8) {
+    if ((bad >> ((32 * c + e) / box_rows)) & 1) v &= ~(0xffu << e);
+  }
+  return v;
+}
+
+__device__ __forceinline__ void both_groups_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+template <int HD, bool DUAL>
+__global__ void __launch_bounds__(kThreadsTc, 1)
+    tree_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
+                   const __grid_constant__ CUtensorMap tv, const TreeArgs a) {
+  grid_dependency_wait();
+  using L = Layout<HD, DUAL>;
+  constexpr uint32_t kIdescS = instr_desc_bf16(false, false, kTile, kTile);
+  constexpr uint32_t kIdescO = instr_desc_bf16(false, true, HD, kTile);
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                                         ~static_cast<uintptr_t>(1023));
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int cta = static_cast<int>(blockIdx.x);
+  const int tpt = tokens_per_tile(a);      // tokens of a row tile
+  const int per = tpt * L::kTiles;         // and of an item
+
+  uint64_t* kfull = reinterpret_cast<uint64_t*>(smem + L::kOffBar);
+  uint64_t* kempty = kfull + L::kKS;
+  uint64_t* vfull = kempty + L::kKS;
+  uint64_t* vempty = vfull + L::kVS;
+  uint64_t* sfull = vempty + L::kVS;  // scores in TMEM       (commit)
+  uint64_t* pfull = sfull + 2;        // weights in TMEM      (one arrival per warp of the group)
+  uint64_t* pvdone = pfull + 2;       // mix done             (commit)
+  uint64_t* qfull = pvdone + 2;
+  uint64_t* qempty = qfull + 1;       // the segment's last scores are done (commit)
+  uint64_t* ofree = qempty + 1;       // the segment's O has been read (one arrival per softmax warp)
+  uint64_t* mma_done = ofree + 1;
+  Plan* plan = reinterpret_cast<Plan*>(smem + L::kOffPlan);
+  int64_t* scan = reinterpret_cast<int64_t*>(smem + L::kOffPlan + 64);
+  volatile uint32_t* bad_ring = reinterpret_cast<volatile uint32_t*>(scan + 16);
+  uint32_t* tmem_base_s = const_cast<uint32_t*>(bad_ring) + kBadRing;
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_base_s + 1);
+  Record* records = reinterpret_cast<Record*>(a.ws);
+  float* slots = a.ws + records_bytes(gridDim.x) / sizeof(float);
+
+  // ---------------- the plan ----------------
+  {
+    const int64_t share = (a.batch + kThreadsTc - 1) / kThreadsTc;
+    const int64_t b_lo = min(a.batch, tid * share), b_hi = min(a.batch, b_lo + share);
+    int64_t mine = 0;
+    for (int64_t b = b_lo; b < b_hi; ++b) {
+      Seq s;
+      const int32_t bad = read_seq(a, b, &s);
+      if (bad && cta == 0) raise_status(a.status, bad);
+      int items;
+      mine += a.hkv * head_tiles(a, s, per, &items);
+    }
+    int64_t incl = mine;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const int64_t v = __shfl_up_sync(0xffffffffu, incl, off);
+      if (lane >= off) incl += v;
+    }
+    if (lane == 31) scan[warp] = incl;
+    __syncthreads();
+    int64_t total = 0, before = incl - mine;
+    for (int w = 0; w < kThreadsTc / 32; ++w) {
+      if (w < warp) before += scan[w];
+      total += scan[w];
+    }
+    const int nc = static_cast<int>(min(static_cast<int64_t>(gridDim.x), (total + kMinTiles - 1) / kMinTiles));
+    if (cta >= nc) {  // nothing for this CTA (the same for all its threads)
+      if (tid == 0) records[cta] = Record{0, total, -1, 0, 0, -1, 0, nc};
+      return;
+    }
+    const int64_t lo = total * cta / nc, hi = total * (cta + 1) / nc;
+    if (before <= lo && lo < before + mine) {
+      int64_t at = before;
+      for (int64_t b = b_lo; b < b_hi; ++b) {
+        Seq s;
+        read_seq(a, b, &s);
+        int items;
+        const int64_t n = a.hkv * head_tiles(a, s, per, &items);
+        if (lo < at + n) {
+          *plan = Plan{lo, hi - lo, total, b, lo - at, nc};
+          break;
+        }
+        at += n;
+      }
+    }
+    if (tid == 0) {
+      for (int i = 0; i < L::kKS; ++i) {
+        mbar_init(&kfull[i], 1);
+        mbar_init(&kempty[i], 1);
+      }
+      for (int i = 0; i < L::kVS; ++i) {
+        mbar_init(&vfull[i], 1);
+        mbar_init(&vempty[i], 1);
+      }
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(&sfull[i], 1);
+        mbar_init(&pfull[i], 4);
+        mbar_init(&pvdone[i], 1);
+      }
+      mbar_init(qfull, 1);
+      mbar_init(qempty, 1);
+      mbar_init(ofree, 8);
+      mbar_init(mma_done, 1);
+      *abort_flag = 0;
+      fence_barrier_init();
+    }
+    if (warp == 1) tmem_alloc(tmem_base_s, L::kCols);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+  }
+  const uint32_t tmem = *tmem_base_s;
+  Walk walk;
+  walk.start(a, plan->b, plan->off, plan->n, per);
+  if (tid == 0) {
+    records[cta] = Record{plan->lo, plan->total, static_cast<int32_t>(walk.b), walk.kvh, walk.p, walk.t, walk.tiles, plan->nc};
+  }
+
+  if (warp == 0) {
+    // ---------------- K and V ----------------
+    const int box_rows = min(a.page_size, kTile);
+    const int boxes = kTile / box_rows;  // pages of a tile: at most 16
+    int kt = 0, nk = 0, nv = 0;  // the tile; K and V tiles asked for
+    bool ok = true;
+    for (; ok && walk.left > 0; walk.next(a, per)) {
+      const int n = walk.segment();
+      const int32_t* pages = a.page_table + static_cast<int64_t>(walk.s.seq) * a.max_pages;
+      const int total = walk.s.ctx + walk.s.n;
+      auto row_of = [&](int t) {  // this lane's box of tile t: its row in the tensor map, -1 bad, -2 none
+        const int slot = t * kTile + lane * box_rows;
+        if (lane >= boxes || slot >= total) return -2;
+        const int nth = slot / a.page_size;
+        const int32_t page = __ldg(pages + nth);
+        if (page < 0 || page >= a.num_pages) return -1;
+        return (page * a.hkv + walk.kvh) * a.page_size + (slot - nth * a.page_size);
+      };
+      int row = row_of(walk.t);
+      for (int i = 0; i < n; ++i, ++kt) {
+        const int next_row = i + 1 < n ? row_of(walk.t + i + 1) : -2;  // looked up while this tile waits
+        const uint32_t have = __ballot_sync(0xffffffffu, row >= 0);
+        const uint32_t bad = __ballot_sync(0xffffffffu, row == -1);
+        const uint32_t bytes = __popc(have) * box_rows * 128 * (HD / 64);
+        const int ks = kt % L::kKS, vs = kt % L::kVS;
+        unsigned char* kd = smem + L::kOffK + ks * L::kOperand + lane * box_rows * 128;
+        unsigned char* vd = smem + L::kOffV + vs * L::kOperand + lane * box_rows * 128;
+        if (!warp_wait(&kempty[ks], ((kt / L::kKS) & 1) ^ 1u, abort_flag, a.status)) {
+          ok = false;
+          break;
+        }
+        if (lane == 0) {
+          bad_ring[kt % kBadRing] = bad;
+          if (bad) raise_status(a.status, BM_DEVERR_BAD_PAGE);
+          mbar_expect_tx(&kfull[ks], bytes);
+        }
+        __syncwarp();
+        if (row >= 0) {
+#pragma unroll
+          for (int h = 0; h < HD / 64; ++h) tma_load_2d(kd + h * L::kBox, &tk, &kfull[ks], 64 * h, row);
+        }
+        nk = kt + 1;
+        if (!warp_wait(&vempty[vs], ((kt / L::kVS) & 1) ^ 1u, abort_flag, a.status)) {
+          ok = false;
+          break;
+        }
+        if (lane == 0) mbar_expect_tx(&vfull[vs], bytes);
+        __syncwarp();
+        if (row >= 0) {
+#pragma unroll
+          for (int h = 0; h < HD / 64; ++h) tma_load_2d(vd + h * L::kBox, &tv, &vfull[vs], 64 * h, row);
+        }
+        nv = kt + 1;
+        row = next_row;
+      }
+    }
+    if (lane == 0) {  // copies still in flight land before the CTA ends
+      for (int i = max(0, nk - L::kKS); i < nk; ++i) {
+        wait_phase(&kfull[i % L::kKS], (i / L::kKS) & 1, abort_flag, a.status, kDrainNs, false);
+      }
+      for (int i = max(0, nv - L::kVS); i < nv; ++i) {
+        wait_phase(&vfull[i % L::kVS], (i / L::kVS) & 1, abort_flag, a.status, kDrainNs, false);
+      }
+    }
+    __syncwarp();
+  } else if (warp == 2 && lane == 0) {
+    // ---------------- queries ----------------
+    int seg = 0;
+    for (; walk.left > 0; walk.next(a, per), ++seg) {
+      if (!wait_phase(qempty, (seg & 1) ^ 1u, abort_flag, a.status, kWaitNs, true)) break;
+      mbar_expect_tx(qfull, L::kTiles * (HD / 64) * a.group * tpt * 128);
+#pragma unroll
+      for (int w = 0; w < L::kTiles; ++w) {
+        const int token = static_cast<int>(walk.s.row0) + walk.p * per + w * tpt;
+#pragma unroll
+        for (int h = 0; h < HD / 64; ++h) {
+          tma_load_3d(smem + w * L::kOperand + h * L::kBox, &tq, qfull, 64 * h, walk.kvh * a.group, token);
+        }
+      }
+    }
+    if (seg > 0) wait_phase(qfull, (seg - 1) & 1, abort_flag, a.status, kDrainNs, false);
+  } else if (warp == 1 && lane == 0) {
+    // ---------------- MMA issuer ----------------
+    // Step x: the mix of unit x - 2, then the scores of unit x into the TMEM buffer that
+    // mix has done with.
+    const uint32_t q_addr = smem_u32(smem), k_base = smem_u32(smem + L::kOffK), v_base = smem_u32(smem + L::kOffV);
+    bool issued = false, ok = true;
+    int x = 0, seg = 0;         // scores: the next unit, its segment
+    int pseg = 0;               // mix: its segment's number
+    int pu = 0;                 // and the next unit
+    struct Span {
+      int first, units;
+    };
+    Span span[4] = {{0, 0}, {0, 0}, {0, 0}, {0, 0}};  // the last segments, by number mod 4
+    auto mix = [&]() {
+      const int u = pu++, w = u & 1;
+      while (u >= span[pseg & 3].first + span[pseg & 3].units) ++pseg;
+      const Span sp = span[pseg & 3];
+      if (!wait_phase(&pfull[w], (u >> 1) & 1, abort_flag, a.status, kWaitNs, true)) return false;
+      // the segment's first mix overwrites O: its last reader was the previous segment's end
+      if (u == sp.first && pseg > 0 && !wait_phase(ofree, (pseg - 1) & 1, abort_flag, a.status, kWaitNs, true)) return false;
+      const int kt = DUAL ? u >> 1 : u;
+      const int vs = kt % L::kVS;
+      if (!wait_phase(&vfull[vs], (kt / L::kVS) & 1, abort_flag, a.status, kWaitNs, true)) return false;
+      tc_fence_after();
+      const uint32_t v_addr = v_base + vs * L::kOperand;
+      const uint32_t fresh = u < sp.first + 2 ? 0u : 1u;  // the group's first unit of the segment
+#pragma unroll
+      for (int kk = 0; kk < kTile / 16; ++kk) {
+        mma_bf16_ts(tmem + L::kColO + w * HD, tmem + w * kTile + kk * 8, smem_desc(v_addr + kk * 2048, L::kBox, 1024), kIdescO,
+                    kk > 0 ? 1u : fresh);
+      }
+      issued = true;
+      mma_commit(&pvdone[w]);
+      if (!DUAL || w == 1) mma_commit(&vempty[vs]);
+      return true;
+    };
+    for (; ok && walk.left > 0; walk.next(a, per), ++seg) {
+      const int units = walk.segment() * L::kTiles;
+      span[seg & 3] = Span{x, units};
+      for (int i = 0; i < units; ++i, ++x) {
+        const int w = x & 1;
+        if (x >= 2 && !(ok = mix())) break;
+        if (i == 0 && !(ok = wait_phase(qfull, seg & 1, abort_flag, a.status, kWaitNs, true))) break;
+        const int kt = DUAL ? x >> 1 : x;
+        const int ks = kt % L::kKS;
+        if (!(ok = wait_phase(&kfull[ks], (kt / L::kKS) & 1, abort_flag, a.status, kWaitNs, true))) break;
+        if (x >= 2 && !(ok = wait_phase(&pvdone[w], ((x - 2) >> 1) & 1, abort_flag, a.status, kWaitNs, true))) break;
+        tc_fence_after();
+        const uint32_t k_addr = k_base + ks * L::kOperand;
+        const uint32_t qa = q_addr + (DUAL ? w * L::kOperand : 0);
+#pragma unroll
+        for (int kk = 0; kk < HD / 16; ++kk) {
+          const uint32_t off = (kk >> 2) * L::kBox + (kk & 3) * 32;
+          mma_bf16(tmem + w * kTile, smem_desc(qa + off, 16, 1024), smem_desc(k_addr + off, 16, 1024), kIdescS,
+                   kk > 0 ? 1u : 0u);
+        }
+        issued = true;
+        mma_commit(&sfull[w]);
+        if (!DUAL || w == 1) mma_commit(&kempty[ks]);
+        if (i == units - 1) mma_commit(qempty);
+      }
+    }
+    while (ok && pu < x) ok = mix();
+    if (issued) {
+      mma_commit(mma_done);
+      wait_phase(mma_done, 0, abort_flag, a.status, kDrainNs, false);
+    }
+  } else if (warp >= 4) {
+    // ---------------- softmax ----------------
+    const int w = (warp - 4) >> 2;      // group
+    const int quarter = warp & 3;
+    const int r = quarter * 32 + lane;  // row of the row tile: this thread's TMEM lane
+    const uint32_t lane_addr = static_cast<uint32_t>(quarter * 32) << 16;
+    const uint32_t s_addr = tmem + lane_addr + w * kTile;
+    const uint32_t o_addr = tmem + lane_addr + L::kColO + w * HD;
+    const int box_rows = min(a.page_size, kTile);
+    float2* ml = reinterpret_cast<float2*>(smem + L::kOffMl);
+    int x = 0;  // the segment's first unit
+    for (int seg = 0; walk.left > 0; walk.next(a, per), ++seg) {
+      const int n = walk.segment();
+      const int units = n * L::kTiles;
+      const Seq s = walk.s;
+      const int i0 = walk.p * per + (DUAL ? w * tpt : 0);
+      const int live = max(0, min(tpt, s.n - i0)) * a.group;
+      const bool warp_live = quarter * 32 < live;
+      const int token = i0 + r / a.group;  // a row past `live` computes on what it finds and is not stored
+      const int total = s.ctx + s.n;
+      float m = -INFINITY, l = 0.f;
+      const int u0 = x + ((x & 1) == w ? 0 : 1);
+      for (int u = u0; u < x + units; u += 2) {
+        const int kt = DUAL ? u >> 1 : u;
+        const int t = walk.t + (DUAL ? (u - x) >> 1 : u - x);  // tile of the item
+        warp_wait(&sfull[w], (u >> 1) & 1, abort_flag, a.status);
+        tc_fence_after();
+        const int slot0 = t * kTile;
+        const uint32_t bad = bad_ring[kt % kBadRing];
+        const bool masked = slot0 + kTile > s.ctx || bad != 0;
+        if (warp_live) {
+          uint32_t see[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
+          if (masked) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              see[c] = r < live ? seen32(a, s, token, slot0 + 32 * c) : 0u;
+              if (bad) see[c] &= sound32(bad, c, box_rows);
+            }
+          }
+          float top = -INFINITY;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            uint32_t v[32];
+            tmem_load32(s_addr + 32 * c, v);
+            tmem_wait_ld();
+            if (masked) {
+#pragma unroll
+              for (int e = 0; e < 32; ++e) {
+                if ((see[c] >> e) & 1) top = fmaxf(top, __uint_as_float(v[e]));
+              }
+            } else {
+#pragma unroll
+              for (int e = 0; e < 32; ++e) top = fmaxf(top, __uint_as_float(v[e]));
+            }
+          }
+          top = r < live ? top * a.qscale : -INFINITY;
+          const bool first = u == u0;
+          const bool rise = top > m + kRescaleAt || (m == -INFINITY && top > -INFINITY);
+          const float m_new = rise ? top : m;
+          const float alpha = rise ? ex2(m - m_new) : 1.f;  // m = -inf: 0
+          if (!first && __any_sync(0xffffffffu, rise)) {
+            // the group's previous mix is done: these scores were issued after it
+            l *= alpha;
+#pragma unroll
+            for (int c = 0; c < HD / 32; ++c) {
+              uint32_t v[32];
+              tmem_load32(o_addr + 32 * c, v);
+              tmem_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * alpha);
+              tmem_store32(o_addr + 32 * c, v);
+            }
+          }
+          m = m_new;
+          const float base = m == -INFINITY ? 0.f : m;
+          float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            uint32_t v[32], pk[16];
+            tmem_load32(s_addr + 32 * c, v);
+            tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) {
+              float p0 = ex2(fmaf(__uint_as_float(v[e]), a.qscale, -base));
+              float p1 = ex2(fmaf(__uint_as_float(v[e + 1]), a.qscale, -base));
+              if (masked) {
+                if (!((see[c] >> e) & 1)) p0 = 0.f;
+                if (!((see[c] >> (e + 1)) & 1)) p1 = 0.f;
+              }
+              sum[e / 2 % 4] += p0 + p1;
+              pk[e / 2] = pack_bf16x2(p0, p1);
+            }
+            tmem_store16(s_addr + 16 * c, pk);  // columns that have been read
+          }
+          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+          tmem_wait_st();
+        }
+        if (slot0 + kTile > total || bad != 0) {
+          // V rows that no copy filled, or stale slots behind the last token: zero
+          const int vs = kt % L::kVS;
+          warp_wait(&vfull[vs], (kt / L::kVS) & 1, abort_flag, a.status);
+          if (slot0 + r >= total || ((bad >> (r / box_rows)) & 1)) {
+            unsigned char* row = smem + L::kOffV + vs * L::kOperand + r * 128;
+#pragma unroll
+            for (int h = 0; h < HD / 64; ++h) {
+#pragma unroll
+              for (int c = 0; c < 8; ++c) *reinterpret_cast<uint4*>(row + h * L::kBox + c * 16) = make_uint4(0u, 0u, 0u, 0u);
+            }
+          }
+          fence_proxy_async_smem();
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&pfull[w]);
+      }
+
+      // The segment's end: sums out of TMEM, to out (whole item) or to a partial.
+      const bool whole = walk.t == 0 && n == walk.tiles;
+      float* slot = slots + (2 * static_cast<int64_t>(cta) + (seg > 0)) * L::kSlotFloats;
+      const int end = x + units;
+      const int h = r - (r / a.group) * a.group;
+      bf16* out = static_cast<bf16*>(a.out) + ((s.row0 + token) * a.hq + walk.kvh * a.group + h) * HD;
+      if constexpr (DUAL) {
+        warp_wait(&pvdone[w], ((end - 2 + w) >> 1) & 1, abort_flag, a.status);
+        tc_fence_after();
+        const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
+        if (warp_live) {
+#pragma unroll
+          for (int c = 0; c < HD / 32; ++c) {
+            uint32_t v[32];
+            tmem_load32(o_addr + 32 * c, v);
+            tmem_wait_ld();
+            if (r < live) {
+              if (whole) {
+#pragma unroll
+                for (int e = 0; e < 32; e += 8) {
+                  float f[8];
+#pragma unroll
+                  for (int d = 0; d < 8; ++d) f[d] = __uint_as_float(v[e + d]) * inv;
+                  st_plain(out + 32 * c + e, pack16<bf16>(f));
+                }
+              } else {
+                float* dst = slot + (w * kTile + r) * HD + 32 * c;
+#pragma unroll
+                for (int e = 0; e < 32; e += 4) st_plain(dst + e, make_uint4(v[e], v[e + 1], v[e + 2], v[e + 3]));
+              }
+            }
+          }
+          if (!whole && r < live) {
+            slot[L::kRows * HD + w * kTile + r] = m;
+            slot[L::kRows * (HD + 1) + w * kTile + r] = l;
+          }
+        }
+      } else {
+        // both groups' maxima and sums, then each takes half of the dims of both
+        ml[((seg & 1) * 2 + w) * kTile + r] = make_float2(m, l);
+        both_groups_sync();
+        const float2 other = ml[((seg & 1) * 2 + (w ^ 1)) * kTile + r];
+        const int last0 = end - 1 - ((end - 1) & 1), last1 = end - 1 - (~(end - 1) & 1);  // last units of groups 0, 1
+        if (last0 >= x) warp_wait(&pvdone[0], (last0 >> 1) & 1, abort_flag, a.status);
+        if (last1 >= x) warp_wait(&pvdone[1], (last1 >> 1) & 1, abort_flag, a.status);
+        tc_fence_after();
+        if (warp_live) {
+          const float top = fmaxf(m, other.x), base = top == -INFINITY ? 0.f : top;
+          const float own_f = m == -INFINITY ? 0.f : ex2(m - base), other_f = other.x == -INFINITY ? 0.f : ex2(other.x - base);
+          const float sum = l * own_f + other.y * other_f;
+          const float inv = !whole ? 1.f : sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
+          const float f0 = (w == 0 ? own_f : other_f) * inv, f1 = (w == 0 ? other_f : own_f) * inv;
+          const bool two = last0 >= x && last1 >= x;  // otherwise one group had no unit and its O is stale
+#pragma unroll
+          for (int c = 0; c < HD / 64; ++c) {
+            const int col = w * (HD / 2) + 32 * c;
+            uint32_t v[32];
+            float f[32];
+            tmem_load32(tmem + lane_addr + L::kColO + (last0 >= x ? 0 : HD) + col, v);
+            tmem_wait_ld();
+            const float fa = last0 >= x ? f0 : f1;
+#pragma unroll
+            for (int e = 0; e < 32; ++e) f[e] = fa == 0.f ? 0.f : __uint_as_float(v[e]) * fa;
+            if (two) {
+              tmem_load32(tmem + lane_addr + L::kColO + HD + col, v);
+              tmem_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 32; ++e) f[e] = f1 == 0.f ? f[e] : fmaf(__uint_as_float(v[e]), f1, f[e]);
+            }
+            if (r < live) {
+              if (whole) {
+#pragma unroll
+                for (int e = 0; e < 32; e += 8) st_plain(out + col + e, pack16<bf16>(f + e));
+              } else {
+                float* dst = slot + r * HD + col;
+#pragma unroll
+                for (int e = 0; e < 32; e += 4) *reinterpret_cast<float4*>(dst + e) = make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]);
+              }
+            }
+          }
+          if (!whole && w == 0 && r < live) {
+            slot[L::kRows * HD + r] = top;
+            slot[L::kRows * (HD + 1) + r] = sum;
+          }
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(ofree);
+      x = end;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, L::kCols);
+  }
+}
+
+// Adds up the partials of the item that CTA k's first tile continues: block (k, rows
+// 16 y .. 16 y + 15) by the first border inside the item.
+template <int HD, bool DUAL>
+__global__ void __launch_bounds__(256) tree_merge_kernel(const TreeArgs a, int ctas) {
+  grid_dependency_wait();
+  using L = Layout<HD, DUAL>;
+  const Record* records = reinterpret_cast<const Record*>(a.ws);
+  const float* slots = a.ws + records_bytes(ctas) / sizeof(float);
+  const int k = static_cast<int>(blockIdx.x) + 1;
+  const Record rec = records[k];
+  if (rec.t0 <= 0) return;  // no tiles, or its first tile begins an item
+  const int64_t first = rec.lo - rec.t0;  // the item's first tile
+  auto border = [&](int c) { return rec.total * c / rec.nc; };
+  if (border(k - 1) > first) return;  // an earlier border is inside it, too
+  Seq s;
+  read_seq(a, rec.b, &s);
+  const int tpt = tokens_per_tile(a);
+  constexpr int kLanes = 16;  // threads of a row
+  const int r = static_cast<int>(blockIdx.y) * 16 + threadIdx.x / kLanes;
+  const int tile = r / kTile, rr = r - tile * kTile;
+  const int i0 = rec.p * tpt * L::kTiles + tile * tpt;
+  if (rr >= max(0, min(tpt, s.n - i0)) * a.group) return;
+  const int last = static_cast<int>([&] {  // one past the last CTA with a part of the item
+    int c = k + 1;
+    while (c < rec.nc && border(c) < first + rec.tiles) ++c;
+    return c;
+  }());
+  auto part = [&](int c) { return slots + (2 * static_cast<int64_t>(c) + (c == k - 1 && border(c) != first)) * L::kSlotFloats; };
+  float m = -INFINITY;
+  for (int c = k - 1; c < last; ++c) m = fmaxf(m, part(c)[L::kRows * HD + r]);
+  const float base = m == -INFINITY ? 0.f : m;
+  constexpr int kDims = HD / kLanes;  // 4 or 8 dims of a thread
+  const int d = (threadIdx.x % kLanes) * kDims;
+  float l = 0.f, o[kDims];
+#pragma unroll
+  for (int e = 0; e < kDims; ++e) o[e] = 0.f;
+#pragma unroll 4
+  for (int c = k - 1; c < last; ++c) {
+    const float* ps = part(c);
+    const float f = ex2(ps[L::kRows * HD + r] - base);
+    l = fmaf(ps[L::kRows * (HD + 1) + r], f, l);
+#pragma unroll
+    for (int e = 0; e < kDims; e += 4) {
+      const float4 v = *reinterpret_cast<const float4*>(ps + r * HD + d + e);
+      o[e] = fmaf(v.x, f, o[e]);
+      o[e + 1] = fmaf(v.y, f, o[e + 1]);
+      o[e + 2] = fmaf(v.z, f, o[e + 2]);
+      o[e + 3] = fmaf(v.w, f, o[e + 3]);
+    }
+  }
+  const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
+  const int token = i0 + rr / a.group, h = rr - (rr / a.group) * a.group;
+  bf16* out = static_cast<bf16*>(a.out) + ((s.row0 + token) * a.hq + rec.kvh * a.group + h) * HD + d;
+#pragma unroll
+  for (int e = 0; e < kDims; e += 4) {
+    *reinterpret_cast<uint2*>(out + e) = make_uint2(pack_bf16x2(o[e] * inv, o[e + 1] * inv),
+                                                    pack_bf16x2(o[e + 2] * inv, o[e + 3] * inv));
+  }
+}
+
+// Whether an item holds two row tiles: more rows per kv head than one tile has.
+bool dual(int group, int max_tree) { return max_tree > kTile / group; }
+
+// CTAs for the bounds: one per SM, no more than the tiles there can be.
+int ctas_for(int64_t batch, int hkv, int group, int max_ctx, int max_tree) {
+  const int per = kTile / group * (dual(group, max_tree) ? 2 : 1);
+  const int64_t tiles = batch * hkv * ((max_tree + per - 1) / per) * ((static_cast<int64_t>(max_ctx) + max_tree + kTile - 1) / kTile);
+  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(sm_count(), (tiles + kMinTiles - 1) / kMinTiles)));
+}
+
+template <int HD, bool DUAL>
+int launch_form(const TreeArgs& a, cudaStream_t stream, const char* what) {
+  using L = Layout<HD, DUAL>;
+  const int tpt = kTile / a.group;
+  const uint64_t rows = static_cast<uint64_t>(a.num_pages) * a.hkv * a.page_size;
+  const uint32_t box_rows = static_cast<uint32_t>(std::min(a.page_size, kTile));
+  CUtensorMap tq, tk, tv;
+  if (int st = make_tensor_map_bf16(&tk, a.k_pages, HD, rows, 64, box_rows, what)) return st;
+  if (int st = make_tensor_map_bf16(&tv, a.v_pages, HD, rows, 64, box_rows, what)) return st;
+  if (int st = make_tensor_map_3d_bf16(&tq, a.q, HD, a.hq, a.total_q, 64, a.group, tpt, what)) return st;
+  auto kernel = tree_tc_kernel<HD, DUAL>;
+  if (int st = allow_dynamic_smem(reinterpret_cast<const void*>(kernel), L::kBytes, what)) return st;
+  const int nc = ctas_for(a.batch, a.hkv, a.group, a.max_ctx, a.max_tree);
+  if (int st = launch_kernel(what, kernel, dim3(nc), dim3(kThreadsTc), L::kBytes, stream, nullptr, tq, tk, tv, a)) return st;
+  // items of one tile, and a single CTA, are never cut
+  if (nc == 1 || a.max_ctx + a.max_tree <= kTile) return BM_OK;
+  return launch_kernel(what, tree_merge_kernel<HD, DUAL>, dim3(nc - 1, L::kRows / 16), dim3(256), 0, stream, nullptr, a, nc);
+}
+
+}  // namespace
+
+bool tc_takes(const TreeArgs& a, bm_dtype_t dtype) {
+  const int64_t rows = static_cast<int64_t>(a.num_pages) * a.hkv * a.page_size;
+  const bool pages = a.page_size >= 8 && (kTile % a.page_size == 0 || a.page_size % kTile == 0);
+  return dtype == BM_BF16 && (a.hd == 64 || a.hd == 128) && pages && rows + kTile < (int64_t{1} << 31);
+}
+
+size_t tc_workspace_bytes(int64_t batch, int hkv, int hd, int group, int max_ctx, int max_tree) {
+  if (hd != 64 && hd != 128) return 0;
+  const int nc = ctas_for(batch, hkv, group, max_ctx, max_tree);
+  const size_t rows = dual(group, max_tree) ? 2 * kTile : kTile;
+  return records_bytes(nc) + 2 * static_cast<size_t>(nc) * rows * (hd + 2) * sizeof(float);
+}
+
+int launch_tc(const TreeArgs& a, cudaStream_t stream, const char* what) {
+  if (a.hd == 128) {
+    return dual(a.group, a.max_tree) ? launch_form<128, true>(a, stream, what) : launch_form<128, false>(a, stream, what);
+  }
+  return dual(a.group, a.max_tree) ? launch_form<64, true>(a, stream, what) : launch_form<64, false>(a, stream, what);
+}
 
 }  // namespace paged
 }  // namespace bm

@@ -57,4 +57,19 @@ int make_tensor_map_2d(CUtensorMap* map, const void* base, bm_dtype_t dtype, uin
   return BM_OK;
 }
 
+int make_tensor_map_3d_bf16(CUtensorMap* map, const void* base, uint64_t inner, uint64_t middle, uint64_t outer,
+                            uint32_t box_inner, uint32_t box_middle, uint32_t box_outer, const char* what) {
+  EncodeTiled enc = encoder();
+  if (enc == nullptr) return fail(BM_ERR_CUDA, "%s: cuTensorMapEncodeTiled is not available", what);
+  const cuuint64_t dims[3] = {inner, middle, outer};
+  const cuuint64_t strides[2] = {inner * 2, inner * middle * 2};
+  const cuuint32_t box[3] = {box_inner, box_middle, box_outer};
+  const cuuint32_t elem[3] = {1, 1, 1};
+  CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, elem,
+                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(BM_ERR_CUDA, "%s: cuTensorMapEncodeTiled failed (%d)", what, static_cast<int>(r));
+  return BM_OK;
+}
+
 }  // namespace bm
