@@ -159,6 +159,8 @@ def lib_path() -> str:
 def load() -> ctypes.CDLL:
     """Loads the library once; raises if it is missing (no fallback path)."""
     global _lib
+    if _lib is not None:
+        return _lib
     with _lock:
         if _lib is None:
             if not os.path.exists(LIB_PATH):

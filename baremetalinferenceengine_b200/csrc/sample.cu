@@ -10,8 +10,8 @@
 // answer. Weights are 64-bit fixed point, 2^bits for the largest with 2^bits * vocab <=
 // 2^62, rounded once from fp64; every sum that decides is an integer sum, the same in any
 // order, and p * sum and u * sum are compared exactly. The fp64 2^-y is table-driven (the
-// method of Tang, ACM TOMS 15, 1989): y = (j + r) / 64, a table of 2^(-j/64) and a
-// polynomial of degree 5 in r, off by less than 2^-50 of the weight.
+// method of Tang, ACM TOMS 15, 1989): y = (j + r) / 128, a table of 2^(-j/128) and a
+// polynomial of degree 4 in r, off by less than 2^-49 of the weight.
 //
 // Bound: a row is read from HBM once (the passes below find it in L2), so bytes count
 // only for many rows; there the fp64 operations (eleven a logit where all weigh) cost as
@@ -46,7 +46,7 @@ constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxCluster = 8;
 constexpr int kBins = 4096;
-constexpr int kBinsPerThread = kBins / kThreads;
+constexpr int kCoarse = kBins / 64;
 constexpr int kList = 1024;  // logits of the border's bins that are collected
 constexpr double kLog2e = 1.4426950408889634074;
 
@@ -78,79 +78,68 @@ __device__ __forceinline__ float logit_of(uint32_t key) {
 }
 
 // A finite fp32 value in fp64 by its bits: the conversion instruction runs at a quarter
-// of the fp64 units' rate.
+// of the fp64 units' rate. What is below 2^-126 comes out as 2^-126 at most, which is
+// nothing beside a temperature of 2^-60 or more.
 __device__ __forceinline__ double widen(float x) {
-  const uint32_t u = __float_as_uint(x);
-  if ((u & 0x7f800000u) == 0) return static_cast<double>(x);  // zeros and denormals
-  return __hiloint2double(static_cast<int>((u & 0x80000000u) | (((u & 0x7fffffffu) >> 3) + 0x38000000u)),
-                          static_cast<int>(u << 29));
+  const int u = __float_as_int(x);
+  return __hiloint2double(((u >> 3) & 0x8fffffff) + 0x38000000, u << 29);
 }
 
 // Weights of a row.
 struct Weigher {
-  double top;            // the largest logit (0 when it is +inf: no other has a weight)
-  double scale;          // 64 log2(e) / T
-  double one, least;     // 2^bits; min_p in it
-  const double* table;   // 2^(bits - j/64), j < 64
-  float top_f, scale_f;  // the same in fp32, scale_f per octave
-  float limit;           // octaves past which a weight rounds to 0
+  double top;            // the largest logit (finite: see `remap`)
+  double scale;          // 128 log2(e) / T
+  double least;          // min_p in units of the weights
+  const double* table;   // 2^(bits - j/128), j < 128
+  float top_f, bins;     // bins of the histogram per logit
 
-  // log2 of the largest weight over this one, rounded: never falls as the logit does.
-  // NaN for -inf at T = inf.
-  __device__ __forceinline__ float octaves(float x) const { return (top_f - x) * scale_f; }
-  // The weight before it is rounded to a whole number, for x < top with octaves < limit.
+  // The weight's place in the histogram, from 0 at the largest logit; never falls as the
+  // logit does. Below kLimit the weight may round to something; NaN for a NaN logit, and
+  // for -inf at T = inf.
+  static constexpr float kLimit = kBins - 1.5f;
+  __device__ __forceinline__ float place(float x) const { return (top_f - x) * bins; }
+  // The weight before it is rounded to a whole number, for places below kLimit (anything
+  // for others).
   __device__ __forceinline__ double real(float x) const {
     constexpr double kRound = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to a whole number
-    constexpr double kStep = 0.010830424696249145;  // ln(2) / 64
-    const double y = (top - widen(x)) * scale;
-    const double shifted = y + kRound;
+    constexpr double c1 = -0.69314718055994530942 / 128, c2 = c1 * c1 / 2, c3 = c1 * c2 / 3, c4 = c1 * c3 / 4;
+    const double d = top - widen(x);
+    const double shifted = fma(d, scale, kRound);
     const int j = __double2loint(shifted);
-    const double z = (y - (shifted - kRound)) * -kStep;
-    double q = fma(z, 1.0 / 120.0, 1.0 / 24.0);
-    q = fma(z, q, 1.0 / 6.0);
-    q = fma(z, q, 0.5);
-    q = fma(z, q, 1.0);
-    q = fma(z, q, 1.0);
-    const double w = q * table[j & 63];
-    return __hiloint2double(__double2hiint(w) - ((j >> 6) << 20), __double2loint(w));
+    const double r = fma(d, scale, kRound - shifted);
+    double q = fma(r, c4, c3);
+    q = fma(r, q, c2);
+    q = fma(r, q, c1);
+    q = fma(r, q, 1.0);
+    const double w = q * table[j & 127];
+    return __hiloint2double(__double2hiint(w) - ((j >> 7) << 20), __double2loint(w));
   }
   __device__ __forceinline__ static u64 whole(double w) {  // w < 2^52, rounded
     return static_cast<u64>(__double_as_longlong(w + 4503599627370496.0)) & 0xfffffffffffffull;
   }
-  // The weight, and (kept) the same or 0 where min_p drops it.
-  __device__ __forceinline__ u64 weigh(float x, u64* kept) const {
-    if (x == top_f) {
-      *kept = static_cast<u64>(one);
-      return *kept;
-    }
-    *kept = 0;
-    if (!(octaves(x) < limit)) return 0;
-    const double w = real(x);
-    const u64 n = whole(w);
-    if (w >= least) *kept = n;
-    return n;
-  }
-  __device__ __forceinline__ u64 operator()(float x) const {
-    u64 kept;
-    return weigh(x, &kept);
-  }
+  __device__ __forceinline__ u64 operator()(float x) const { return place(x) < kLimit ? whole(real(x)) : 0; }
 };
+
+// Adding it to 0 <= x < 2^22 rounds x to a whole number, in the sum's low bits.
+constexpr float kMagic = 12582912.f;  // 1.5 * 2^23
+__device__ __forceinline__ int bits_of(float magic_sum) { return __float_as_int(magic_sum) - 0x4b400000; }
 
 struct Shared {
   union {
-    u64 wide[kBins];
     uint32_t hist[kBins];
+    u64 split[kThreads];   // of an interval of keys
   };
-  double table[64];
+  double table[128];
+  u64 coarse[kCoarse];     // the histogram by 64 bins
   u64 best[kMaxCluster];   // per CTA of the cluster: key << 32 | ~index
-  u64 sum[kMaxCluster], above[kMaxCluster], slice[kMaxCluster];
-  u64 warp[kWarps], sub[kWarps], kept[kWarps];
+  u64 sum[kMaxCluster], above[kMaxCluster];
+  u64 warp[kWarps], sub[kWarps];
   u64 before;              // value above the bin found
-  u64 ties;                // how many logits equal to t stay,
+  u64 ties;                // how many logits equal to t stay
   u64 cand_weight[kList];  // the leader's: collected logits
   uint32_t cand_key[kList];
   uint32_t list_key[kList], list_index[kList];  // this CTA's share of them
-  uint32_t own_count;
+  uint32_t own_count, offset;
   uint32_t count, key_min, key_max;             // the leader's: logits of the border's bins
   uint32_t bin_lo, bin_hi, bin;
   uint32_t key;            // t
@@ -192,14 +181,19 @@ __device__ __forceinline__ u64 portion(float f, u64 s, bool* fraction) {
   return __umul64hi(f64, s);
 }
 
+// In a row with +inf these are its largest logits and the others have no weight.
+__device__ __forceinline__ float remapped(float x, bool remap) {
+  return remap ? (x == INFINITY ? 0.f : -INFINITY) : x;
+}
+
 // The logits [lo, hi) of a row by one warp: f(index, logit), U 16-byte loads in flight
 // per lane besides those being worked on. Lanes may call f a different number of times.
 template <int U, typename T, typename F>
-__device__ __forceinline__ void each(const T* x, int lo, int hi, bool vec, F f) {
+__device__ __forceinline__ void each(const T* x, int lo, int hi, bool vec, bool remap, F f) {
   constexpr int VEC = VecWidth<T>::value;
   const int lane = threadIdx.x & 31;
   if (!vec) {
-    for (int i = lo + lane; i < hi; i += 32) f(i, load1(x + i));
+    for (int i = lo + lane; i < hi; i += 32) f(i, remapped(load1(x + i), remap));
     return;
   }
   const int whole = lo + (hi - lo) / VEC * VEC;  // a multiple of VEC, as lo is
@@ -223,12 +217,16 @@ __device__ __forceinline__ void each(const T* x, int lo, int hi, bool vec, F f) 
       if (i < whole) {
         float v[VEC];
         unpack16<T>(raw[u], v);
+        if (remap) {
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) v[e] = remapped(v[e], true);
+        }
 #pragma unroll
         for (int e = 0; e < VEC; ++e) f(i + e, v[e]);
       }
     }
   }
-  if (whole + lane < hi) f(whole + lane, load1(x + whole + lane));  // fewer than VEC are left
+  if (whole + lane < hi) f(whole + lane, remapped(load1(x + whole + lane), remap));  // fewer than VEC are left
 }
 
 template <typename T>
@@ -262,23 +260,26 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
 
   // ---------------- the largest logit ----------------
   {
-    uint32_t key = 0;
-    int at = 0;
-    each<4>(x, lo, hi, a.vec, [&](int i, float v) {
-      const uint32_t c = key_of(v);
-      if (c > key) {  // a lane's indexes ascend
-        key = c;
-        at = i;
-      }
-    });
-    u64 best = static_cast<u64>(key) << 32 | static_cast<uint32_t>(~at);
+    float m = -INFINITY;
+    int at = c_hi;
+    if (temp == 0.f) {  // and its first index
+      each<4>(x, lo, hi, a.vec, false, [&](int i, float v) {
+        if (v > m) {  // a lane's indexes ascend
+          m = v;
+          at = i;
+        }
+      });
+    } else {
+      each<4>(x, lo, hi, a.vec, false, [&](int, float v) { m = fmaxf(m, v); });
+    }
+    u64 best = static_cast<u64>(key_of(m)) << 32 | static_cast<uint32_t>(~at);
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) {
       const u64 o = __shfl_xor_sync(0xffffffffu, best, off);
       best = o > best ? o : best;
     }
     if (lane == 0) sh.warp[warp] = best;
-    if (tid < 64) sh.table[tid] = exp2(static_cast<double>(a.bits) - tid / 64.0);
+    if (tid < 128) sh.table[tid] = exp2(static_cast<double>(a.bits) - tid / 128.0);
     __syncthreads();
     if (tid < C) {
       for (int w = 0; w < kWarps; ++w) best = sh.warp[w] > best ? sh.warp[w] : best;
@@ -288,21 +289,22 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
   cluster.sync();
   u64 best = 0;
   for (int r = 0; r < C; ++r) best = sh.best[r] > best ? sh.best[r] : best;
-  const uint32_t top = static_cast<uint32_t>(best >> 32);
-  Weigher weigh;
-  weigh.top_f = logit_of(top);
-  if (weigh.top_f == -INFINITY || temp == 0.f) {
-    if (rank == 0 && tid == 0) a.tokens[row] = weigh.top_f == -INFINITY ? -1 : static_cast<int32_t>(~static_cast<uint32_t>(best));
+  const float top = logit_of(static_cast<uint32_t>(best >> 32));
+  if (top == -INFINITY || temp == 0.f) {
+    if (rank == 0 && tid == 0) a.tokens[row] = top == -INFINITY ? -1 : static_cast<int32_t>(~static_cast<uint32_t>(best));
     return;  // nobody reads another CTA's shared memory after the sync above
   }
-  weigh.top = weigh.top_f == INFINITY ? 0.0 : widen(weigh.top_f);
-  weigh.scale = 64.0 * kLog2e / static_cast<double>(temp);
-  weigh.one = exp2(static_cast<double>(a.bits));
-  weigh.least = weigh.one * static_cast<double>(fminf(mp, 1.f));
+  const bool remap = top == INFINITY;
+  const float octaves = static_cast<float>(a.bits + 2);  // past these a weight rounds to 0
+  const float bins_per_octave = Weigher::kLimit / octaves;
+  const double per_logit = kLog2e / fmax(static_cast<double>(temp), 0x1p-60);
+  Weigher weigh;
+  weigh.top_f = remap ? 0.f : top;
+  weigh.top = widen(weigh.top_f);
+  weigh.scale = 128.0 * per_logit;
+  weigh.least = exp2(static_cast<double>(a.bits)) * static_cast<double>(fminf(mp, 1.f));
   weigh.table = sh.table;
-  weigh.scale_f = static_cast<float>(kLog2e / static_cast<double>(temp));
-  weigh.limit = static_cast<float>(a.bits + 2);
-  const float bins_per_octave = static_cast<float>(kBins - 1) / weigh.limit;
+  weigh.bins = static_cast<float>(per_logit * static_cast<double>(bins_per_octave));
 
   uint32_t t = 0;         // what stays: keys above t,
   u64 ties = 0;           // and the first `ties` equal to it,
@@ -311,119 +313,165 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
   u64 kept = 0;
 
   // ---------------- t for top-k (stage 0) and top-p (stage 1) ----------------
+  const bool has_min_p = mp > 0.f;
   for (int stage = 0; stage < 2; ++stage) {
     if (stage == 0 ? !(k > 0 && k < a.vocab) : !(p < 1.f)) continue;
     const uint32_t t0 = t;  // top-p works on what top-k left: keys above t0
-    const u64 tied = stage == 1 && t0 != 0 ? ties * weigh(logit_of(t0)) : 0;  // and these
-    auto bin_of = [&](float x) -> int {  // by octaves; a logit without a weight has the last
-      if (x == weigh.top_f) return 0;
-      const float b = weigh.octaves(x) * bins_per_octave;
-      return b < static_cast<float>(kBins - 1) ? static_cast<int>(b) : kBins - 1;
+    const float t0_f = t0 != 0 ? logit_of(t0) : -INFINITY;
+    const u64 tied = stage == 1 && t0 != 0 ? ties * weigh(t0_f) : 0;  // and these
+    auto bin_of = [&](float x) -> int {  // a logit without a weight has the last
+      const float b = weigh.place(x);
+      return b < Weigher::kLimit ? bits_of(b + kMagic) : kBins - 1;
     };
-    // the fp32 weight in units of its bin's: at most 2^unit
-    auto coarse = [&](float x, int bin) -> uint32_t {
-      const float y = x == weigh.top_f ? 0.f : weigh.octaves(x) - static_cast<float>(bin) / bins_per_octave;
-      return __float2uint_rn(exp2f(static_cast<float>(a.unit) - fmaxf(y, 0.f)));
-    };
-    for (int b = tid; b < kBins; b += kThreads) sh.hist[b] = 0;
+    for (int b = tid; b < kBins / 4; b += kThreads) reinterpret_cast<uint4*>(sh.hist)[b] = make_uint4(0u, 0u, 0u, 0u);
     if (tid == 0) {
       sh.own_count = 0;
       sh.count = 0;
       sh.key_min = 0xffffffffu;
       sh.key_max = 0;
-      sh.bin_lo = sh.bin_hi = kBins - 1;
     }
     __syncthreads();
-    each<1>(x, lo, hi, a.vec, [&](int, float v) {
-      if (stage == 0) {
-        atomicAdd(&sh.hist[bin_of(v == v ? v : -INFINITY)], 1u);
-      } else if (key_of(v) > t0 && (v == weigh.top_f || weigh.octaves(v) < weigh.limit)) {
-        const int b = bin_of(v);
-        atomicAdd(&sh.hist[b], coarse(v, b));
-      }
-    });
-    cluster.sync();
-    // this CTA's slice of the bins, over the cluster
-    const int per_thread = kBins / C / kThreads;  // 8, 4, 2 or 1 bins
-    const int first_bin = rank * (kBins / C) + tid * per_thread;
-    u64 v[kBinsPerThread], mine = 0;
-#pragma unroll
-    for (int i = 0; i < kBinsPerThread; ++i) {
-      v[i] = 0;
-      if (i < per_thread) {
-        for (int r = 0; r < C; ++r) v[i] += peer(r)->hist[first_bin + i];
-        if (stage == 1) {  // units of the bin to units of the largest weight's 2^-40
-          v[i] = static_cast<u64>(static_cast<double>(v[i]) *
-                                  static_cast<double>(exp2f(static_cast<float>(40 - a.unit) -
-                                                            static_cast<float>(first_bin + i) / bins_per_octave)));
-          if (tied != 0 && bin_of(logit_of(t0)) == first_bin + i) v[i] += static_cast<u64>(static_cast<double>(tied) / weigh.one * 1099511627776.0);
+    if (stage == 0) {
+      each<1>(x, lo, hi, a.vec, remap, [&](int, float v) { atomicAdd(&sh.hist[bin_of(v)], 1u); });
+    } else {
+      // the fp32 weight in units of its bin's middle, 2^unit: linear within the bin
+      const float unit = exp2f(static_cast<float>(a.unit));
+      const float slope = unit * -0.69314718f / bins_per_octave;
+      each<1>(x, lo, hi, a.vec, remap, [&](int, float v) {
+        const float b = weigh.place(v);
+        if (b < Weigher::kLimit && v > t0_f) {
+          const float m = b + kMagic;
+          atomicAdd(&sh.hist[bits_of(m)], static_cast<uint32_t>(bits_of(fmaf(b - (m - kMagic), slope, unit) + kMagic)));
         }
-      }
-      mine += v[i];
+      });
     }
-    u64 all;
-    u64 at = block_scan64(mine, sh.sub, &all);
-    if (tid < C) peer(tid)->slice[rank] = all;
+    __syncthreads();
+    // a bin's value: its count, or its weight in units of 2^-40 of the largest
+    auto bin_value = [&](u64 h, int bin) -> u64 {
+      if (stage == 0) return h;
+      return static_cast<u64>(static_cast<double>(h) * static_cast<double>(exp2f(static_cast<float>(40 - a.unit) - static_cast<float>(bin) / bins_per_octave)));
+    };
+    const u64 tied_value = tied == 0 ? 0 : static_cast<u64>(static_cast<double>(tied) * exp2(40.0 - a.bits));
+    const int tied_bin = tied == 0 ? -1 : bin_of(t0_f);
+    {
+      u64 v = 0;  // eight bins a thread, 64 by eight threads
+#pragma unroll 1
+      for (int i = 0; i < kBins / kThreads; ++i) v += bin_value(sh.hist[tid * (kBins / kThreads) + i], tid * (kBins / kThreads) + i);
+#pragma unroll
+      for (int off = 4; off > 0; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
+      if ((lane & 7) == 0) sh.coarse[tid >> 3] = v + (rank == 0 && tied_bin >> 6 == tid >> 3 ? tied_value : 0);
+    }
     cluster.sync();
-    u64 sum = 0;
-    for (int r = 0; r < C; ++r) {
-      if (r < rank) at += sh.slice[r];
-      sum += sh.slice[r];
-    }
     // The bins that can hold the border: the first whose running value reaches the target,
-    // for top-p from the least to the most that the sums' errors allow. Octave counts here
-    // and above are off by 5 * 2^-24 of at most 53 octaves, a coarse weight by half a unit
-    // of at least 0.99 * 2^unit: a sum by e = 2^-16 + 1.01 * 2^-(unit + 1) of itself, a
-    // running sum against p * sum by 2 e (1 + e), below the 2^-13 + 2^(1 - unit) taken.
-    u64 least_target = k, most_target = k;
-    if (stage == 1) {
-      const double ps = static_cast<double>(fmaxf(p, 0.f)) * static_cast<double>(sum);
-      const double width = 0x1p-13 + exp2f(static_cast<float>(1 - a.unit));
-      least_target = max(static_cast<u64>(ps * fmax(1.0 - width, 0.0)), static_cast<u64>(1));
-      most_target = static_cast<u64>(ps * (1.0 + width)) + 2 * kBins;  // each bin's sum was cut to a whole number
-    }
+    // for top-p from the least to the most that the sums' errors allow. A place is off by
+    // 4 * 2^-24 of at most 53 octaves, the line within a bin by 2^-16.5 of the weight (half a
+    // bin is 53 / 8192 octaves at most), a coarse weight by half a unit of at least
+    // 0.99 * 2^unit: a sum by e = 2^-15.5 + 1.01 * 2^-(unit + 1) of itself, a running sum
+    // against p * sum by 2 e (1 + e), below the 2^-13 + 2^(1 - unit) taken.
+    if (warp == 0) {
+      static_assert(kCoarse == 64, "two coarse bins a lane");
+      u64 c0 = 0, c1 = 0;
+      for (int r = 0; r < C; ++r) {
+        c0 += peer(r)->coarse[2 * lane];
+        c1 += peer(r)->coarse[2 * lane + 1];
+      }
+      auto scan = [&](u64 v) {  // the sum of the lanes before, v included
 #pragma unroll
-    for (int i = 0; i < kBinsPerThread; ++i) {
-      const u64 next = at + v[i];
-      if (at < least_target && least_target <= next) {
-        for (int r = 0; r < C; ++r) peer(r)->bin_lo = first_bin + i;
-        if (stage == 0) {
-          for (int r = 0; r < C; ++r) peer(r)->before = at;
+        for (int off = 1; off < 32; off <<= 1) {
+          const u64 o = __shfl_up_sync(0xffffffffu, v, off);
+          if (lane >= off) v += o;
+        }
+        return v;
+      };
+      const u64 coarse_incl = scan(c0 + c1);
+      const u64 sum = __shfl_sync(0xffffffffu, coarse_incl, 31);
+      u64 least_target = k, most_target = k;
+      if (stage == 1) {
+        const double ps = static_cast<double>(fmaxf(p, 0.f)) * static_cast<double>(sum);
+        const double width = 0x1p-13 + exp2f(static_cast<float>(1 - a.unit));
+        least_target = max(static_cast<u64>(ps * fmax(1.0 - width, 0.0)), static_cast<u64>(1));
+        most_target = static_cast<u64>(ps * (1.0 + width)) + 2 * kBins;  // each bin's value was cut to a whole number
+      }
+#pragma unroll 1
+      for (int side = 0; side < 2; ++side) {
+        const u64 target = side == 0 ? least_target : most_target;
+        int bin = kBins - 1;
+        u64 at = 0;
+        const uint32_t hit = __ballot_sync(0xffffffffu, target <= coarse_incl);
+        if (hit != 0) {
+          const int l = __ffs(hit) - 1;
+          const u64 before = __shfl_sync(0xffffffffu, coarse_incl - c0 - c1, l), first = __shfl_sync(0xffffffffu, c0, l);
+          const int group = 2 * l + (target > before + first);
+          at = before + (target > before + first ? first : 0);
+          // its 64 bins, two a lane; rounding by bin and by CTA sums to what coarse holds
+          u64 f0 = 0, f1 = 0;
+          const int b0 = group * 64 + 2 * lane;
+          for (int r = 0; r < C; ++r) {
+            f0 += bin_value(peer(r)->hist[b0], b0);
+            f1 += bin_value(peer(r)->hist[b0 + 1], b0 + 1);
+          }
+          if (tied_bin == b0) f0 += tied_value;
+          if (tied_bin == b0 + 1) f1 += tied_value;
+          const u64 incl = at + scan(f0 + f1);
+          const int fl = __ffs(__ballot_sync(0xffffffffu, target <= incl)) - 1;
+          const u64 fine = __shfl_sync(0xffffffffu, incl - f0 - f1, fl), f = __shfl_sync(0xffffffffu, f0, fl);
+          bin = group * 64 + 2 * fl + (target > fine + f);
+          at = fine + (target > fine + f ? f : 0);
+        }
+        if (lane == 0) {
+          if (side == 0) {
+            sh.bin_lo = bin;
+            sh.before = at;
+          } else {
+            sh.bin_hi = bin;
+          }
         }
       }
-      if (at < most_target && most_target <= next) {
-        for (int r = 0; r < C; ++r) peer(r)->bin_hi = first_bin + i;
-      }
-      at = next;
     }
-    cluster.sync();
+    __syncthreads();
     const int bin_lo = static_cast<int>(sh.bin_lo), bin_hi = static_cast<int>(sh.bin_hi);
-    // Exact weights: of the row's part (sum), of what is above these bins, and of that
-    // what min_p keeps; and the bins' logits.
+    // Exact weights: of the row, of what is above these bins, and of that what min_p keeps;
+    // and the bins' logits.
     u64 own_sum = 0, own_above = 0;
-    uint32_t key_lo = 0xffffffffu, key_hi = 0;
+    uint32_t from = 0xffffffffu, to = 0;  // keys
     kept = 0;
-    each<1>(x, lo, hi, a.vec, [&](int i, float lv) {
+    auto collect = [&](int i, float lv) {
       const uint32_t key = key_of(lv);
-      if (key < t0) return;
-      const int b = bin_of(lv == lv ? lv : -INFINITY);
-      u64 w = 0, keep = 0;
-      if (key > t0 && (stage == 1 || b < bin_lo)) w = weigh.weigh(lv, &keep);
-      own_sum += w;
-      if (b < bin_lo) {
-        own_above += w;
-        kept += keep;
-      } else if (b <= bin_hi && (stage == 0 || w != 0 || key == t0)) {  // a logit without weight is no border
-        key_lo = min(key_lo, key);
-        key_hi = max(key_hi, key);
-        const uint32_t n = atomicAdd(&sh.own_count, 1u);
-        if (n < kList) {
-          sh.list_key[n] = key;
-          sh.list_index[n] = static_cast<uint32_t>(i);
-        }
+      from = min(from, key);
+      to = max(to, key);
+      const uint32_t n = atomicAdd(&sh.own_count, 1u);
+      if (n < kList) {
+        sh.list_key[n] = key;
+        sh.list_index[n] = static_cast<uint32_t>(i);
       }
-    });
-    if (stage == 1) {
+    };
+    if (stage == 0) {
+      each<1>(x, lo, hi, a.vec, remap, [&](int i, float lv) {
+        const int b = bin_of(lv);
+        if (b > bin_hi) return;
+        if (b >= bin_lo) {
+          collect(i, lv);
+        } else {
+          const double w = weigh.real(lv);
+          if (w >= weigh.least) kept += Weigher::whole(w);
+        }
+      });
+    } else {
+      const float m_lo = kMagic + static_cast<float>(bin_lo), m_hi = kMagic + static_cast<float>(bin_hi);
+      each<1>(x, lo, hi, a.vec, remap, [&](int i, float lv) {
+        const float b = weigh.place(lv), m = b + kMagic;
+        const double w = weigh.real(lv);
+        const u64 n = b < Weigher::kLimit && lv > t0_f ? Weigher::whole(w) : 0;
+        own_sum += n;
+        if (m < m_lo) {
+          own_above += n;
+          if (has_min_p && w >= weigh.least) kept += n;
+        } else if (m <= m_hi && n != 0) {  // a logit without weight is no border
+          collect(i, lv);
+        }
+        if (t0 != 0 && lv == t0_f && m <= m_hi) collect(i, lv);
+      });
+      if (!has_min_p) kept = own_above;
       own_sum = warp_sum64(own_sum);
       own_above = warp_sum64(own_above);
       if (lane == 0) {
@@ -431,19 +479,31 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
         sh.sub[warp] = own_above;
       }
     }
+    // This CTA's collected logits go behind the others' in the leader's list.
+    auto value = [&](uint32_t key) -> u64 { return stage == 0 ? 1 : key == t0 ? 0 : weigh(logit_of(key)); };
+    auto hand_over = [&]() {
 #pragma unroll
-    for (int off = 16; off > 0; off >>= 1) {
-      key_lo = min(key_lo, __shfl_xor_sync(0xffffffffu, key_lo, off));
-      key_hi = max(key_hi, __shfl_xor_sync(0xffffffffu, key_hi, off));
-    }
-    if (lane == 0 && key_hi != 0) {
-      atomicMin(&peer(0)->key_min, key_lo);
-      atomicMax(&peer(0)->key_max, key_hi);
-    }
-    __syncthreads();
-    // this CTA's collected logits go behind the others' in the leader's list
-    const uint32_t own_count = sh.own_count;
-    if (tid == 0) sh.bin = own_count == 0 ? 0 : atomicAdd(&peer(0)->count, own_count);
+      for (int off = 16; off > 0; off >>= 1) {
+        from = min(from, __shfl_xor_sync(0xffffffffu, from, off));
+        to = max(to, __shfl_xor_sync(0xffffffffu, to, off));
+      }
+      if (lane == 0 && to != 0) {
+        atomicMin(&peer(0)->key_min, from);
+        atomicMax(&peer(0)->key_max, to);
+      }
+      __syncthreads();
+      const uint32_t own = sh.own_count;
+      if (tid == 0 && own != 0) sh.offset = atomicAdd(&peer(0)->count, own);
+      __syncthreads();
+      for (uint32_t i = tid; i < min(own, static_cast<uint32_t>(kList)); i += kThreads) {
+        const uint32_t at = sh.offset + i, key = sh.list_key[i];
+        if (at < kList) {
+          peer(0)->cand_key[at] = key;
+          peer(0)->cand_weight[at] = value(key);
+        }
+      }
+    };
+    hand_over();
     if (stage == 1 && tid < C) {
       u64 s = 0, b = 0;
       for (int w = 0; w < kWarps; ++w) {
@@ -452,12 +512,6 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
       }
       peer(tid)->sum[rank] = s;
       peer(tid)->above[rank] = b;
-    }
-    __syncthreads();
-    for (uint32_t i = tid; i < own_count; i += kThreads) {
-      if (sh.bin + i >= kList || i >= kList) break;
-      peer(0)->cand_key[sh.bin + i] = sh.list_key[i];
-      peer(0)->cand_weight[sh.bin + i] = stage == 0 ? 1 : sh.list_key[i] == t0 ? 0 : weigh(logit_of(sh.list_key[i]));
     }
     cluster.sync();
     u64 target = k, passed = stage == 0 ? sh.before : 0;
@@ -472,127 +526,69 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
       if (fraction || target == 0) ++target;  // a token stays while the weight before it is below target
     }
     uint32_t count = peer(0)->count;
-    key_lo = peer(0)->key_min;
-    key_hi = peer(0)->key_max;
+    from = peer(0)->key_min;
+    to = peer(0)->key_max;
     summed = count <= kList;
-    auto value = [&](uint32_t key) -> u64 { return stage == 0 ? 1 : key == t0 ? 0 : weigh(logit_of(key)); };
-    // the interval's bins, descending, at most kBins of 2^shift keys
-    auto shift_of = [](uint32_t from, uint32_t to) {
-      int s = 0;
-      while (((to - from) >> s) >= static_cast<uint32_t>(kBins)) ++s;
-      return s;
-    };
-    // More than the list holds: the cluster splits the interval of keys until it does.
-    for (int round = 0; round < 3 && count > kList && key_lo != key_hi; ++round) {  // 12 bits a round
-      cluster.sync();  // the leader's counters have been read
-      const int shift = shift_of(key_lo, key_hi);
-      for (int b = tid; b < kBins; b += kThreads) sh.wide[b] = 0;
+    // Split the keys from..to, 512 equal parts a round, down to the border's key: by the
+    // whole cluster while the list does not hold them, then by the leader.
+    for (int round = 0; round < 4 && from != to; ++round) {
+      const bool all = count > kList;
+      if (!all && rank != 0) break;
+      if (all) cluster.sync();  // the leader's counters have been read
+      int shift = 0;
+      while (((to - from) >> shift) >= static_cast<uint32_t>(kThreads)) ++shift;
+      sh.split[tid] = 0;
       if (tid == 0) {
-        sh.own_count = 0;
-        sh.count = 0;
+        sh.own_count = all ? 0 : sh.own_count;
+        if (all) sh.count = 0;
         sh.key_min = 0xffffffffu;
         sh.key_max = 0;
       }
       __syncthreads();
-      each<1>(x, lo, hi, a.vec, [&](int, float lv) {
-        const uint32_t key = key_of(lv);
-        if (key < key_lo || key > key_hi) return;
-        const u64 w = value(key);
-        if (w != 0) atomicAdd(&sh.wide[(key_hi - key) >> shift], w);
-      });
-      cluster.sync();
-      mine = 0;
-#pragma unroll
-      for (int i = 0; i < kBinsPerThread; ++i) {
-        v[i] = 0;
-        if (i < per_thread) {
-          for (int r = 0; r < C; ++r) v[i] += peer(r)->wide[first_bin + i];
-          if (tied != 0 && t0 >= key_lo && t0 <= key_hi && (key_hi - t0) >> shift == static_cast<uint32_t>(first_bin + i)) v[i] += tied;
+      if (all) {
+        each<1>(x, lo, hi, a.vec, remap, [&](int, float lv) {
+          const uint32_t key = key_of(lv);
+          if (key >= from && key <= to) atomicAdd(&sh.split[(to - key) >> shift], value(key));
+        });
+        cluster.sync();
+      } else {
+        for (uint32_t i = tid; i < count; i += kThreads) {
+          const uint32_t key = sh.cand_key[i];
+          if (key >= from && key <= to) atomicAdd(&sh.split[(to - key) >> shift], sh.cand_weight[i]);
         }
-        mine += v[i];
+        __syncthreads();
       }
-      at = block_scan64(mine, sh.sub, &all) + passed;
-      if (tid < C) peer(tid)->slice[rank] = all;
-      cluster.sync();
-      for (int r = 0; r < rank; ++r) at += sh.slice[r];
-#pragma unroll
-      for (int i = 0; i < kBinsPerThread; ++i) {
-        if (at < target && target <= at + v[i]) {
-          for (int r = 0; r < C; ++r) {
-            peer(r)->bin = first_bin + i;
-            peer(r)->before = at;
-          }
-        }
-        at += v[i];
+      u64 v = 0, total;
+      if (all) {
+        for (int r = 0; r < C; ++r) v += peer(r)->split[tid];
+      } else {
+        v = sh.split[tid];
       }
-      cluster.sync();
+      if (tied != 0 && t0 >= from && t0 <= to && (to - t0) >> shift == static_cast<uint32_t>(tid)) v += tied;
+      const u64 at = block_scan64(v, sh.sub, &total) + passed;
+      if (at < target && target <= at + v) {
+        sh.bin = tid;
+        sh.before = at;
+      }
+      __syncthreads();
       passed = sh.before;
-      const uint32_t bin = sh.bin;
-      const uint32_t from = key_lo, to = key_hi;
-      key_lo = 0xffffffffu;
-      key_hi = 0;
-      __syncthreads();  // sh.bin has been read
-      each<1>(x, lo, hi, a.vec, [&](int i, float lv) {
-        const uint32_t key = key_of(lv);
-        if (key < from || key > to || (to - key) >> shift != bin) return;
-        key_lo = min(key_lo, key);
-        key_hi = max(key_hi, key);
-        const uint32_t n = atomicAdd(&sh.own_count, 1u);
-        if (n < kList) sh.list_key[n] = key;
-      });
-      if (key_hi != 0) {
-        atomicMin(&peer(0)->key_min, key_lo);
-        atomicMax(&peer(0)->key_max, key_hi);
-      }
-      __syncthreads();
-      const uint32_t own = sh.own_count;
-      if (tid == 0) sh.bin = own == 0 ? 0 : atomicAdd(&peer(0)->count, own);
-      __syncthreads();
-      for (uint32_t i = tid; i < own; i += kThreads) {
-        if (sh.bin + i >= kList || i >= kList) break;
-        peer(0)->cand_key[sh.bin + i] = sh.list_key[i];
-        peer(0)->cand_weight[sh.bin + i] = value(sh.list_key[i]);
-      }
-      cluster.sync();
-      count = peer(0)->count;
-      key_lo = peer(0)->key_min;
-      key_hi = peer(0)->key_max;
-    }
-    if (rank == 0) {
-      uint32_t from = key_lo, to = key_hi;
-      for (int round = 0; round < 3 && from != to; ++round) {  // count <= kList; 12 bits a round
-        const int shift = shift_of(from, to);
-        __syncthreads();
-        for (int b = tid; b < kBins; b += kThreads) sh.wide[b] = 0;
-        __syncthreads();
+      const uint32_t bin = sh.bin, old_from = from, old_to = to;
+      if (all) {
+        from = 0xffffffffu;
+        to = 0;
+        each<1>(x, lo, hi, a.vec, remap, [&](int i, float lv) {
+          const uint32_t key = key_of(lv);
+          if (key >= old_from && key <= old_to && (old_to - key) >> shift == bin) collect(i, lv);
+        });
+        hand_over();
+        cluster.sync();
+        count = peer(0)->count;
+        from = peer(0)->key_min;
+        to = peer(0)->key_max;
+      } else {
         for (uint32_t i = tid; i < count; i += kThreads) {
           const uint32_t key = sh.cand_key[i];
-          if (key >= from && key <= to) atomicAdd(&sh.wide[(to - key) >> shift], sh.cand_weight[i]);
-        }
-        if (tid == 0 && tied != 0 && t0 >= from && t0 <= to) atomicAdd(&sh.wide[(to - t0) >> shift], tied);
-        __syncthreads();
-        mine = 0;
-#pragma unroll
-        for (int i = 0; i < kBinsPerThread; ++i) {
-          v[i] = sh.wide[tid * kBinsPerThread + i];
-          mine += v[i];
-        }
-        at = block_scan64(mine, sh.sub, &all) + passed;
-#pragma unroll
-        for (int i = 0; i < kBinsPerThread; ++i) {
-          if (at < target && target <= at + v[i]) {
-            sh.bin = tid * kBinsPerThread + i;
-            sh.before = at;
-            sh.key_min = 0xffffffffu;
-            sh.key_max = 0;
-          }
-          at += v[i];
-        }
-        __syncthreads();
-        passed = sh.before;
-        for (uint32_t i = tid; i < count; i += kThreads) {
-          const uint32_t key = sh.cand_key[i];
-          if (key >= from && key <= to && (to - key) >> shift == sh.bin) {
+          if (key >= from && key <= to && (to - key) >> shift == bin) {
             atomicMin(&sh.key_min, key);
             atomicMax(&sh.key_max, key);
           }
@@ -601,29 +597,20 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
         from = sh.key_min;
         to = sh.key_max;
       }
-      uint32_t equal = count;  // logits of key t
-      if (count <= kList) {
-        int n = 0;
-        for (uint32_t i = tid; i < count; i += kThreads) n += sh.cand_key[i] == from;
-        u64 total;
-        block_scan64(n, sh.sub, &total);
-        equal = static_cast<uint32_t>(total);
-      }
-      if (tid == 0) {
-        u64 rest;
-        if (stage == 1 && from == t0) {
-          const u64 w = max(weigh(logit_of(t0)), static_cast<u64>(1));
-          rest = min((target - passed + w - 1) / w, ties);
-        } else {
-          const u64 w = max(value(from), static_cast<u64>(1));  // a border lies in logits of some value
-          rest = (target - passed + w - 1) / w;
-        }
-        if (rest > equal) rest = equal;
-        for (int r = 0; r < C; ++r) {
-          peer(r)->key = from;
-          peer(r)->ties = rest;
-          peer(r)->cut = rest < equal;
-        }
+    }
+    if (rank == 0) {
+      int n = 0;
+      for (uint32_t i = tid; i < count && count <= kList; i += kThreads) n += sh.cand_key[i] == from;
+      u64 total;
+      block_scan64(static_cast<u64>(n), sh.sub, &total);
+      if (tid < C) {
+        const u64 equal = count > kList ? count : total;  // logits of key t (over the list: one key)
+        const u64 w = max(stage == 1 && from == t0 ? weigh(t0_f) : value(from), static_cast<u64>(1));
+        u64 rest = min((target - passed + w - 1) / w, equal);
+        if (stage == 1 && from == t0) rest = min(rest, ties);
+        peer(tid)->key = from;
+        peer(tid)->ties = rest;
+        peer(tid)->cut = rest < equal;
       }
     }
     cluster.sync();
@@ -632,12 +619,40 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
     cut = sh.cut;
   }
 
-  // ---------------- the index where a running sum passes a target ----------------
-  // f(index, logit) -> its value. The sums by warp's stretch are in sh.warp; then those by
-  // sixteenths of the stretch that holds the target, then its logits. Writes the index to
-  // every CTA's sh.index.
-  auto find = [&](auto f, auto target_of) -> void {
+  // ---------------- the token ----------------
+  // An index by running sums of values: the sums by warp's stretch (own) meet over the
+  // cluster; then those by sixteenths of the stretch that holds the target, then its
+  // logits. First (if not all logits equal to t stay) the last of those that do, then the
+  // token.
+  const float t_f = t != 0 ? logit_of(t) : -INFINITY;
+  uint32_t last_tie = 0xffffffffu;
+  for (int what = cut ? 0 : 1; what < 2; ++what) {
+    auto value = [&](int i, float v) -> u64 {
+      if (what == 0) return v == t_f;
+      if (!(weigh.place(v) < Weigher::kLimit) || v < t_f || (v == t_f && static_cast<uint32_t>(i) > last_tie)) return 0;
+      const double w = weigh.real(v);
+      return w >= weigh.least ? Weigher::whole(w) : 0;
+    };
+    // What stays above the border's bins was summed on the way; their logits are collected.
+    u64 own = 0;
+    const bool have = what == 1 && summed;
+    if (have) {
+      own = kept;
+    } else {
+      each<1>(x, lo, hi, a.vec, remap, [&](int i, float v) { own += value(i, v); });
+    }
+    own = warp_sum64(own);
     __syncthreads();
+    if (lane == 0) sh.warp[warp] = own;
+    __syncthreads();
+    if (have) {
+      for (uint32_t i = tid; i < sh.own_count; i += kThreads) {
+        const int index = static_cast<int>(sh.list_index[i]);
+        const u64 w = value(index, logit_of(sh.list_key[i]));
+        if (w != 0) atomicAdd(&sh.warp[(index - c_lo) / span], w);
+      }
+      __syncthreads();
+    }
     if (tid < C) {
       u64 s = 0;
       for (int w = 0; w < kWarps; ++w) s += sh.warp[w];
@@ -649,82 +664,51 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
       if (r < rank) at += sh.sum[r];
       total += sh.sum[r];
     }
-    const u64 want = target_of(total);             // the first index whose running sum exceeds it
+    bool fraction;
+    const u64 want = what == 0 ? ties - 1 : portion(u, total, &fraction);  // the first index whose running sum exceeds it
     if (at <= want && want < at + sh.sum[rank]) {  // this CTA's stretch (all its threads agree)
       int w = 0;
-      while (want >= at + sh.warp[w]) at += sh.warp[w++];
+      while (w < kWarps - 1 && want >= at + sh.warp[w]) at += sh.warp[w++];
       const int w_lo = min(c_hi, c_lo + w * span), w_hi = min(c_hi, w_lo + span);
       const int part = ((w_hi - w_lo + kWarps - 1) / kWarps + VEC - 1) / VEC * VEC;
       int s_lo = min(w_hi, w_lo + warp * part), s_hi = min(w_hi, s_lo + part);
-      u64 own = 0;
-      each<1>(x, s_lo, s_hi, a.vec, [&](int i, float v) { own += f(i, v); });
+      own = 0;
+      each<1>(x, s_lo, s_hi, a.vec, remap, [&](int i, float v) { own += value(i, v); });
       own = warp_sum64(own);
       if (lane == 0) sh.sub[warp] = own;
       __syncthreads();
       if (warp == 0) {
         int q = 0;
-        while (want >= at + sh.sub[q]) at += sh.sub[q++];
+        while (q < kWarps - 1 && want >= at + sh.sub[q]) at += sh.sub[q++];
         s_lo = min(w_hi, w_lo + q * part);
         s_hi = min(w_hi, s_lo + part);
         for (int i0 = s_lo; i0 < s_hi; i0 += 32) {
           const int i = i0 + lane;
-          u64 incl = i < s_hi ? f(i, load1(x + i)) : 0;
+          u64 incl = i < s_hi ? value(i, remapped(load1(x + i), remap)) : 0;
 #pragma unroll
           for (int off = 1; off < 32; off <<= 1) {
             const u64 o = __shfl_up_sync(0xffffffffu, incl, off);
             if (lane >= off) incl += o;
           }
-          const unsigned int hit = __ballot_sync(0xffffffffu, want < at + incl);
+          const uint32_t hit = __ballot_sync(0xffffffffu, want < at + incl);
           if (hit != 0) {
-            if (lane < C) peer(lane)->index = i0 + __ffs(hit) - 1;
+            const int index = i0 + __ffs(hit) - 1;
+            if (what == 1) {
+              if (lane == 0) a.tokens[row] = index;
+            } else if (lane < C) {
+              peer(lane)->index = index;
+            }
             break;
           }
           at += __shfl_sync(0xffffffffu, incl, 31);
         }
       }
     }
-    cluster.sync();
-  };
-
-  uint32_t last_tie = 0xffffffffu;  // index of the last logit equal to t that stays
-  if (cut) {
-    auto is_tie = [&](int, float v) -> u64 { return key_of(v) == t; };
-    u64 own = 0;
-    each<1>(x, lo, hi, a.vec, [&](int i, float v) { own += is_tie(i, v); });
-    own = warp_sum64(own);
-    __syncthreads();
-    if (lane == 0) sh.warp[warp] = own;
-    find(is_tie, [&](u64) { return ties - 1; });
-    last_tie = sh.index;
-  }
-  auto staying = [&](int i, float v) -> u64 {
-    const uint32_t key = key_of(v);
-    if (key < t || (key == t && static_cast<uint32_t>(i) > last_tie)) return 0;
-    u64 keep;
-    weigh.weigh(v, &keep);
-    return keep;
-  };
-  // What stays, by warp's stretch: summed above the border's bins on the way, and of
-  // their collected logits here; or all of it now.
-  if (!summed) {
-    kept = 0;
-    each<1>(x, lo, hi, a.vec, [&](int i, float v) { kept += staying(i, v); });
-  }
-  kept = warp_sum64(kept);
-  __syncthreads();
-  if (lane == 0) sh.warp[warp] = kept;
-  if (summed) {
-    __syncthreads();
-    for (uint32_t i = tid; i < min(sh.own_count, static_cast<uint32_t>(kList)); i += kThreads) {
-      const u64 w = staying(static_cast<int>(sh.list_index[i]), logit_of(sh.list_key[i]));
-      if (w != 0) atomicAdd(&sh.warp[(static_cast<int>(sh.list_index[i]) - c_lo) / span], w);
+    if (what == 0) {
+      cluster.sync();
+      last_tie = sh.index;
     }
   }
-  find(staying, [&](u64 total) {
-    bool fraction;
-    return portion(u, total, &fraction);
-  });
-  if (rank == 0 && tid == 0) a.tokens[row] = static_cast<int32_t>(sh.index);
 }
 
 }  // namespace

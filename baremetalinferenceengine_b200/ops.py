@@ -451,18 +451,19 @@ def _empty(shape, dtype: torch.dtype, device: torch.device, stream) -> torch.Ten
         return torch.empty(shape, dtype=dtype, device=device)
 
 
-def _head_rows(t: torch.Tensor, name: str, ref: torch.Tensor) -> None:
-    """[rows, heads, head_dim] of ref's device and dtype with dense heads (rows may be
-    slices of wider ones)."""
-    if t.dim() != 3 or t.dtype != ref.dtype or t.device != ref.device or t.shape[2] != ref.shape[2]:
+def _head_rows(t: torch.Tensor, name: str, dtype: torch.dtype, device: torch.device, hd: int):
+    """(rows, heads, elements between rows) of [rows, heads, hd] with dense heads; rows may
+    be slices of wider ones."""
+    shape = t.shape
+    if len(shape) != 3 or shape[2] != hd or t.dtype != dtype or t.device != device:
         raise _invalid(f"{name} must be [rows, heads, head_dim] of the other tensors' device, dtype and head_dim")
-    if t.numel() > 0 and ((t.shape[2] > 1 and t.stride(2) != 1) or (t.shape[1] > 1 and t.stride(1) != t.shape[2])):
+    rows, heads, _ = shape
+    if t.is_contiguous():
+        return rows, heads, heads * hd
+    s0, s1, s2 = t.stride()
+    if (hd > 1 and s2 != 1) or (heads > 1 and s1 != hd):
         raise _invalid(f"{name} must have dense heads")
-
-
-def _row_stride(t: torch.Tensor) -> int:
-    """Elements between rows (a single row's or an empty tensor's stride means nothing)."""
-    return t.stride(0) if t.shape[0] > 1 and t.numel() > 0 else t.shape[1] * t.shape[2]
+    return rows, heads, s0 if rows > 1 else heads * hd
 
 
 def _same_device_i32(t: Optional[torch.Tensor], name: str, device: torch.device, numel: Optional[int] = None) -> None:
@@ -477,6 +478,35 @@ def _same_device_i32(t: Optional[torch.Tensor], name: str, device: torch.device,
 def _table_device(table: Optional[RopeTable], device: torch.device) -> None:
     if table is not None and table.data.device != device:
         raise _invalid("the rope table is on another device")
+
+
+class _On:
+    """Makes `device` current for a call, at no cost where it is already."""
+
+    __slots__ = ("device", "guard")
+
+    def __init__(self, device: torch.device):
+        self.device = device
+
+    def __enter__(self):
+        self.guard = None
+        if torch.cuda.current_device() != self.device.index:
+            self.guard = torch.cuda.device(self.device)
+            self.guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+
+
+# The current stream's handle without a Stream object around it, where torch has that.
+_current_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def _raw_stream(device: torch.device, stream: Optional[torch.cuda.Stream]) -> int:
+    if stream is None and _current_raw_stream is not None:
+        return _current_raw_stream(device.index)
+    return _stream(device, stream)
 
 
 def _status_ptr(status: Optional[DeviceStatus], device: torch.device) -> Optional[int]:
@@ -501,32 +531,38 @@ def rotary(q: Optional[torch.Tensor], k: Optional[torch.Tensor], positions, tabl
         raise _invalid("neither q nor k given")
     if ref.dim() != 3:
         raise _invalid("q and k must be [rows, heads, head_dim]")
-    dev, rows = _dev(ref), ref.shape[0]
-    outs = []
-    for name, x, out in (("q", q, q_out), ("k", k, k_out)):
-        if x is None:
-            if out is not None:
-                raise _invalid(f"{name}_out without {name}")
-            outs.append(None)
-            continue
-        _head_rows(x, name, ref)
-        if out is None:
-            out = _empty(x.shape, x.dtype, dev, stream)
-        _head_rows(out, name + "_out", ref)
-        if x.shape[0] != rows or out.shape != x.shape:
-            raise _invalid("q, k and their outputs must have the same rows, and an output its input's shape")
-        outs.append(out)
+    dev, dtype, hd = _dev(ref), ref.dtype, ref.shape[2]
+    code = bm_dtype(ref)
+    rows = hq = hkv = qs = ks = qos = kos = 0
+    qp = kp = qop = kop = None
+    if q is not None:
+        rows, hq, qs = _head_rows(q, "q", dtype, dev, hd)
+        if q_out is None:
+            q_out = _empty(q.shape, dtype, dev, stream)
+        out_rows, out_heads, qos = _head_rows(q_out, "q_out", dtype, dev, hd)
+        if out_rows != rows or out_heads != hq:
+            raise _invalid("q_out must have q's shape")
+        qp, qop = q.data_ptr(), q_out.data_ptr()
+    elif q_out is not None:
+        raise _invalid("q_out without q")
+    if k is not None:
+        k_rows, hkv, ks = _head_rows(k, "k", dtype, dev, hd)
+        if k_out is None:
+            k_out = _empty(k.shape, dtype, dev, stream)
+        out_rows, out_heads, kos = _head_rows(k_out, "k_out", dtype, dev, hd)
+        if out_rows != k_rows or out_heads != hkv or (q is not None and k_rows != rows):
+            raise _invalid("k must have q's rows, and k_out k's shape")
+        rows = k_rows
+        kp, kop = k.data_ptr(), k_out.data_ptr()
+    elif k_out is not None:
+        raise _invalid("k_out without k")
     pos_t, pos0 = (None, positions) if isinstance(positions, int) else (positions, 0)
     _same_device_i32(pos_t, "positions", dev, rows)
     _table_device(table, dev)
-    q_out, k_out = outs
-    none = torch.empty(0, 0, 0)
-    qs, ks, qo, ko = (none if t is None else t for t in (q, k, q_out, k_out))
-    with torch.cuda.device(dev):
-        check(load().bm_rotary(_ptr(q_out), _ptr(k_out), _ptr(q), _ptr(k), _ptr(pos_t), pos0, table.ptr, table.max_pos,
-                               table.head_dim, int(interleaved), rows, qs.shape[1], ks.shape[1], ref.shape[2],
-                               _row_stride(qs), _row_stride(ks), _row_stride(qo), _row_stride(ko), bm_dtype(ref),
-                               _status_ptr(status, dev), _stream(dev, stream)))
+    with _On(dev):
+        check(load().bm_rotary(qop, kop, qp, kp, None if pos_t is None else pos_t.data_ptr(), pos0, table.ptr,
+                               table.max_pos, table.head_dim, int(interleaved), rows, hq, hkv, hd, qs, ks, qos, kos, code,
+                               _status_ptr(status, dev), _raw_stream(dev, stream)))
     return q_out, k_out
 
 
@@ -542,7 +578,6 @@ class PagedKV:
             raise _invalid("k_pages and v_pages must be [num_pages, kv_heads, page_size, head_dim]")
         _dense(k_pages, "k_pages")
         _dense(v_pages, "v_pages")
-        bm_dtype(k_pages)
         _same(k_pages, v_pages)
         if page_table.dim() != 2:
             raise _invalid("page_table must be [num_seqs, max_pages]")
@@ -553,6 +588,7 @@ class PagedKV:
         self.device, self.dtype = k_pages.device, k_pages.dtype
         self.c = _lib.PagedKVC(k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr(), self.num_pages,
                                self.page_size, self.max_pages, self.num_seqs, self.num_kv_heads, self.head_dim)
+        self.ref, self.code = ctypes.byref(self.c), bm_dtype(k_pages)
 
 
 def paged_kv_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, positions: Optional[torch.Tensor],
@@ -565,36 +601,41 @@ def paged_kv_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor,
     ``seq_ids[r]`` (0 without) and returns q [rows, Hq, hd] rotated (``q_out``, made when
     not given; ``q_out=q`` in place; None without q). Without a table nothing is
     rotated."""
-    dev, rows = _dev(k), k.shape[0]
     if k.dim() != 3:
         raise _invalid("k and v must be [rows, kv_heads, head_dim]")
-    for name, t in (("k", k), ("v", v), ("q", q)):
-        if t is not None:
-            _head_rows(t, name, k)
-    if v.shape != k.shape or k.shape[1] != cache.num_kv_heads or k.shape[2] != cache.head_dim:
-        raise _invalid("k and v do not match the cache")
-    if cache.dtype != k.dtype or cache.device != dev:
+    dev, dtype, hd = _dev(k), k.dtype, cache.head_dim
+    if cache.dtype != dtype or cache.device != dev:
         raise _invalid("the cache has another dtype or device")
-    if q is None:
-        if q_out is not None:
-            raise _invalid("q_out without q")
-    else:
+    rows, hkv, ks = _head_rows(k, "k", dtype, dev, hd)
+    v_rows, v_heads, vs = _head_rows(v, "v", dtype, dev, hd)
+    if hkv != cache.num_kv_heads or v_rows != rows or v_heads != hkv:
+        raise _invalid("k and v do not match the cache or each other")
+    hq = qs = qos = 0
+    qp = qop = None
+    if q is not None:
+        q_rows, hq, qs = _head_rows(q, "q", dtype, dev, hd)
         if q_out is None:
-            q_out = _empty(q.shape, q.dtype, dev, stream)
-        _head_rows(q_out, "q_out", k)
-        if q.shape[0] != rows or q_out.shape != q.shape:
+            q_out = _empty(q.shape, dtype, dev, stream)
+        out_rows, out_heads, qos = _head_rows(q_out, "q_out", dtype, dev, hd)
+        if q_rows != rows or out_rows != rows or out_heads != hq:
             raise _invalid("q must have k's rows, and q_out q's shape")
-    for name, t in (("positions", positions), ("seq_ids", seq_ids), ("slots", slots)):
-        _same_device_i32(t, name, dev, rows)
-    _table_device(table, dev)
-    with torch.cuda.device(dev):
-        check(load().bm_paged_kv_append(_ptr(q_out), _ptr(q), _ptr(k), _ptr(v), _ptr(positions), _ptr(slots),
-                                        _ptr(seq_ids), ctypes.byref(cache.c), None if table is None else table.ptr,
-                                        0 if table is None else table.max_pos, 0 if table is None else table.head_dim,
-                                        int(interleaved), rows, 0 if q is None else q.shape[1],
-                                        0 if q is None else _row_stride(q), _row_stride(k), _row_stride(v),
-                                        0 if q is None else _row_stride(q_out), bm_dtype(k), _status_ptr(status, dev),
-                                        _stream(dev, stream)))
+        qp, qop = q.data_ptr(), q_out.data_ptr()
+    elif q_out is not None:
+        raise _invalid("q_out without q")
+    _same_device_i32(positions, "positions", dev, rows)
+    _same_device_i32(seq_ids, "seq_ids", dev, rows)
+    _same_device_i32(slots, "slots", dev, rows)
+    tp, tn, rd = None, 0, 0
+    if table is not None:
+        _table_device(table, dev)
+        tp, tn, rd = table.ptr, table.max_pos, table.head_dim
+    with _On(dev):
+        check(load().bm_paged_kv_append(qop, qp, k.data_ptr(), v.data_ptr(),
+                                        None if positions is None else positions.data_ptr(),
+                                        None if slots is None else slots.data_ptr(),
+                                        None if seq_ids is None else seq_ids.data_ptr(), cache.ref, tp, tn, rd,
+                                        int(interleaved), rows, hq, qs, ks, vs, qos, cache.code,
+                                        _status_ptr(status, dev), _raw_stream(dev, stream)))
     return q_out
 
 
@@ -648,12 +689,13 @@ def paged_tree_attention(q: torch.Tensor, cache: PagedKV, ctx_lens: torch.Tensor
         workspace = paged_tree_attention_workspace(q, cache, batch, max_ctx, max_tree, stream)
     if workspace.device != dev or not workspace.is_contiguous():
         raise _invalid("workspace must be contiguous on q's device")
-    with torch.cuda.device(dev):
-        check(load().bm_paged_tree_attention(_ptr(out), _ptr(q), ctypes.byref(cache.c), _ptr(seq_ids), _ptr(ctx_lens),
-                                             _ptr(q_starts), _ptr(tree_mask), words, q.shape[0], batch, q.shape[1],
-                                             max_ctx, max_tree, scale, workspace.data_ptr(),
-                                             workspace.numel() * workspace.element_size(), bm_dtype(q),
-                                             _status_ptr(status, dev), _stream(dev, stream)))
+    with _On(dev):
+        check(load().bm_paged_tree_attention(out.data_ptr(), q.data_ptr(), cache.ref,
+                                             None if seq_ids is None else seq_ids.data_ptr(), ctx_lens.data_ptr(),
+                                             q_starts.data_ptr(), None if tree_mask is None else tree_mask.data_ptr(),
+                                             words, q.shape[0], batch, q.shape[1], max_ctx, max_tree, scale,
+                                             workspace.data_ptr(), workspace.numel() * workspace.element_size(), cache.code,
+                                             _status_ptr(status, dev), _raw_stream(dev, stream)))
     return out
 
 
@@ -670,17 +712,24 @@ def sample(logits: torch.Tensor, uniforms: torch.Tensor, temperature: Optional[t
     if logits.dim() != 2 or logits.shape[1] == 0 or (logits.shape[1] > 1 and logits.stride(1) != 1):
         raise _invalid("logits must be [rows, vocab] with unit inner stride")
     rows, vocab = logits.shape
-    for name, t in (("uniforms", uniforms), ("temperature", temperature), ("top_p", top_p), ("min_p", min_p)):
-        if t is not None and (t.dtype != torch.float32 or t.numel() != rows or not t.is_contiguous() or t.device != dev):
-            raise _invalid(f"{name} must be a contiguous float32 tensor of one entry per row on the logits' device")
-    _same_device_i32(top_k, "top_k", dev, rows)
+    ptrs = []
+    for name, t in (("uniforms", uniforms), ("temperature", temperature), ("top_k", top_k), ("top_p", top_p),
+                    ("min_p", min_p)):
+        if t is None:
+            ptrs.append(None)
+            continue
+        want = torch.int32 if name == "top_k" else torch.float32
+        if t.dtype != want or t.numel() != rows or not t.is_contiguous() or t.device != dev:
+            raise _invalid(f"{name} must be a contiguous {want} tensor of one entry per row on the logits' device")
+        ptrs.append(t.data_ptr())
     if out is None:
         out = _empty((rows,), torch.int32, dev, stream)
-    _same_device_i32(out, "out", dev, rows)
-    with torch.cuda.device(dev):
-        check(load().bm_sample(_ptr(out), _ptr(logits), _ptr(uniforms), _ptr(temperature), _ptr(top_k), _ptr(top_p),
-                               _ptr(min_p), rows, vocab, logits.stride(0) if rows > 1 else vocab, bm_dtype(logits),
-                               _status_ptr(status, dev), _stream(dev, stream)))
+    else:
+        _same_device_i32(out, "out", dev, rows)
+    with _On(dev):
+        check(load().bm_sample(out.data_ptr(), logits.data_ptr(), *ptrs, rows, vocab,
+                               logits.stride(0) if rows > 1 else vocab, bm_dtype(logits), _status_ptr(status, dev),
+                               _raw_stream(dev, stream)))
     return out
 
 
