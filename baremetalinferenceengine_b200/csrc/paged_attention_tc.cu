@@ -14,9 +14,13 @@
 // the mix, the row sums take them before rounding.
 //
 // Bound: memory while group * tokens is below about 200 (two operations per K and V
-// element and row against 2.25 bytes per ns and SM), the tensor cores above. Padding
-// to M = 128 costs nothing that bounds: a tile's two products take 1024 cycles, its
-// 64 KB of K and V 2800 at the SM's share of HBM.
+// element and row against 2.25 bytes per ns and SM), the tensor cores and the
+// exponentials above. Padding to M = 128 costs nothing that bounds: a tile's two
+// products take 1024 cycles, its 64 KB of K and V 2800 at the SM's share of HBM. What few
+// rows would leave idle is the softmax: a thread walks its row's 128 scores however few
+// rows there are. So with at most 64 (32) rows the row tile holds them twice (four times),
+// and each copy weighs a half (quarter) of the tile's slots, with zero weights elsewhere;
+// the copies' sums meet at the segment's end.
 //
 // Split: the host does not see the lengths, so one CTA per SM takes an equal share of
 // all tiles of the batch, counted on the device: items (sequence, kv head, row tile) laid
@@ -31,9 +35,9 @@
 //   warp 2     TMA of the queries, once per segment (an item's part in this CTA);
 //   warps 4-7, 8-11  two softmax groups. Unit u of the CTA's sequence goes to group
 //              u & 1 with TMEM buffers S[u & 1] and O[u & 1]: with one row tile per
-//              item (kDual = false) units are its tiles in turn, and both groups' sums
-//              meet at the segment's end; with more rows (kDual = true) a tile is two
-//              units, one per row tile, so K and V are read once for 256 rows.
+//              item units are its tiles in turn, and both groups' sums meet at the
+//              segment's end; with more rows (kDual) a tile is two units, one per row
+//              tile, so K and V are read once for 256 rows.
 // Every mbarrier wait is bounded in time: past the limit the CTA raises
 // BM_DEVERR_TIMEOUT, lets its copies and MMAs land, frees TMEM and returns.
 #include <cuda.h>
@@ -59,23 +63,38 @@ constexpr uint64_t kWaitNs = 2000000000ull;
 constexpr uint64_t kDrainNs = 200000000ull;
 constexpr float kRescaleAt = 8.f;
 
-template <int HD, bool DUAL>
+// How an item's rows lie in row tiles: two tiles of rows, or one holding them COPIES times.
+constexpr int kDual = 0;
+
+template <int HD, int COPIES>
 struct Layout {
-  static constexpr int kTiles = DUAL ? 2 : 1;               // row tiles of an item
+  static constexpr bool kTwo = COPIES == kDual;
+  static constexpr int kTiles = kTwo ? 2 : 1;               // row tiles of an item
+  static constexpr int kCopies = kTwo ? 1 : COPIES;
+  static constexpr int kCopyRows = kTile / kCopies;         // rows of a copy
+  static constexpr int kCols = kTile / kCopies;             // slots of a tile that a copy weighs
+  static constexpr int kRows = kTiles * kCopyRows;          // rows of an item
   static constexpr int kBox = kTile * 128;                  // 128 rows x 64 dims of bf16
   static constexpr int kOperand = HD / 64 * kBox;           // a tile of Q, K or V
   static constexpr int kKS = HD == 128 ? 2 : 4;             // K ring: freed by the scores
   static constexpr int kVS = HD == 128 ? 3 : 6;             // V ring: freed by the mix
   static constexpr int kOffK = kTiles * kOperand;
   static constexpr int kOffV = kOffK + kKS * kOperand;
-  static constexpr int kOffMl = kOffV + kVS * kOperand;     // [2][2][128] (maximum, sum), kDual = false
-  static constexpr int kOffBar = kOffMl + (DUAL ? 0 : 2 * 2 * kTile * 8);
+  static constexpr int kOffMl = kOffV + kVS * kOperand;     // [2][2][128] (maximum, sum), not with two tiles
+  // The copies' sums meet in shared memory, kDims dims of all rows at a time, each of the
+  // kWriters (group, copy) adding its own kStep dims in turn.
+  static constexpr int kWriters = 2 * kCopies;  // (unused with one copy)
+  static constexpr int kDims = 4096 / kCopyRows < HD ? 4096 / kCopyRows : HD;
+  static constexpr int kStep = kDims / kWriters;
+  static constexpr int kPitch = kDims + 4;
+  static constexpr int kOffSum = kOffMl + (kTwo ? 0 : 2 * 2 * kTile * 8);
+  static constexpr int kOffBar = kOffSum + (kCopies > 1 ? kCopyRows * kPitch * 4 : 0);
   static constexpr int kBars = 2 * kKS + 2 * kVS + 6 + 4;
   static constexpr int kOffPlan = kOffBar + kBars * 8;      // Plan, scan, bad-page ring
   static constexpr int kBytes = kOffPlan + 64 + 16 * 8 + kBadRing * 4 + 16 + 1024 /* alignment slack */;
+  static_assert(kBytes <= 232448, "shared memory of a CTA");
   static constexpr uint32_t kColO = 256;                    // TMEM: S0, S1 (128 each), O0, O1 (HD each)
-  static constexpr uint32_t kCols = 512;
-  static constexpr int kRows = kTiles * kTile;
+  static constexpr uint32_t kTmemCols = 512;
   static constexpr int kSlotFloats = kRows * (HD + 2);      // a partial: sums, then maxima, then weight sums
 };
 
@@ -89,8 +108,6 @@ struct Record {
 static_assert(sizeof(Record) == 40, "record layout");
 
 __host__ __device__ constexpr size_t records_bytes(int nc) { return (static_cast<size_t>(nc) * sizeof(Record) + 255) / 256 * 256; }
-
-__device__ __forceinline__ int tokens_per_tile(const TreeArgs& a) { return kTile / a.group; }
 
 // Tiles of item p (its row tiles hold `per` tokens) of a sequence.
 __device__ __forceinline__ int item_tiles(const TreeArgs& a, const Seq& s, int p, int per) {
@@ -169,7 +186,7 @@ __device__ __forceinline__ void mma_bf16_ts(uint32_t d_tmem, uint32_t a_tmem, ui
       ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
-// 16 or 32 consecutive 32-bit columns of this thread's TMEM lane.
+// 16 consecutive 32-bit columns of this thread's TMEM lane.
 __device__ __forceinline__ void tmem_store16(uint32_t taddr, const uint32_t (&r)[16]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], "
@@ -178,16 +195,11 @@ __device__ __forceinline__ void tmem_store16(uint32_t taddr, const uint32_t (&r)
       "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
       : "memory");
 }
-__device__ __forceinline__ void tmem_store32(uint32_t taddr, const uint32_t (&r)[32]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
-      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};" ::"r"(r[0]),
-      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
-      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]),
-      "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]),
-      "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr)
-      : "memory");
+// 8 consecutive fp32 columns of this thread's TMEM lane, into r's first.
+__device__ __forceinline__ void tmem_load8(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(taddr));
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
@@ -230,6 +242,30 @@ __device__ __forceinline__ uint32_t sound32(uint32_t bad, int c, int box_rows) {
   return v;
 }
 
+// Pairs of fp32 in one register pair: one instruction for two multiply-adds or adds.
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t pair(uint32_t a, uint32_t b) { return static_cast<uint64_t>(b) << 32 | a; }
+__device__ __forceinline__ float2 unpair(uint64_t p) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(p));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) { return fmaxf(fmaxf(a, b), c); }
+
 __device__ __forceinline__ void both_groups_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 
 __device__ __forceinline__ float ex2(float x) {
@@ -238,12 +274,13 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-template <int HD, bool DUAL>
+template <int HD, int COPIES>
 __global__ void __launch_bounds__(kThreadsTc, 1)
     tree_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
                    const __grid_constant__ CUtensorMap tv, const TreeArgs a) {
   grid_dependency_wait();
-  using L = Layout<HD, DUAL>;
+  using L = Layout<HD, COPIES>;
+  constexpr bool DUAL = L::kTwo;
   constexpr uint32_t kIdescS = instr_desc_bf16(false, false, kTile, kTile);
   constexpr uint32_t kIdescO = instr_desc_bf16(false, true, HD, kTile);
   extern __shared__ __align__(1024) unsigned char smem_raw[];
@@ -251,7 +288,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
                                                          ~static_cast<uintptr_t>(1023));
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int cta = static_cast<int>(blockIdx.x);
-  const int tpt = tokens_per_tile(a);      // tokens of a row tile
+  const int tpt = L::kCopyRows / a.group;  // tokens of a row tile
   const int per = tpt * L::kTiles;         // and of an item
 
   uint64_t* kfull = reinterpret_cast<uint64_t*>(smem + L::kOffBar);
@@ -339,7 +376,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
       *abort_flag = 0;
       fence_barrier_init();
     }
-    if (warp == 1) tmem_alloc(tmem_base_s, L::kCols);
+    if (warp == 1) tmem_alloc(tmem_base_s, L::kTmemCols);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -421,13 +458,16 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
     int seg = 0;
     for (; walk.left > 0; walk.next(a, per), ++seg) {
       if (!wait_phase(qempty, (seg & 1) ^ 1u, abort_flag, a.status, kWaitNs, true)) break;
-      mbar_expect_tx(qfull, L::kTiles * (HD / 64) * a.group * tpt * 128);
+      mbar_expect_tx(qfull, L::kTiles * L::kCopies * (HD / 64) * a.group * tpt * 128);
 #pragma unroll
       for (int w = 0; w < L::kTiles; ++w) {
         const int token = static_cast<int>(walk.s.row0) + walk.p * per + w * tpt;
 #pragma unroll
         for (int h = 0; h < HD / 64; ++h) {
-          tma_load_3d(smem + w * L::kOperand + h * L::kBox, &tq, qfull, 64 * h, walk.kvh * a.group, token);
+#pragma unroll
+          for (int c = 0; c < L::kCopies; ++c) {
+            tma_load_3d(smem + w * L::kOperand + h * L::kBox + c * L::kCopyRows * 128, &tq, qfull, 64 * h, walk.kvh * a.group, token);
+          }
         }
       }
     }
@@ -501,14 +541,17 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
     }
   } else if (warp >= 4) {
     // ---------------- softmax ----------------
+    constexpr int NC = L::kCols;
     const int w = (warp - 4) >> 2;      // group
     const int quarter = warp & 3;
-    const int r = quarter * 32 + lane;  // row of the row tile: this thread's TMEM lane
+    const int copy = quarter * 32 / L::kCopyRows;
+    const int r = quarter * 32 % L::kCopyRows + lane;  // row of the row tile; lane quarter * 32 + lane of TMEM is its
     const uint32_t lane_addr = static_cast<uint32_t>(quarter * 32) << 16;
     const uint32_t s_addr = tmem + lane_addr + w * kTile;
     const uint32_t o_addr = tmem + lane_addr + L::kColO + w * HD;
     const int box_rows = min(a.page_size, kTile);
     float2* ml = reinterpret_cast<float2*>(smem + L::kOffMl);
+    const uint64_t scale2 = pair(a.qscale, a.qscale);
     int x = 0;  // the segment's first unit
     for (int seg = 0; walk.left > 0; walk.next(a, per), ++seg) {
       const int n = walk.segment();
@@ -516,7 +559,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
       const Seq s = walk.s;
       const int i0 = walk.p * per + (DUAL ? w * tpt : 0);
       const int live = max(0, min(tpt, s.n - i0)) * a.group;
-      const bool warp_live = quarter * 32 < live;
+      const bool warp_live = r - lane < live;
       const int token = i0 + r / a.group;  // a row past `live` computes on what it finds and is not stored
       const int total = s.ctx + s.n;
       float m = -INFINITY, l = 0.f;
@@ -528,80 +571,106 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
         tc_fence_after();
         const int slot0 = t * kTile;
         const uint32_t bad = bad_ring[kt % kBadRing];
-        const bool masked = slot0 + kTile > s.ctx || bad != 0;
         if (warp_live) {
-          uint32_t see[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
-          if (masked) {
+          // This copy's scores of the row: at most 64 are held, of 128 the second half is
+          // loaded twice (its weights go where the first half's scores were).
+          constexpr int kHeld = NC < 64 ? NC : 64;
+          uint32_t v[kHeld / 32][32];
+          auto load = [&](int col) {
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              see[c] = r < live ? seen32(a, s, token, slot0 + 32 * c) : 0u;
-              if (bad) see[c] &= sound32(bad, c, box_rows);
-            }
-          }
-          float top = -INFINITY;
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            uint32_t v[32];
-            tmem_load32(s_addr + 32 * c, v);
+            for (int c = 0; c < kHeld / 32; ++c) tmem_load32(s_addr + copy * NC + col + 32 * c, v[c]);
             tmem_wait_ld();
-            if (masked) {
+            if (slot0 + kTile > s.ctx || bad != 0) {
 #pragma unroll
-              for (int e = 0; e < 32; ++e) {
-                if ((see[c] >> e) & 1) top = fmaxf(top, __uint_as_float(v[e]));
+              for (int c = 0; c < kHeld / 32; ++c) {
+                const int at = copy * NC + col + 32 * c;
+                uint32_t see = r < live ? seen32(a, s, token, slot0 + at) : 0u;
+                if (bad) see &= sound32(bad, at / 32, box_rows);
+#pragma unroll
+                for (int e = 0; e < 32; ++e) {
+                  if (!((see >> e) & 1)) v[c][e] = 0xff800000u;  // -inf: no weight
+                }
               }
-            } else {
-#pragma unroll
-              for (int e = 0; e < 32; ++e) top = fmaxf(top, __uint_as_float(v[e]));
+              __syncwarp();
             }
+          };
+          float top = -INFINITY, top1 = -INFINITY;
+          auto highest = [&]() {
+#pragma unroll
+            for (int c = 0; c < kHeld / 32; ++c) {
+#pragma unroll
+              for (int e = 0; e < 32; e += 4) {
+                top = max3(top, __uint_as_float(v[c][e]), __uint_as_float(v[c][e + 1]));
+                top1 = max3(top1, __uint_as_float(v[c][e + 2]), __uint_as_float(v[c][e + 3]));
+              }
+            }
+          };
+          if constexpr (NC == 128) {
+            load(64);
+            highest();
           }
-          top = r < live ? top * a.qscale : -INFINITY;
-          const bool first = u == u0;
+          load(0);
+          highest();
+          top = r < live ? fmaxf(top, top1) * a.qscale : -INFINITY;
           const bool rise = top > m + kRescaleAt || (m == -INFINITY && top > -INFINITY);
           const float m_new = rise ? top : m;
           const float alpha = rise ? ex2(m - m_new) : 1.f;  // m = -inf: 0
-          if (!first && __any_sync(0xffffffffu, rise)) {
+          if (u != u0 && __any_sync(0xffffffffu, rise)) {
             // the group's previous mix is done: these scores were issued after it
             l *= alpha;
-#pragma unroll
-            for (int c = 0; c < HD / 32; ++c) {
-              uint32_t v[32];
-              tmem_load32(o_addr + 32 * c, v);
+#pragma unroll 1
+            for (int c = 0; c < HD / 16; ++c) {
+              uint32_t o[16];
+              tmem_load16(o_addr + 16 * c, o);
               tmem_wait_ld();
 #pragma unroll
-              for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * alpha);
-              tmem_store32(o_addr + 32 * c, v);
+              for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+              tmem_store16(o_addr + 16 * c, o);
             }
           }
           m = m_new;
           const float base = m == -INFINITY ? 0.f : m;
-          float sum[4] = {0.f, 0.f, 0.f, 0.f};
+          const uint64_t minus = pair(-base, -base);
+          uint64_t sum[2] = {0, 0};
+          auto weigh = [&](int col) {
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            uint32_t v[32], pk[16];
-            tmem_load32(s_addr + 32 * c, v);
-            tmem_wait_ld();
+            for (int c = 0; c < kHeld / 32; ++c) {
+              uint32_t pk[16];
 #pragma unroll
-            for (int e = 0; e < 32; e += 2) {
-              float p0 = ex2(fmaf(__uint_as_float(v[e]), a.qscale, -base));
-              float p1 = ex2(fmaf(__uint_as_float(v[e + 1]), a.qscale, -base));
-              if (masked) {
-                if (!((see[c] >> e) & 1)) p0 = 0.f;
-                if (!((see[c] >> (e + 1)) & 1)) p1 = 0.f;
+              for (int e = 0; e < 32; e += 2) {
+                const float2 y = unpair(fma2(pair(v[c][e], v[c][e + 1]), scale2, minus));
+                const float p0 = ex2(y.x), p1 = ex2(y.y);
+                sum[e / 2 % 2] = add2(sum[e / 2 % 2], pair(p0, p1));
+                pk[e / 2] = pack_bf16x2(p0, p1);
               }
-              sum[e / 2 % 4] += p0 + p1;
-              pk[e / 2] = pack_bf16x2(p0, p1);
+              tmem_store16(s_addr + (copy * NC + col) / 2 + 16 * c, pk);
             }
-            tmem_store16(s_addr + 16 * c, pk);  // columns that have been read
+          };
+          weigh(0);
+          if constexpr (NC == 128) {
+            load(64);
+            weigh(64);
           }
-          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+          if constexpr (L::kCopies > 1) {  // no weights for the slots of the other copies
+            uint32_t zero[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) zero[e] = 0;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              if (c / (NC / 32) != copy) tmem_store16(s_addr + 16 * c, zero);
+            }
+          }
+          const float2 sums = unpair(add2(sum[0], sum[1]));
+          l += sums.x + sums.y;
           tmem_wait_st();
         }
         if (slot0 + kTile > total || bad != 0) {
           // V rows that no copy filled, or stale slots behind the last token: zero
           const int vs = kt % L::kVS;
           warp_wait(&vfull[vs], (kt / L::kVS) & 1, abort_flag, a.status);
-          if (slot0 + r >= total || ((bad >> (r / box_rows)) & 1)) {
-            unsigned char* row = smem + L::kOffV + vs * L::kOperand + r * 128;
+          const int vr = quarter * 32 + lane;
+          if (slot0 + vr >= total || ((bad >> (vr / box_rows)) & 1)) {
+            unsigned char* row = smem + L::kOffV + vs * L::kOperand + vr * 128;
 #pragma unroll
             for (int h = 0; h < HD / 64; ++h) {
 #pragma unroll
@@ -651,6 +720,80 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
             slot[L::kRows * HD + w * kTile + r] = m;
             slot[L::kRows * (HD + 1) + w * kTile + r] = l;
           }
+        }
+      } else if constexpr (L::kCopies > 1) {
+        // maxima and sums of every group and copy, then their sums of values in shared memory
+        ml[((seg & 1) * 2 + w) * kTile + copy * L::kCopyRows + r] = make_float2(m, l);
+        both_groups_sync();
+        float top = -INFINITY, sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < L::kWriters; ++i) {
+          top = fmaxf(top, ml[((seg & 1) * 2 + i / L::kCopies) * kTile + i % L::kCopies * L::kCopyRows + r].x);
+        }
+        const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+        for (int i = 0; i < L::kWriters; ++i) {
+          const float2 part = ml[((seg & 1) * 2 + i / L::kCopies) * kTile + i % L::kCopies * L::kCopyRows + r];
+          sum = fmaf(part.y, ex2(part.x - base), sum);  // a maximum of -inf: 0
+        }
+        const float inv = !whole ? 1.f : sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
+        const int last = end - 1 - ((end - 1 - w) & 1);  // this group's last unit; none: its O is stale
+        const bool had = last >= x && warp_live;
+        if (last >= x) warp_wait(&pvdone[w], (last >> 1) & 1, abort_flag, a.status);
+        tc_fence_after();
+        const float f = m == -INFINITY || r >= live ? 0.f : ex2(m - base) * inv;
+        float* acc = reinterpret_cast<float*>(smem + L::kOffSum);
+        for (int d0 = 0; d0 < HD; d0 += L::kDims) {
+#pragma unroll 1
+          for (int step = 0; step < L::kWriters; ++step) {
+            const int col = (w * L::kCopies + copy + step) % L::kWriters * L::kStep;
+            uint32_t o[16];
+            if (had) {  // the same for the warp
+              if constexpr (L::kStep == 16) {
+                tmem_load16(o_addr + d0 + col, o);
+              } else {
+                tmem_load8(o_addr + d0 + col, o);
+              }
+              tmem_wait_ld();
+            }
+            float* to = acc + r * L::kPitch + col;
+#pragma unroll
+            for (int e = 0; e < L::kStep; e += 4) {
+              float4 add = make_float4(0.f, 0.f, 0.f, 0.f);
+              if (had && f != 0.f) {
+                add = make_float4(__uint_as_float(o[e]) * f, __uint_as_float(o[e + 1]) * f, __uint_as_float(o[e + 2]) * f,
+                                  __uint_as_float(o[e + 3]) * f);
+              }
+              if (step > 0) {
+                const float4 old = *reinterpret_cast<const float4*>(to + e);
+                add = make_float4(add.x + old.x, add.y + old.y, add.z + old.z, add.w + old.w);
+              }
+              *reinterpret_cast<float4*>(to + e) = add;
+            }
+            __syncwarp();
+            both_groups_sync();
+          }
+          for (int c = tid - 128; c < live * (L::kDims / 8); c += 256) {
+            const int row = c / (L::kDims / 8), d = c % (L::kDims / 8) * 8;
+            const float* from = acc + row * L::kPitch + d;
+            if (whole) {
+              const int tok = i0 + row / a.group, head = row % a.group;
+              float f8[8];
+#pragma unroll
+              for (int e = 0; e < 8; ++e) f8[e] = from[e];
+              st_plain(static_cast<bf16*>(a.out) + ((s.row0 + tok) * a.hq + walk.kvh * a.group + head) * HD + d0 + d, pack16<bf16>(f8));
+            } else {
+              float* to = slot + row * HD + d0 + d;
+              *reinterpret_cast<float4*>(to) = *reinterpret_cast<const float4*>(from);
+              *reinterpret_cast<float4*>(to + 4) = *reinterpret_cast<const float4*>(from + 4);
+            }
+          }
+          __syncwarp();
+          both_groups_sync();  // the sums have been read
+        }
+        if (!whole && w == 0 && copy == 0 && r < live) {
+          slot[L::kRows * HD + r] = top;
+          slot[L::kRows * (HD + 1) + r] = sum;
         }
       } else {
         // both groups' maxima and sums, then each takes half of the dims of both
@@ -711,16 +854,16 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
   __syncthreads();
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem, L::kCols);
+    tmem_dealloc(tmem, L::kTmemCols);
   }
 }
 
 // Adds up the partials of the item that CTA k's first tile continues: block (k, rows
 // 16 y .. 16 y + 15) by the first border inside the item.
-template <int HD, bool DUAL>
+template <int HD, int COPIES>
 __global__ void __launch_bounds__(256) tree_merge_kernel(const TreeArgs a, int ctas) {
   grid_dependency_wait();
-  using L = Layout<HD, DUAL>;
+  using L = Layout<HD, COPIES>;
   const Record* records = reinterpret_cast<const Record*>(a.ws);
   const float* slots = a.ws + records_bytes(ctas) / sizeof(float);
   const int k = static_cast<int>(blockIdx.x) + 1;
@@ -731,7 +874,7 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(const TreeArgs a, int c
   if (border(k - 1) > first) return;  // an earlier border is inside it, too
   Seq s;
   read_seq(a, rec.b, &s);
-  const int tpt = tokens_per_tile(a);
+  const int tpt = L::kCopyRows / a.group;
   constexpr int kLanes = 16;  // threads of a row
   const int r = static_cast<int>(blockIdx.y) * 16 + threadIdx.x / kLanes;
   const int tile = r / kTile, rr = r - tile * kTile;
@@ -775,33 +918,53 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(const TreeArgs a, int c
   }
 }
 
-// Whether an item holds two row tiles: more rows per kv head than one tile has.
-bool dual(int group, int max_tree) { return max_tree > kTile / group; }
+// The form for the bounds' rows per kv head: the widest that holds them in one item, else
+// two row tiles.
+int copies_for(int group, int max_tree) {
+  const int64_t rows = static_cast<int64_t>(group) * max_tree;
+  return rows <= 32 ? 4 : rows <= 64 ? 2 : rows <= kTile / group * group ? 1 : kDual;
+}
+int rows_of(int copies) { return copies == kDual ? 2 * kTile : kTile / copies; }
+int tokens_of(int copies, int group) { return copies == kDual ? kTile / group * 2 : kTile / copies / group; }
 
 // CTAs for the bounds: one per SM, no more than the tiles there can be.
 int ctas_for(int64_t batch, int hkv, int group, int max_ctx, int max_tree) {
-  const int per = kTile / group * (dual(group, max_tree) ? 2 : 1);
+  const int per = tokens_of(copies_for(group, max_tree), group);
   const int64_t tiles = batch * hkv * ((max_tree + per - 1) / per) * ((static_cast<int64_t>(max_ctx) + max_tree + kTile - 1) / kTile);
   return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(sm_count(), (tiles + kMinTiles - 1) / kMinTiles)));
 }
 
-template <int HD, bool DUAL>
+template <int HD, int COPIES>
 int launch_form(const TreeArgs& a, cudaStream_t stream, const char* what) {
-  using L = Layout<HD, DUAL>;
-  const int tpt = kTile / a.group;
+  using L = Layout<HD, COPIES>;
+  const int tpt = L::kCopyRows / a.group;
   const uint64_t rows = static_cast<uint64_t>(a.num_pages) * a.hkv * a.page_size;
   const uint32_t box_rows = static_cast<uint32_t>(std::min(a.page_size, kTile));
   CUtensorMap tq, tk, tv;
   if (int st = make_tensor_map_bf16(&tk, a.k_pages, HD, rows, 64, box_rows, what)) return st;
   if (int st = make_tensor_map_bf16(&tv, a.v_pages, HD, rows, 64, box_rows, what)) return st;
   if (int st = make_tensor_map_3d_bf16(&tq, a.q, HD, a.hq, a.total_q, 64, a.group, tpt, what)) return st;
-  auto kernel = tree_tc_kernel<HD, DUAL>;
+  auto kernel = tree_tc_kernel<HD, COPIES>;
   if (int st = allow_dynamic_smem(reinterpret_cast<const void*>(kernel), L::kBytes, what)) return st;
   const int nc = ctas_for(a.batch, a.hkv, a.group, a.max_ctx, a.max_tree);
   if (int st = launch_kernel(what, kernel, dim3(nc), dim3(kThreadsTc), L::kBytes, stream, nullptr, tq, tk, tv, a)) return st;
   // items of one tile, and a single CTA, are never cut
   if (nc == 1 || a.max_ctx + a.max_tree <= kTile) return BM_OK;
-  return launch_kernel(what, tree_merge_kernel<HD, DUAL>, dim3(nc - 1, L::kRows / 16), dim3(256), 0, stream, nullptr, a, nc);
+  return launch_kernel(what, tree_merge_kernel<HD, COPIES>, dim3(nc - 1, L::kRows / 16), dim3(256), 0, stream, nullptr, a, nc);
+}
+
+template <int HD>
+int launch_hd(const TreeArgs& a, cudaStream_t stream, const char* what) {
+  switch (copies_for(a.group, a.max_tree)) {
+    case 4:
+      return launch_form<HD, 4>(a, stream, what);
+    case 2:
+      return launch_form<HD, 2>(a, stream, what);
+    case 1:
+      return launch_form<HD, 1>(a, stream, what);
+    default:
+      return launch_form<HD, kDual>(a, stream, what);
+  }
 }
 
 }  // namespace
@@ -815,15 +978,12 @@ bool tc_takes(const TreeArgs& a, bm_dtype_t dtype) {
 size_t tc_workspace_bytes(int64_t batch, int hkv, int hd, int group, int max_ctx, int max_tree) {
   if (hd != 64 && hd != 128) return 0;
   const int nc = ctas_for(batch, hkv, group, max_ctx, max_tree);
-  const size_t rows = dual(group, max_tree) ? 2 * kTile : kTile;
+  const size_t rows = static_cast<size_t>(rows_of(copies_for(group, max_tree)));
   return records_bytes(nc) + 2 * static_cast<size_t>(nc) * rows * (hd + 2) * sizeof(float);
 }
 
 int launch_tc(const TreeArgs& a, cudaStream_t stream, const char* what) {
-  if (a.hd == 128) {
-    return dual(a.group, a.max_tree) ? launch_form<128, true>(a, stream, what) : launch_form<128, false>(a, stream, what);
-  }
-  return dual(a.group, a.max_tree) ? launch_form<64, true>(a, stream, what) : launch_form<64, false>(a, stream, what);
+  return a.hd == 128 ? launch_hd<128>(a, stream, what) : launch_hd<64>(a, stream, what);
 }
 
 }  // namespace paged

@@ -9,9 +9,10 @@
 //
 // Bound: memory. Every element of q, k (and v) is read once and written once; the
 // table rows come from L2. Layout of the work: a unit is N pairs of one head, two
-// 16-byte chunks (i and i + rd/2, or two chunks side by side), and a lane keeps the N
-// (cos, sin) of its unit's place in the head for all heads that it visits, so the
-// table is read once per token and lane and not once per head. A warp takes one token,
+// 16-byte chunks (i and i + rd/2, or two chunks side by side; copied elements are units of
+// two chunks, too), and a lane keeps the N (cos, sin) of its unit's place in the head for
+// all heads that it visits, so the table is read once per token and lane and not once
+// per head, and neighbouring lanes cover whole heads. A warp takes one token,
 // or one of `parts` shares of a token's heads when there are few tokens: a decode
 // batch is bound by the chain position -> (cos, sin), sequence -> page -> store, which
 // more warps with one pass each overlap. Data loads are issued before that chain is
@@ -47,7 +48,7 @@ struct RotaryArgs {
   int hq, hkv, hd, rd;      // rd: rotated elements of a head (0 without a table)
   int num_pages, page_size, max_pages, num_seqs;
   int parts;                // warps per token
-  int units, rest;          // rotated units and copied chunks of a head
+  int units, rest;          // rotated and copied units of a head
   int32_t* status;
 };
 
@@ -108,7 +109,7 @@ __device__ __forceinline__ void rotate(Piece<T, N>& p1, Piece<T, N>& p2, const f
 // PAGED: k goes into the cache's pages and v with it; otherwise k into k_out.
 template <typename T, int N, bool INTER, bool PAGED>
 __global__ void __launch_bounds__(kThreads) rotary_kernel(RotaryArgs a) {
-  constexpr int U = 4;  // passes whose loads a lane keeps in flight
+  constexpr int U = PAGED ? 4 : 2;  // passes whose loads a lane keeps in flight (the other way round: 9 % and 4 % slower on prompts)
   const int lane = threadIdx.x & 31;
   const int64_t job0 = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) >> 5;
   const int64_t njobs = a.rows * a.parts;
@@ -120,8 +121,7 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(RotaryArgs a) {
   }
   grid_dependency_wait();
   const int64_t step = (static_cast<int64_t>(gridDim.x) * kThreads) >> 5;
-  const int heads = a.hq + a.hkv;
-  const int second = INTER ? N : a.rd / 2;  // the unit's second chunk, from its first
+  const int heads = a.hq + a.hkv + (PAGED ? a.hkv : 0);
   constexpr int kUnit = INTER ? 2 * N : N;  // elements between neighbouring units
 
   for (int64_t job = job0; job < njobs; job += step) {
@@ -151,19 +151,35 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(RotaryArgs a) {
     }
     const T* qrow = static_cast<const T*>(a.q) + row * a.q_stride;
     const T* krow = static_cast<const T*>(a.k) + row * a.k_stride;
+    const T* vrow = static_cast<const T*>(a.v) + row * a.v_stride;
     T* qdst = static_cast<T*>(a.q_out) + row * a.q_out_stride;
     T* kdst = PAGED ? static_cast<T*>(a.k_pages) + cache_base : static_cast<T*>(a.k_out) + row * a.k_out_stride;
-    const int64_t kstep = PAGED ? head_stride : a.hd;
-    auto src = [&](int h) { return h < a.hq ? qrow + static_cast<int64_t>(h) * a.hd : krow + static_cast<int64_t>(h - a.hq) * a.hd; };
-    auto dst = [&](int h) { return h < a.hq ? qdst + static_cast<int64_t>(h) * a.hd : kdst + static_cast<int64_t>(h - a.hq) * kstep; };
+    T* vdst = static_cast<T*>(a.v_pages) + cache_base;
+    // heads in turn: q's, k's, then (PAGED) v's
+    auto src = [&](int h) -> const T* {
+      if (h < a.hq) return qrow + static_cast<int64_t>(h) * a.hd;
+      if (!PAGED || h < a.hq + a.hkv) return krow + static_cast<int64_t>(h - a.hq) * a.hd;
+      return vrow + static_cast<int64_t>(h - a.hq - a.hkv) * a.hd;
+    };
+    auto dst = [&](int h) -> T* {
+      if (h < a.hq) return qdst + static_cast<int64_t>(h) * a.hd;
+      if (!PAGED) return kdst + static_cast<int64_t>(h - a.hq) * a.hd;
+      if (h < a.hq + a.hkv) return kdst + (h - a.hq) * head_stride;
+      return vdst + (h - a.hq - a.hkv) * head_stride;
+    };
+    const int turning = a.hq + a.hkv;
 
-    // rotated units: lane -> unit c of heads h, h + hpi, ... (this part's heads)
-    for (int c0 = 0; c0 < a.units; c0 += 32) {
-      const int n = min(32, a.units - c0);
+    for (int c0 = 0; c0 < a.units + a.rest; c0 += 32) {
+      const int n = min(32, a.units + a.rest - c0);
       const int hpi = 32 / n;
       const int c = c0 + lane % n;
       const int hl = lane / n;
       if (hl >= hpi) continue;
+      const bool turns = c < a.units;
+      // this unit's two chunks of every head; the last copied one may have no second
+      const int first = turns ? c * kUnit : a.rd + (c - a.units) * 2 * N;
+      const int second = first + (turns && !INTER ? a.rd / 2 : N);
+      const bool pair = second < a.hd;
       const int passes = (heads + hpi - 1) / hpi;
       const int mine = (passes + a.parts - 1) / a.parts;
       const int h_end = min(heads, (part + 1) * mine * hpi);
@@ -175,11 +191,11 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(RotaryArgs a) {
         for (int u = 0; u < U; ++u) {
           const int h = hb + u * hpi;
           if (h < h_end) {
-            x1[u].load(src(h) + c * kUnit);
-            x2[u].load(src(h) + c * kUnit + second);
+            x1[u].load(src(h) + first);
+            if (pair) x2[u].load(src(h) + second);
           }
         }
-        if (!have) {
+        if (turns && !have) {
           const float2* t = a.table + static_cast<int64_t>(pos) * (a.rd / 2) + c * N;
           if constexpr (N % 2 == 0) {  // 16-byte loads: the host checked the table's alignment
 #pragma unroll
@@ -198,46 +214,10 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(RotaryArgs a) {
         for (int u = 0; u < U; ++u) {
           const int h = hb + u * hpi;
           if (h < h_end) {
-            rotate<T, N, INTER>(x1[u], x2[u], cs);
-            x1[u].store(dst(h) + c * kUnit);
-            x2[u].store(dst(h) + c * kUnit + second);
+            if (turns && h < turning) rotate<T, N, INTER>(x1[u], x2[u], cs);
+            x1[u].store(dst(h) + first);
+            if (pair) x2[u].store(dst(h) + second);
           }
-        }
-      }
-    }
-    // copied elements: the rest of each head (nothing to do where q is rotated in place)
-    if (a.rest > 0) {
-      const int total = heads * a.rest;
-      for (int i0 = part * 32 + lane; i0 < total; i0 += 32 * a.parts * U) {
-        Piece<T, N> x[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const int i = i0 + u * 32 * a.parts;
-          if (i < total) x[u].load(src(i / a.rest) + a.rd + (i % a.rest) * N);
-        }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const int i = i0 + u * 32 * a.parts;
-          if (i < total) x[u].store(dst(i / a.rest) + a.rd + (i % a.rest) * N);
-        }
-      }
-    }
-    if constexpr (PAGED) {
-      const int per = a.hd / N;
-      const int total = a.hkv * per;
-      const T* vrow = static_cast<const T*>(a.v) + row * a.v_stride;
-      T* vdst = static_cast<T*>(a.v_pages) + cache_base;
-      for (int i0 = part * 32 + lane; i0 < total; i0 += 32 * a.parts * U) {
-        Piece<T, N> x[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const int i = i0 + u * 32 * a.parts;
-          if (i < total) x[u].load(vrow + static_cast<int64_t>(i) * N);
-        }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const int i = i0 + u * 32 * a.parts;
-          if (i < total) x[u].store(vdst + static_cast<int64_t>(i / per) * head_stride + (i % per) * N);
         }
       }
     }
@@ -264,7 +244,7 @@ int launch(RotaryArgs a, bool interleaved, bm_dtype_t dtype, cudaStream_t stream
   int n = 16 / es;
   if (!fits(n)) n = es == 2 && fits(4) ? 4 : 1;
   a.units = a.rd / 2 / n;
-  a.rest = (a.hd - a.rd) / n;
+  a.rest = (a.hd - a.rd + 2 * n - 1) / (2 * n);
   // One warp per token for a batch that fills the GPU (2048 warps: 14 per SM); fewer
   // tokens are shared out over up to 8 warps each.
   a.parts = static_cast<int>(std::min<int64_t>(8, std::max<int64_t>(1, 2048 / std::max<int64_t>(1, a.rows))));
