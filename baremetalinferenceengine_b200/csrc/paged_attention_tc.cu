@@ -170,10 +170,22 @@ struct Plan {
   int nc;
 };
 
+// The whole warp waits; lane 0 watches the clock where it is not over at once.
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int32_t* status) {
+  if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
   int ok = 1;
   if ((threadIdx.x & 31) == 0) ok = wait_phase(bar, parity, abort_flag, status, kWaitNs, true);
   return __shfl_sync(0xffffffffu, ok, 0) != 0;
+}
+// One thread of a converged warp, always the same.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(p));
+  return p != 0;
 }
 
 // D[tmem] (+)= A[tmem] * B[smem], kind::f16: A's rows are TMEM lanes, two bf16 a column.
@@ -472,72 +484,92 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
       }
     }
     if (seg > 0) wait_phase(qfull, (seg - 1) & 1, abort_flag, a.status, kDrainNs, false);
-  } else if (warp == 1 && lane == 0) {
+  } else if (warp == 1) {
     // ---------------- MMA issuer ----------------
     // Step x: the mix of unit x - 2, then the scores of unit x into the TMEM buffer that
-    // mix has done with.
-    const uint32_t q_addr = smem_u32(smem), k_base = smem_u32(smem + L::kOffK), v_base = smem_u32(smem + L::kOffV);
-    bool issued = false, ok = true;
-    int x = 0, seg = 0;         // scores: the next unit, its segment
-    int pseg = 0;               // mix: its segment's number
-    int pu = 0;                 // and the next unit
-    struct Span {
-      int first, units;
-    };
-    Span span[4] = {{0, 0}, {0, 0}, {0, 0}, {0, 0}};  // the last segments, by number mod 4
-    auto mix = [&]() {
-      const int u = pu++, w = u & 1;
-      while (u >= span[pseg & 3].first + span[pseg & 3].units) ++pseg;
-      const Span sp = span[pseg & 3];
-      if (!wait_phase(&pfull[w], (u >> 1) & 1, abort_flag, a.status, kWaitNs, true)) return false;
-      // the segment's first mix overwrites O: its last reader was the previous segment's end
-      if (u == sp.first && pseg > 0 && !wait_phase(ofree, (pseg - 1) & 1, abort_flag, a.status, kWaitNs, true)) return false;
-      const int kt = DUAL ? u >> 1 : u;
-      const int vs = kt % L::kVS;
-      if (!wait_phase(&vfull[vs], (kt / L::kVS) & 1, abort_flag, a.status, kWaitNs, true)) return false;
-      tc_fence_after();
-      const uint32_t v_addr = v_base + vs * L::kOperand;
-      const uint32_t fresh = u < sp.first + 2 ? 0u : 1u;  // the group's first unit of the segment
-#pragma unroll
-      for (int kk = 0; kk < kTile / 16; ++kk) {
-        mma_bf16_ts(tmem + L::kColO + w * HD, tmem + w * kTile + kk * 8, smem_desc(v_addr + kk * 2048, L::kBox, 1024), kIdescO,
-                    kk > 0 ? 1u : fresh);
-      }
-      issued = true;
-      mma_commit(&pvdone[w]);
-      if (!DUAL || w == 1) mma_commit(&vempty[vs]);
-      return true;
-    };
-    for (; ok && walk.left > 0; walk.next(a, per), ++seg) {
-      const int units = walk.segment() * L::kTiles;
-      span[seg & 3] = Span{x, units};
-      for (int i = 0; i < units; ++i, ++x) {
-        const int w = x & 1;
-        if (x >= 2 && !(ok = mix())) break;
-        if (i == 0 && !(ok = wait_phase(qfull, seg & 1, abort_flag, a.status, kWaitNs, true))) break;
-        const int kt = DUAL ? x >> 1 : x;
-        const int ks = kt % L::kKS;
-        if (!(ok = wait_phase(&kfull[ks], (kt / L::kKS) & 1, abort_flag, a.status, kWaitNs, true))) break;
-        if (x >= 2 && !(ok = wait_phase(&pvdone[w], ((x - 2) >> 1) & 1, abort_flag, a.status, kWaitNs, true))) break;
+    // mix has done with. The whole warp walks, one thread issues: descriptors stay in
+    // uniform registers, and a product of 64 cycles is not held up by its issue.
+    const uint64_t q_desc = smem_desc(smem_u32(smem), 16, 1024);
+    const uint64_t k_desc = smem_desc(smem_u32(smem + L::kOffK), 16, 1024);
+    const uint64_t v_desc = smem_desc(smem_u32(smem + L::kOffV), L::kBox, 1024);
+    constexpr uint32_t kStage = L::kOperand >> 4;
+    bool issued = false, ok = true, first = true;
+    int seg = 0, mix_seg = -1, end = -1;  // segments of the scores and of the mix; units in all, once known
+    int ks = 0, vs = 0;                   // ring slots of the next scores and mix
+    uint32_t k_phase = 0, v_phase = 0;
+    uint32_t firsts = 0;                  // bit i: unit x - 1 - i is its segment's first
+    int left = __shfl_sync(0xffffffffu, walk.segment(), 0) * L::kTiles;
+    for (int x = 0; ok; ++x) {
+      const int w = x & 1;
+      if (x >= 2) {
+        const bool opens = (firsts & 2) != 0;
+        if (opens) ++mix_seg;
+        ok = warp_wait(&pfull[w], ((x - 2) >> 1) & 1, abort_flag, a.status);
+        // the segment's first mix overwrites O: its last reader was the previous segment's end
+        if (ok && opens && mix_seg > 0) ok = warp_wait(ofree, (mix_seg - 1) & 1, abort_flag, a.status);
+        if (ok) ok = warp_wait(&vfull[vs], v_phase, abort_flag, a.status);
+        if (!ok) break;
         tc_fence_after();
-        const uint32_t k_addr = k_base + ks * L::kOperand;
-        const uint32_t qa = q_addr + (DUAL ? w * L::kOperand : 0);
+        if (elect_one()) {
+          const uint32_t fresh = (firsts & 6) != 0 ? 0u : 1u;  // the group's first unit of the segment
 #pragma unroll
-        for (int kk = 0; kk < HD / 16; ++kk) {
-          const uint32_t off = (kk >> 2) * L::kBox + (kk & 3) * 32;
-          mma_bf16(tmem + w * kTile, smem_desc(qa + off, 16, 1024), smem_desc(k_addr + off, 16, 1024), kIdescS,
-                   kk > 0 ? 1u : 0u);
+          for (int kk = 0; kk < kTile / 16; ++kk) {
+            mma_bf16_ts(tmem + L::kColO + w * HD, tmem + w * kTile + kk * 8, v_desc + vs * kStage + kk * 128, kIdescO,
+                        kk > 0 ? 1u : fresh);
+          }
+          mma_commit(&pvdone[w]);
+          if (!DUAL || w == 1) mma_commit(&vempty[vs]);
         }
+        __syncwarp();
         issued = true;
-        mma_commit(&sfull[w]);
-        if (!DUAL || w == 1) mma_commit(&kempty[ks]);
-        if (i == units - 1) mma_commit(qempty);
+        if ((!DUAL || w == 1) && ++vs == L::kVS) {
+          vs = 0;
+          v_phase ^= 1;
+        }
+      }
+      if (left > 0) {
+        if (first) ok = warp_wait(qfull, seg & 1, abort_flag, a.status);
+        if (ok) ok = warp_wait(&kfull[ks], k_phase, abort_flag, a.status);
+        if (ok && x >= 2) ok = warp_wait(&pvdone[w], ((x - 2) >> 1) & 1, abort_flag, a.status);
+        if (!ok) break;
+        tc_fence_after();
+        if (elect_one()) {
+#pragma unroll
+          for (int kk = 0; kk < HD / 16; ++kk) {
+            constexpr uint32_t kAtom = L::kBox >> 4;
+            const uint32_t off = (kk >> 2) * kAtom + (kk & 3) * 2;
+            mma_bf16(tmem + w * kTile, q_desc + (DUAL ? w * kStage : 0) + off, k_desc + ks * kStage + off, kIdescS,
+                     kk > 0 ? 1u : 0u);
+          }
+          mma_commit(&sfull[w]);
+          if (!DUAL || w == 1) mma_commit(&kempty[ks]);
+          if (left == 1) mma_commit(qempty);
+        }
+        __syncwarp();
+        issued = true;
+        firsts = firsts << 1 | (first ? 1u : 0u);
+        first = false;
+        if ((!DUAL || w == 1) && ++ks == L::kKS) {
+          ks = 0;
+          k_phase ^= 1;
+        }
+        if (--left == 0) {
+          walk.next(a, per);
+          ++seg;
+          left = __shfl_sync(0xffffffffu, walk.left > 0 ? walk.segment() : 0, 0) * L::kTiles;
+          first = left > 0;
+          if (left == 0) end = x + 1;
+        }
+      } else {
+        firsts <<= 1;
+        if (x == end + 1) break;  // the last unit's mix is issued
       }
     }
-    while (ok && pu < x) ok = mix();
     if (issued) {
-      mma_commit(mma_done);
-      wait_phase(mma_done, 0, abort_flag, a.status, kDrainNs, false);
+      if (elect_one()) mma_commit(mma_done);
+      __syncwarp();
+      if (lane == 0) wait_phase(mma_done, 0, abort_flag, a.status, kDrainNs, false);
+      __syncwarp();
     }
   } else if (warp >= 4) {
     // ---------------- softmax ----------------
