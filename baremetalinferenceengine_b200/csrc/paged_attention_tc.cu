@@ -29,8 +29,8 @@
 // up; a whole one is written directly.
 //
 // Twelve warps:
-//   warp 0     TMA of K and V, pages looked up by its lanes, one box of page_size rows
-//              (128 at most) x 64 dims each, into separate rings;
+//   warps 0, 3 TMA of K and of V, pages looked up by their lanes, one box of page_size
+//              rows (128 at most) x 64 dims each, into separate rings;
 //   warp 1     owns TMEM; one thread issues every MMA;
 //   warp 2     TMA of the queries, once per segment (an item's part in this CTA);
 //   warps 4-7, 8-11  two softmax groups. Unit u of the CTA's sequence goes to group
@@ -400,11 +400,18 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
     records[cta] = Record{plan->lo, plan->total, static_cast<int32_t>(walk.b), walk.kvh, walk.p, walk.t, walk.tiles, plan->nc};
   }
 
-  if (warp == 0) {
-    // ---------------- K and V ----------------
+  if (warp == 0 || warp == 3) {
+    // ---------------- K (warp 0) and V (warp 3) ----------------
+    const bool is_v = warp == 3;
+    const CUtensorMap* map = is_v ? &tv : &tk;
+    uint64_t* full = is_v ? vfull : kfull;
+    uint64_t* empty = is_v ? vempty : kempty;
+    unsigned char* ring = smem + (is_v ? L::kOffV : L::kOffK);
+    const int stages = is_v ? L::kVS : L::kKS;
     const int box_rows = min(a.page_size, kTile);
     const int boxes = kTile / box_rows;  // pages of a tile: at most 16
-    int kt = 0, nk = 0, nv = 0;  // the tile; K and V tiles asked for
+    int kt = 0, stage = 0;               // tiles asked for; the next one's ring slot
+    uint32_t phase = 1;
     bool ok = true;
     for (; ok && walk.left > 0; walk.next(a, per)) {
       const int n = walk.segment();
@@ -419,49 +426,35 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
         return (page * a.hkv + walk.kvh) * a.page_size + (slot - nth * a.page_size);
       };
       int row = row_of(walk.t);
-      for (int i = 0; i < n; ++i, ++kt) {
+      for (int i = 0; i < n; ++i) {
         const int next_row = i + 1 < n ? row_of(walk.t + i + 1) : -2;  // looked up while this tile waits
         const uint32_t have = __ballot_sync(0xffffffffu, row >= 0);
         const uint32_t bad = __ballot_sync(0xffffffffu, row == -1);
-        const uint32_t bytes = __popc(have) * box_rows * 128 * (HD / 64);
-        const int ks = kt % L::kKS, vs = kt % L::kVS;
-        unsigned char* kd = smem + L::kOffK + ks * L::kOperand + lane * box_rows * 128;
-        unsigned char* vd = smem + L::kOffV + vs * L::kOperand + lane * box_rows * 128;
-        if (!warp_wait(&kempty[ks], ((kt / L::kKS) & 1) ^ 1u, abort_flag, a.status)) {
-          ok = false;
-          break;
-        }
+        if (!(ok = warp_wait(&empty[stage], phase, abort_flag, a.status))) break;
         if (lane == 0) {
-          bad_ring[kt % kBadRing] = bad;
-          if (bad) raise_status(a.status, BM_DEVERR_BAD_PAGE);
-          mbar_expect_tx(&kfull[ks], bytes);
+          if (!is_v) {
+            bad_ring[kt % kBadRing] = bad;
+            if (bad) raise_status(a.status, BM_DEVERR_BAD_PAGE);
+          }
+          mbar_expect_tx(&full[stage], __popc(have) * box_rows * 128 * (HD / 64));
         }
         __syncwarp();
         if (row >= 0) {
+          unsigned char* to = ring + stage * L::kOperand + lane * box_rows * 128;
 #pragma unroll
-          for (int h = 0; h < HD / 64; ++h) tma_load_2d(kd + h * L::kBox, &tk, &kfull[ks], 64 * h, row);
+          for (int h = 0; h < HD / 64; ++h) tma_load_2d(to + h * L::kBox, map, &full[stage], 64 * h, row);
         }
-        nk = kt + 1;
-        if (!warp_wait(&vempty[vs], ((kt / L::kVS) & 1) ^ 1u, abort_flag, a.status)) {
-          ok = false;
-          break;
+        ++kt;
+        if (++stage == stages) {
+          stage = 0;
+          phase ^= 1;
         }
-        if (lane == 0) mbar_expect_tx(&vfull[vs], bytes);
-        __syncwarp();
-        if (row >= 0) {
-#pragma unroll
-          for (int h = 0; h < HD / 64; ++h) tma_load_2d(vd + h * L::kBox, &tv, &vfull[vs], 64 * h, row);
-        }
-        nv = kt + 1;
         row = next_row;
       }
     }
     if (lane == 0) {  // copies still in flight land before the CTA ends
-      for (int i = max(0, nk - L::kKS); i < nk; ++i) {
-        wait_phase(&kfull[i % L::kKS], (i / L::kKS) & 1, abort_flag, a.status, kDrainNs, false);
-      }
-      for (int i = max(0, nv - L::kVS); i < nv; ++i) {
-        wait_phase(&vfull[i % L::kVS], (i / L::kVS) & 1, abort_flag, a.status, kDrainNs, false);
+      for (int i = max(0, kt - stages); i < kt; ++i) {
+        wait_phase(&full[i % stages], (i / stages) & 1, abort_flag, a.status, kDrainNs, false);
       }
     }
     __syncwarp();
