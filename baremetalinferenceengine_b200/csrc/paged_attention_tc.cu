@@ -91,7 +91,7 @@ struct Layout {
   static constexpr int kOffBar = kOffSum + (kCopies > 1 ? kCopyRows * kPitch * 4 : 0);
   static constexpr int kBars = 2 * kKS + 2 * kVS + 6 + 4;
   static constexpr int kOffPlan = kOffBar + kBars * 8;      // Plan, scan, bad-page ring
-  static constexpr int kBytes = kOffPlan + 64 + 16 * 8 + kBadRing * 4 + 16 + 1024 /* alignment slack */;
+  static constexpr int kBytes = kOffPlan + 96 + 16 * 8 + kBadRing * 4 + 16 + 1024 /* alignment slack */;
   static_assert(kBytes <= 232448, "shared memory of a CTA");
   static constexpr uint32_t kColO = 256;                    // TMEM: S0, S1 (128 each), O0, O1 (HD each)
   static constexpr uint32_t kTmemCols = 512;
@@ -130,10 +130,10 @@ struct Walk {
   Seq s;
 
   // Tile `off` of sequence b is the CTA's first, and `n` tiles are its own.
-  __device__ void start(const TreeArgs& a, int64_t b0, int64_t off, int64_t n, int per) {
+  __device__ void start(const TreeArgs& a, const Seq& sequence, int64_t b0, int64_t off, int64_t n, int per) {
     b = b0;
     left = n;
-    read_seq(a, b, &s);
+    s = sequence;
     const int64_t head = head_tiles(a, s, per, &items);
     kvh = static_cast<int>(off / head);
     off -= kvh * head;
@@ -167,8 +167,10 @@ struct Walk {
 
 struct Plan {
   int64_t lo, n, total, b, off;
+  Seq s;  // sequence b
   int nc;
 };
+static_assert(sizeof(Plan) <= 96, "room in the layout");
 
 // The whole warp waits; lane 0 watches the clock where it is not over at once.
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int32_t* status) {
@@ -315,7 +317,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
   uint64_t* ofree = qempty + 1;       // the segment's O has been read (one arrival per softmax warp)
   uint64_t* mma_done = ofree + 1;
   Plan* plan = reinterpret_cast<Plan*>(smem + L::kOffPlan);
-  int64_t* scan = reinterpret_cast<int64_t*>(smem + L::kOffPlan + 64);
+  int64_t* scan = reinterpret_cast<int64_t*>(smem + L::kOffPlan + 96);
   volatile uint32_t* bad_ring = reinterpret_cast<volatile uint32_t*>(scan + 16);
   uint32_t* tmem_base_s = const_cast<uint32_t*>(bad_ring) + kBadRing;
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_base_s + 1);
@@ -324,49 +326,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
 
   // ---------------- the plan ----------------
   {
-    const int64_t share = (a.batch + kThreadsTc - 1) / kThreadsTc;
-    const int64_t b_lo = min(a.batch, tid * share), b_hi = min(a.batch, b_lo + share);
-    int64_t mine = 0;
-    for (int64_t b = b_lo; b < b_hi; ++b) {
-      Seq s;
-      const int32_t bad = read_seq(a, b, &s);
-      if (bad && cta == 0) raise_status(a.status, bad);
-      int items;
-      mine += a.hkv * head_tiles(a, s, per, &items);
-    }
-    int64_t incl = mine;
-#pragma unroll
-    for (int off = 1; off < 32; off <<= 1) {
-      const int64_t v = __shfl_up_sync(0xffffffffu, incl, off);
-      if (lane >= off) incl += v;
-    }
-    if (lane == 31) scan[warp] = incl;
-    __syncthreads();
-    int64_t total = 0, before = incl - mine;
-    for (int w = 0; w < kThreadsTc / 32; ++w) {
-      if (w < warp) before += scan[w];
-      total += scan[w];
-    }
-    const int nc = static_cast<int>(min(static_cast<int64_t>(gridDim.x), (total + kMinTiles - 1) / kMinTiles));
-    if (cta >= nc) {  // nothing for this CTA (the same for all its threads)
-      if (tid == 0) records[cta] = Record{0, total, -1, 0, 0, -1, 0, nc};
-      return;
-    }
-    const int64_t lo = total * cta / nc, hi = total * (cta + 1) / nc;
-    if (before <= lo && lo < before + mine) {
-      int64_t at = before;
-      for (int64_t b = b_lo; b < b_hi; ++b) {
-        Seq s;
-        read_seq(a, b, &s);
-        int items;
-        const int64_t n = a.hkv * head_tiles(a, s, per, &items);
-        if (lo < at + n) {
-          *plan = Plan{lo, hi - lo, total, b, lo - at, nc};
-          break;
-        }
-        at += n;
-      }
-    }
+    // barriers and TMEM come up while the lengths are read
     if (tid == 0) {
       for (int i = 0; i < L::kKS; ++i) {
         mbar_init(&kfull[i], 1);
@@ -389,13 +349,56 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
       fence_barrier_init();
     }
     if (warp == 1) tmem_alloc(tmem_base_s, L::kTmemCols);
+    const int64_t share = (a.batch + kThreadsTc - 1) / kThreadsTc;
+    const int64_t b_lo = min(a.batch, tid * share), b_hi = min(a.batch, b_lo + share);
+    int64_t mine = 0;
+    Seq s;
+    for (int64_t b = b_lo; b < b_hi; ++b) {
+      const int32_t bad = read_seq(a, b, &s);
+      if (bad && cta == 0) raise_status(a.status, bad);
+      int items;
+      mine += a.hkv * head_tiles(a, s, per, &items);
+    }
+    int64_t incl = mine;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const int64_t v = __shfl_up_sync(0xffffffffu, incl, off);
+      if (lane >= off) incl += v;
+    }
+    if (lane == 31) scan[warp] = incl;
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    int64_t total = 0, before = incl - mine;
+    for (int w = 0; w < kThreadsTc / 32; ++w) {
+      if (w < warp) before += scan[w];
+      total += scan[w];
+    }
+    const int nc = static_cast<int>(min(static_cast<int64_t>(gridDim.x), (total + kMinTiles - 1) / kMinTiles));
+    if (cta >= nc) {  // nothing for this CTA (the same for all its threads)
+      if (tid == 0) records[cta] = Record{0, total, -1, 0, 0, -1, 0, nc};
+      if (warp == 1) tmem_dealloc(*tmem_base_s, L::kTmemCols);
+      return;
+    }
+    const int64_t lo = total * cta / nc, hi = total * (cta + 1) / nc;
+    if (before <= lo && lo < before + mine) {
+      int64_t at = before;
+      for (int64_t b = b_lo; b < b_hi; ++b) {
+        if (share > 1) read_seq(a, b, &s);
+        int items;
+        const int64_t n = a.hkv * head_tiles(a, s, per, &items);
+        if (lo < at + n) {
+          *plan = Plan{lo, hi - lo, total, b, lo - at, s, nc};
+          break;
+        }
+        at += n;
+      }
+    }
+    __syncthreads();
   }
   const uint32_t tmem = *tmem_base_s;
   Walk walk;
-  walk.start(a, plan->b, plan->off, plan->n, per);
+  walk.start(a, plan->s, plan->b, plan->off, plan->n, per);
   if (tid == 0) {
     records[cta] = Record{plan->lo, plan->total, static_cast<int32_t>(walk.b), walk.kvh, walk.p, walk.t, walk.tiles, plan->nc};
   }
@@ -884,7 +887,9 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
 }
 
 // Adds up the partials of the item that CTA k's first tile continues: block (k, rows
-// 16 y .. 16 y + 15) by the first border inside the item.
+// 8 y .. 8 y + 7) by the first border inside the item. A warp takes a row, its halves
+// every other part: an item of few rows and many parts is bound by the latency of the
+// parts' loads, so many are in flight over many SMs.
 template <int HD, int COPIES>
 __global__ void __launch_bounds__(256) tree_merge_kernel(const TreeArgs a, int ctas) {
   grid_dependency_wait();
@@ -900,39 +905,52 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(const TreeArgs a, int c
   Seq s;
   read_seq(a, rec.b, &s);
   const int tpt = L::kCopyRows / a.group;
-  constexpr int kLanes = 16;  // threads of a row
-  const int r = static_cast<int>(blockIdx.y) * 16 + threadIdx.x / kLanes;
+  constexpr int kLanes = 16;  // threads of a part's row
+  const int lane = threadIdx.x & 31;
+  const int r = static_cast<int>(blockIdx.y) * 8 + threadIdx.x / 32;
   const int tile = r / kTile, rr = r - tile * kTile;
   const int i0 = rec.p * tpt * L::kTiles + tile * tpt;
   if (rr >= max(0, min(tpt, s.n - i0)) * a.group) return;
-  const int last = static_cast<int>([&] {  // one past the last CTA with a part of the item
-    int c = k + 1;
-    while (c < rec.nc && border(c) < first + rec.tiles) ++c;
-    return c;
-  }());
-  auto part = [&](int c) { return slots + (2 * static_cast<int64_t>(c) + (c == k - 1 && border(c) != first)) * L::kSlotFloats; };
+  // one past the last CTA with a part: the one that holds the item's last tile
+  const int last = static_cast<int>(((first + rec.tiles) * rec.nc - 1) / rec.total) + 1;
+  const int skip = border(k - 1) != first;  // in the first CTA the item is not the first segment
+  auto part = [&](int c) { return slots + (2 * static_cast<int64_t>(c) + (c == k - 1 ? skip : 0)) * L::kSlotFloats; };
   float m = -INFINITY;
-  for (int c = k - 1; c < last; ++c) m = fmaxf(m, part(c)[L::kRows * HD + r]);
+  for (int c = k - 1 + lane; c < last; c += 32) m = fmaxf(m, part(c)[L::kRows * HD + r]);
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
   const float base = m == -INFINITY ? 0.f : m;
   constexpr int kDims = HD / kLanes;  // 4 or 8 dims of a thread
-  const int d = (threadIdx.x % kLanes) * kDims;
+  const int d = lane % kLanes * kDims, half = lane / kLanes;
   float l = 0.f, o[kDims];
 #pragma unroll
   for (int e = 0; e < kDims; ++e) o[e] = 0.f;
-#pragma unroll 4
-  for (int c = k - 1; c < last; ++c) {
-    const float* ps = part(c);
-    const float f = ex2(ps[L::kRows * HD + r] - base);
-    l = fmaf(ps[L::kRows * (HD + 1) + r], f, l);
+  for (int c0 = k - 1; c0 < last; c0 += 32) {
+    float f = 0.f;  // of part c0 + lane
+    if (c0 + lane < last) {
+      f = ex2(part(c0 + lane)[L::kRows * HD + r] - base);
+      l = fmaf(part(c0 + lane)[L::kRows * (HD + 1) + r], f, l);
+    }
+    const int n = min(32, last - c0);
+#pragma unroll 8
+    for (int i = half; i < n + half; i += 2) {
+      const float w = __shfl_sync(0xffffffffu, f, i & 31);  // past n: 0
+      const float* ps = part(min(c0 + i, last - 1)) + r * HD + d;
 #pragma unroll
-    for (int e = 0; e < kDims; e += 4) {
-      const float4 v = *reinterpret_cast<const float4*>(ps + r * HD + d + e);
-      o[e] = fmaf(v.x, f, o[e]);
-      o[e + 1] = fmaf(v.y, f, o[e + 1]);
-      o[e + 2] = fmaf(v.z, f, o[e + 2]);
-      o[e + 3] = fmaf(v.w, f, o[e + 3]);
+      for (int e = 0; e < kDims; e += 4) {
+        const float4 v = *reinterpret_cast<const float4*>(ps + e);
+        o[e] = fmaf(v.x, w, o[e]);
+        o[e + 1] = fmaf(v.y, w, o[e + 1]);
+        o[e + 2] = fmaf(v.z, w, o[e + 2]);
+        o[e + 3] = fmaf(v.w, w, o[e + 3]);
+      }
     }
   }
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
+#pragma unroll
+  for (int e = 0; e < kDims; ++e) o[e] += __shfl_xor_sync(0xffffffffu, o[e], 16);
+  if (half != 0) return;
   const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
   const int token = i0 + rr / a.group, h = rr - (rr / a.group) * a.group;
   bf16* out = static_cast<bf16*>(a.out) + ((s.row0 + token) * a.hq + rec.kvh * a.group + h) * HD + d;
@@ -975,7 +993,7 @@ int launch_form(const TreeArgs& a, cudaStream_t stream, const char* what) {
   if (int st = launch_kernel(what, kernel, dim3(nc), dim3(kThreadsTc), L::kBytes, stream, nullptr, tq, tk, tv, a)) return st;
   // items of one tile, and a single CTA, are never cut
   if (nc == 1 || a.max_ctx + a.max_tree <= kTile) return BM_OK;
-  return launch_kernel(what, tree_merge_kernel<HD, COPIES>, dim3(nc - 1, L::kRows / 16), dim3(256), 0, stream, nullptr, a, nc);
+  return launch_kernel(what, tree_merge_kernel<HD, COPIES>, dim3(nc - 1, L::kRows / 8), dim3(256), 0, stream, nullptr, a, nc);
 }
 
 template <int HD>
