@@ -10,13 +10,14 @@
 // Bound: with R = group * n rows per kv head a slot costs 4 R hd operations and
 // 2 hd * es bytes, so few rows are bound by memory and many, in fp32 on CUDA cores, by
 // the multiply-adds. All rows of a kv head therefore share a CTA's tile of K and V
-// (16 or 64 rows against 64 slots), and both products run from shared memory in
+// (16, 32 or 64 rows against 64 slots), and both products run from shared memory in
 // register tiles (4 x 4 scores and 4 x hd/16 outputs per thread for 64 rows), 64
 // multiply-adds for 8 16-byte shared loads. Slots are shared out over CTAs when the
 // (sequence, kv head) pairs do not fill the GPU; the shares' partial sums meet in
 // tree_combine_kernel.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "paged_attention.cuh"
 
@@ -282,16 +283,16 @@ __global__ void __launch_bounds__(kThreads) tree_combine_kernel(const TreeArgs a
   }
 }
 
-int rows_per_tile(int rows) { return rows > 16 ? 64 : 16; }
+int rows_per_tile(int rows) { return rows > 32 ? 64 : rows > 16 ? 32 : 16; }
 
-// The CUDA-core form's split: enough CTAs for two per SM, none shorter than two tiles.
+// The CUDA-core form's split: enough CTAs for four per SM, none shorter than a tile.
 void plan(int64_t batch, int hkv, int group, int max_ctx, int max_tree, int* row_tiles, int* splits, int* split_len) {
   const int rows = group * max_tree, bm = rows_per_tile(rows);
   *row_tiles = (rows + bm - 1) / bm;
   const int len = max_ctx + max_tree;
   const int64_t ctas = batch * hkv * *row_tiles;
-  const int64_t want = (2 * static_cast<int64_t>(sm_count()) + ctas - 1) / ctas;
-  const int most = std::max(1, len / (2 * kBN));
+  const int64_t want = (4 * static_cast<int64_t>(sm_count()) + ctas - 1) / ctas;
+  const int most = std::max(1, len / kBN);
   const int n = static_cast<int>(std::min<int64_t>(want, std::min(most, 64)));
   *split_len = ((len + n - 1) / n + kBN - 1) / kBN * kBN;
   *splits = (len + *split_len - 1) / *split_len;
@@ -310,14 +311,14 @@ int launch_one(const TreeArgs& a, cudaStream_t stream, const char* what) {
 template <typename T>
 int launch(TreeArgs a, cudaStream_t stream, const char* what) {
   const int nj = (a.hd + 63) / 64;
-  int st;
-  if (rows_per_tile(a.group * a.max_tree) == 16) {
-    st = nj == 1 ? launch_one<T, 16, 1>(a, stream, what) : nj == 2 ? launch_one<T, 16, 2>(a, stream, what)
-                                                                 : launch_one<T, 16, 4>(a, stream, what);
-  } else {
-    st = nj == 1 ? launch_one<T, 64, 1>(a, stream, what) : nj == 2 ? launch_one<T, 64, 2>(a, stream, what)
-                                                                 : launch_one<T, 64, 4>(a, stream, what);
-  }
+  auto by_width = [&](auto bm) {
+    constexpr int BM = decltype(bm)::value;
+    return nj == 1 ? launch_one<T, BM, 1>(a, stream, what) : nj == 2 ? launch_one<T, BM, 2>(a, stream, what)
+                                                                   : launch_one<T, BM, 4>(a, stream, what);
+  };
+  const int rows = rows_per_tile(a.group * a.max_tree);
+  const int st = rows == 16 ? by_width(std::integral_constant<int, 16>{})
+                 : rows == 32 ? by_width(std::integral_constant<int, 32>{}) : by_width(std::integral_constant<int, 64>{});
   if (st != BM_OK || a.splits == 1) return st;
   const int64_t warps = a.batch * a.max_tree * a.hq;
   const int64_t grid = (warps + kThreads / 32 - 1) / (kThreads / 32);
