@@ -10,7 +10,7 @@
 // Bound: with R = group * n rows per kv head a slot costs 4 R hd operations and
 // 2 hd * es bytes, so few rows are bound by memory and many, in fp32 on CUDA cores, by
 // the multiply-adds. All rows of a kv head therefore share a CTA's tile of K and V
-// (16, 32 or 64 rows against 64 slots), and both products run from shared memory in
+// (32 or 64 rows against 64 slots), and both products run from shared memory in
 // register tiles (4 x 4 scores and 4 x hd/16 outputs per thread for 64 rows), 64
 // multiply-adds for 8 16-byte shared loads. Slots are shared out over CTAs when the
 // (sequence, kv head) pairs do not fill the GPU; the shares' partial sums meet in
@@ -241,6 +241,227 @@ __global__ void __launch_bounds__(kThreads) tree_attention_kernel(const TreeArgs
   }
 }
 
+// Few rows (MR at most): each warp walks groups of eight slots of its own with its own
+// running softmax, K and V straight from memory into registers (a quarter warp's 16-byte
+// chunks of a slot's K, a warp's of a slot's V), so every byte is loaded once and no
+// barrier stands between a load and its use; the four warps' sums meet at the end. The
+// tiled kernel above would read its shared K and V eight times over for a few rows. J:
+// 16-byte chunks of a row of V per lane.
+constexpr int kRowThreads = 128;
+constexpr int kGroup = 8;  // slots of a warp's step
+
+template <typename T, int MR, int J>
+__global__ void __launch_bounds__(kRowThreads) tree_rows_kernel(const TreeArgs a) {
+  grid_dependency_wait();
+  constexpr int VEC = VecWidth<T>::value;
+  constexpr int kWarps = kRowThreads / 32;
+  const int hd = a.hd, cpr = hd / VEC;
+  int64_t id = blockIdx.x;
+  const int split = static_cast<int>(id % a.splits);
+  id /= a.splits;
+  const int rt = static_cast<int>(id % a.row_tiles);
+  id /= a.row_tiles;
+  const int kvh = static_cast<int>(id % a.hkv);
+  const int64_t b = id / a.hkv;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  Seq s;
+  const int32_t bad = read_seq(a, b, &s);
+  if (bad) {
+    if (tid == 0 && split == 0 && rt == 0 && kvh == 0) raise_status(a.status, bad);
+    return;
+  }
+  const int R = a.group * s.n, r_lo = rt * MR;
+  if (r_lo >= R) return;
+  const int rows = min(MR, R - r_lo);
+  const int total = s.ctx + s.n;
+  const int seen = a.mask ? total : s.ctx + min(s.n, (r_lo + rows - 1) / a.group + 1);
+  const int start = split * a.split_len, end = min(seen, start + a.split_len);
+
+  extern __shared__ __align__(16) float smem[];
+  float* Qs = smem;                                   // [MR][hd], then the warps' sums [kWarps][MR][hd]
+  float* Ps = smem + kWarps * MR * hd + warp * kGroup * MR;  // this warp's weights [kGroup][MR]
+  float* ml = smem + kWarps * MR * (hd + kGroup);     // [kWarps][MR] maxima, then sums
+  const T* q = static_cast<const T*>(a.q);
+  for (int c = tid; c < MR * cpr; c += kRowThreads) {
+    const int r = c / cpr, col = (c - r * cpr) * VEC;
+    float f[VEC];
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) f[e] = 0.f;
+    if (r < rows) {
+      const int i = (r_lo + r) / a.group, g = (r_lo + r) - i * a.group;
+      unpack16<T>(ld_keep(q + ((s.row0 + i) * a.hq + kvh * a.group + g) * hd + col), f);
+    }
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) Qs[r * hd + col + e] = f[e] * a.qscale;
+  }
+  __syncthreads();
+  const T* kp = static_cast<const T*>(a.k_pages);
+  const T* vp = static_cast<const T*>(a.v_pages);
+  const int32_t* pages = a.page_table + static_cast<int64_t>(s.seq) * a.max_pages;
+  const int own = lane >> 2, sub = lane & 3;  // this lane's slot of the group, its quarter of K's chunks
+
+  float m[MR], l[MR], acc[MR][J * VEC];
+#pragma unroll
+  for (int r = 0; r < MR; ++r) {
+    m[r] = -INFINITY;
+    l[r] = 0.f;
+#pragma unroll
+    for (int e = 0; e < J * VEC; ++e) acc[r][e] = 0.f;
+  }
+  for (int g0 = start + warp * kGroup; g0 < end; g0 += kWarps * kGroup) {
+    const int slot = g0 + own;
+    int64_t at = -1;  // the slot's row of the pages
+    if (slot < end) {
+      const int nth = slot / a.page_size;
+      const int32_t page = __ldg(pages + nth);
+      if (page >= 0 && page < a.num_pages) {
+        at = ((static_cast<int64_t>(page) * a.hkv + kvh) * a.page_size + (slot - nth * a.page_size)) * hd;
+      } else if (sub == 0) {
+        raise_status(a.status, BM_DEVERR_BAD_PAGE);
+      }
+    }
+    uint4 v[kGroup][J];  // V of the eight slots, on its way while the scores are made
+#pragma unroll
+    for (int i = 0; i < kGroup; ++i) {
+      const int64_t vat = __shfl_sync(0xffffffffu, at, i * 4);
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+        v[i][j] = make_uint4(0u, 0u, 0u, 0u);
+        if (vat >= 0 && lane + 32 * j < cpr) v[i][j] = ld_stream(vp + vat + (lane + 32 * j) * VEC);
+      }
+    }
+    float sc[MR];
+#pragma unroll
+    for (int r = 0; r < MR; ++r) sc[r] = 0.f;
+    for (int c0 = sub; c0 < cpr; c0 += 16) {
+      uint4 k[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        k[u] = make_uint4(0u, 0u, 0u, 0u);
+        if (at >= 0 && c0 + 4 * u < cpr) k[u] = ld_stream(kp + at + (c0 + 4 * u) * VEC);
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        float f[VEC];
+        unpack16<T>(k[u], f);
+        const int col = min(c0 + 4 * u, cpr - 1) * VEC;  // past the row k is 0
+#pragma unroll
+        for (int r = 0; r < MR; ++r) {
+#pragma unroll
+          for (int e = 0; e < VEC; e += 4) {
+            const float4 q4 = *reinterpret_cast<const float4*>(Qs + r * hd + col + e);
+            sc[r] = fmaf(q4.x, f[e], sc[r]);
+            sc[r] = fmaf(q4.y, f[e + 1], sc[r]);
+            sc[r] = fmaf(q4.z, f[e + 2], sc[r]);
+            sc[r] = fmaf(q4.w, f[e + 3], sc[r]);
+          }
+        }
+      }
+    }
+    const int j0 = slot - s.ctx;
+    __syncwarp();  // the last group's weights have been read
+#pragma unroll
+    for (int r = 0; r < MR; ++r) {
+      sc[r] += __shfl_xor_sync(0xffffffffu, sc[r], 1);
+      sc[r] += __shfl_xor_sync(0xffffffffu, sc[r], 2);
+      if (at < 0 || r >= rows || (j0 >= 0 && !sees(a, s.row0, (r_lo + r) / a.group, j0))) sc[r] = -INFINITY;
+      float mx = sc[r];
+#pragma unroll
+      for (int off = 4; off < 32; off <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+      const float m_new = fmaxf(m[r], mx);
+      const float base = m_new == -INFINITY ? 0.f : m_new;
+      const float alpha = exp2f(m[r] - base), p = exp2f(sc[r] - base);
+      m[r] = m_new;
+      l[r] = l[r] * alpha + p;  // this slot's share, the same in its four lanes
+      if (sub == 0) Ps[own * MR + r] = p;
+#pragma unroll
+      for (int e = 0; e < J * VEC; ++e) acc[r][e] *= alpha;
+    }
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < kGroup; ++i) {
+      float p[MR];
+#pragma unroll
+      for (int r = 0; r < MR; r += 4) {
+        const float4 p4 = *reinterpret_cast<const float4*>(Ps + i * MR + r);
+        p[r] = p4.x;
+        p[r + 1] = p4.y;
+        p[r + 2] = p4.z;
+        p[r + 3] = p4.w;
+      }
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+        float f[VEC];
+        unpack16<T>(v[i][j], f);
+#pragma unroll
+        for (int r = 0; r < MR; ++r) {
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) acc[r][j * VEC + e] = fmaf(p[r], f[e], acc[r][j * VEC + e]);
+        }
+      }
+    }
+  }
+  // the warps' maxima, sums of weights and of values
+#pragma unroll
+  for (int r = 0; r < MR; ++r) {
+#pragma unroll
+    for (int off = 4; off < 32; off <<= 1) l[r] += __shfl_xor_sync(0xffffffffu, l[r], off);
+    if (lane == 0) {
+      ml[warp * MR + r] = m[r];
+      ml[(kWarps + warp) * MR + r] = l[r];
+    }
+  }
+  __syncthreads();  // Q has been read, too
+#pragma unroll
+  for (int r = 0; r < MR; ++r) {
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      if (lane + 32 * j < cpr) {
+#pragma unroll
+        for (int e = 0; e < VEC; e += 4) {
+          *reinterpret_cast<float4*>(smem + (warp * MR + r) * hd + (lane + 32 * j) * VEC + e) =
+              make_float4(acc[r][j * VEC + e], acc[r][j * VEC + e + 1], acc[r][j * VEC + e + 2], acc[r][j * VEC + e + 3]);
+        }
+      }
+    }
+  }
+  __syncthreads();
+  for (int c = tid; c < rows * (hd / 4); c += kRowThreads) {
+    const int r = c / (hd / 4), d = (c - r * (hd / 4)) * 4;
+    float top = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, ml[w * MR + r]);
+    const float base = top == -INFINITY ? 0.f : top;
+    float sum = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const float f = exp2f(ml[w * MR + r] - base);
+      sum = fmaf(ml[(kWarps + w) * MR + r], f, sum);
+      const float4 part = *reinterpret_cast<const float4*>(smem + (w * MR + r) * hd + d);
+      o = make_float4(fmaf(part.x, f, o.x), fmaf(part.y, f, o.y), fmaf(part.z, f, o.z), fmaf(part.w, f, o.w));
+    }
+    const int i = (r_lo + r) / a.group, h = kvh * a.group + (r_lo + r - i * a.group);
+    const int64_t row = (s.row0 + i) * a.hq + h;
+    if (a.splits == 1) {
+      const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
+      T* out = static_cast<T*>(a.out) + row * hd + d;
+      if constexpr (sizeof(T) == 4) {
+        *reinterpret_cast<float4*>(out) = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+      } else {
+        *reinterpret_cast<uint2*>(out) = make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
+      }
+    } else {
+      float* w = a.ws + (row * a.splits + split) * (hd + 4);
+      *reinterpret_cast<float4*>(w + d) = o;
+      if (d == 0) {
+        w[hd] = sum;
+        w[hd + 1] = top;
+      }
+    }
+  }
+}
+
 // One warp per (row, head): the splits' partials, each scaled to the common maximum.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) tree_combine_kernel(const TreeArgs a) {
@@ -283,15 +504,17 @@ __global__ void __launch_bounds__(kThreads) tree_combine_kernel(const TreeArgs a
   }
 }
 
-int rows_per_tile(int rows) { return rows > 32 ? 64 : rows > 16 ? 32 : 16; }
+// Rows of a CTA: 4 and 8 are tree_rows_kernel's, the others the tiled kernel's.
+int rows_per_tile(int rows) { return rows > 32 ? 64 : rows > 16 ? 32 : rows > 4 ? 8 : 4; }
 
-// The CUDA-core form's split: enough CTAs for four per SM, none shorter than a tile.
+// The CUDA-core form's split: enough CTAs for four per SM (eight of the few-row kernel's),
+// none shorter than a tile.
 void plan(int64_t batch, int hkv, int group, int max_ctx, int max_tree, int* row_tiles, int* splits, int* split_len) {
   const int rows = group * max_tree, bm = rows_per_tile(rows);
   *row_tiles = (rows + bm - 1) / bm;
   const int len = max_ctx + max_tree;
   const int64_t ctas = batch * hkv * *row_tiles;
-  const int64_t want = (4 * static_cast<int64_t>(sm_count()) + ctas - 1) / ctas;
+  const int64_t want = ((bm <= 8 ? 8 : 4) * static_cast<int64_t>(sm_count()) + ctas - 1) / ctas;
   const int most = std::max(1, len / kBN);
   const int n = static_cast<int>(std::min<int64_t>(want, std::min(most, 64)));
   *split_len = ((len + n - 1) / n + kBN - 1) / kBN * kBN;
@@ -316,8 +539,16 @@ int launch(TreeArgs a, cudaStream_t stream, const char* what) {
     return nj == 1 ? launch_one<T, BM, 1>(a, stream, what) : nj == 2 ? launch_one<T, BM, 2>(a, stream, what)
                                                                    : launch_one<T, BM, 4>(a, stream, what);
   };
+  auto few = [&](auto mr) {
+    constexpr int MR = decltype(mr)::value;
+    const int smem = (kRowThreads / 32 * MR * (a.hd + kGroup) + 2 * (kRowThreads / 32) * MR) * 4;
+    const int64_t grid = a.batch * a.hkv * a.row_tiles * a.splits;
+    auto kernel = a.hd / VecWidth<T>::value <= 32 ? tree_rows_kernel<T, MR, 1> : tree_rows_kernel<T, MR, 2>;
+    if (int st = allow_dynamic_smem(reinterpret_cast<const void*>(kernel), smem, what)) return st;
+    return launch_kernel(what, kernel, dim3(static_cast<unsigned>(grid)), dim3(kRowThreads), smem, stream, nullptr, a);
+  };
   const int rows = rows_per_tile(a.group * a.max_tree);
-  const int st = rows == 16 ? by_width(std::integral_constant<int, 16>{})
+  const int st = rows == 4 ? few(std::integral_constant<int, 4>{}) : rows == 8 ? few(std::integral_constant<int, 8>{})
                  : rows == 32 ? by_width(std::integral_constant<int, 32>{}) : by_width(std::integral_constant<int, 64>{});
   if (st != BM_OK || a.splits == 1) return st;
   const int64_t warps = a.batch * a.max_tree * a.hq;

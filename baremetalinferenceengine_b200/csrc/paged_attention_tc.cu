@@ -1,8 +1,9 @@
 // Tree attention over a paged KV cache on the tensor cores (tcgen05, TMA, TMEM), for
-// bf16 caches with head_dim 64 or 128. Same contract as paged_attention.cu.
+// bf16 caches with head_dim up to 128 (filled up with zeros to 64 or 128 by TMA). Same
+// contract as paged_attention.cu.
 //
-// Mathematics: the running softmax of paged_attention.cu on tiles of 128 slots, with
-// both products as tcgen05.mma:
+// Mathematics: the running softmax of paged_attention.cu on tiles of 128 slots (fewer
+// where whole pages do not make 128), with both products as tcgen05.mma:
 //   scores  S[row][slot] = Q[row][:] . K[slot][:]    M = 128 rows, N = 128 slots
 //   mix     O[row][:]   += P[row][slot] V[slot][:]   M = 128 rows, N = head_dim
 // A row is (token, head of the group), token-major: 128 / group tokens share a tile of
@@ -29,8 +30,8 @@
 // up; a whole one is written directly.
 //
 // Twelve warps:
-//   warps 0, 3 TMA of K and of V, pages looked up by their lanes, one box of page_size
-//              rows (128 at most) x 64 dims each, into separate rings;
+//   warps 0, 3 TMA of K and of V, pages looked up by their lanes, one box of a page's
+//              rows (or an equal part of them) x 64 dims each, into separate rings;
 //   warp 1     owns TMEM; one thread issues every MMA;
 //   warp 2     TMA of the queries, once per segment (an item's part in this CTA);
 //   warps 4-7, 8-11  two softmax groups. Unit u of the CTA's sequence goes to group
@@ -112,7 +113,7 @@ __host__ __device__ constexpr size_t records_bytes(int nc) { return (static_cast
 // Tiles of item p (its row tiles hold `per` tokens) of a sequence.
 __device__ __forceinline__ int item_tiles(const TreeArgs& a, const Seq& s, int p, int per) {
   const int seen = s.ctx + (a.mask ? s.n : min(s.n, (p + 1) * per));
-  return (seen + kTile - 1) / kTile;
+  return (seen + a.tile - 1) / a.tile;
 }
 // All tiles of one kv head of a sequence, and its items.
 __device__ __forceinline__ int64_t head_tiles(const TreeArgs& a, const Seq& s, int per, int* items) {
@@ -247,11 +248,11 @@ __device__ __forceinline__ uint32_t seen32(const TreeArgs& a, const Seq& s, int 
 }
 
 // Which of the 32 slots at column 32c of a tile have a sound page (bit b of bad: the
-// tile's page b is not). Boxes hold at least 8 slots.
+// tile's box b has not). Two boxes or more hold whole groups of 8 slots each.
 __device__ __forceinline__ uint32_t sound32(uint32_t bad, int c, int box_rows) {
   uint32_t v = 0xffffffffu;
   for (int e = 0; e < 32; e += 8) {
-    if ((bad >> ((32 * c + e) / box_rows)) & 1) v &= ~(0xffu << e);
+    if ((bad >> min((32 * c + e) / box_rows, 31)) & 1) v &= ~(0xffu << e);
   }
   return v;
 }
@@ -349,6 +350,14 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
       fence_barrier_init();
     }
     if (warp == 1) tmem_alloc(tmem_base_s, L::kTmemCols);
+    if (a.tile < kTile) {  // V rows that no copy ever fills: zero, since their weights of 0 meet them
+      const int rows = kTile - a.tile;
+      for (int c = tid; c < L::kVS * (HD / 64) * rows * 8; c += kThreadsTc) {
+        const int row = a.tile + c / 8 % rows, block = c / 8 / rows;
+        *reinterpret_cast<uint4*>(smem + L::kOffV + block * L::kBox + row * 128 + c % 8 * 16) = make_uint4(0u, 0u, 0u, 0u);
+      }
+      fence_proxy_async_smem();
+    }
     const int64_t share = (a.batch + kThreadsTc - 1) / kThreadsTc;
     const int64_t b_lo = min(a.batch, tid * share), b_hi = min(a.batch, b_lo + share);
     int64_t mine = 0;
@@ -411,8 +420,8 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
     uint64_t* empty = is_v ? vempty : kempty;
     unsigned char* ring = smem + (is_v ? L::kOffV : L::kOffK);
     const int stages = is_v ? L::kVS : L::kKS;
-    const int box_rows = min(a.page_size, kTile);
-    const int boxes = kTile / box_rows;  // pages of a tile: at most 16
+    constexpr int halves = HD / 64;      // 64 dims each; past head_dim the copy fills in zeros
+    const int boxes = a.tile / a.box;    // of a tile: at most 16
     int kt = 0, stage = 0;               // tiles asked for; the next one's ring slot
     uint32_t phase = 1;
     bool ok = true;
@@ -421,7 +430,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
       const int32_t* pages = a.page_table + static_cast<int64_t>(walk.s.seq) * a.max_pages;
       const int total = walk.s.ctx + walk.s.n;
       auto row_of = [&](int t) {  // this lane's box of tile t: its row in the tensor map, -1 bad, -2 none
-        const int slot = t * kTile + lane * box_rows;
+        const int slot = t * a.tile + lane * a.box;
         if (lane >= boxes || slot >= total) return -2;
         const int nth = slot / a.page_size;
         const int32_t page = __ldg(pages + nth);
@@ -439,13 +448,12 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
             bad_ring[kt % kBadRing] = bad;
             if (bad) raise_status(a.status, BM_DEVERR_BAD_PAGE);
           }
-          mbar_expect_tx(&full[stage], __popc(have) * box_rows * 128 * (HD / 64));
+          mbar_expect_tx(&full[stage], __popc(have) * a.box * 128 * halves);
         }
         __syncwarp();
         if (row >= 0) {
-          unsigned char* to = ring + stage * L::kOperand + lane * box_rows * 128;
-#pragma unroll
-          for (int h = 0; h < HD / 64; ++h) tma_load_2d(to + h * L::kBox, map, &full[stage], 64 * h, row);
+          unsigned char* to = ring + stage * L::kOperand + lane * a.box * 128;
+          for (int h = 0; h < halves; ++h) tma_load_2d(to + h * L::kBox, map, &full[stage], 64 * h, row);
         }
         ++kt;
         if (++stage == stages) {
@@ -577,7 +585,6 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
     const uint32_t lane_addr = static_cast<uint32_t>(quarter * 32) << 16;
     const uint32_t s_addr = tmem + lane_addr + w * kTile;
     const uint32_t o_addr = tmem + lane_addr + L::kColO + w * HD;
-    const int box_rows = min(a.page_size, kTile);
     float2* ml = reinterpret_cast<float2*>(smem + L::kOffMl);
     const uint64_t scale2 = pair(a.qscale, a.qscale);
     int x = 0;  // the segment's first unit
@@ -597,7 +604,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
         const int t = walk.t + (DUAL ? (u - x) >> 1 : u - x);  // tile of the item
         warp_wait(&sfull[w], (u >> 1) & 1, abort_flag, a.status);
         tc_fence_after();
-        const int slot0 = t * kTile;
+        const int slot0 = t * a.tile;
         const uint32_t bad = bad_ring[kt % kBadRing];
         if (warp_live) {
           // This copy's scores of the row: at most 64 are held, of 128 the second half is
@@ -608,12 +615,12 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
 #pragma unroll
             for (int c = 0; c < kHeld / 32; ++c) tmem_load32(s_addr + copy * NC + col + 32 * c, v[c]);
             tmem_wait_ld();
-            if (slot0 + kTile > s.ctx || bad != 0) {
+            if (slot0 + a.tile > s.ctx || a.tile < kTile || bad != 0) {
 #pragma unroll
               for (int c = 0; c < kHeld / 32; ++c) {
                 const int at = copy * NC + col + 32 * c;
-                uint32_t see = r < live ? seen32(a, s, token, slot0 + at) : 0u;
-                if (bad) see &= sound32(bad, at / 32, box_rows);
+                uint32_t see = r < live ? seen32(a, s, token, slot0 + at) & low_bits(a.tile - at) : 0u;
+                if (bad) see &= sound32(bad, at / 32, a.box);
 #pragma unroll
                 for (int e = 0; e < 32; ++e) {
                   if (!((see >> e) & 1)) v[c][e] = 0xff800000u;  // -inf: no weight
@@ -692,12 +699,12 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
           l += sums.x + sums.y;
           tmem_wait_st();
         }
-        if (slot0 + kTile > total || bad != 0) {
+        if (slot0 + a.tile > total || bad != 0) {
           // V rows that no copy filled, or stale slots behind the last token: zero
           const int vs = kt % L::kVS;
           warp_wait(&vfull[vs], (kt / L::kVS) & 1, abort_flag, a.status);
           const int vr = quarter * 32 + lane;
-          if (slot0 + vr >= total || ((bad >> (vr / box_rows)) & 1)) {
+          if (slot0 + vr >= total || (vr < a.tile && ((bad >> (vr / a.box)) & 1))) {
             unsigned char* row = smem + L::kOffV + vs * L::kOperand + vr * 128;
 #pragma unroll
             for (int h = 0; h < HD / 64; ++h) {
@@ -717,7 +724,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
       float* slot = slots + (2 * static_cast<int64_t>(cta) + (seg > 0)) * L::kSlotFloats;
       const int end = x + units;
       const int h = r - (r / a.group) * a.group;
-      bf16* out = static_cast<bf16*>(a.out) + ((s.row0 + token) * a.hq + walk.kvh * a.group + h) * HD;
+      bf16* out = static_cast<bf16*>(a.out) + ((s.row0 + token) * a.hq + walk.kvh * a.group + h) * a.hd;
       if constexpr (DUAL) {
         warp_wait(&pvdone[w], ((end - 2 + w) >> 1) & 1, abort_flag, a.status);
         tc_fence_after();
@@ -735,7 +742,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
                   float f[8];
 #pragma unroll
                   for (int d = 0; d < 8; ++d) f[d] = __uint_as_float(v[e + d]) * inv;
-                  st_plain(out + 32 * c + e, pack16<bf16>(f));
+                  if (32 * c + e < a.hd) st_plain(out + 32 * c + e, pack16<bf16>(f));
                 }
               } else {
                 float* dst = slot + (w * kTile + r) * HD + 32 * c;
@@ -809,7 +816,9 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
               float f8[8];
 #pragma unroll
               for (int e = 0; e < 8; ++e) f8[e] = from[e];
-              st_plain(static_cast<bf16*>(a.out) + ((s.row0 + tok) * a.hq + walk.kvh * a.group + head) * HD + d0 + d, pack16<bf16>(f8));
+              if (d0 + d < a.hd) {
+                st_plain(static_cast<bf16*>(a.out) + ((s.row0 + tok) * a.hq + walk.kvh * a.group + head) * a.hd + d0 + d, pack16<bf16>(f8));
+              }
             } else {
               float* to = slot + row * HD + d0 + d;
               *reinterpret_cast<float4*>(to) = *reinterpret_cast<const float4*>(from);
@@ -858,7 +867,9 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
             if (r < live) {
               if (whole) {
 #pragma unroll
-                for (int e = 0; e < 32; e += 8) st_plain(out + col + e, pack16<bf16>(f + e));
+                for (int e = 0; e < 32; e += 8) {
+                  if (col + e < a.hd) st_plain(out + col + e, pack16<bf16>(f + e));
+                }
               } else {
                 float* dst = slot + r * HD + col;
 #pragma unroll
@@ -953,9 +964,10 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(const TreeArgs a, int c
   if (half != 0) return;
   const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
   const int token = i0 + rr / a.group, h = rr - (rr / a.group) * a.group;
-  bf16* out = static_cast<bf16*>(a.out) + ((s.row0 + token) * a.hq + rec.kvh * a.group + h) * HD + d;
+  if (d >= a.hd) return;
+  bf16* out = static_cast<bf16*>(a.out) + ((s.row0 + token) * a.hq + rec.kvh * a.group + h) * a.hd + d;
 #pragma unroll
-  for (int e = 0; e < kDims; e += 4) {
+  for (int e = 0; e < kDims; e += 4) {  // head_dim is a multiple of 8
     *reinterpret_cast<uint2*>(out + e) = make_uint2(pack_bf16x2(o[e] * inv, o[e + 1] * inv),
                                                     pack_bf16x2(o[e + 2] * inv, o[e + 3] * inv));
   }
@@ -970,29 +982,47 @@ int copies_for(int group, int max_tree) {
 int rows_of(int copies) { return copies == kDual ? 2 * kTile : kTile / copies; }
 int tokens_of(int copies, int group) { return copies == kDual ? kTile / group * 2 : kTile / copies / group; }
 
-// CTAs for the bounds: one per SM, no more than the tiles there can be.
+// Slots of a tile and rows of the boxes that fill it: whole pages or equal parts of one,
+// so that a box never crosses a page, at 1024-byte steps of shared memory unless there is
+// one. A tile below half full is left to the CUDA cores.
+bool tile_of(int page_size, int* tile, int* box) {
+  if (page_size <= kTile) {
+    const int n = page_size % 8 == 0 ? kTile / page_size : 1;
+    *box = page_size;
+    *tile = n * page_size;
+  } else {
+    int parts = (page_size + kTile - 1) / kTile;
+    while (page_size % parts != 0) ++parts;  // ends at parts = page_size
+    *box = *tile = page_size / parts;
+  }
+  return *tile >= kTile / 2;
+}
+
+// CTAs for the bounds: one per SM, no more than the tiles there can be (a tile holds at
+// least half of 128 slots).
 int ctas_for(int64_t batch, int hkv, int group, int max_ctx, int max_tree) {
   const int per = tokens_of(copies_for(group, max_tree), group);
-  const int64_t tiles = batch * hkv * ((max_tree + per - 1) / per) * ((static_cast<int64_t>(max_ctx) + max_tree + kTile - 1) / kTile);
+  const int64_t tiles = batch * hkv * ((max_tree + per - 1) / per) *
+                        ((static_cast<int64_t>(max_ctx) + max_tree + kTile / 2 - 1) / (kTile / 2));
   return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(sm_count(), (tiles + kMinTiles - 1) / kMinTiles)));
 }
 
 template <int HD, int COPIES>
-int launch_form(const TreeArgs& a, cudaStream_t stream, const char* what) {
+int launch_form(TreeArgs a, cudaStream_t stream, const char* what) {
   using L = Layout<HD, COPIES>;
+  tile_of(a.page_size, &a.tile, &a.box);
   const int tpt = L::kCopyRows / a.group;
   const uint64_t rows = static_cast<uint64_t>(a.num_pages) * a.hkv * a.page_size;
-  const uint32_t box_rows = static_cast<uint32_t>(std::min(a.page_size, kTile));
   CUtensorMap tq, tk, tv;
-  if (int st = make_tensor_map_bf16(&tk, a.k_pages, HD, rows, 64, box_rows, what)) return st;
-  if (int st = make_tensor_map_bf16(&tv, a.v_pages, HD, rows, 64, box_rows, what)) return st;
-  if (int st = make_tensor_map_3d_bf16(&tq, a.q, HD, a.hq, a.total_q, 64, a.group, tpt, what)) return st;
+  if (int st = make_tensor_map_bf16(&tk, a.k_pages, a.hd, rows, 64, a.box, what)) return st;
+  if (int st = make_tensor_map_bf16(&tv, a.v_pages, a.hd, rows, 64, a.box, what)) return st;
+  if (int st = make_tensor_map_3d_bf16(&tq, a.q, a.hd, a.hq, a.total_q, 64, a.group, tpt, what)) return st;
   auto kernel = tree_tc_kernel<HD, COPIES>;
   if (int st = allow_dynamic_smem(reinterpret_cast<const void*>(kernel), L::kBytes, what)) return st;
   const int nc = ctas_for(a.batch, a.hkv, a.group, a.max_ctx, a.max_tree);
   if (int st = launch_kernel(what, kernel, dim3(nc), dim3(kThreadsTc), L::kBytes, stream, nullptr, tq, tk, tv, a)) return st;
   // items of one tile, and a single CTA, are never cut
-  if (nc == 1 || a.max_ctx + a.max_tree <= kTile) return BM_OK;
+  if (nc == 1 || a.max_ctx + a.max_tree <= a.tile) return BM_OK;
   return launch_kernel(what, tree_merge_kernel<HD, COPIES>, dim3(nc - 1, L::kRows / 8), dim3(256), 0, stream, nullptr, a, nc);
 }
 
@@ -1014,19 +1044,19 @@ int launch_hd(const TreeArgs& a, cudaStream_t stream, const char* what) {
 
 bool tc_takes(const TreeArgs& a, bm_dtype_t dtype) {
   const int64_t rows = static_cast<int64_t>(a.num_pages) * a.hkv * a.page_size;
-  const bool pages = a.page_size >= 8 && (kTile % a.page_size == 0 || a.page_size % kTile == 0);
-  return dtype == BM_BF16 && (a.hd == 64 || a.hd == 128) && pages && rows + kTile < (int64_t{1} << 31);
+  int tile, box;
+  return dtype == BM_BF16 && a.hd <= 128 && tile_of(a.page_size, &tile, &box) && rows + kTile < (int64_t{1} << 31);
 }
 
 size_t tc_workspace_bytes(int64_t batch, int hkv, int hd, int group, int max_ctx, int max_tree) {
-  if (hd != 64 && hd != 128) return 0;
+  if (hd > 128 || hd % 8) return 0;
   const int nc = ctas_for(batch, hkv, group, max_ctx, max_tree);
   const size_t rows = static_cast<size_t>(rows_of(copies_for(group, max_tree)));
-  return records_bytes(nc) + 2 * static_cast<size_t>(nc) * rows * (hd + 2) * sizeof(float);
+  return records_bytes(nc) + 2 * static_cast<size_t>(nc) * rows * ((hd <= 64 ? 64 : 128) + 2) * sizeof(float);
 }
 
 int launch_tc(const TreeArgs& a, cudaStream_t stream, const char* what) {
-  return a.hd == 128 ? launch_hd<128>(a, stream, what) : launch_hd<64>(a, stream, what);
+  return a.hd > 64 ? launch_hd<128>(a, stream, what) : launch_hd<64>(a, stream, what);
 }
 
 }  // namespace paged

@@ -98,6 +98,8 @@ LENS = {
 @pytest.mark.parametrize("dtype,hq,hkv,hd,page", [
     (BF16, 8, 2, 128, 16), (BF16, 4, 4, 128, 64), (BF16, 16, 2, 128, 8), (BF16, 7, 1, 128, 128), (BF16, 8, 1, 64, 32),
     (BF16, 6, 2, 64, 256), (BF16, 4, 2, 128, 24), (BF16, 4, 2, 48, 16), (BF16, 2, 1, 256, 16), (BF16, 24, 2, 128, 512),
+    (BF16, 4, 2, 80, 100), (BF16, 8, 1, 8, 72), (BF16, 3, 1, 120, 200), (BF16, 4, 1, 96, 7), (BF16, 16, 1, 56, 250),
+    (BF16, 32, 1, 112, 24),
     (F32, 6, 6, 48, 16), (F32, 8, 2, 128, 7), (F32, 4, 1, 256, 100), (F32, 2, 2, 4, 1), (F32, 6, 1, 100, 32)])
 @pytest.mark.parametrize("lens", LENS)
 @pytest.mark.parametrize("tree", [True, False])
