@@ -9,7 +9,7 @@ import ctypes
 import os
 import threading
 
-from .build import LIB_PATH
+from .build import BINDING_PATH, LIB_PATH
 
 c_int, c_int32, c_int64, c_float, c_double = (ctypes.c_int, ctypes.c_int32, ctypes.c_int64,
                                               ctypes.c_float, ctypes.c_double)
@@ -174,6 +174,32 @@ def load() -> ctypes.CDLL:
                 fn.argtypes = argtypes
             _lib = lib
         return _lib
+
+
+_serving = None
+
+
+def serving_ops():
+    """The CPython module over the paged-cache serving operators (csrc/binding/); raises if
+    it is missing (no fallback path)."""
+    global _serving
+    if _serving is not None:
+        return _serving
+    load()
+    with _lock:
+        if _serving is None:
+            if not os.path.exists(BINDING_PATH):
+                raise RuntimeError(f"{BINDING_PATH} is missing: build it first (python -m baremetalinferenceengine_b200.build)")
+            import importlib.machinery
+            import importlib.util
+
+            name = __package__ + "._serving_ops"
+            spec = importlib.util.spec_from_file_location(
+                name, BINDING_PATH, loader=importlib.machinery.ExtensionFileLoader(name, BINDING_PATH))
+            module = importlib.util.module_from_spec(spec)
+            spec.loader.exec_module(module)
+            _serving = module
+        return _serving
 
 
 def check(status: int) -> None:

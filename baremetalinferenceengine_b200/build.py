@@ -1,11 +1,13 @@
-"""Compiles the sm_100a layer-op kernels into the in-tree shared library.
+"""Compiles the sm_100a layer-op kernels into the in-tree shared library, and the Python
+module over it.
 
     python -m baremetalinferenceengine_b200.build [--force]
 
 produces ``baremetalinferenceengine_b200/libbm_layer_ops.so`` from ``csrc/*.cu``
 with nvcc (``-gencode arch=compute_100a,code=sm_100a``), static cudart, C++17.
 Objects go to ``_build/`` at the repository root. A source newer than the
-library (or a changed header) triggers a rebuild.
+library (or a changed header) triggers a rebuild. ``_serving_ops.so`` beside it is the
+CPython module of ``csrc/binding/`` (g++ against torch's headers), linked to the library.
 """
 from __future__ import annotations
 
@@ -23,6 +25,8 @@ INCLUDE = os.path.join(REPO_ROOT, "include")
 BUILD_DIR = os.path.join(REPO_ROOT, "_build", "bm_layer_ops")
 LIB_NAME = "libbm_layer_ops.so"
 LIB_PATH = os.path.join(PKG_DIR, LIB_NAME)
+BINDING_SRC = os.path.join(CSRC, "binding", "serving_ops.cpp")
+BINDING_PATH = os.path.join(PKG_DIR, "_serving_ops.so")
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ARCH_FLAGS + [
@@ -67,6 +71,28 @@ def _run(cmd: list[str]) -> None:
         raise RuntimeError("command failed:\n  " + " ".join(cmd) + "\n" + proc.stdout)
 
 
+def _build_binding(force: bool) -> None:
+    """_serving_ops.so: g++ against torch's headers and libraries, and libbm_layer_ops.so
+    (found beside it at run time)."""
+    if not (force or _stale(BINDING_PATH, [BINDING_SRC, os.path.join(INCLUDE, "bm_layer_ops.h")])):
+        return
+    import sysconfig
+
+    import torch
+
+    root = os.path.dirname(torch.__file__)
+    cuda = os.path.dirname(os.path.dirname(nvcc_path()))
+    includes = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
+                os.path.join(cuda, "include"), sysconfig.get_paths()["include"], INCLUDE]
+    tmp = BINDING_PATH + ".tmp"
+    _run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+          f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
+         + [f"-I{i}" for i in includes] + [BINDING_SRC, "-o", tmp, LIB_PATH, f"-L{os.path.join(root, 'lib')}",
+                                           "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda",
+                                           "-Wl,-rpath,$ORIGIN"])
+    os.replace(tmp, BINDING_PATH)
+
+
 def build(force: bool = False, verbose: bool = False) -> str:
     """Builds (if needed) and returns the path of libbm_layer_ops.so."""
     nvcc = nvcc_path()
@@ -88,8 +114,9 @@ def build(force: bool = False, verbose: bool = False) -> str:
                     print(" ".join(j))
     if force or jobs or _stale(LIB_PATH, objs):
         tmp = LIB_PATH + ".tmp"
-        _run([nvcc] + ARCH_FLAGS + ["-shared", "-o", tmp] + objs + ["-lcudart_static", "-lrt", "-ldl", "-lpthread"])
+        _run([nvcc] + ARCH_FLAGS + ["-shared", "-Xlinker", f"-soname={LIB_NAME}", "-o", tmp] + objs + ["-lcudart_static", "-lrt", "-ldl", "-lpthread"])
         os.replace(tmp, LIB_PATH)
+    _build_binding(force)
     return LIB_PATH
 
 

@@ -451,70 +451,18 @@ def _empty(shape, dtype: torch.dtype, device: torch.device, stream) -> torch.Ten
         return torch.empty(shape, dtype=dtype, device=device)
 
 
-def _head_rows(t: torch.Tensor, name: str, dtype: torch.dtype, device: torch.device, hd: int):
-    """(rows, heads, elements between rows) of [rows, heads, hd] with dense heads; rows may
-    be slices of wider ones."""
-    shape = t.shape
-    if len(shape) != 3 or shape[2] != hd or t.dtype != dtype or t.device != device:
-        raise _invalid(f"{name} must be [rows, heads, head_dim] of the other tensors' device, dtype and head_dim")
-    rows, heads, _ = shape
-    if t.is_contiguous():
-        return rows, heads, heads * hd
-    s0, s1, s2 = t.stride()
-    if (hd > 1 and s2 != 1) or (heads > 1 and s1 != hd):
-        raise _invalid(f"{name} must have dense heads")
-    return rows, heads, s0 if rows > 1 else heads * hd
+def _like(t: Optional[torch.Tensor], stream):
+    """Room for an output like `t`, made on the stream that will write it."""
+    return _empty(t.shape, t.dtype, t.device, stream)
 
 
-def _same_device_i32(t: Optional[torch.Tensor], name: str, device: torch.device, numel: Optional[int] = None) -> None:
-    if t is None:
-        return
-    if t.dtype != torch.int32 or not t.is_contiguous() or t.device != device:
-        raise _invalid(f"{name} must be a contiguous int32 tensor on {device}")
-    if numel is not None and t.numel() != numel:
-        raise _invalid(f"{name} must have {numel} entries")
+def _word(status: Optional[DeviceStatus]) -> Optional[torch.Tensor]:
+    return None if status is None else status.word
 
 
-def _table_device(table: Optional[RopeTable], device: torch.device) -> None:
-    if table is not None and table.data.device != device:
-        raise _invalid("the rope table is on another device")
-
-
-class _On:
-    """Makes `device` current for a call, at no cost where it is already."""
-
-    __slots__ = ("device", "guard")
-
-    def __init__(self, device: torch.device):
-        self.device = device
-
-    def __enter__(self):
-        self.guard = None
-        if torch.cuda.current_device() != self.device.index:
-            self.guard = torch.cuda.device(self.device)
-            self.guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
-
-
-# The current stream's handle without a Stream object around it, where torch has that.
-_current_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-
-
-def _raw_stream(device: torch.device, stream: Optional[torch.cuda.Stream]) -> int:
-    if stream is None and _current_raw_stream is not None:
-        return _current_raw_stream(device.index)
-    return _stream(device, stream)
-
-
-def _status_ptr(status: Optional[DeviceStatus], device: torch.device) -> Optional[int]:
-    if status is None:
-        return None
-    if status.word.device != device:
-        raise _invalid("the status word is on another device")
-    return status.ptr
+def _handle(stream: Optional[torch.cuda.Stream]) -> Optional[int]:
+    """A stream's handle; None is the current stream of the tensors' device."""
+    return None if stream is None else stream.cuda_stream
 
 
 def rotary(q: Optional[torch.Tensor], k: Optional[torch.Tensor], positions, table: RopeTable,
@@ -526,44 +474,14 @@ def rotary(q: Optional[torch.Tensor], k: Optional[torch.Tensor], positions, tabl
     or (2i, 2i + 1) with ``interleaved``. q and k may be slices of a fused projection's
     rows. ``positions``: int32 tensor, or an int pos0 (row r at pos0 + r). A position
     outside the table leaves its row unwritten and sets BAD_POSITION."""
-    ref = q if q is not None else k
-    if ref is None:
-        raise _invalid("neither q nor k given")
-    if ref.dim() != 3:
-        raise _invalid("q and k must be [rows, heads, head_dim]")
-    dev, dtype, hd = _dev(ref), ref.dtype, ref.shape[2]
-    code = bm_dtype(ref)
-    rows = hq = hkv = qs = ks = qos = kos = 0
-    qp = kp = qop = kop = None
-    if q is not None:
-        rows, hq, qs = _head_rows(q, "q", dtype, dev, hd)
-        if q_out is None:
-            q_out = _empty(q.shape, dtype, dev, stream)
-        out_rows, out_heads, qos = _head_rows(q_out, "q_out", dtype, dev, hd)
-        if out_rows != rows or out_heads != hq:
-            raise _invalid("q_out must have q's shape")
-        qp, qop = q.data_ptr(), q_out.data_ptr()
-    elif q_out is not None:
-        raise _invalid("q_out without q")
-    if k is not None:
-        k_rows, hkv, ks = _head_rows(k, "k", dtype, dev, hd)
-        if k_out is None:
-            k_out = _empty(k.shape, dtype, dev, stream)
-        out_rows, out_heads, kos = _head_rows(k_out, "k_out", dtype, dev, hd)
-        if out_rows != k_rows or out_heads != hkv or (q is not None and k_rows != rows):
-            raise _invalid("k must have q's rows, and k_out k's shape")
-        rows = k_rows
-        kp, kop = k.data_ptr(), k_out.data_ptr()
-    elif k_out is not None:
-        raise _invalid("k_out without k")
-    pos_t, pos0 = (None, positions) if isinstance(positions, int) else (positions, 0)
-    _same_device_i32(pos_t, "positions", dev, rows)
-    _table_device(table, dev)
-    with _On(dev):
-        check(load().bm_rotary(qop, kop, qp, kp, None if pos_t is None else pos_t.data_ptr(), pos0, table.ptr,
-                               table.max_pos, table.head_dim, int(interleaved), rows, hq, hkv, hd, qs, ks, qos, kos, code,
-                               _status_ptr(status, dev), _raw_stream(dev, stream)))
-    return q_out, k_out
+    if table is None:
+        raise _invalid("rotary needs a table")
+    if stream is not None:
+        q_out = _like(q, stream) if q is not None and q_out is None else q_out
+        k_out = _like(k, stream) if k is not None and k_out is None else k_out
+    pos, pos0 = (None, positions) if isinstance(positions, int) else (positions, 0)
+    return _lib.serving_ops().rotary(q, k, pos, pos0, table.data, table.max_pos, table.head_dim, interleaved, q_out, k_out,
+                                     _word(status), _handle(stream))
 
 
 class PagedKV:
@@ -578,17 +496,19 @@ class PagedKV:
             raise _invalid("k_pages and v_pages must be [num_pages, kv_heads, page_size, head_dim]")
         _dense(k_pages, "k_pages")
         _dense(v_pages, "v_pages")
+        bm_dtype(k_pages)
         _same(k_pages, v_pages)
         if page_table.dim() != 2:
             raise _invalid("page_table must be [num_seqs, max_pages]")
-        _same_device_i32(page_table, "page_table", _dev(k_pages))
+        if page_table.dtype != torch.int32 or not page_table.is_contiguous() or page_table.device != _dev(k_pages):
+            raise _invalid("page_table must be a contiguous int32 tensor on the pages' device")
         self.k_pages, self.v_pages, self.page_table = k_pages, v_pages, page_table
         self.num_pages, self.num_kv_heads, self.page_size, self.head_dim = k_pages.shape
         self.num_seqs, self.max_pages = page_table.shape
         self.device, self.dtype = k_pages.device, k_pages.dtype
         self.c = _lib.PagedKVC(k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr(), self.num_pages,
                                self.page_size, self.max_pages, self.num_seqs, self.num_kv_heads, self.head_dim)
-        self.ref, self.code = ctypes.byref(self.c), bm_dtype(k_pages)
+        self.address = ctypes.addressof(self.c)
 
 
 def paged_kv_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, positions: Optional[torch.Tensor],
@@ -601,42 +521,14 @@ def paged_kv_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor,
     ``seq_ids[r]`` (0 without) and returns q [rows, Hq, hd] rotated (``q_out``, made when
     not given; ``q_out=q`` in place; None without q). Without a table nothing is
     rotated."""
-    if k.dim() != 3:
-        raise _invalid("k and v must be [rows, kv_heads, head_dim]")
-    dev, dtype, hd = _dev(k), k.dtype, cache.head_dim
-    if cache.dtype != dtype or cache.device != dev:
-        raise _invalid("the cache has another dtype or device")
-    rows, hkv, ks = _head_rows(k, "k", dtype, dev, hd)
-    v_rows, v_heads, vs = _head_rows(v, "v", dtype, dev, hd)
-    if hkv != cache.num_kv_heads or v_rows != rows or v_heads != hkv:
-        raise _invalid("k and v do not match the cache or each other")
-    hq = qs = qos = 0
-    qp = qop = None
-    if q is not None:
-        q_rows, hq, qs = _head_rows(q, "q", dtype, dev, hd)
-        if q_out is None:
-            q_out = _empty(q.shape, dtype, dev, stream)
-        out_rows, out_heads, qos = _head_rows(q_out, "q_out", dtype, dev, hd)
-        if q_rows != rows or out_rows != rows or out_heads != hq:
-            raise _invalid("q must have k's rows, and q_out q's shape")
-        qp, qop = q.data_ptr(), q_out.data_ptr()
-    elif q_out is not None:
-        raise _invalid("q_out without q")
-    _same_device_i32(positions, "positions", dev, rows)
-    _same_device_i32(seq_ids, "seq_ids", dev, rows)
-    _same_device_i32(slots, "slots", dev, rows)
-    tp, tn, rd = None, 0, 0
-    if table is not None:
-        _table_device(table, dev)
-        tp, tn, rd = table.ptr, table.max_pos, table.head_dim
-    with _On(dev):
-        check(load().bm_paged_kv_append(qop, qp, k.data_ptr(), v.data_ptr(),
-                                        None if positions is None else positions.data_ptr(),
-                                        None if slots is None else slots.data_ptr(),
-                                        None if seq_ids is None else seq_ids.data_ptr(), cache.ref, tp, tn, rd,
-                                        int(interleaved), rows, hq, qs, ks, vs, qos, cache.code,
-                                        _status_ptr(status, dev), _raw_stream(dev, stream)))
-    return q_out
+    if stream is not None and q is not None and q_out is None:
+        q_out = _like(q, stream)
+    if table is None:
+        tdata, max_pos, rotary_dim = None, 0, 0
+    else:
+        tdata, max_pos, rotary_dim = table.data, table.max_pos, table.head_dim
+    return _lib.serving_ops().paged_kv_append(q, k, v, positions, slots, seq_ids, cache.address, cache.k_pages, tdata, max_pos,
+                                              rotary_dim, interleaved, q_out, _word(status), _handle(stream))
 
 
 def paged_tree_attention_workspace(q: torch.Tensor, cache: PagedKV, batch: int, max_ctx: int, max_tree: int,
@@ -645,6 +537,7 @@ def paged_tree_attention_workspace(q: torch.Tensor, cache: PagedKV, batch: int, 
     bounds). Calls that overlap on the GPU need one each."""
     if q.dim() != 3:
         raise _invalid("q must be [rows, heads, head_dim]")
+    _dev(q)
     n = ctypes.c_size_t()
     with torch.cuda.device(cache.device):
         check(load().bm_paged_tree_attention_workspace_size(q.shape[0], batch, q.shape[1], cache.num_kv_heads,
@@ -666,37 +559,12 @@ def paged_tree_attention(q: torch.Tensor, cache: PagedKV, ctx_lens: torch.Tensor
     max_ctx and max_tree bound ctx_lens and a sequence's rows. Rows outside every
     sequence are left as they were in ``out``. ``workspace``:
     paged_tree_attention_workspace's, made for the call when None."""
-    dev = _dev(q)
-    if q.dim() != 3 or not q.is_contiguous() or q.shape[2] != cache.head_dim:
-        raise _invalid("q must be contiguous [rows, heads, head_dim] with the cache's head_dim")
-    if cache.dtype != q.dtype or cache.device != dev:
-        raise _invalid("the cache has another dtype or device")
-    batch = ctx_lens.numel()
-    _same_device_i32(ctx_lens, "ctx_lens", dev)
-    _same_device_i32(q_starts, "q_starts", dev, batch + 1)
-    _same_device_i32(seq_ids, "seq_ids", dev, batch)
-    words = 0
-    if tree_mask is not None:
-        if (tree_mask.dtype != torch.int64 or tree_mask.dim() != 2 or tree_mask.shape[0] != q.shape[0]
-                or not tree_mask.is_contiguous() or tree_mask.device != dev):
-            raise _invalid("tree_mask must be contiguous int64 [rows, words] on q's device")
-        words = tree_mask.shape[1]
-    if out is None:
-        out = _empty(q.shape, q.dtype, dev, stream)
-    if out.shape != q.shape or out.dtype != q.dtype or out.device != dev or not out.is_contiguous():
-        raise _invalid("out must be contiguous and like q")
     if workspace is None:
-        workspace = paged_tree_attention_workspace(q, cache, batch, max_ctx, max_tree, stream)
-    if workspace.device != dev or not workspace.is_contiguous():
-        raise _invalid("workspace must be contiguous on q's device")
-    with _On(dev):
-        check(load().bm_paged_tree_attention(out.data_ptr(), q.data_ptr(), cache.ref,
-                                             None if seq_ids is None else seq_ids.data_ptr(), ctx_lens.data_ptr(),
-                                             q_starts.data_ptr(), None if tree_mask is None else tree_mask.data_ptr(),
-                                             words, q.shape[0], batch, q.shape[1], max_ctx, max_tree, scale,
-                                             workspace.data_ptr(), workspace.numel() * workspace.element_size(), cache.code,
-                                             _status_ptr(status, dev), _raw_stream(dev, stream)))
-    return out
+        workspace = paged_tree_attention_workspace(q, cache, ctx_lens.numel(), max_ctx, max_tree, stream)
+    if stream is not None and out is None:
+        out = _like(q, stream)
+    return _lib.serving_ops().paged_tree_attention(q, cache.address, cache.k_pages, ctx_lens, q_starts, max_ctx, max_tree,
+                                                   tree_mask, seq_ids, scale, out, workspace, _word(status), _handle(stream))
 
 
 def sample(logits: torch.Tensor, uniforms: torch.Tensor, temperature: Optional[torch.Tensor] = None,
@@ -708,29 +576,9 @@ def sample(logits: torch.Tensor, uniforms: torch.Tensor, temperature: Optional[t
     off), then the first index whose running weight exceeds its uniform's share. Ties
     go to the lowest index; temperature 0 takes the largest logit; a row without any
     weight gives -1. Returns int32 [rows]."""
-    dev = _dev(logits)
-    if logits.dim() != 2 or logits.shape[1] == 0 or (logits.shape[1] > 1 and logits.stride(1) != 1):
-        raise _invalid("logits must be [rows, vocab] with unit inner stride")
-    rows, vocab = logits.shape
-    ptrs = []
-    for name, t in (("uniforms", uniforms), ("temperature", temperature), ("top_k", top_k), ("top_p", top_p),
-                    ("min_p", min_p)):
-        if t is None:
-            ptrs.append(None)
-            continue
-        want = torch.int32 if name == "top_k" else torch.float32
-        if t.dtype != want or t.numel() != rows or not t.is_contiguous() or t.device != dev:
-            raise _invalid(f"{name} must be a contiguous {want} tensor of one entry per row on the logits' device")
-        ptrs.append(t.data_ptr())
-    if out is None:
-        out = _empty((rows,), torch.int32, dev, stream)
-    else:
-        _same_device_i32(out, "out", dev, rows)
-    with _On(dev):
-        check(load().bm_sample(out.data_ptr(), logits.data_ptr(), *ptrs, rows, vocab,
-                               logits.stride(0) if rows > 1 else vocab, bm_dtype(logits), _status_ptr(status, dev),
-                               _raw_stream(dev, stream)))
-    return out
+    if stream is not None and out is None:
+        out = _empty((logits.shape[0],), torch.int32, _dev(logits), stream)
+    return _lib.serving_ops().sample(logits, uniforms, temperature, top_k, top_p, min_p, out, _word(status), _handle(stream))
 
 
 # --------------------------------------------------------------------------
