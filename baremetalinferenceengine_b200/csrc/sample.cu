@@ -134,10 +134,10 @@ struct Shared {
   u64 best[kMaxCluster];   // per CTA of the cluster: key << 32 | ~index
   u64 sum[kMaxCluster], above[kMaxCluster];
   u64 warp[kWarps], sub[kWarps];
-  u64 before;              // value above the bin found
+  u64 before, through;     // value above the bin found, and up to its end
   u64 ties;                // how many logits equal to t stay
   u64 cand_weight[kList];  // the leader's: collected logits
-  uint32_t cand_key[kList];
+  uint32_t cand_key[kList], cand_index[kList];
   uint32_t list_key[kList], list_index[kList];  // this CTA's share of them
   uint32_t own_count, offset;
   uint32_t count, key_min, key_max;             // the leader's: logits of the border's bins
@@ -227,6 +227,121 @@ __device__ __forceinline__ void each(const T* x, int lo, int hi, bool vec, bool 
     }
   }
   if (whole + lane < hi) f(whole + lane, remapped(load1(x + whole + lane), remap));  // fewer than VEC are left
+}
+
+// The border among the block's elements, kEach a thread, taken by descending field: the
+// field of the first whose running value (equal fields together) reaches the target, and
+// in *before the value above it. 512 equal parts of the fields' range a round. All values
+// together reach the target.
+constexpr int kEach = kList / kThreads;
+__device__ uint32_t border(Shared& sh, const uint32_t (&field)[kEach], const u64 (&value)[kEach], u64 target, u64* before) {
+  const int tid = threadIdx.x;
+  u64 passed = 0;
+  uint32_t from = 0, to = 0xffffffffu;
+  for (int round = 0; round < 5; ++round) {
+    __syncthreads();
+    if (tid == 0) {
+      sh.key_min = 0xffffffffu;
+      sh.key_max = 0;
+    }
+    sh.split[tid] = 0;
+    __syncthreads();
+    uint32_t mn = 0xffffffffu, mx = 0;
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+      if (value[e] != 0 && field[e] >= from && field[e] <= to) {
+        mn = min(mn, field[e]);
+        mx = max(mx, field[e]);
+      }
+    }
+    mn = __reduce_min_sync(0xffffffffu, mn);
+    mx = __reduce_max_sync(0xffffffffu, mx);
+    if ((tid & 31) == 0) {
+      atomicMin(&sh.key_min, mn);
+      atomicMax(&sh.key_max, mx);
+    }
+    __syncthreads();
+    from = sh.key_min;
+    to = sh.key_max;
+    if (from >= to) break;
+    const int shift = max(0, 32 - __clz(to - from) - 9);
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+      if (value[e] != 0 && field[e] >= from && field[e] <= to) atomicAdd(&sh.split[(to - field[e]) >> shift], value[e]);
+    }
+    __syncthreads();
+    const u64 v = sh.split[tid];
+    u64 total;
+    const u64 at = block_scan64(v, sh.sub, &total) + passed;
+    if (at < target && target <= at + v) {
+      sh.bin = tid;
+      sh.before = at;
+    }
+    __syncthreads();
+    passed = sh.before;
+    to -= sh.bin << shift;
+    from = max(from, shift == 0 ? to : to - ((1u << shift) - 1));
+  }
+  *before = passed;
+  return to;
+}
+
+// The rest of a row whose top-k logits are in the leader's list (some more may be).
+__device__ __noinline__ void finish_alone(Shared& sh, const SampleArgs& a, const Weigher& weigh, int k, float p, float u,
+                                          int64_t row) {
+  const int tid = threadIdx.x;
+  const uint32_t n = sh.count;
+  uint32_t key[kEach], later[kEach];  // later: descends as the index rises
+  u64 one[kEach], weight[kEach], before, all;
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) {
+    const uint32_t i = tid + e * kThreads;
+    key[e] = i < n ? sh.cand_key[i] : 0;
+    later[e] = i < n ? ~sh.cand_index[i] : 0;
+    one[e] = i < n;
+    weight[e] = i < n ? weigh(logit_of(key[e])) : 0;
+  }
+  // top-k, then top-p: a key, how many of those equal to it stay, and (if not all) the last
+  for (int stage = 0; stage < 2; ++stage) {
+    if (stage == 1 && !(p < 1.f)) break;
+    u64 target = k;
+    if (stage == 1) {
+      u64 mine = 0;
+#pragma unroll
+      for (int e = 0; e < kEach; ++e) mine += weight[e];
+      block_scan64(mine, sh.sub, &all);
+      bool fraction;
+      target = portion(fmaxf(p, 0.f), all, &fraction);
+      if (fraction || target == 0) ++target;
+    }
+    const uint32_t t = border(sh, key, stage == 0 ? one : weight, target, &before);
+    u64 tie[kEach], equal = 0;
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+      tie[e] = one[e] != 0 && key[e] == t;
+      equal += tie[e];
+    }
+    block_scan64(equal, sh.sub, &all);
+    const u64 w = stage == 0 ? 1 : max(weigh(logit_of(t)), static_cast<u64>(1));
+    const u64 rest = (target - before + w - 1) / w;
+    uint32_t last = 0;  // of the `later` order: those below it go
+    if (rest < all) last = border(sh, later, tie, rest, &before);
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+      if (key[e] < t || (key[e] == t && later[e] < last)) one[e] = weight[e] = 0;
+    }
+  }
+  u64 mine = 0;
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) {
+    if (weight[e] != 0 && weigh.real(logit_of(key[e])) < weigh.least) weight[e] = 0;  // min-p
+    mine += weight[e];
+  }
+  block_scan64(mine, sh.sub, &all);
+  bool fraction;
+  const u64 want = portion(u, all, &fraction);
+  const uint32_t token = ~border(sh, later, weight, want + 1, &before);
+  if (tid == 0) a.tokens[row] = static_cast<int32_t>(token);
 }
 
 template <typename T>
@@ -396,7 +511,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
       for (int side = 0; side < 2; ++side) {
         const u64 target = side == 0 ? least_target : most_target;
         int bin = kBins - 1;
-        u64 at = 0;
+        u64 at = 0, through = 0;
         const uint32_t hit = __ballot_sync(0xffffffffu, target <= coarse_incl);
         if (hit != 0) {
           const int l = __ffs(hit) - 1;
@@ -415,13 +530,16 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
           const u64 incl = at + scan(f0 + f1);
           const int fl = __ffs(__ballot_sync(0xffffffffu, target <= incl)) - 1;
           const u64 fine = __shfl_sync(0xffffffffu, incl - f0 - f1, fl), f = __shfl_sync(0xffffffffu, f0, fl);
-          bin = group * 64 + 2 * fl + (target > fine + f);
-          at = fine + (target > fine + f ? f : 0);
+          const bool second = target > fine + f;
+          bin = group * 64 + 2 * fl + second;
+          at = fine + (second ? f : 0);
+          through = second ? __shfl_sync(0xffffffffu, incl, fl) : fine + f;
         }
         if (lane == 0) {
           if (side == 0) {
             sh.bin_lo = bin;
             sh.before = at;
+            sh.through = through;
           } else {
             sh.bin_hi = bin;
           }
@@ -445,7 +563,14 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
         sh.list_index[n] = static_cast<uint32_t>(i);
       }
     };
-    if (stage == 0) {
+    // All of a small top-k's logits, and those that share its last bin, fit the list: the
+    // leader goes on alone.
+    const bool alone = stage == 0 && sh.through <= kList;
+    if (alone) {
+      each<1>(x, lo, hi, a.vec, remap, [&](int i, float lv) {
+        if (bin_of(lv) <= bin_hi && i < hi) collect(i, lv);
+      });
+    } else if (stage == 0) {
       each<1>(x, lo, hi, a.vec, remap, [&](int i, float lv) {
         const int b = bin_of(lv);
         if (b > bin_hi) return;
@@ -499,7 +624,11 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
         const uint32_t at = sh.offset + i, key = sh.list_key[i];
         if (at < kList) {
           peer(0)->cand_key[at] = key;
-          peer(0)->cand_weight[at] = value(key);
+          if (alone) {
+            peer(0)->cand_index[at] = sh.list_index[i];
+          } else {
+            peer(0)->cand_weight[at] = value(key);
+          }
         }
       }
     };
@@ -514,6 +643,10 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
       peer(tid)->above[rank] = b;
     }
     cluster.sync();
+    if (alone) {
+      if (rank == 0) finish_alone(sh, a, weigh, k, p, u, row);
+      return;  // nobody reads another CTA's shared memory any more
+    }
     u64 target = k, passed = stage == 0 ? sh.before : 0;
     if (stage == 1) {
       u64 s = tied;
@@ -742,9 +875,10 @@ extern "C" int bm_sample(int32_t* tokens, const void* logits, const float* unifo
   a.bits = std::min(51, 62 - log2_up);  // an fp64 weight is made whole below 2^52
   a.vec = aligned16(logits) && row_stride * es % 16 == 0;
   a.status = d_status;
-  // CTAs per row: enough to fill two per SM, none with fewer than 2048 logits.
+  // CTAs per row: as many as keep all rows resident at once, two CTAs to an SM, none with
+  // fewer than 2048 logits. 64 rows of 128256 logits: 84, 71 and 91 us with 2, 4 and 8.
   int c = 1;
-  while (c < kMaxCluster && rows * c < 2 * sm_count() && vocab > int64_t{2048} * c) c *= 2;
+  while (c < kMaxCluster && rows * c * 2 <= 2 * sm_count() && vocab >= int64_t{2048} * c * 2) c *= 2;
   a.chunk = static_cast<int>(((vocab + c - 1) / c + 7) / 8 * 8);
   a.unit = 16;
   while ((static_cast<int64_t>(a.chunk) << a.unit) >= int64_t{1} << 32) --a.unit;
