@@ -18,7 +18,9 @@
 // much, and one or few rows are bound by the chain of passes. A cluster of up to 8 CTAs
 // shares a row:
 //   1. the largest logit and its first index;
-//   2. for top-k, then for top-p: a histogram over 4096 bins of equal ratio of weight, in
+//   2. for a small top-k: the logits that reach the k-th largest of the maxima of 512 or
+//      1024 parts of the row, which one CTA then finishes alone. For others, first top-k,
+//      then top-p: a histogram over 4096 bins of equal ratio of weight, in
 //      32-bit counts (top-k) or fixed-point fp32 weights (top-p; shared-memory atomics
 //      on 64 bits are many times slower). Each CTA adds up a slice of the bins over the
 //      cluster. The bins that can hold the border are one or, with the fp32 weights'
@@ -344,8 +346,9 @@ __device__ __noinline__ void finish_alone(Shared& sh, const SampleArgs& a, const
   if (tid == 0) a.tokens[row] = static_cast<int32_t>(token);
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a) {
+// RESIDENT: CTAs per SM that the registers are cut for.
+template <typename T, int RESIDENT>
+__global__ void __launch_bounds__(kThreads, RESIDENT) sample_kernel(const SampleArgs a) {
   grid_dependency_wait();
   extern __shared__ __align__(16) unsigned char smem[];
   Shared& sh = *reinterpret_cast<Shared*>(smem);
@@ -373,6 +376,12 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
   const int span = ((c_hi - c_lo + kWarps - 1) / kWarps + VEC - 1) / VEC * VEC;
   const int lo = min(c_hi, c_lo + warp * span), hi = min(c_hi, lo + span);
 
+  // A small top-k: the k-th largest of the maxima of `groups` parts of the row is a bound
+  // that k logits reach, and few more where k is small beside the groups.
+  const int share = max(1, C / 2);                   // threads of a group
+  const int groups = C * (kThreads / share);         // 512 or 1024
+  const bool bounded = k > 0 && k < a.vocab && 2 * k <= groups && temp > 0.f;
+
   // ---------------- the largest logit ----------------
   {
     float m = -INFINITY;
@@ -386,6 +395,12 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
       });
     } else {
       each<4>(x, lo, hi, a.vec, false, [&](int, float v) { m = fmaxf(m, v); });
+      if (bounded) {
+        float g = m;
+        if (share > 1) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, 1));
+        if (share > 2) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, 2));
+        if (tid % share == 0) peer(0)->cand_key[(rank * kThreads + tid) / share] = key_of(g);
+      }
     }
     u64 best = static_cast<u64>(key_of(m)) << 32 | static_cast<uint32_t>(~at);
 #pragma unroll
@@ -427,6 +442,79 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
   bool summed = false;    // kept: the weights of what stays by warp's stretch
   u64 kept = 0;
 
+  // Logits set aside on the way, in no order, with the range of their keys.
+  uint32_t from = 0xffffffffu, to = 0;
+  auto collect = [&](int i, float lv) {
+    const uint32_t key = key_of(lv);
+    from = min(from, key);
+    to = max(to, key);
+    const uint32_t n = atomicAdd(&sh.own_count, 1u);
+    if (n < kList) {
+      sh.list_key[n] = key;
+      sh.list_index[n] = static_cast<uint32_t>(i);
+    }
+  };
+  // This CTA's go behind the others' in the leader's list: put(place, key, index).
+  auto hand_over = [&](auto put) {
+    from = __reduce_min_sync(0xffffffffu, from);
+    to = __reduce_max_sync(0xffffffffu, to);
+    if (lane == 0 && to != 0) {
+      atomicMin(&peer(0)->key_min, from);
+      atomicMax(&peer(0)->key_max, to);
+    }
+    __syncthreads();
+    const uint32_t own = sh.own_count;
+    if (tid == 0 && own != 0) sh.offset = atomicAdd(&peer(0)->count, own);
+    __syncthreads();
+    for (uint32_t i = tid; i < min(own, static_cast<uint32_t>(kList)); i += kThreads) {
+      const uint32_t at = sh.offset + i;
+      if (at < kList) put(at, sh.list_key[i], sh.list_index[i]);
+    }
+  };
+  auto clear_lists = [&]() {
+    if (tid == 0) {
+      sh.own_count = 0;
+      sh.count = 0;
+      sh.key_min = 0xffffffffu;
+      sh.key_max = 0;
+    }
+  };
+  auto put_index = [&](uint32_t at, uint32_t key, uint32_t index) {
+    peer(0)->cand_key[at] = key;
+    peer(0)->cand_index[at] = index;
+  };
+
+  if (bounded && !remap) {
+    if (rank == 0) {
+      uint32_t key[kEach];
+      u64 one[kEach], before;
+#pragma unroll
+      for (int e = 0; e < kEach; ++e) {
+        one[e] = tid + e * kThreads < groups;
+        key[e] = one[e] != 0 ? sh.cand_key[tid + e * kThreads] : 0;
+      }
+      const uint32_t bound = border(sh, key, one, k, &before);
+      if (tid < C) peer(tid)->key = bound;
+      __syncthreads();
+    }
+    clear_lists();
+    cluster.sync();
+    const float bound = logit_of(sh.key);
+    if (bound > -INFINITY) {
+      each<1>(x, lo, hi, a.vec, false, [&](int i, float v) {
+        if (v >= bound) collect(i, v);
+      });
+      hand_over(put_index);
+      cluster.sync();
+      if (peer(0)->count <= kList) {
+        cluster.sync();  // the count has been read: a CTA's shared memory outlives its readers
+        if (rank == 0) finish_alone(sh, a, weigh, k, p, u, row);
+        return;
+      }
+      cluster.sync();
+    }
+  }
+
   // ---------------- t for top-k (stage 0) and top-p (stage 1) ----------------
   const bool has_min_p = mp > 0.f;
   for (int stage = 0; stage < 2; ++stage) {
@@ -439,12 +527,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
       return b < Weigher::kLimit ? bits_of(b + kMagic) : kBins - 1;
     };
     for (int b = tid; b < kBins / 4; b += kThreads) reinterpret_cast<uint4*>(sh.hist)[b] = make_uint4(0u, 0u, 0u, 0u);
-    if (tid == 0) {
-      sh.own_count = 0;
-      sh.count = 0;
-      sh.key_min = 0xffffffffu;
-      sh.key_max = 0;
-    }
+    clear_lists();
     __syncthreads();
     if (stage == 0) {
       each<1>(x, lo, hi, a.vec, remap, [&](int, float v) { atomicAdd(&sh.hist[bin_of(v)], 1u); });
@@ -551,18 +634,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
     // Exact weights: of the row, of what is above these bins, and of that what min_p keeps;
     // and the bins' logits.
     u64 own_sum = 0, own_above = 0;
-    uint32_t from = 0xffffffffu, to = 0;  // keys
+    from = 0xffffffffu;
+    to = 0;
     kept = 0;
-    auto collect = [&](int i, float lv) {
-      const uint32_t key = key_of(lv);
-      from = min(from, key);
-      to = max(to, key);
-      const uint32_t n = atomicAdd(&sh.own_count, 1u);
-      if (n < kList) {
-        sh.list_key[n] = key;
-        sh.list_index[n] = static_cast<uint32_t>(i);
-      }
-    };
     // All of a small top-k's logits, and those that share its last bin, fit the list: the
     // leader goes on alone.
     const bool alone = stage == 0 && sh.through <= kList;
@@ -604,35 +678,16 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
         sh.sub[warp] = own_above;
       }
     }
-    // This CTA's collected logits go behind the others' in the leader's list.
     auto value = [&](uint32_t key) -> u64 { return stage == 0 ? 1 : key == t0 ? 0 : weigh(logit_of(key)); };
-    auto hand_over = [&]() {
-#pragma unroll
-      for (int off = 16; off > 0; off >>= 1) {
-        from = min(from, __shfl_xor_sync(0xffffffffu, from, off));
-        to = max(to, __shfl_xor_sync(0xffffffffu, to, off));
-      }
-      if (lane == 0 && to != 0) {
-        atomicMin(&peer(0)->key_min, from);
-        atomicMax(&peer(0)->key_max, to);
-      }
-      __syncthreads();
-      const uint32_t own = sh.own_count;
-      if (tid == 0 && own != 0) sh.offset = atomicAdd(&peer(0)->count, own);
-      __syncthreads();
-      for (uint32_t i = tid; i < min(own, static_cast<uint32_t>(kList)); i += kThreads) {
-        const uint32_t at = sh.offset + i, key = sh.list_key[i];
-        if (at < kList) {
-          peer(0)->cand_key[at] = key;
-          if (alone) {
-            peer(0)->cand_index[at] = sh.list_index[i];
-          } else {
-            peer(0)->cand_weight[at] = value(key);
-          }
-        }
-      }
+    auto put_weight = [&](uint32_t at, uint32_t key, uint32_t) {
+      peer(0)->cand_key[at] = key;
+      peer(0)->cand_weight[at] = value(key);
     };
-    hand_over();
+    if (alone) {
+      hand_over(put_index);
+    } else {
+      hand_over(put_weight);
+    }
     if (stage == 1 && tid < C) {
       u64 s = 0, b = 0;
       for (int w = 0; w < kWarps; ++w) {
@@ -713,7 +768,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
           const uint32_t key = key_of(lv);
           if (key >= old_from && key <= old_to && (old_to - key) >> shift == bin) collect(i, lv);
         });
-        hand_over();
+        hand_over(put_weight);
         cluster.sync();
         count = peer(0)->count;
         from = peer(0)->key_min;
@@ -875,10 +930,13 @@ extern "C" int bm_sample(int32_t* tokens, const void* logits, const float* unifo
   a.bits = std::min(51, 62 - log2_up);  // an fp64 weight is made whole below 2^52
   a.vec = aligned16(logits) && row_stride * es % 16 == 0;
   a.status = d_status;
-  // CTAs per row: as many as keep all rows resident at once, two CTAs to an SM, none with
-  // fewer than 2048 logits. 64 rows of 128256 logits: 84, 71 and 91 us with 2, 4 and 8.
+  // CTAs per row: as many as leave every SM at most one, with all the registers they like;
+  // twice as many, at half the registers, where a CTA had more than 16384 logits (64 rows
+  // of 128256: 53 against 64 us; 32 rows of 32000: 31 against 27). None with fewer than 2048.
   int c = 1;
-  while (c < kMaxCluster && rows * c * 2 <= 2 * sm_count() && vocab >= int64_t{2048} * c * 2) c *= 2;
+  while (c < kMaxCluster && rows * c * 2 <= sm_count() && vocab >= int64_t{2048} * c * 2) c *= 2;
+  if (c < kMaxCluster && rows * c * 2 <= 2 * sm_count() && vocab > int64_t{16384} * c) c *= 2;
+  const bool crowded = rows * c > sm_count();
   a.chunk = static_cast<int>(((vocab + c - 1) / c + 7) / 8 * 8);
   a.unit = 16;
   while ((static_cast<int64_t>(a.chunk) << a.unit) >= int64_t{1} << 32) --a.unit;
@@ -892,5 +950,6 @@ extern "C" int bm_sample(int32_t* tokens, const void* logits, const float* unifo
     if (int st = allow_dynamic_smem(reinterpret_cast<const void*>(kernel), sizeof(Shared), what)) return st;
     return launch_kernel(what, kernel, grid, dim3(kThreads), sizeof(Shared), as_stream(stream), &attr, a);
   };
-  return dtype == BM_F32 ? go(sample_kernel<float>) : go(sample_kernel<bf16>);
+  if (dtype == BM_F32) return crowded ? go(sample_kernel<float, 2>) : go(sample_kernel<float, 1>);
+  return crowded ? go(sample_kernel<bf16, 2>) : go(sample_kernel<bf16, 1>);
 }
