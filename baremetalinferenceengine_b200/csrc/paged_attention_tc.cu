@@ -619,8 +619,9 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
 #pragma unroll
               for (int c = 0; c < kHeld / 32; ++c) {
                 const int at = copy * NC + col + 32 * c;
-                uint32_t see = r < live ? seen32(a, s, token, slot0 + at) & low_bits(a.tile - at) : 0u;
+                uint32_t see = r < live ? seen32(a, s, token, slot0 + at) & low_bits(a.tile - at) : 0xffffffffu;
                 if (bad) see &= sound32(bad, at / 32, a.box);
+                if (__all_sync(0xffffffffu, see == 0xffffffffu)) continue;  // a prompt's chunks are mostly seen
 #pragma unroll
                 for (int e = 0; e < 32; ++e) {
                   if (!((see >> e) & 1)) v[c][e] = 0xff800000u;  // -inf: no weight
@@ -898,7 +899,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
 }
 
 // Adds up the partials of the item that CTA k's first tile continues: block (k, rows
-// 8 y .. 8 y + 7) by the first border inside the item. A warp takes a row, its halves
+// 8 y .. 8 y + 7, and so on) by the first border inside the item. A warp takes a row, its halves
 // every other part: an item of few rows and many parts is bound by the latency of the
 // parts' loads, so many are in flight over many SMs.
 template <int HD, int COPIES>
@@ -918,58 +919,59 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(const TreeArgs a, int c
   const int tpt = L::kCopyRows / a.group;
   constexpr int kLanes = 16;  // threads of a part's row
   const int lane = threadIdx.x & 31;
-  const int r = static_cast<int>(blockIdx.y) * 8 + threadIdx.x / 32;
-  const int tile = r / kTile, rr = r - tile * kTile;
-  const int i0 = rec.p * tpt * L::kTiles + tile * tpt;
-  if (rr >= max(0, min(tpt, s.n - i0)) * a.group) return;
   // one past the last CTA with a part: the one that holds the item's last tile
   const int last = static_cast<int>(((first + rec.tiles) * rec.nc - 1) / rec.total) + 1;
   const int skip = border(k - 1) != first;  // in the first CTA the item is not the first segment
   auto part = [&](int c) { return slots + (2 * static_cast<int64_t>(c) + (c == k - 1 ? skip : 0)) * L::kSlotFloats; };
-  float m = -INFINITY;
-  for (int c = k - 1 + lane; c < last; c += 32) m = fmaxf(m, part(c)[L::kRows * HD + r]);
+  for (int r = static_cast<int>(blockIdx.y) * 8 + threadIdx.x / 32; r < L::kRows; r += 8 * gridDim.y) {
+    const int tile = r / kTile, rr = r - tile * kTile;
+    const int i0 = rec.p * tpt * L::kTiles + tile * tpt;
+    if (rr >= max(0, min(tpt, s.n - i0)) * a.group) continue;
+    float m = -INFINITY;
+    for (int c = k - 1 + lane; c < last; c += 32) m = fmaxf(m, part(c)[L::kRows * HD + r]);
 #pragma unroll
-  for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
-  const float base = m == -INFINITY ? 0.f : m;
-  constexpr int kDims = HD / kLanes;  // 4 or 8 dims of a thread
-  const int d = lane % kLanes * kDims, half = lane / kLanes;
-  float l = 0.f, o[kDims];
+    for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
+    const float base = m == -INFINITY ? 0.f : m;
+    constexpr int kDims = HD / kLanes;  // 4 or 8 dims of a thread
+    const int d = lane % kLanes * kDims, half = lane / kLanes;
+    float l = 0.f, o[kDims];
 #pragma unroll
-  for (int e = 0; e < kDims; ++e) o[e] = 0.f;
-  for (int c0 = k - 1; c0 < last; c0 += 32) {
-    float f = 0.f;  // of part c0 + lane
-    if (c0 + lane < last) {
-      f = ex2(part(c0 + lane)[L::kRows * HD + r] - base);
-      l = fmaf(part(c0 + lane)[L::kRows * (HD + 1) + r], f, l);
-    }
-    const int n = min(32, last - c0);
+    for (int e = 0; e < kDims; ++e) o[e] = 0.f;
+    for (int c0 = k - 1; c0 < last; c0 += 32) {
+      float f = 0.f;  // of part c0 + lane
+      if (c0 + lane < last) {
+        f = ex2(part(c0 + lane)[L::kRows * HD + r] - base);
+        l = fmaf(part(c0 + lane)[L::kRows * (HD + 1) + r], f, l);
+      }
+      const int n = min(32, last - c0);
 #pragma unroll 8
-    for (int i = half; i < n + half; i += 2) {
-      const float w = __shfl_sync(0xffffffffu, f, i & 31);  // past n: 0
-      const float* ps = part(min(c0 + i, last - 1)) + r * HD + d;
+      for (int i = half; i < n + half; i += 2) {
+        const float w = __shfl_sync(0xffffffffu, f, i & 31);  // past n: 0
+        const float* ps = part(min(c0 + i, last - 1)) + r * HD + d;
 #pragma unroll
-      for (int e = 0; e < kDims; e += 4) {
-        const float4 v = *reinterpret_cast<const float4*>(ps + e);
-        o[e] = fmaf(v.x, w, o[e]);
-        o[e + 1] = fmaf(v.y, w, o[e + 1]);
-        o[e + 2] = fmaf(v.z, w, o[e + 2]);
-        o[e + 3] = fmaf(v.w, w, o[e + 3]);
+        for (int e = 0; e < kDims; e += 4) {
+          const float4 v = *reinterpret_cast<const float4*>(ps + e);
+          o[e] = fmaf(v.x, w, o[e]);
+          o[e + 1] = fmaf(v.y, w, o[e + 1]);
+          o[e + 2] = fmaf(v.z, w, o[e + 2]);
+          o[e + 3] = fmaf(v.w, w, o[e + 3]);
+        }
       }
     }
-  }
 #pragma unroll
-  for (int off = 16; off > 0; off >>= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
+    for (int off = 16; off > 0; off >>= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
 #pragma unroll
-  for (int e = 0; e < kDims; ++e) o[e] += __shfl_xor_sync(0xffffffffu, o[e], 16);
-  if (half != 0) return;
-  const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
-  const int token = i0 + rr / a.group, h = rr - (rr / a.group) * a.group;
-  if (d >= a.hd) return;
-  bf16* out = static_cast<bf16*>(a.out) + ((s.row0 + token) * a.hq + rec.kvh * a.group + h) * a.hd + d;
+    for (int e = 0; e < kDims; ++e) o[e] += __shfl_xor_sync(0xffffffffu, o[e], 16);
+    if (half != 0) continue;
+    const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
+    const int token = i0 + rr / a.group, h = rr - (rr / a.group) * a.group;
+    if (d >= a.hd) continue;
+    bf16* out = static_cast<bf16*>(a.out) + ((s.row0 + token) * a.hq + rec.kvh * a.group + h) * a.hd + d;
 #pragma unroll
-  for (int e = 0; e < kDims; e += 4) {  // head_dim is a multiple of 8
-    *reinterpret_cast<uint2*>(out + e) = make_uint2(pack_bf16x2(o[e] * inv, o[e + 1] * inv),
-                                                    pack_bf16x2(o[e + 2] * inv, o[e + 3] * inv));
+    for (int e = 0; e < kDims; e += 4) {  // head_dim is a multiple of 8
+      *reinterpret_cast<uint2*>(out + e) = make_uint2(pack_bf16x2(o[e] * inv, o[e + 1] * inv),
+                                                      pack_bf16x2(o[e + 2] * inv, o[e + 3] * inv));
+    }
   }
 }
 
@@ -1023,7 +1025,7 @@ int launch_form(TreeArgs a, cudaStream_t stream, const char* what) {
   if (int st = launch_kernel(what, kernel, dim3(nc), dim3(kThreadsTc), L::kBytes, stream, nullptr, tq, tk, tv, a)) return st;
   // items of one tile, and a single CTA, are never cut
   if (nc == 1 || a.max_ctx + a.max_tree <= a.tile) return BM_OK;
-  return launch_kernel(what, tree_merge_kernel<HD, COPIES>, dim3(nc - 1, L::kRows / 8), dim3(256), 0, stream, nullptr, a, nc);
+  return launch_kernel(what, tree_merge_kernel<HD, COPIES>, dim3(nc - 1, std::min(L::kRows / 8, 8)), dim3(256), 0, stream, nullptr, a, nc);
 }
 
 template <int HD>
