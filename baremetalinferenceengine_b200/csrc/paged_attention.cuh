@@ -25,6 +25,7 @@ struct TreeArgs {
   int num_pages, page_size, max_pages, num_seqs;
   int max_ctx, max_tree;
   int tile, box;              // tensor-core form: slots of a tile, rows of the boxes that fill it
+  bool whole;                 // and whether items stay whole
   int splits, split_len;      // CUDA-core form: the slots shared out over CTAs
   int row_tiles;              // and the query rows of a sequence and kv head
   float qscale;               // scale * log2(e): the softmax runs in base 2

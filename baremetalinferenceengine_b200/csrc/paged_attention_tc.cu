@@ -27,7 +27,9 @@
 // all tiles of the batch, counted on the device: items (sequence, kv head, row tile) laid
 // end to end, CTA c walking tiles [c T / nc, (c + 1) T / nc). An item cut at a CTA border
 // leaves partials in the workspace (at most two per CTA), which tree_merge_kernel adds
-// up; a whole one is written directly.
+// up; a whole one is written directly. Where the bounds allow no item of more than
+// kWholeTiles tiles, borders move on to the next item instead: walking the rest of a short
+// item costs less than a merge.
 //
 // Twelve warps:
 //   warps 0, 3 TMA of K and of V, pages looked up by their lanes, one box of a page's
@@ -58,7 +60,8 @@ namespace {
 
 constexpr int kTile = 128;      // slots per tile, rows per row tile
 constexpr int kThreadsTc = 384;
-constexpr int kMinTiles = 2;    // tiles that make a CTA worth starting
+constexpr int kMinTiles = 2;    // tiles that make a CTA worth starting, where items are cut
+constexpr int kWholeTiles = 8;  // of the longest item, up to which items stay whole
 constexpr int kBadRing = 16;    // tiles whose bad-page bits are kept
 constexpr uint64_t kWaitNs = 2000000000ull;
 constexpr uint64_t kDrainNs = 200000000ull;
@@ -124,6 +127,16 @@ __device__ __forceinline__ int64_t head_tiles(const TreeArgs& a, const Seq& s, i
   return t;
 }
 
+// Tiles from tile `off` of a sequence to the next beginning of an item (0: it is one).
+__device__ __forceinline__ int64_t to_next_item(const TreeArgs& a, const Seq& s, int64_t off, int64_t head, int per) {
+  off %= head;
+  for (int p = 0;; ++p) {
+    const int tiles = item_tiles(a, s, p, per);
+    if (off < tiles) return off == 0 ? 0 : tiles - off;
+    off -= tiles;
+  }
+}
+
 // The walk over a CTA's segments: every role runs its own, with the same results.
 struct Walk {
   int64_t b, left;
@@ -135,7 +148,15 @@ struct Walk {
     b = b0;
     left = n;
     s = sequence;
-    const int64_t head = head_tiles(a, s, per, &items);
+    int64_t head = head_tiles(a, s, per, &items);
+    if (off >= a.hkv * head) {  // behind the sequence's last item: the next one with tiles
+      do {
+        ++b;
+        read_seq(a, b, &s);
+      } while (s.n == 0);
+      head = head_tiles(a, s, per, &items);
+      off = 0;
+    }
     kvh = static_cast<int>(off / head);
     off -= kvh * head;
     p = 0;
@@ -167,9 +188,8 @@ struct Walk {
 };
 
 struct Plan {
-  int64_t lo, n, total, b, off;
-  Seq s;  // sequence b
-  int nc;
+  int64_t lo, hi, b, off;  // this CTA's tiles; the first is tile `off` of sequence b
+  Seq s;                   // sequence b
 };
 static_assert(sizeof(Plan) <= 96, "room in the layout");
 
@@ -326,6 +346,8 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
   float* slots = a.ws + records_bytes(gridDim.x) / sizeof(float);
 
   // ---------------- the plan ----------------
+  int64_t plan_total;
+  int plan_nc;
   {
     // barriers and TMEM come up while the lengths are read
     if (tid == 0) {
@@ -383,33 +405,54 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
       if (w < warp) before += scan[w];
       total += scan[w];
     }
-    const int nc = static_cast<int>(min(static_cast<int64_t>(gridDim.x), (total + kMinTiles - 1) / kMinTiles));
+    const int nc = static_cast<int>(min(static_cast<int64_t>(gridDim.x), a.whole ? total : (total + kMinTiles - 1) / kMinTiles));
     if (cta >= nc) {  // nothing for this CTA (the same for all its threads)
       if (tid == 0) records[cta] = Record{0, total, -1, 0, 0, -1, 0, nc};
       if (warp == 1) tmem_dealloc(*tmem_base_s, L::kTmemCols);
       return;
     }
+    // Tile x lies in one thread's sequences; a.whole moves both ends on to the next beginning
+    // of an item.
     const int64_t lo = total * cta / nc, hi = total * (cta + 1) / nc;
-    if (before <= lo && lo < before + mine) {
+    auto locate = [&](int64_t x, bool first) {
+      if (x < before || x >= before + mine) return;
       int64_t at = before;
       for (int64_t b = b_lo; b < b_hi; ++b) {
         if (share > 1) read_seq(a, b, &s);
         int items;
-        const int64_t n = a.hkv * head_tiles(a, s, per, &items);
-        if (lo < at + n) {
-          *plan = Plan{lo, hi - lo, total, b, lo - at, s, nc};
-          break;
+        const int64_t head = head_tiles(a, s, per, &items), n = a.hkv * head;
+        if (x < at + n) {
+          const int64_t on = a.whole ? to_next_item(a, s, x - at, head, per) : 0;
+          if (first) {
+            plan->lo = x + on;
+            plan->b = b;
+            plan->off = x - at + on;
+            plan->s = s;
+          } else {
+            plan->hi = x + on;
+          }
+          return;
         }
         at += n;
       }
-    }
+    };
+    locate(lo, true);
+    locate(hi, false);
+    if (tid == 0 && hi == total) plan->hi = total;
     __syncthreads();
+    plan_total = total;
+    plan_nc = nc;
+    if (plan->lo >= plan->hi) {  // another CTA's item fills the whole range
+      if (tid == 0) records[cta] = Record{0, total, -1, 0, 0, -1, 0, nc};
+      if (warp == 1) tmem_dealloc(*tmem_base_s, L::kTmemCols);
+      return;
+    }
   }
   const uint32_t tmem = *tmem_base_s;
   Walk walk;
-  walk.start(a, plan->s, plan->b, plan->off, plan->n, per);
+  walk.start(a, plan->s, plan->b, plan->off, plan->hi - plan->lo, per);
   if (tid == 0) {
-    records[cta] = Record{plan->lo, plan->total, static_cast<int32_t>(walk.b), walk.kvh, walk.p, walk.t, walk.tiles, plan->nc};
+    records[cta] = Record{plan->lo, plan_total, static_cast<int32_t>(walk.b), walk.kvh, walk.p, walk.t, walk.tiles, plan_nc};
   }
 
   if (warp == 0 || warp == 3) {
@@ -1006,7 +1049,7 @@ int ctas_for(int64_t batch, int hkv, int group, int max_ctx, int max_tree) {
   const int per = tokens_of(copies_for(group, max_tree), group);
   const int64_t tiles = batch * hkv * ((max_tree + per - 1) / per) *
                         ((static_cast<int64_t>(max_ctx) + max_tree + kTile / 2 - 1) / (kTile / 2));
-  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(sm_count(), (tiles + kMinTiles - 1) / kMinTiles)));
+  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(sm_count(), tiles)));
 }
 
 template <int HD, int COPIES>
@@ -1021,10 +1064,15 @@ int launch_form(TreeArgs a, cudaStream_t stream, const char* what) {
   if (int st = make_tensor_map_3d_bf16(&tq, a.q, a.hd, a.hq, a.total_q, 64, a.group, tpt, what)) return st;
   auto kernel = tree_tc_kernel<HD, COPIES>;
   if (int st = allow_dynamic_smem(reinterpret_cast<const void*>(kernel), L::kBytes, what)) return st;
+  // Whole items up to kWholeTiles tiles where they make CTAs for a quarter of the SMs or more
+  // (80 items of 5 tiles: 15.9 us, cut 18.6), else up to half of that (8 items of 8: 18.7,
+  // cut 15.8).
+  const int per = tokens_of(COPIES, a.group);
+  const int64_t items = a.batch * a.hkv * ((a.max_tree + per - 1) / per);
+  a.whole = a.max_ctx + a.max_tree <= (4 * items >= sm_count() ? kWholeTiles : kWholeTiles / 2) * a.tile;
   const int nc = ctas_for(a.batch, a.hkv, a.group, a.max_ctx, a.max_tree);
   if (int st = launch_kernel(what, kernel, dim3(nc), dim3(kThreadsTc), L::kBytes, stream, nullptr, tq, tk, tv, a)) return st;
-  // items of one tile, and a single CTA, are never cut
-  if (nc == 1 || a.max_ctx + a.max_tree <= a.tile) return BM_OK;
+  if (nc == 1 || a.whole) return BM_OK;  // no item is cut
   return launch_kernel(what, tree_merge_kernel<HD, COPIES>, dim3(nc - 1, std::min(L::kRows / 8, 8)), dim3(256), 0, stream, nullptr, a, nc);
 }
 
