@@ -119,8 +119,29 @@ struct Weigher {
   __device__ __forceinline__ static u64 whole(double w) {  // w < 2^52, rounded
     return static_cast<u64>(__double_as_longlong(w + 4503599627370496.0)) & 0xfffffffffffffull;
   }
+  // A whole number that never rises as the logit falls, linear in it: kEven for the
+  // largest, 0 for those without a weight.
+  static constexpr uint32_t kEven = 1u << 31;
+  __device__ __forceinline__ uint32_t even(float x) const {
+    const float b = place(x);
+    return b < kLimit ? kEven - static_cast<uint32_t>(b * 524288.f) : 0;
+  }
   __device__ __forceinline__ u64 operator()(float x) const { return place(x) < kLimit ? whole(real(x)) : 0; }
 };
+
+// Of a row with this largest logit. Past bits + 2 octaves a weight rounds to 0.
+__device__ __forceinline__ Weigher weigher(float top, float temperature, float min_p, int bits, const double* table) {
+  const float bins_per_octave = Weigher::kLimit / static_cast<float>(bits + 2);
+  const double per_logit = kLog2e / fmax(static_cast<double>(temperature), 0x1p-60);
+  Weigher w;
+  w.top_f = top;
+  w.top = widen(top);
+  w.scale = 128.0 * per_logit;
+  w.least = exp2(static_cast<double>(bits)) * static_cast<double>(fminf(min_p, 1.f));
+  w.table = table;
+  w.bins = static_cast<float>(per_logit * static_cast<double>(bins_per_octave));
+  return w;
+}
 
 // Adding it to 0 <= x < 2^22 rounds x to a whole number, in the sum's low bits.
 constexpr float kMagic = 12582912.f;  // 1.5 * 2^23
@@ -144,6 +165,8 @@ struct Shared {
   uint32_t own_count, offset;
   uint32_t count, key_min, key_max;             // the leader's: logits of the border's bins
   uint32_t bin_lo, bin_hi, bin;
+  uint32_t members, member[32];                 // of the border's part of a split
+  u64 member_value[32];
   uint32_t key;            // t
   uint32_t index;
   bool cut;                // not all logits equal to t stay
@@ -231,45 +254,68 @@ __device__ __forceinline__ void each(const T* x, int lo, int hi, bool vec, bool 
   if (whole + lane < hi) f(whole + lane, remapped(load1(x + whole + lane), remap));  // fewer than VEC are left
 }
 
-// The border among the block's elements, kEach a thread, taken by descending field: the
-// field of the first whose running value (equal fields together) reaches the target, and
-// in *before the value above it. 512 equal parts of the fields' range a round. All values
-// together reach the target.
+// The border among the block's elements, kEach a thread, taken by descending `fine`: the
+// fine of the first whose running value (equal ones together) reaches the target, and in
+// *before the value above it. All values together reach the target; elements of value 0
+// are none. `coarse` never rises where fine falls: its range is split in
+// 512 equal parts a round, so elements should lie evenly in it (64-bit shared-memory atomics
+// on one address take turns). Up to 32 elements in the border's part are ranked by every
+// warp alike; more that share one coarse are split by their fine.
 constexpr int kEach = kList / kThreads;
-__device__ uint32_t border(Shared& sh, const uint32_t (&field)[kEach], const u64 (&value)[kEach], u64 target, u64* before) {
-  const int tid = threadIdx.x;
+__device__ uint32_t border(Shared& sh, const uint32_t (&coarse)[kEach], const uint32_t (&fine)[kEach],
+                           const u64 (&value)[kEach], u64 target, u64* before) {
+  const int tid = threadIdx.x, lane = tid & 31;
   u64 passed = 0;
-  uint32_t from = 0, to = 0xffffffffu;
-  for (int round = 0; round < 5; ++round) {
+  uint32_t from = 0, to = 0xffffffffu, fine_from = 0, fine_to = 0xffffffffu;
+  bool by_fine = false;
+  for (int round = 0; round < 10; ++round) {  // at most 4 by coarse, 5 by fine
     __syncthreads();
+    sh.split[tid] = 0;
     if (tid == 0) {
+      sh.members = 0;
       sh.key_min = 0xffffffffu;
       sh.key_max = 0;
     }
-    sh.split[tid] = 0;
     __syncthreads();
-    uint32_t mn = 0xffffffffu, mx = 0;
+    {  // the range that is left
+      uint32_t mn = 0xffffffffu, mx = 0;
 #pragma unroll
-    for (int e = 0; e < kEach; ++e) {
-      if (value[e] != 0 && field[e] >= from && field[e] <= to) {
-        mn = min(mn, field[e]);
-        mx = max(mx, field[e]);
+      for (int e = 0; e < kEach; ++e) {
+        const uint32_t f = by_fine ? fine[e] : coarse[e];
+        if (value[e] != 0 && coarse[e] >= from && coarse[e] <= to && fine[e] >= fine_from && fine[e] <= fine_to) {
+          mn = min(mn, f);
+          mx = max(mx, f);
+        }
+      }
+      mn = __reduce_min_sync(0xffffffffu, mn);
+      mx = __reduce_max_sync(0xffffffffu, mx);
+      if (lane == 0) {
+        atomicMin(&sh.key_min, mn);
+        atomicMax(&sh.key_max, mx);
+      }
+      __syncthreads();
+      if (by_fine) {
+        fine_from = sh.key_min;
+        fine_to = sh.key_max;
+        if (fine_from >= fine_to) {
+          *before = passed;
+          return fine_to;
+        }
+      } else {
+        from = sh.key_min;
+        to = sh.key_max;
       }
     }
-    mn = __reduce_min_sync(0xffffffffu, mn);
-    mx = __reduce_max_sync(0xffffffffu, mx);
-    if ((tid & 31) == 0) {
-      atomicMin(&sh.key_min, mn);
-      atomicMax(&sh.key_max, mx);
-    }
-    __syncthreads();
-    from = sh.key_min;
-    to = sh.key_max;
-    if (from >= to) break;
-    const int shift = max(0, 32 - __clz(to - from) - 9);
+    const uint32_t range = by_fine ? fine_to - fine_from : to - from;
+    const int shift = max(0, 32 - __clz(range) - 9);
+    auto part = [&](int e) { return by_fine ? (fine_to - fine[e]) >> shift : (to - coarse[e]) >> shift; };
+    auto within = [&](int e) {
+      if (value[e] == 0) return false;
+      return by_fine ? coarse[e] == to && fine[e] >= fine_from && fine[e] <= fine_to : coarse[e] >= from && coarse[e] <= to;
+    };
 #pragma unroll
     for (int e = 0; e < kEach; ++e) {
-      if (value[e] != 0 && field[e] >= from && field[e] <= to) atomicAdd(&sh.split[(to - field[e]) >> shift], value[e]);
+      if (within(e)) atomicAdd(&sh.split[part(e)], value[e]);
     }
     __syncthreads();
     const u64 v = sh.split[tid];
@@ -281,31 +327,65 @@ __device__ uint32_t border(Shared& sh, const uint32_t (&field)[kEach], const u64
     }
     __syncthreads();
     passed = sh.before;
-    to -= sh.bin << shift;
-    from = max(from, shift == 0 ? to : to - ((1u << shift) - 1));
+    const uint32_t bin = sh.bin;
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+      if (within(e) && part(e) == bin) {
+        const uint32_t n = atomicAdd(&sh.members, 1u);
+        if (n < 32) {
+          sh.member[n] = fine[e];
+          sh.member_value[n] = value[e];
+        }
+      }
+    }
+    __syncthreads();
+    if (sh.members <= 32) {
+      const bool is = lane < static_cast<int>(sh.members);
+      const uint32_t own = is ? sh.member[lane] : 0;
+      const u64 worth = is ? sh.member_value[lane] : 0;
+      u64 above = passed;
+      for (int j = 0; j < static_cast<int>(sh.members); ++j) {
+        if (sh.member[j] > own) above += sh.member_value[j];
+      }
+      // the lowest of those with less than the target above them
+      const uint32_t found = __reduce_min_sync(0xffffffffu, worth != 0 && above < target ? own : 0xffffffffu);
+      const int who = __ffs(__ballot_sync(0xffffffffu, is && own == found)) - 1;
+      *before = __shfl_sync(0xffffffffu, above, who);
+      return found;
+    }
+    if (by_fine) {
+      fine_to -= bin << shift;
+      if (shift < 31) fine_from = max(fine_from, fine_to - min(fine_to, (1u << shift) - 1));
+    } else {
+      to -= bin << shift;
+      from = max(from, to - min(to, (1u << shift) - 1));
+      by_fine = from == to;
+    }
   }
   *before = passed;
-  return to;
+  return fine_to;
 }
 
-// The rest of a row whose top-k logits are in the leader's list (some more may be).
+// The rest of a row whose top-k logits are in the leader's list (some more may be), or all
+// of whose logits are (k at least their number).
 __device__ __noinline__ void finish_alone(Shared& sh, const SampleArgs& a, const Weigher& weigh, int k, float p, float u,
                                           int64_t row) {
   const int tid = threadIdx.x;
   const uint32_t n = sh.count;
-  uint32_t key[kEach], later[kEach];  // later: descends as the index rises
+  uint32_t key[kEach], even[kEach], later[kEach];  // even: as the logits lie; later: descends as the index rises
   u64 one[kEach], weight[kEach], before, all;
 #pragma unroll
   for (int e = 0; e < kEach; ++e) {
     const uint32_t i = tid + e * kThreads;
     key[e] = i < n ? sh.cand_key[i] : 0;
+    even[e] = weigh.even(logit_of(key[e]));
     later[e] = i < n ? ~sh.cand_index[i] : 0;
     one[e] = i < n;
     weight[e] = i < n ? weigh(logit_of(key[e])) : 0;
   }
   // top-k, then top-p: a key, how many of those equal to it stay, and (if not all) the last
   for (int stage = 0; stage < 2; ++stage) {
-    if (stage == 1 && !(p < 1.f)) break;
+    if (stage == 1 ? !(p < 1.f) : k >= static_cast<int>(n)) continue;
     u64 target = k;
     if (stage == 1) {
       u64 mine = 0;
@@ -316,7 +396,7 @@ __device__ __noinline__ void finish_alone(Shared& sh, const SampleArgs& a, const
       target = portion(fmaxf(p, 0.f), all, &fraction);
       if (fraction || target == 0) ++target;
     }
-    const uint32_t t = border(sh, key, stage == 0 ? one : weight, target, &before);
+    const uint32_t t = border(sh, even, key, stage == 0 ? one : weight, target, &before);
     u64 tie[kEach], equal = 0;
 #pragma unroll
     for (int e = 0; e < kEach; ++e) {
@@ -327,7 +407,7 @@ __device__ __noinline__ void finish_alone(Shared& sh, const SampleArgs& a, const
     const u64 w = stage == 0 ? 1 : max(weigh(logit_of(t)), static_cast<u64>(1));
     const u64 rest = (target - before + w - 1) / w;
     uint32_t last = 0;  // of the `later` order: those below it go
-    if (rest < all) last = border(sh, later, tie, rest, &before);
+    if (rest < all) last = border(sh, later, later, tie, rest, &before);
 #pragma unroll
     for (int e = 0; e < kEach; ++e) {
       if (key[e] < t || (key[e] == t && later[e] < last)) one[e] = weight[e] = 0;
@@ -342,8 +422,72 @@ __device__ __noinline__ void finish_alone(Shared& sh, const SampleArgs& a, const
   block_scan64(mine, sh.sub, &all);
   bool fraction;
   const u64 want = portion(u, all, &fraction);
-  const uint32_t token = ~border(sh, later, weight, want + 1, &before);
+  const uint32_t token = ~border(sh, later, later, weight, want + 1, &before);
   if (tid == 0) a.tokens[row] = static_cast<int32_t>(token);
+}
+
+// A row of at most kList logits: one CTA holds it, and there is nothing to search for
+// in memory.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) sample_short_kernel(const SampleArgs a) {
+  grid_dependency_wait();
+  extern __shared__ __align__(16) unsigned char smem[];
+  Shared& sh = *reinterpret_cast<Shared*>(smem);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int64_t row = blockIdx.x;
+  const T* x = static_cast<const T*>(a.logits) + row * a.stride;
+  float v[kEach];
+  uint32_t most = 0;
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) {
+    const int i = tid + e * kThreads;
+    v[e] = i < a.vocab ? load1(x + i) : -INFINITY;
+    most = max(most, key_of(v[e]));
+  }
+  const float temp = a.temperature ? a.temperature[row] : 1.f;
+  const float u = a.uniforms[row];
+  const int k = a.top_k ? a.top_k[row] : 0;
+  const float p = a.top_p ? a.top_p[row] : 1.f;
+  const float mp = a.min_p ? a.min_p[row] : 0.f;
+  if (!(temp >= 0.f) || !(u >= 0.f && u < 1.f) || p != p || mp != mp) {
+    if (tid == 0) {
+      a.tokens[row] = -1;
+      raise_status(a.status, BM_DEVERR_BAD_PARAMETER);
+    }
+    return;
+  }
+  most = __reduce_max_sync(0xffffffffu, most);
+  if (lane == 0) sh.list_key[warp] = most;
+  if (tid < 128) sh.table[tid] = exp2(static_cast<double>(a.bits) - tid / 128.0);
+  if (tid == 0) sh.index = 0xffffffffu;
+  __syncthreads();
+  for (int w = 0; w < kWarps; ++w) most = max(most, sh.list_key[w]);
+  const float top = logit_of(most);
+  if (top == -INFINITY || temp == 0.f) {
+    uint32_t first = 0xffffffffu;
+#pragma unroll
+    for (int e = kEach - 1; e >= 0; --e) {
+      if (tid + e * kThreads < a.vocab && key_of(v[e]) == most) first = tid + e * kThreads;
+    }
+    first = __reduce_min_sync(0xffffffffu, first);
+    if (lane == 0) atomicMin(&sh.index, first);
+    __syncthreads();
+    if (tid == 0) a.tokens[row] = top == -INFINITY ? -1 : static_cast<int32_t>(sh.index);
+    return;
+  }
+  const bool remap = top == INFINITY;
+  const Weigher weigh = weigher(remap ? 0.f : top, temp, mp, a.bits, sh.table);
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) {
+    const int i = tid + e * kThreads;
+    if (i < a.vocab) {
+      sh.cand_key[i] = key_of(remapped(v[e], remap));
+      sh.cand_index[i] = i;
+    }
+  }
+  if (tid == 0) sh.count = a.vocab;
+  __syncthreads();
+  finish_alone(sh, a, weigh, k > 0 ? min(k, a.vocab) : a.vocab, p, u, row);
 }
 
 // RESIDENT: CTAs per SM that the registers are cut for.
@@ -425,16 +569,8 @@ __global__ void __launch_bounds__(kThreads, RESIDENT) sample_kernel(const Sample
     return;  // nobody reads another CTA's shared memory after the sync above
   }
   const bool remap = top == INFINITY;
-  const float octaves = static_cast<float>(a.bits + 2);  // past these a weight rounds to 0
-  const float bins_per_octave = Weigher::kLimit / octaves;
-  const double per_logit = kLog2e / fmax(static_cast<double>(temp), 0x1p-60);
-  Weigher weigh;
-  weigh.top_f = remap ? 0.f : top;
-  weigh.top = widen(weigh.top_f);
-  weigh.scale = 128.0 * per_logit;
-  weigh.least = exp2(static_cast<double>(a.bits)) * static_cast<double>(fminf(mp, 1.f));
-  weigh.table = sh.table;
-  weigh.bins = static_cast<float>(per_logit * static_cast<double>(bins_per_octave));
+  const float bins_per_octave = Weigher::kLimit / static_cast<float>(a.bits + 2);
+  const Weigher weigh = weigher(remap ? 0.f : top, temp, mp, a.bits, sh.table);
 
   uint32_t t = 0;         // what stays: keys above t,
   u64 ties = 0;           // and the first `ties` equal to it,
@@ -486,14 +622,15 @@ __global__ void __launch_bounds__(kThreads, RESIDENT) sample_kernel(const Sample
 
   if (bounded && !remap) {
     if (rank == 0) {
-      uint32_t key[kEach];
+      uint32_t key[kEach], even[kEach];
       u64 one[kEach], before;
 #pragma unroll
       for (int e = 0; e < kEach; ++e) {
         one[e] = tid + e * kThreads < groups;
         key[e] = one[e] != 0 ? sh.cand_key[tid + e * kThreads] : 0;
+        even[e] = weigh.even(logit_of(key[e]));
       }
-      const uint32_t bound = border(sh, key, one, k, &before);
+      const uint32_t bound = border(sh, even, key, one, k, &before);
       if (tid < C) peer(tid)->key = bound;
       __syncthreads();
     }
@@ -553,7 +690,7 @@ __global__ void __launch_bounds__(kThreads, RESIDENT) sample_kernel(const Sample
     const int tied_bin = tied == 0 ? -1 : bin_of(t0_f);
     {
       u64 v = 0;  // eight bins a thread, 64 by eight threads
-#pragma unroll 1
+#pragma unroll
       for (int i = 0; i < kBins / kThreads; ++i) v += bin_value(sh.hist[tid * (kBins / kThreads) + i], tid * (kBins / kThreads) + i);
 #pragma unroll
       for (int off = 4; off > 0; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
@@ -623,10 +760,10 @@ __global__ void __launch_bounds__(kThreads, RESIDENT) sample_kernel(const Sample
             sh.bin_lo = bin;
             sh.before = at;
             sh.through = through;
-          } else {
-            sh.bin_hi = bin;
           }
+          sh.bin_hi = bin;
         }
+        if (most_target <= through) break;  // both ends in one bin
       }
     }
     __syncthreads();
@@ -946,6 +1083,11 @@ extern "C" int bm_sample(int32_t* tokens, const void* logits, const float* unifo
   attr.val.clusterDim.y = 1;
   attr.val.clusterDim.z = 1;
   const dim3 grid(static_cast<unsigned>(rows * c));
+  if (vocab <= kList) {
+    auto kernel = dtype == BM_F32 ? sample_short_kernel<float> : sample_short_kernel<bf16>;
+    if (int st = allow_dynamic_smem(reinterpret_cast<const void*>(kernel), sizeof(Shared), what)) return st;
+    return launch_kernel(what, kernel, dim3(static_cast<unsigned>(rows)), dim3(kThreads), sizeof(Shared), as_stream(stream), nullptr, a);
+  }
   auto go = [&](auto kernel) {
     if (int st = allow_dynamic_smem(reinterpret_cast<const void*>(kernel), sizeof(Shared), what)) return st;
     return launch_kernel(what, kernel, grid, dim3(kThreads), sizeof(Shared), as_stream(stream), &attr, a);
