@@ -480,8 +480,8 @@ typedef struct bm_paged_kv {
  *   slot slots[r] of sequence seq_ids[r]: K = k[r] rotated, V = v[r].
  * slots NULL: slot = positions[r]. A drafted tree's tokens share rotary positions and
  * have slots of their own. seq_ids NULL: all 0. table NULL: nothing is rotated (q_out
- * and K are copies; positions may be NULL when slots is given). q, k, v and q_out rows are *_stride elements apart;
- * num_q_heads may be 0 (q and q_out NULL). Rows whose slot is -1 are padding: nothing of
+ * and K are copies; positions may be NULL when slots is given). q, k, v and q_out rows
+ * are *_stride elements apart; num_q_heads may be 0 (q and q_out NULL). Rows whose slot is -1 are padding: nothing of
  * theirs is read or written. Bad positions (outside the table), slots (negative or
  * outside max_pages pages), sequences and page ids flag *d_status; such a row is
  * skipped. The rows of one call name distinct slots: with two rows on one slot either
@@ -502,14 +502,16 @@ int bm_paged_kv_append(void* q_out, const void* q, const void* k, const void* v,
  * over the context and the drafted slots j that it sees: bit j%64 of
  * tree_mask[row][j/64] (uint64 [total_q][mask_words], bits past n_b ignored), or j <= i
  * when tree_mask is NULL. G = num_q_heads / num_kv_heads <= 64, scale <= 0 means
- * 1/sqrt(head_dim), head_dim <= 256 with whole 16-byte rows. A row that sees nothing
+ * 1/sqrt(head_dim), head_dim <= 256 with whole 16-byte rows, and
+ * batch * max_tree * num_q_heads <= 2^25. out must not overlap q. A row that sees nothing
  * gets zeros. Rows outside [q_starts[0], q_starts[batch]) are left as they were.
  * max_ctx and max_tree are host-side upper bounds of ctx_lens and n_b that size the
  * work split; with a mask max_tree <= 64 * mask_words. K and V of the ctx + n_b slots
  * must be finite; slots behind them may hold anything. Softmax statistics and sums are
- * fp32; bf16 caches with head_dim 64 or 128 and page sizes that divide 128 or are multiples of it
- * (at least 8) run on the tensor cores with weights rounded to bf16, as
- * bm_decode_attention does.
+ * fp32. bf16 caches with head_dim a multiple of 8 up to 128 run on the tensor cores, with
+ * weights rounded to bf16 as bm_decode_attention does, for page sizes up to 128 that are
+ * multiples of 8 or at least 64, and larger ones with an equal part of 64 to 128 slots;
+ * all others run on the CUDA cores.
  * A sequence with n_b or ctx outside [0, bound], slots outside its max_pages pages or
  * rows outside [0, total_q) flags BM_DEVERR_BAD_POSITION, one with a bad sequence id
  * BM_DEVERR_BAD_SEQUENCE: it is skipped, its rows unwritten. A bad page id flags
@@ -540,10 +542,11 @@ int bm_paged_tree_attention(void* out, const void* q, const bm_paged_kv_t* cache
  * logit's lowest index. temperature, top_k, top_p and min_p are device arrays of one
  * entry per row, or NULL (1, off, off, off); k <= 0 or >= vocab, p >= 1 and m <= 0 are
  * off, p <= 0 leaves the largest alone. A NaN logit counts as -inf; -inf has no weight;
- * with +inf logits only these have one, all alike. A row without any weight gets token
- * -1. Weights are held in 64-bit fixed point (2^min(52, 62 - ceil(log2 vocab)) for the
- * largest, from fp64 exponentials) and summed as integers, so a result does not depend
- * on the order of any sum. A row whose temperature, top_p, min_p or uniform number is
+ * with +inf logits only these have one, all alike; a logit more than FLT_MAX below the
+ * largest has none. A row without any weight gets token -1. Weights are held in 64-bit
+ * fixed point (2^min(51, 62 - ceil(log2 vocab)) for the largest, from fp64 exponentials)
+ * and summed as integers, so a result does not depend on the order of any sum.
+ * Temperatures between 0 and 2^-60 count as 2^-60. A row whose temperature, top_p, min_p or uniform number is
  * NaN, or whose temperature is negative or uniform outside [0, 1), gets -1 and flags
  * BM_DEVERR_BAD_PARAMETER. vocab <= 2^24. */
 int bm_sample(int32_t* tokens, const void* logits, const float* uniforms, const float* temperature,
