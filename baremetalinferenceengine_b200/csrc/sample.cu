@@ -867,7 +867,11 @@ __global__ void __launch_bounds__(kThreads, RESIDENT) sample_kernel(const Sample
     for (int round = 0; round < 4 && from != to; ++round) {
       const bool all = count > kList;
       if (!all && rank != 0) break;
-      if (all) cluster.sync();  // the leader's counters have been read
+      if (all) {  // the leader's counters have been read
+        cluster.sync();
+      } else {
+        __syncthreads();
+      }
       int shift = 0;
       while (((to - from) >> shift) >= static_cast<uint32_t>(kThreads)) ++shift;
       sh.split[tid] = 0;

@@ -153,3 +153,22 @@ def test_frequencies_follow_the_weights(cuda):
     got = ops.sample(row.expand(n, 7).contiguous().to(cuda), u.to(cuda)).cpu().long()
     p = torch.softmax(row.double(), 0)
     assert bool(((torch.bincount(got, minlength=7) / n - p).abs() <= 2.0 / n).all())
+
+
+@pytest.mark.parametrize("which", ["tp", "tkp"])
+def test_many_rows_at_once_and_again(cuda, which):
+    """More rows than SMs (two CTAs on each), with equal logits at the borders: the same
+    tokens every time."""
+    g = gen(11)
+    rows, vocab = 250, 128000
+    x = (torch.randn(rows, vocab, generator=g) * 2.0).to(BF16)
+    u = torch.rand(rows, generator=g)
+    s = dict(temperature=0.7 + torch.rand(rows, generator=g), top_k=None, top_p=0.5 + 0.49 * torch.rand(rows, generator=g),
+             min_p=None)
+    if "k" in which:
+        s["top_k"] = torch.randint(1100, 90000, (rows,), generator=g).to(torch.int32)
+    got = check(cuda, x, u, s)
+    dev = {n: None if t is None else t.to(cuda) for n, t in s.items()}
+    x, u = x.to(cuda), u.to(cuda)
+    for _ in range(30):
+        assert torch.equal(ops.sample(x, u, **dev), got)
