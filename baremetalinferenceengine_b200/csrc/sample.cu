@@ -101,9 +101,10 @@ struct Weigher {
 
   // The weight's place in the histogram, from 0 at the largest logit; never falls as the
   // logit does. Below kLimit the weight may round to something; NaN for a NaN logit, and
-  // for -inf at T = inf.
+  // for -inf at T = inf. Rounded here in every use: fused with the addition of kMagic in some
+  // of them, a place half way between two bins would be now in one, now in the other.
   static constexpr float kLimit = kBins - 1.5f;
-  __device__ __forceinline__ float place(float x) const { return (top_f - x) * bins; }
+  __device__ __forceinline__ float place(float x) const { return __fmul_rn(top_f - x, bins); }
   // The weight before it is rounded to a whole number, for places below kLimit (anything
   // for others).
   __device__ __forceinline__ double real(float x) const {

@@ -172,3 +172,31 @@ def test_many_rows_at_once_and_again(cuda, which):
     x, u = x.to(cuda), u.to(cuda)
     for _ in range(30):
         assert torch.equal(ops.sample(x, u, **dev), got)
+
+
+def test_ties_between_two_bins_of_the_histogram(cuda):
+    """Equal logits at the border of top-p whose place in the histogram lies half way
+    between two bins, but for its rounding: all of them fall into the same one."""
+    g = np.random.default_rng(12)
+    vocab, rows, top, ties = 2100, 160, np.float32(8.0), 100
+    values = torch.arange(-4.0, 4.0, 2.0 ** -6).to(BF16).float().numpy()
+    bins_per_octave = np.float32(np.float32(4094.5) / np.float32(min(51, 62 - 12) + 2))
+    found = []
+    while len(found) < rows:
+        t = np.float32(g.uniform(0.5, 2.0))
+        bins = np.float32(1.4426950408889634074 / np.float64(t) * np.float64(bins_per_octave))
+        exact = (np.float64(top) - values) * np.float64(bins)
+        place = exact.astype(np.float32)
+        for i in np.flatnonzero((place % 1 == 0.5) & (exact != place))[:1]:
+            found.append((t, values[i]))
+    x = np.full((rows, vocab), -30.0, dtype=np.float32)
+    p = np.empty(rows)
+    for r, (t, v) in enumerate(found):
+        at = g.permutation(vocab)
+        x[r, at[0]], x[r, at[1:1 + ties]] = top, v
+        w = np.exp((np.float64(v) - 8.0) / t)
+        x[r, at[1 + ties:1 + 2 * ties]] = v - 0.5  # and less of what goes
+        p[r] = (1 + w * (ties // 2 + 0.4)) / np.exp((x[r].astype(np.float64) - 8.0) / t).sum()
+    s = dict(temperature=torch.tensor([float(t) for t, _ in found]), top_k=None, top_p=torch.tensor(p).float(), min_p=None)
+    for u in (0.999, 0.9999, 1 - 2.0 ** -24):
+        check(cuda, torch.from_numpy(x).to(BF16), torch.full((rows,), u), s)
