@@ -242,13 +242,27 @@ __global__ void __launch_bounds__(kThreads) tree_attention_kernel(const TreeArgs
 }
 
 // Few rows (MR at most): each warp walks groups of eight slots of its own with its own
-// running softmax, K and V straight from memory into registers (a quarter warp's 16-byte
-// chunks of a slot's K, a warp's of a slot's V), so every byte is loaded once and no
-// barrier stands between a load and its use; the four warps' sums meet at the end. The
-// tiled kernel above would read its shared K and V eight times over for a few rows. J:
-// 16-byte chunks of a row of V per lane.
+// running softmax; K and V of the next groups are on their way into its ring of shared
+// memory (cp.async) meanwhile, and no barrier but the warp's own stands between. A lane
+// makes a quarter of its slot's score and owns 16-byte chunks of every row of V; the four
+// warps' sums meet at the end. The tiled kernel above would read its shared K and V eight
+// times over for a few rows. J: 16-byte chunks of a row of V per lane.
 constexpr int kRowThreads = 128;
-constexpr int kGroup = 8;  // slots of a warp's step
+constexpr int kGroup = 8;   // slots of a warp's step
+constexpr int kStages = 2;  // groups of a warp in flight or in use
+
+// The ring, in whose place the warps' sums [4][MR][hd] meet at the end; then Q [MR][hd], the
+// warps' weights [4][kGroup][MR], their maxima and sums.
+__host__ __device__ constexpr int ring_bytes(int hd, int es) { return kRowThreads / 32 * kStages * 2 * kGroup * hd * es; }
+__host__ __device__ constexpr int rows_smem(int hd, int es, int mr) {
+  return ring_bytes(hd, es) + (mr * hd + kRowThreads / 32 * mr * (kGroup + 2)) * 4;
+}
+
+__device__ __forceinline__ void copy16_async(void* to, const void* from, bool real) {  // zeros where not real
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(to))),
+               "l"(from), "r"(real ? 16 : 0)
+               : "memory");
+}
 
 template <typename T, int MR, int J>
 __global__ void __launch_bounds__(kRowThreads) tree_rows_kernel(const TreeArgs a) {
@@ -278,9 +292,45 @@ __global__ void __launch_bounds__(kRowThreads) tree_rows_kernel(const TreeArgs a
   const int start = split * a.split_len, end = min(seen, start + a.split_len);
 
   extern __shared__ __align__(16) float smem[];
-  float* Qs = smem;                                   // [MR][hd], then the warps' sums [kWarps][MR][hd]
-  float* Ps = smem + kWarps * MR * hd + warp * kGroup * MR;  // this warp's weights [kGroup][MR]
-  float* ml = smem + kWarps * MR * (hd + kGroup);     // [kWarps][MR] maxima, then sums
+  T* ring = reinterpret_cast<T*>(smem) + warp * kStages * 2 * kGroup * hd;
+  float* Qs = smem + ring_bytes(hd, sizeof(T)) / 4;       // [MR][hd]
+  float* Ps = Qs + MR * hd + warp * kGroup * MR;          // this warp's weights [kGroup][MR]
+  float* ml = Qs + MR * (hd + kWarps * kGroup);           // [kWarps][MR] maxima, then sums
+  const T* kp = static_cast<const T*>(a.k_pages);
+  const T* vp = static_cast<const T*>(a.v_pages);
+  const int32_t* pages = a.page_table + static_cast<int64_t>(s.seq) * a.max_pages;
+  const int own = lane >> 2, sub = lane & 3;  // this lane's slot of the group, its quarter of K's chunks
+  // Neighbouring rows' chunks lie 64 bytes apart in the banks, by the pitch or by a swap.
+  const int swap = cpr % 8 == 0 ? 4 : 0;
+
+  uint32_t sound = 0;  // bit i: this lane's slot in stage i has a sound page
+  auto fetch = [&](int g0, int stage) {
+    const int slot = g0 + own;
+    int64_t at = -1;  // the slot's row of the pages
+    if (slot < end) {
+      const int nth = slot / a.page_size;
+      const int32_t page = __ldg(pages + nth);
+      if (page >= 0 && page < a.num_pages) {
+        at = ((static_cast<int64_t>(page) * a.hkv + kvh) * a.page_size + (slot - nth * a.page_size)) * hd;
+      } else if (sub == 0) {
+        raise_status(a.status, BM_DEVERR_BAD_PAGE);
+      }
+    }
+    const bool real = at >= 0;
+    sound = (sound & ~(1u << stage)) | (real ? 1u << stage : 0u);
+    if (g0 < end) {
+      const T* k_from = kp + (real ? at : 0);
+      const T* v_from = vp + (real ? at : 0);
+      T* k_to = ring + (stage * 2 * kGroup + own) * hd;
+      T* v_to = k_to + kGroup * hd;
+      for (int c = sub; c < cpr; c += 4) copy16_async(k_to + (c ^ (own & 1 ? swap : 0)) * VEC, k_from + c * VEC, real);
+      for (int c = sub; c < cpr; c += 4) copy16_async(v_to + (c ^ (own & 1 ? swap : 0)) * VEC, v_from + c * VEC, real);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  const int first = start + warp * kGroup;
+  for (int i = 0; i < kStages; ++i) fetch(first + i * kWarps * kGroup, i);
+
   const T* q = static_cast<const T*>(a.q);
   for (int c = tid; c < MR * cpr; c += kRowThreads) {
     const int r = c / cpr, col = (c - r * cpr) * VEC;
@@ -295,10 +345,6 @@ __global__ void __launch_bounds__(kRowThreads) tree_rows_kernel(const TreeArgs a
     for (int e = 0; e < VEC; ++e) Qs[r * hd + col + e] = f[e] * a.qscale;
   }
   __syncthreads();
-  const T* kp = static_cast<const T*>(a.k_pages);
-  const T* vp = static_cast<const T*>(a.v_pages);
-  const int32_t* pages = a.page_table + static_cast<int64_t>(s.seq) * a.max_pages;
-  const int own = lane >> 2, sub = lane & 3;  // this lane's slot of the group, its quarter of K's chunks
 
   float m[MR], l[MR], acc[MR][J * VEC];
 #pragma unroll
@@ -308,63 +354,42 @@ __global__ void __launch_bounds__(kRowThreads) tree_rows_kernel(const TreeArgs a
 #pragma unroll
     for (int e = 0; e < J * VEC; ++e) acc[r][e] = 0.f;
   }
-  for (int g0 = start + warp * kGroup; g0 < end; g0 += kWarps * kGroup) {
-    const int slot = g0 + own;
-    int64_t at = -1;  // the slot's row of the pages
-    if (slot < end) {
-      const int nth = slot / a.page_size;
-      const int32_t page = __ldg(pages + nth);
-      if (page >= 0 && page < a.num_pages) {
-        at = ((static_cast<int64_t>(page) * a.hkv + kvh) * a.page_size + (slot - nth * a.page_size)) * hd;
-      } else if (sub == 0) {
-        raise_status(a.status, BM_DEVERR_BAD_PAGE);
-      }
-    }
-    uint4 v[kGroup][J];  // V of the eight slots, on its way while the scores are made
-#pragma unroll
-    for (int i = 0; i < kGroup; ++i) {
-      const int64_t vat = __shfl_sync(0xffffffffu, at, i * 4);
-#pragma unroll
-      for (int j = 0; j < J; ++j) {
-        v[i][j] = make_uint4(0u, 0u, 0u, 0u);
-        if (vat >= 0 && lane + 32 * j < cpr) v[i][j] = ld_stream(vp + vat + (lane + 32 * j) * VEC);
-      }
-    }
+  int stage = 0;
+  for (int g0 = first; g0 < end; g0 += kWarps * kGroup) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
+    __syncwarp();  // all lanes' copies of this group are there
+    const T* ks = ring + (stage * 2 * kGroup + own) * hd;
+    const T* vs = ring + (stage * 2 + 1) * kGroup * hd;
     float sc[MR];
 #pragma unroll
     for (int r = 0; r < MR; ++r) sc[r] = 0.f;
-    for (int c0 = sub; c0 < cpr; c0 += 16) {
-      uint4 k[4];
+#pragma unroll 4
+    for (int c = sub; c < cpr; c += 4) {
+      float f[VEC];
+      unpack16<T>(*reinterpret_cast<const uint4*>(ks + (c ^ (own & 1 ? swap : 0)) * VEC), f);
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        k[u] = make_uint4(0u, 0u, 0u, 0u);
-        if (at >= 0 && c0 + 4 * u < cpr) k[u] = ld_stream(kp + at + (c0 + 4 * u) * VEC);
-      }
+      for (int r = 0; r < MR; ++r) {
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        float f[VEC];
-        unpack16<T>(k[u], f);
-        const int col = min(c0 + 4 * u, cpr - 1) * VEC;  // past the row k is 0
-#pragma unroll
-        for (int r = 0; r < MR; ++r) {
-#pragma unroll
-          for (int e = 0; e < VEC; e += 4) {
-            const float4 q4 = *reinterpret_cast<const float4*>(Qs + r * hd + col + e);
-            sc[r] = fmaf(q4.x, f[e], sc[r]);
-            sc[r] = fmaf(q4.y, f[e + 1], sc[r]);
-            sc[r] = fmaf(q4.z, f[e + 2], sc[r]);
-            sc[r] = fmaf(q4.w, f[e + 3], sc[r]);
-          }
+        for (int e = 0; e < VEC; e += 4) {
+          const float4 q4 = *reinterpret_cast<const float4*>(Qs + r * hd + c * VEC + e);
+          sc[r] = fmaf(q4.x, f[e], sc[r]);
+          sc[r] = fmaf(q4.y, f[e + 1], sc[r]);
+          sc[r] = fmaf(q4.z, f[e + 2], sc[r]);
+          sc[r] = fmaf(q4.w, f[e + 3], sc[r]);
         }
       }
     }
-    const int j0 = slot - s.ctx;
-    __syncwarp();  // the last group's weights have been read
+    __syncwarp();  // lanes may have left the loop apart; the last group's weights have been read
+    const bool real = (sound >> stage) & 1;
+    const int j0 = g0 + own - s.ctx;
 #pragma unroll
     for (int r = 0; r < MR; ++r) {
       sc[r] += __shfl_xor_sync(0xffffffffu, sc[r], 1);
       sc[r] += __shfl_xor_sync(0xffffffffu, sc[r], 2);
-      if (at < 0 || r >= rows || (j0 >= 0 && !sees(a, s.row0, (r_lo + r) / a.group, j0))) sc[r] = -INFINITY;
+      if (!real || r >= rows || (j0 >= 0 && !sees(a, s.row0, (r_lo + r) / a.group, j0))) sc[r] = -INFINITY;
+    }
+#pragma unroll
+    for (int r = 0; r < MR; ++r) {
       float mx = sc[r];
 #pragma unroll
       for (int off = 4; off < 32; off <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
@@ -391,8 +416,9 @@ __global__ void __launch_bounds__(kRowThreads) tree_rows_kernel(const TreeArgs a
       }
 #pragma unroll
       for (int j = 0; j < J; ++j) {
+        if (lane + 32 * j >= cpr) continue;
         float f[VEC];
-        unpack16<T>(v[i][j], f);
+        unpack16<T>(*reinterpret_cast<const uint4*>(vs + i * hd + ((lane + 32 * j) ^ (i & 1 ? swap : 0)) * VEC), f);
 #pragma unroll
         for (int r = 0; r < MR; ++r) {
 #pragma unroll
@@ -400,7 +426,11 @@ __global__ void __launch_bounds__(kRowThreads) tree_rows_kernel(const TreeArgs a
         }
       }
     }
+    __syncwarp();  // this group has been read
+    fetch(g0 + kStages * kWarps * kGroup, stage);
+    if (++stage == kStages) stage = 0;
   }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
   // the warps' maxima, sums of weights and of values
 #pragma unroll
   for (int r = 0; r < MR; ++r) {
@@ -411,7 +441,7 @@ __global__ void __launch_bounds__(kRowThreads) tree_rows_kernel(const TreeArgs a
       ml[(kWarps + warp) * MR + r] = l[r];
     }
   }
-  __syncthreads();  // Q has been read, too
+  __syncthreads();  // the rings have been read
 #pragma unroll
   for (int r = 0; r < MR; ++r) {
 #pragma unroll
@@ -541,7 +571,7 @@ int launch(TreeArgs a, cudaStream_t stream, const char* what) {
   };
   auto few = [&](auto mr) {
     constexpr int MR = decltype(mr)::value;
-    const int smem = (kRowThreads / 32 * MR * (a.hd + kGroup) + 2 * (kRowThreads / 32) * MR) * 4;
+    const int smem = rows_smem(a.hd, sizeof(T), MR);
     const int64_t grid = a.batch * a.hkv * a.row_tiles * a.splits;
     auto kernel = a.hd / VecWidth<T>::value <= 32 ? tree_rows_kernel<T, MR, 1> : tree_rows_kernel<T, MR, 2>;
     if (int st = allow_dynamic_smem(reinterpret_cast<const void*>(kernel), smem, what)) return st;
