@@ -10,11 +10,12 @@
 // Bound: with R = group * n rows per kv head a slot costs 4 R hd operations and
 // 2 hd * es bytes, so few rows are bound by memory and many, in fp32 on CUDA cores, by
 // the multiply-adds. All rows of a kv head therefore share a CTA's tile of K and V
-// (32 or 64 rows against 64 slots), and both products run from shared memory in
-// register tiles (4 x 4 scores and 4 x hd/16 outputs per thread for 64 rows), 64
-// multiply-adds for 8 16-byte shared loads. Slots are shared out over CTAs when the
-// (sequence, kv head) pairs do not fill the GPU; the shares' partial sums meet in
-// tree_combine_kernel.
+// (64 rows against 64 slots), and both products run from shared memory in register
+// tiles (4 x 4 scores and 4 x hd/16 outputs per thread), 64 multiply-adds for 8 16-byte
+// shared loads; up to 32 rows have a kernel of their own, bound by its shared loads of Q
+// (8 rows of 128 in fp32 over 16 sequences of 1000 to 2000, 8 heads: 82 us, floor 30). Slots
+// are shared out over CTAs when the (sequence, kv head, row tile) triples do not fill the
+// GPU; the shares' partial sums meet in tree_combine_kernel.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -26,11 +27,11 @@ namespace paged {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int BM = 64;   // query rows of a CTA
 constexpr int kBN = 64;  // slots per tile
 
-// BM: query rows of a CTA. NJ: 16-byte groups of four outputs a thread owns per row,
-// ceil(hd / 64).
-template <typename T, int BM, int NJ>
+// NJ: 16-byte groups of four outputs a thread owns per row, ceil(hd / 64).
+template <typename T, int NJ>
 __global__ void __launch_bounds__(kThreads) tree_attention_kernel(const TreeArgs a) {
   grid_dependency_wait();
   constexpr int MR = BM / 16;
@@ -243,10 +244,12 @@ __global__ void __launch_bounds__(kThreads) tree_attention_kernel(const TreeArgs
 
 // Few rows (MR at most): each warp walks groups of eight slots of its own with its own
 // running softmax; K and V of the next groups are on their way into its ring of shared
-// memory (cp.async) meanwhile, and no barrier but the warp's own stands between. A lane
-// makes a quarter of its slot's score and owns 16-byte chunks of every row of V; the four
-// warps' sums meet at the end. The tiled kernel above would read its shared K and V eight
-// times over for a few rows. J: 16-byte chunks of a row of V per lane.
+// memory (cp.async) meanwhile, and no barrier but the warp's own stands between. Four lanes
+// share a slot: each makes a quarter of all its scores, then, these summed up, weighs a
+// quarter of the rows; and a lane owns 16-byte chunks of every row of V. Multiply-adds go
+// two to an instruction. The four warps' sums meet at the end. The tiled kernel above would
+// read its shared K and V eight times over for a few rows. J: 16-byte chunks of a row of V
+// per lane.
 constexpr int kRowThreads = 128;
 constexpr int kGroup = 8;   // slots of a warp's step
 constexpr int kStages = 2;  // groups of a warp in flight or in use
@@ -262,6 +265,20 @@ __device__ __forceinline__ void copy16_async(void* to, const void* from, bool re
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(to))),
                "l"(from), "r"(real ? 16 : 0)
                : "memory");
+}
+
+// A 16-byte chunk as pairs of fp32.
+template <typename T>
+__device__ __forceinline__ void unpack_pairs(const uint4& raw, uint64_t* f) {
+  if constexpr (sizeof(T) == 4) {
+    f[0] = pair(raw.x, raw.y);
+    f[1] = pair(raw.z, raw.w);
+  } else {
+    f[0] = pair(bf16_lo(raw.x), bf16_hi(raw.x));
+    f[1] = pair(bf16_lo(raw.y), bf16_hi(raw.y));
+    f[2] = pair(bf16_lo(raw.z), bf16_hi(raw.z));
+    f[3] = pair(bf16_lo(raw.w), bf16_hi(raw.w));
+  }
 }
 
 template <typename T, int MR, int J>
@@ -346,13 +363,20 @@ __global__ void __launch_bounds__(kRowThreads) tree_rows_kernel(const TreeArgs a
   }
   __syncthreads();
 
-  float m[MR], l[MR], acc[MR][J * VEC];
+  constexpr int RL = MR / 4;        // rows that a lane weighs for its slot, from
+  const int r_own = sub * RL;       // this one on
+  constexpr int P2 = J * VEC / 2;   // pairs of a row's dims that a lane owns
+  float m[RL], l[RL];
+  uint64_t acc[MR][P2];
 #pragma unroll
-  for (int r = 0; r < MR; ++r) {
+  for (int r = 0; r < RL; ++r) {
     m[r] = -INFINITY;
     l[r] = 0.f;
+  }
 #pragma unroll
-    for (int e = 0; e < J * VEC; ++e) acc[r][e] = 0.f;
+  for (int r = 0; r < MR; ++r) {
+#pragma unroll
+    for (int e = 0; e < P2; ++e) acc[r][e] = 0;
   }
   int stage = 0;
   for (int g0 = first; g0 < end; g0 += kWarps * kGroup) {
@@ -360,69 +384,89 @@ __global__ void __launch_bounds__(kRowThreads) tree_rows_kernel(const TreeArgs a
     __syncwarp();  // all lanes' copies of this group are there
     const T* ks = ring + (stage * 2 * kGroup + own) * hd;
     const T* vs = ring + (stage * 2 + 1) * kGroup * hd;
-    float sc[MR];
+    uint64_t s2[MR];
 #pragma unroll
-    for (int r = 0; r < MR; ++r) sc[r] = 0.f;
+    for (int r = 0; r < MR; ++r) s2[r] = 0;
 #pragma unroll 4
     for (int c = sub; c < cpr; c += 4) {
-      float f[VEC];
-      unpack16<T>(*reinterpret_cast<const uint4*>(ks + (c ^ (own & 1 ? swap : 0)) * VEC), f);
+      uint64_t k2[VEC / 2];
+      unpack_pairs<T>(*reinterpret_cast<const uint4*>(ks + (c ^ (own & 1 ? swap : 0)) * VEC), k2);
 #pragma unroll
       for (int r = 0; r < MR; ++r) {
 #pragma unroll
         for (int e = 0; e < VEC; e += 4) {
-          const float4 q4 = *reinterpret_cast<const float4*>(Qs + r * hd + c * VEC + e);
-          sc[r] = fmaf(q4.x, f[e], sc[r]);
-          sc[r] = fmaf(q4.y, f[e + 1], sc[r]);
-          sc[r] = fmaf(q4.z, f[e + 2], sc[r]);
-          sc[r] = fmaf(q4.w, f[e + 3], sc[r]);
+          const ulonglong2 q4 = *reinterpret_cast<const ulonglong2*>(Qs + r * hd + c * VEC + e);
+          s2[r] = fma2(q4.x, k2[e / 2], s2[r]);
+          s2[r] = fma2(q4.y, k2[e / 2 + 1], s2[r]);
         }
       }
     }
     __syncwarp();  // lanes may have left the loop apart; the last group's weights have been read
+    float sc[MR];
+#pragma unroll
+    for (int r = 0; r < MR; ++r) {
+      const float2 two = unpair(s2[r]);
+      sc[r] = two.x + two.y;
+    }
+    // the four quarters' sums: half of the rows stay with a lane, then half of these
+#pragma unroll
+    for (int keep = MR / 2; keep >= RL; keep /= 2) {
+      const int bit = keep == MR / 2 ? 2 : 1;
+      const bool upper = sub & bit;
+#pragma unroll
+      for (int r = 0; r < keep; ++r) {
+        const float give = upper ? sc[r] : sc[r + keep], have = upper ? sc[r + keep] : sc[r];
+        sc[r] = have + __shfl_xor_sync(0xffffffffu, give, bit);
+      }
+    }
     const bool real = (sound >> stage) & 1;
     const int j0 = g0 + own - s.ctx;
+    float alpha[RL], p[RL];
+    bool rise = false;
 #pragma unroll
-    for (int r = 0; r < MR; ++r) {
-      sc[r] += __shfl_xor_sync(0xffffffffu, sc[r], 1);
-      sc[r] += __shfl_xor_sync(0xffffffffu, sc[r], 2);
-      if (!real || r >= rows || (j0 >= 0 && !sees(a, s.row0, (r_lo + r) / a.group, j0))) sc[r] = -INFINITY;
-    }
-#pragma unroll
-    for (int r = 0; r < MR; ++r) {
+    for (int r = 0; r < RL; ++r) {
+      if (!real || r_own + r >= rows || (j0 >= 0 && !sees(a, s.row0, (r_lo + r_own + r) / a.group, j0))) sc[r] = -INFINITY;
       float mx = sc[r];
 #pragma unroll
       for (int off = 4; off < 32; off <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
       const float m_new = fmaxf(m[r], mx);
       const float base = m_new == -INFINITY ? 0.f : m_new;
-      const float alpha = exp2f(m[r] - base), p = exp2f(sc[r] - base);
+      rise = rise || m_new > m[r];
+      alpha[r] = exp2f(m[r] - base);
+      p[r] = exp2f(sc[r] - base);
       m[r] = m_new;
-      l[r] = l[r] * alpha + p;  // this slot's share, the same in its four lanes
-      if (sub == 0) Ps[own * MR + r] = p;
+      l[r] = l[r] * alpha[r] + p[r];  // this slot's share
+      Ps[own * MR + r_own + r] = p[r];
+    }
+    if (__any_sync(0xffffffffu, rise)) {
 #pragma unroll
-      for (int e = 0; e < J * VEC; ++e) acc[r][e] *= alpha;
+      for (int r = 0; r < MR; ++r) {
+        const float f = __shfl_sync(0xffffffffu, alpha[r % RL], r / RL);
+#pragma unroll
+        for (int e = 0; e < P2; ++e) acc[r][e] = mul2(acc[r][e], pair(f, f));
+      }
     }
     __syncwarp();
 #pragma unroll
     for (int i = 0; i < kGroup; ++i) {
-      float p[MR];
+      uint64_t w[MR];
 #pragma unroll
       for (int r = 0; r < MR; r += 4) {
         const float4 p4 = *reinterpret_cast<const float4*>(Ps + i * MR + r);
-        p[r] = p4.x;
-        p[r + 1] = p4.y;
-        p[r + 2] = p4.z;
-        p[r + 3] = p4.w;
+        w[r] = pair(p4.x, p4.x);
+        w[r + 1] = pair(p4.y, p4.y);
+        w[r + 2] = pair(p4.z, p4.z);
+        w[r + 3] = pair(p4.w, p4.w);
       }
 #pragma unroll
       for (int j = 0; j < J; ++j) {
         if (lane + 32 * j >= cpr) continue;
-        float f[VEC];
-        unpack16<T>(*reinterpret_cast<const uint4*>(vs + i * hd + ((lane + 32 * j) ^ (i & 1 ? swap : 0)) * VEC), f);
+        uint64_t v2[VEC / 2];
+        unpack_pairs<T>(*reinterpret_cast<const uint4*>(vs + i * hd + ((lane + 32 * j) ^ (i & 1 ? swap : 0)) * VEC), v2);
 #pragma unroll
         for (int r = 0; r < MR; ++r) {
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) acc[r][j * VEC + e] = fmaf(p[r], f[e], acc[r][j * VEC + e]);
+          for (int e = 0; e < VEC / 2; ++e) acc[r][j * VEC / 2 + e] = fma2(w[r], v2[e], acc[r][j * VEC / 2 + e]);
         }
       }
     }
@@ -433,12 +477,12 @@ __global__ void __launch_bounds__(kRowThreads) tree_rows_kernel(const TreeArgs a
   asm volatile("cp.async.wait_group 0;" ::: "memory");
   // the warps' maxima, sums of weights and of values
 #pragma unroll
-  for (int r = 0; r < MR; ++r) {
+  for (int r = 0; r < RL; ++r) {
 #pragma unroll
     for (int off = 4; off < 32; off <<= 1) l[r] += __shfl_xor_sync(0xffffffffu, l[r], off);
-    if (lane == 0) {
-      ml[warp * MR + r] = m[r];
-      ml[(kWarps + warp) * MR + r] = l[r];
+    if (own == 0) {
+      ml[warp * MR + r_own + r] = m[r];
+      ml[(kWarps + warp) * MR + r_own + r] = l[r];
     }
   }
   __syncthreads();  // the rings have been read
@@ -449,8 +493,8 @@ __global__ void __launch_bounds__(kRowThreads) tree_rows_kernel(const TreeArgs a
       if (lane + 32 * j < cpr) {
 #pragma unroll
         for (int e = 0; e < VEC; e += 4) {
-          *reinterpret_cast<float4*>(smem + (warp * MR + r) * hd + (lane + 32 * j) * VEC + e) =
-              make_float4(acc[r][j * VEC + e], acc[r][j * VEC + e + 1], acc[r][j * VEC + e + 2], acc[r][j * VEC + e + 3]);
+          *reinterpret_cast<ulonglong2*>(smem + (warp * MR + r) * hd + (lane + 32 * j) * VEC + e) =
+              make_ulonglong2(acc[r][(j * VEC + e) / 2], acc[r][(j * VEC + e) / 2 + 1]);
         }
       }
     }
@@ -534,8 +578,12 @@ __global__ void __launch_bounds__(kThreads) tree_combine_kernel(const TreeArgs a
   }
 }
 
-// Rows of a CTA: 4 and 8 are tree_rows_kernel's, the others the tiled kernel's.
-int rows_per_tile(int rows) { return rows > 32 ? 64 : rows > 16 ? 32 : rows > 4 ? 8 : 4; }
+// Rows of a CTA: 4 and 8 are tree_rows_kernel's, the others the tiled kernel's. Up to 32
+// rows, tiles of 8 of them beat a tiled kernel cut to 32 rows (16 sequences of 1000 to 2000,
+// 8 heads: 24 rows of 128 in fp32 193 against 244 us, 32 rows of 256 in bf16 361 against 563,
+// though 32 rows of 128 in fp32 268 against 255); a tile of 8 for 4 rows costs twice as much
+// (4 rows of 256 in bf16: 210 against 107 us).
+int rows_per_tile(int rows) { return rows > 32 ? BM : rows > 4 ? 8 : 4; }
 
 // The CUDA-core form's split: enough CTAs for four per SM (eight of the few-row kernel's),
 // none shorter than a tile.
@@ -551,11 +599,11 @@ void plan(int64_t batch, int hkv, int group, int max_ctx, int max_tree, int* row
   *splits = (len + *split_len - 1) / *split_len;
 }
 
-template <typename T, int BM, int NJ>
+template <typename T, int NJ>
 int launch_one(const TreeArgs& a, cudaStream_t stream, const char* what) {
   const int ld = a.hd + 4;
   const int smem = ((BM + 2 * kBN) * ld + BM * (kBN + 4) + kBN) * 4;
-  auto kernel = tree_attention_kernel<T, BM, NJ>;
+  auto kernel = tree_attention_kernel<T, NJ>;
   if (int st = allow_dynamic_smem(reinterpret_cast<const void*>(kernel), smem, what)) return st;
   const int64_t grid = a.batch * a.hkv * a.row_tiles * a.splits;
   return launch_kernel(what, kernel, dim3(static_cast<unsigned>(grid)), dim3(kThreads), smem, stream, nullptr, a);
@@ -564,22 +612,23 @@ int launch_one(const TreeArgs& a, cudaStream_t stream, const char* what) {
 template <typename T>
 int launch(TreeArgs a, cudaStream_t stream, const char* what) {
   const int nj = (a.hd + 63) / 64;
-  auto by_width = [&](auto bm) {
-    constexpr int BM = decltype(bm)::value;
-    return nj == 1 ? launch_one<T, BM, 1>(a, stream, what) : nj == 2 ? launch_one<T, BM, 2>(a, stream, what)
-                                                                   : launch_one<T, BM, 4>(a, stream, what);
-  };
   auto few = [&](auto mr) {
     constexpr int MR = decltype(mr)::value;
     const int smem = rows_smem(a.hd, sizeof(T), MR);
     const int64_t grid = a.batch * a.hkv * a.row_tiles * a.splits;
-    auto kernel = a.hd / VecWidth<T>::value <= 32 ? tree_rows_kernel<T, MR, 1> : tree_rows_kernel<T, MR, 2>;
+    auto kernel = tree_rows_kernel<T, MR, 1>;
+    if constexpr (sizeof(T) == 4) {
+      if (a.hd > 128) kernel = tree_rows_kernel<T, MR, 2>;
+    }
     if (int st = allow_dynamic_smem(reinterpret_cast<const void*>(kernel), smem, what)) return st;
     return launch_kernel(what, kernel, dim3(static_cast<unsigned>(grid)), dim3(kRowThreads), smem, stream, nullptr, a);
   };
   const int rows = rows_per_tile(a.group * a.max_tree);
-  const int st = rows == 4 ? few(std::integral_constant<int, 4>{}) : rows == 8 ? few(std::integral_constant<int, 8>{})
-                 : rows == 32 ? by_width(std::integral_constant<int, 32>{}) : by_width(std::integral_constant<int, 64>{});
+  const int st = rows == 4   ? few(std::integral_constant<int, 4>{})
+                 : rows == 8 ? few(std::integral_constant<int, 8>{})
+                 : nj == 1   ? launch_one<T, 1>(a, stream, what)
+                 : nj == 2   ? launch_one<T, 2>(a, stream, what)
+                             : launch_one<T, 4>(a, stream, what);
   if (st != BM_OK || a.splits == 1) return st;
   const int64_t warps = a.batch * a.max_tree * a.hq;
   const int64_t grid = (warps + kThreads / 32 - 1) / (kThreads / 32);
