@@ -948,35 +948,52 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(const TreeArgs a, int c
     const int tile = r / kTile, rr = r - tile * kTile;
     const int i0 = rec.p * tpt * L::kTiles + tile * tpt;
     if (rr >= max(0, min(tpt, s.n - i0)) * a.group) continue;
-    float m = -INFINITY;
-    for (int c = k - 1 + lane; c < last; c += 32) m = fmaxf(m, part(c)[L::kRows * HD + r]);
+    // the first parts' maxima, sums and values at once: two parts are all there is, mostly
+    constexpr int kDims = HD / kLanes;  // 4 or 8 dims of a thread
+    const int d = lane % kLanes * kDims, half = lane / kLanes;
+    auto values = [&](int c, int e) { return *reinterpret_cast<const float4*>(part(min(c, last - 1)) + r * HD + d + e); };
+    const bool own = k - 1 + lane < last;
+    const float own_m = own ? part(k - 1 + lane)[L::kRows * HD + r] : -INFINITY;
+    const float own_l = own ? part(k - 1 + lane)[L::kRows * (HD + 1) + r] : 0.f;
+    float4 own_v[kDims / 4];
+#pragma unroll
+    for (int e = 0; e < kDims; e += 4) own_v[e / 4] = values(k - 1 + half, e);
+    float m = own_m;
+    for (int c = k - 1 + lane + 32; c < last; c += 32) m = fmaxf(m, part(c)[L::kRows * HD + r]);
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
     const float base = m == -INFINITY ? 0.f : m;
-    constexpr int kDims = HD / kLanes;  // 4 or 8 dims of a thread
-    const int d = lane % kLanes * kDims, half = lane / kLanes;
     float l = 0.f, o[kDims];
 #pragma unroll
     for (int e = 0; e < kDims; ++e) o[e] = 0.f;
+    auto add = [&](const float4& v, float w, int e) {
+      o[e] = fmaf(v.x, w, o[e]);
+      o[e + 1] = fmaf(v.y, w, o[e + 1]);
+      o[e + 2] = fmaf(v.z, w, o[e + 2]);
+      o[e + 3] = fmaf(v.w, w, o[e + 3]);
+    };
     for (int c0 = k - 1; c0 < last; c0 += 32) {
       float f = 0.f;  // of part c0 + lane
-      if (c0 + lane < last) {
+      if (c0 == k - 1) {
+        f = ex2(own_m - base);
+        l = own_l * f;
+      } else if (c0 + lane < last) {
         f = ex2(part(c0 + lane)[L::kRows * HD + r] - base);
         l = fmaf(part(c0 + lane)[L::kRows * (HD + 1) + r], f, l);
       }
       const int n = min(32, last - c0);
-#pragma unroll 8
-      for (int i = half; i < n + half; i += 2) {
-        const float w = __shfl_sync(0xffffffffu, f, i & 31);  // past n: 0
-        const float* ps = part(min(c0 + i, last - 1)) + r * HD + d;
+      int i = half;
+      if (c0 == k - 1) {
+        const float w = __shfl_sync(0xffffffffu, f, i);  // past n: 0
 #pragma unroll
-        for (int e = 0; e < kDims; e += 4) {
-          const float4 v = *reinterpret_cast<const float4*>(ps + e);
-          o[e] = fmaf(v.x, w, o[e]);
-          o[e + 1] = fmaf(v.y, w, o[e + 1]);
-          o[e + 2] = fmaf(v.z, w, o[e + 2]);
-          o[e + 3] = fmaf(v.w, w, o[e + 3]);
-        }
+        for (int e = 0; e < kDims; e += 4) add(own_v[e / 4], w, e);
+        i += 2;
+      }
+#pragma unroll 8
+      for (; i < n + half; i += 2) {
+        const float w = __shfl_sync(0xffffffffu, f, i & 31);
+#pragma unroll
+        for (int e = 0; e < kDims; e += 4) add(values(c0 + i, e), w, e);
       }
     }
 #pragma unroll
