@@ -21,7 +21,10 @@
 // rows would leave idle is the softmax: a thread walks its row's 128 scores however few
 // rows there are. So with at most 64 (32) rows the row tile holds them twice (four times),
 // and each copy weighs a half (quarter) of the tile's slots, with zero weights elsewhere;
-// the copies' sums meet at the segment's end.
+// the copies' sums meet at the segment's end. Measured on a B200 with both launches: 64
+// sequences of 1 to 8192 and up to 8 drafted tokens, 32 / 8 heads of 128: 181 us (1.03 GB,
+// floor 157; one copy everywhere 197); 16 of 4096 to 8192 and 64, 64 / 8 heads: 241 us (floor
+// 124 by products, 120 by bytes); one of 8000 and 12: 23 us (floor 5).
 //
 // Split: the host does not see the lengths, so one CTA per SM takes an equal share of
 // all tiles of the batch, counted on the device: items (sequence, kv head, row tile) laid

@@ -16,7 +16,9 @@
 // or one of `parts` shares of a token's heads when there are few tokens: a decode
 // batch is bound by the chain position -> (cos, sin), sequence -> page -> store, which
 // more warps with one pass each overlap. Data loads are issued before that chain is
-// waited for.
+// waited for. Measured on a B200, bf16: 16384 rows of 64 + 8 heads of 128 in 103 us (604 MB,
+// 0.90 of the copy rate), 32768 rows of 64 + 8 appended to pages of 64 in 226 us (0.91), a
+// decode batch of 64 rows in 3.5 us either way.
 #include <algorithm>
 #include <cmath>
 
