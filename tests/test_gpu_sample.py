@@ -200,3 +200,25 @@ def test_ties_between_two_bins_of_the_histogram(cuda):
     s = dict(temperature=torch.tensor([float(t) for t, _ in found]), top_k=None, top_p=torch.tensor(p).float(), min_p=None)
     for u in (0.999, 0.9999, 1 - 2.0 ** -24):
         check(cuda, torch.from_numpy(x).to(BF16), torch.full((rows,), u), s)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("vocab", [1025, 5000, 40000])
+def test_infinities_and_temperatures_of_long_rows(cuda, vocab, dtype):
+    """The edges of the settings where a row is shared by warps or CTAs."""
+    inf, nan = math.inf, math.nan
+    g = gen(vocab)
+    heads = [[-inf] * 6, [nan] * 6, [nan, -inf, 1.0, nan, -inf, -inf], [inf, 1.0, inf, nan, -inf, inf], [-inf, inf, 3.0, 4.0, 5.0, 6.0]]
+    x = torch.full((100, vocab), -inf)
+    for r in range(100):
+        at = torch.randperm(vocab, generator=g)
+        x[r, at[:6]] = torch.tensor(heads[r % 5])
+        if r % 2:
+            x[r, at[6:vocab // 2]] = torch.randn(vocab // 2 - 6, generator=g) * 3
+    x = x.to(dtype)
+    check(cuda, x, torch.rand(100, generator=g), settings(100, g, "tkpm"))
+    x = (torch.randn(24, vocab, generator=g) * 3).to(dtype)
+    x[:, 5] = -inf
+    t = torch.tensor([0.0, 1e-45, 1e-30, 1e-6, 1e-3, 1e3, 1e30, inf, 0.0, 2.0, inf, 1.0]).repeat(2)
+    for which in ("", "kpm"):
+        check(cuda, x, torch.rand(24, generator=g), dict(settings(24, g, which), temperature=t))

@@ -263,3 +263,30 @@ def test_nothing_to_do(cuda):
     out = torch.full((3, 4, 128), 5.0, dtype=BF16, device=cuda)
     ops.paged_tree_attention(torch.zeros_like(out), b.cache, i32([5], cuda), i32([1, 1], cuda), 8, 4, out=out)
     assert bool((out == 5.0).all())
+
+
+def test_two_streams_at_once(cuda):
+    """Calls that overlap on the GPU, a workspace each: the same results as one after the other."""
+    batches = [Batch(cuda, [(3000, 3), (1500, 2), (17, 4)], 8, 2, 128, 16, BF16, seed=17),
+               Batch(cuda, [(900, 30), (2000, 5)], 8, 2, 64, 32, BF16, seed=18),
+               Batch(cuda, [(700, 4), (90, 9)], 4, 2, 48, 16, F32, seed=19)]
+    first = [b.check() for b in batches]
+    calls = []
+    for b in batches:
+        q = b.q.to(cuda)
+        args = (q, b.cache, i32([c for c, _ in b.lens], cuda), i32(b.starts, cuda), b.max_ctx, b.max_tree)
+        kw = [dict(tree_mask=b.mask.to(cuda), out=torch.empty_like(q),
+                   workspace=ops.paged_tree_attention_workspace(q, b.cache, len(b.lens), b.max_ctx, b.max_tree))
+              for _ in range(3)]
+        calls.append((args, kw))
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    torch.cuda.synchronize()
+    for turn in range(10):
+        for s, stream in enumerate(streams):
+            for i in range(3):
+                args, kw = calls[(s + i) % 3]
+                ops.paged_tree_attention(*args, stream=stream, **kw[s])
+    torch.cuda.synchronize()
+    for (args, kw), want in zip(calls, first):
+        for k in kw:
+            assert bits_equal(k["out"], want)
