@@ -16,9 +16,9 @@
 // Bound: a row is read from HBM once (the passes below find it in L2), so bytes count
 // only for many rows; there the fp64 operations (eleven a logit where all weigh) cost as
 // much, and one or few rows are bound by the chain of passes. Measured on a B200 with
-// top-p alone: 21 us for one fp32 row of 32000, 28 for one of 128256 and 201 for 256 bf16
-// rows of 128256 (floor 10; 94 without top-p); all settings mixed by row, fp32: 19 us for
-// 8 rows of 128256, 52 for 64 (floor 5). A row of up to 1024 logits stays in one CTA's
+// top-p alone: 21 us for one fp32 row of 32000, 28 for one of 128256 and 193 for 256 bf16
+// rows of 128256 (floor 10; 96 without top-p); all settings mixed by row, fp32: 19 us for
+// 8 rows of 128256, 44 for 64 (floor 5). A row of up to 1024 logits stays in one CTA's
 // registers (12 us for 256 rows of 1000; 22 with the passes). A cluster of up to 8 CTAs
 // shares a longer row:
 //   1. the largest logit and its first index;
@@ -1081,11 +1081,14 @@ extern "C" int bm_sample(int32_t* tokens, const void* logits, const float* unifo
   a.vec = aligned16(logits) && row_stride * es % 16 == 0;
   a.status = d_status;
   // CTAs per row: as many as leave every SM at most one, with all the registers they like;
-  // twice as many, at half the registers, where a CTA had more than 16384 logits (64 rows
-  // of 128256: 53 against 64 us; 32 rows of 32000: 31 against 27). None with fewer than 2048.
+  // then twice as many, at half the registers, while a CTA has more than 16384 logits and an
+  // SM gets at most four (rows cost unevenly and SMs fill unevenly: 64 mixed rows of 128256
+  // with 4 CTAs 51, with 8 44 us; 256 rows of 128256 with 1 and 2: top-k 126 and 105, top-p 199
+  // and 193, no filter 94 and 96; 128 rows of 32000 with 2 and 4: 38 and 44). None with fewer
+  // than 2048.
   int c = 1;
   while (c < kMaxCluster && rows * c * 2 <= sm_count() && vocab >= int64_t{2048} * c * 2) c *= 2;
-  if (c < kMaxCluster && rows * c * 2 <= 2 * sm_count() && vocab > int64_t{16384} * c) c *= 2;
+  while (c < kMaxCluster && rows * c * 2 <= 4 * sm_count() && vocab > int64_t{16384} * c) c *= 2;
   const bool crowded = rows * c > sm_count();
   a.chunk = static_cast<int>(((vocab + c - 1) / c + 7) / 8 * 8);
   a.unit = 16;
