@@ -16,8 +16,8 @@
 // or one of `parts` shares of a token's heads when there are few tokens: a decode
 // batch is bound by the chain position -> (cos, sin), sequence -> page -> store, which
 // more warps with one pass each overlap. Data loads are issued before that chain is
-// waited for. Measured on a B200, bf16: 16384 rows of 64 + 8 heads of 128 in 103 us (604 MB,
-// 0.90 of the copy rate), 32768 rows of 64 + 8 appended to pages of 64 in 226 us (0.91), a
+// waited for. Measured on a B200, bf16: 16384 rows of 64 + 8 heads of 128 in 100 us (604 MB,
+// 0.92 of the copy rate), 32768 rows of 64 + 8 appended to pages of 64 in 223 us (0.92), a
 // decode batch of 64 rows in 3.5 us either way.
 #include <algorithm>
 #include <cmath>
@@ -29,7 +29,7 @@ namespace bm {
 namespace {
 
 constexpr int kMaxHeadDim = 1024;
-constexpr int kThreads = 256;
+constexpr int kThreads = 128;  // 256: 1 to 3 % slower on prompts
 
 struct RotaryArgs {
   void* q_out;
@@ -251,7 +251,7 @@ int launch(RotaryArgs a, bool interleaved, bm_dtype_t dtype, cudaStream_t stream
   // tokens are shared out over up to 8 warps each.
   a.parts = static_cast<int>(std::min<int64_t>(8, std::max<int64_t>(1, 2048 / std::max<int64_t>(1, a.rows))));
   const int64_t blocks = (a.rows * a.parts + kThreads / 32 - 1) / (kThreads / 32);
-  const dim3 grid(static_cast<unsigned>(std::min<int64_t>(blocks, static_cast<int64_t>(sm_count()) * 16)));
+  const dim3 grid(static_cast<unsigned>(std::min<int64_t>(blocks, static_cast<int64_t>(sm_count()) * 32)));
   auto go = [&](auto kernel) { return launch_kernel(what, kernel, grid, dim3(kThreads), 0, stream, nullptr, a); };
   if (dtype == BM_F32) {
     if (n == 4) return interleaved ? go(rotary_kernel<float, 4, true, PAGED>) : go(rotary_kernel<float, 4, false, PAGED>);
