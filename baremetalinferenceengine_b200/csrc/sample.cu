@@ -68,7 +68,7 @@ struct SampleArgs {
   int vocab;
   int bits;   // the largest weight is 2^bits
   int chunk;  // logits of a row per CTA of the cluster
-  int unit;   // bits of a fp32 weight in the histogram: chunk * 2^unit < 2^32
+  int unit;   // bits of a fp32 weight in the histogram: chunk * 2^unit * 129 / 128 < 2^32
   bool vec;   // rows are 16-byte aligned
   int32_t* status;
 };
@@ -1091,8 +1091,12 @@ extern "C" int bm_sample(int32_t* tokens, const void* logits, const float* unifo
   while (c < kMaxCluster && rows * c * 2 <= 4 * sm_count() && vocab > int64_t{16384} * c) c *= 2;
   const bool crowded = rows * c > sm_count();
   a.chunk = static_cast<int>(((vocab + c - 1) / c + 7) / 8 * 8);
+  // A bin of the histogram holds a CTA's whole stretch without passing 32 bits. A weight is at
+  // most 2^unit (1 + 0.35 / 77) + 0.5: half a bin above its middle (0.5 ln 2 of an octave's 77
+  // bins or more: kLimit / (51 + 2)), and rounded, where unit is 7 at least (and then an octave has
+  // 102 bins): below 2^unit * 129 / 128.
   a.unit = 16;
-  while ((static_cast<int64_t>(a.chunk) << a.unit) >= int64_t{1} << 32) --a.unit;
+  while ((static_cast<int64_t>(a.chunk) * 129 << a.unit) >= int64_t{128} << 32) --a.unit;
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeClusterDimension;
   attr.val.clusterDim.x = static_cast<unsigned>(c);

@@ -222,3 +222,36 @@ def test_infinities_and_temperatures_of_long_rows(cuda, vocab, dtype):
     t = torch.tensor([0.0, 1e-45, 1e-30, 1e-6, 1e-3, 1e3, 1e30, inf, 0.0, 2.0, inf, 1.0]).repeat(2)
     for which in ("", "kpm"):
         check(cuda, x, torch.rand(24, generator=g), dict(settings(24, g, which), temperature=t))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows,vocab", [(300, 65400), (300, 65528), (150, 130900), (300, 131000), (8, 65528)])
+def test_rows_of_one_bin(cuda, rows, vocab, dtype):
+    """A few largest logits and all others equal: nearly the whole of a CTA's stretch falls into
+    one bin of top-p's histogram, in the half of it whose weights are above its middle's, at
+    stretches just below a power of two. The bulk's places in the histogram are in bins of
+    their own order, from the first few to the last that has much weight."""
+    bits = min(51, 62 - math.ceil(math.log2(vocab)))
+    per_logit = 1.4426950408889634 * 4094.5 / (bits + 2)
+    gaps = torch.linspace(0.02, 12.0, 6000).to(dtype).float().unique()
+    part = (gaps.double() * per_logit) % 1
+    gaps = gaps[(part > 0.505) & (part < 0.56)]
+    gaps = gaps[torch.linspace(0, len(gaps) - 1, 5).long()]
+    x, p, u = [], [], []
+    for gap in gaps.tolist():
+        top = max(1, round(vocab * math.exp(-gap) / 3))  # the bulk has about three quarters of the row
+        row = torch.full((vocab,), 2.0 - gap).to(dtype)
+        row[torch.randperm(vocab, generator=gen(top))[:top]] = 2.0
+        below = 2.0 - float(row.float().min())  # after its rounding
+        share = top / (top + (vocab - top) * math.exp(-below))
+        for at in (0.6 * share, share + 0.3 * (1 - share), share + 0.8 * (1 - share)):
+            x.append(row)
+            p.append(at)
+            u.append(0.9)
+    n = len(x)
+    x, p, u = torch.stack(x), torch.tensor(p), torch.tensor(u)
+    none = dict(temperature=None, top_k=None, min_p=None)
+    want = torch.tensor(ref.sample(x, u, top_p=p, **none), dtype=torch.int32)
+    pick = torch.arange(rows) % n
+    got = ops.sample(x.to(cuda)[pick.to(cuda)], u[pick].to(cuda), top_p=p[pick].to(cuda)).cpu()
+    assert torch.equal(got, want[pick])
