@@ -216,35 +216,54 @@ PyObject* rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
-const bm_paged_kv_t* cache_of(PyObject* address) {
-  return reinterpret_cast<const bm_paged_kv_t*>(static_cast<uintptr_t>(integer(address, "cache")));
+// The cache as its tensors are now: k_pages, v_pages, page_table.
+struct Cache {
+  const at::Tensor& k;
+  bm_paged_kv_t c;
+};
+int32_t size32(const at::Tensor& t, int64_t dim, const char* name) {
+  if (t.size(dim) > INT32_MAX) invalid("%s has more than 2^31 - 1 entries in a dimension", name);
+  return static_cast<int32_t>(t.size(dim));
+}
+Cache cache_of(PyObject* k_pages, PyObject* v_pages, PyObject* page_table) {
+  const at::Tensor &k = required(k_pages, "k_pages"), &v = required(v_pages, "v_pages"), &t = required(page_table, "page_table");
+  if (k.dim() != 4 || v.sizes() != k.sizes() || !k.is_contiguous() || !v.is_contiguous() || v.scalar_type() != k.scalar_type() ||
+      v.device() != k.device()) {
+    invalid("k_pages and v_pages must be contiguous [num_pages, kv_heads, page_size, head_dim] of one dtype and device");
+  }
+  if (t.dim() != 2 || t.scalar_type() != at::kInt || !t.is_contiguous() || t.device() != k.device()) {
+    invalid("page_table must be a contiguous int32 tensor [num_seqs, max_pages] on the pages' device");
+  }
+  return Cache{k, {k.data_ptr(), v.data_ptr(), static_cast<const int32_t*>(t.data_ptr()), size32(k, 0, "k_pages"),
+                   size32(k, 2, "k_pages"), size32(t, 1, "page_table"), size32(t, 0, "page_table"), size32(k, 1, "k_pages"),
+                   size32(k, 3, "k_pages")}};
 }
 
-// q, k, v, positions, slots, seq_ids, cache, k_pages, table, max_pos, rotary_dim, interleaved,
-// q_out, status, stream
+// q, k, v, positions, slots, seq_ids, k_pages, v_pages, page_table, table, max_pos, rotary_dim,
+// interleaved, q_out, status, stream
 PyObject* paged_kv_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  if (!arity(n, 15)) return nullptr;
+  if (!arity(n, 16)) return nullptr;
   return guarded([&]() -> PyObject* {
     const at::Tensor* q = tensor(a[0], "q");
-    const at::Tensor &k = required(a[1], "k"), &v = required(a[2], "v"), &pages = required(a[7], "k_pages");
+    const at::Tensor &k = required(a[1], "k"), &v = required(a[2], "v");
     const at::Tensor *pos = tensor(a[3], "positions"), *slots = tensor(a[4], "slots"), *seqs = tensor(a[5], "seq_ids");
-    const at::Tensor* table = tensor(a[8], "table");
-    const bm_paged_kv_t* cache = cache_of(a[6]);
+    const at::Tensor* table = tensor(a[9], "table");
+    const Cache cache = cache_of(a[6], a[7], a[8]);
     if (k.dim() != 3) invalid("k and v must be [rows, kv_heads, head_dim]");
-    if (q == nullptr && a[12] != Py_None) invalid("q_out without q");
+    if (q == nullptr && a[13] != Py_None) invalid("q_out without q");
     const c10::Device device = cuda_device(k);
     const bm_dtype_t dtype = dtype_of(k);
-    if (pages.scalar_type() != k.scalar_type() || pages.device() != device) invalid("the cache has another dtype or device");
-    const int64_t hd = cache->head_dim;
+    if (cache.k.scalar_type() != k.scalar_type() || cache.k.device() != device) invalid("the cache has another dtype or device");
+    const int64_t hd = cache.c.head_dim;
     const HeadRows kr = head_rows(k, "k", k, hd), vr = head_rows(v, "v", k, hd);
-    if (kr.heads != cache->num_kv_heads || vr.heads != kr.heads || vr.rows != kr.rows) {
+    if (kr.heads != cache.c.num_kv_heads || vr.heads != kr.heads || vr.rows != kr.rows) {
       invalid("k and v do not match the cache or each other");
     }
     HeadRows qr, qor;
     Owned q_out;
     if (q != nullptr) {
       qr = head_rows(*q, "q", k, hd);
-      q_out.p = output(a[12], *q);
+      q_out.p = output(a[13], *q);
       qor = head_rows(required(q_out.p, "q_out"), "q_out", k, hd);
       if (qr.rows != kr.rows || qor.rows != qr.rows || qor.heads != qr.heads) invalid("q must have k's rows, and q_out q's shape");
     }
@@ -255,30 +274,30 @@ PyObject* paged_kv_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const c10::cuda::CUDAGuard guard(device);
     check(bm_paged_kv_append(q ? THPVariable_Unpack(q_out.p).data_ptr() : nullptr, data(q), k.data_ptr(), v.data_ptr(),
                              static_cast<const int32_t*>(data(pos)), static_cast<const int32_t*>(data(slots)),
-                             static_cast<const int32_t*>(data(seqs)), cache, data(table), integer32(a[9], "max_pos"),
-                             integer32(a[10], "rotary_dim"), truth(a[11]), kr.rows, static_cast<int32_t>(qr.heads),
-                             qr.stride, kr.stride, vr.stride, qor.stride, dtype, status_word(a[13], device),
-                             stream_of(a[14], device)));
+                             static_cast<const int32_t*>(data(seqs)), &cache.c, data(table), integer32(a[10], "max_pos"),
+                             integer32(a[11], "rotary_dim"), truth(a[12]), kr.rows, static_cast<int32_t>(qr.heads),
+                             qr.stride, kr.stride, vr.stride, qor.stride, dtype, status_word(a[14], device),
+                             stream_of(a[15], device)));
     if (q_out.p == nullptr) Py_RETURN_NONE;
     return q_out.release();
   });
 }
 
-// q, cache, k_pages, ctx_lens, q_starts, max_ctx, max_tree, tree_mask, seq_ids, scale, out,
-// workspace, status, stream
+// q, k_pages, v_pages, page_table, ctx_lens, q_starts, max_ctx, max_tree, tree_mask, seq_ids, scale,
+// out, workspace, status, stream
 PyObject* paged_tree_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  if (!arity(n, 14)) return nullptr;
+  if (!arity(n, 15)) return nullptr;
   return guarded([&]() -> PyObject* {
-    const at::Tensor &q = required(a[0], "q"), &pages = required(a[2], "k_pages");
-    const at::Tensor &ctx = required(a[3], "ctx_lens"), &starts = required(a[4], "q_starts"), &ws = required(a[11], "workspace");
-    const at::Tensor *mask = tensor(a[7], "tree_mask"), *seqs = tensor(a[8], "seq_ids");
-    const bm_paged_kv_t* cache = cache_of(a[1]);
+    const at::Tensor& q = required(a[0], "q");
+    const at::Tensor &ctx = required(a[4], "ctx_lens"), &starts = required(a[5], "q_starts"), &ws = required(a[12], "workspace");
+    const at::Tensor *mask = tensor(a[8], "tree_mask"), *seqs = tensor(a[9], "seq_ids");
+    const Cache cache = cache_of(a[1], a[2], a[3]);
     const c10::Device device = cuda_device(q);
-    if (q.dim() != 3 || !q.is_contiguous() || q.size(2) != cache->head_dim) {
+    if (q.dim() != 3 || !q.is_contiguous() || q.size(2) != cache.c.head_dim) {
       invalid("q must be contiguous [rows, heads, head_dim] with the cache's head_dim");
     }
     const bm_dtype_t dtype = dtype_of(q);
-    if (pages.scalar_type() != q.scalar_type() || pages.device() != device) invalid("the cache has another dtype or device");
+    if (cache.k.scalar_type() != q.scalar_type() || cache.k.device() != device) invalid("the cache has another dtype or device");
     const int64_t batch = ctx.numel();
     i32(&ctx, "ctx_lens", device, batch);
     i32(&starts, "q_starts", device, batch + 1);
@@ -292,21 +311,21 @@ PyObject* paged_tree_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
       words = mask->size(1);
     }
     Owned out;
-    out.p = output(a[10], q);
+    out.p = output(a[11], q);
     const at::Tensor& o = required(out.p, "out");
     if (o.sizes() != q.sizes() || o.scalar_type() != q.scalar_type() || o.device() != device || !o.is_contiguous()) {
       invalid("out must be contiguous and like q");
     }
     if (ws.device() != device || !ws.is_contiguous()) invalid("workspace must be contiguous on q's device");
-    const double scale = PyFloat_AsDouble(a[9]);
+    const double scale = PyFloat_AsDouble(a[10]);
     if (scale == -1.0 && PyErr_Occurred()) throw Refused();
     const c10::cuda::CUDAGuard guard(device);
-    check(bm_paged_tree_attention(o.data_ptr(), q.data_ptr(), cache, static_cast<const int32_t*>(data(seqs)),
+    check(bm_paged_tree_attention(o.data_ptr(), q.data_ptr(), &cache.c, static_cast<const int32_t*>(data(seqs)),
                                   ctx.data_ptr<int32_t>(), starts.data_ptr<int32_t>(), static_cast<const uint64_t*>(data(mask)),
                                   static_cast<int32_t>(words), q.size(0), batch, static_cast<int32_t>(q.size(1)),
-                                  integer32(a[5], "max_ctx"), integer32(a[6], "max_tree"), static_cast<float>(scale),
+                                  integer32(a[6], "max_ctx"), integer32(a[7], "max_tree"), static_cast<float>(scale),
                                   ws.data_ptr(), static_cast<size_t>(ws.numel()) * ws.element_size(), dtype,
-                                  status_word(a[12], device), stream_of(a[13], device)));
+                                  status_word(a[13], device), stream_of(a[14], device)));
     return out.release();
   });
 }

@@ -488,8 +488,9 @@ class PagedKV:
     """A paged KV cache over the caller's tensors: k_pages and v_pages [num_pages, Hkv,
     page_size, hd] (contiguous, one dtype and device) and page_table int32 [num_seqs,
     max_pages]: slot t of sequence s is in page page_table[s, t // page_size] at
-    t % page_size. The tensors are read by every call, so page_table may be rewritten
-    between calls (on the calls' stream)."""
+    t % page_size. Every call reads (and checks) the three tensors that the object holds then:
+    page_table may be rewritten between calls (on the calls' stream), and each may be replaced
+    by another."""
 
     def __init__(self, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor):
         if k_pages.dim() != 4 or k_pages.shape != v_pages.shape:
@@ -503,12 +504,15 @@ class PagedKV:
         if page_table.dtype != torch.int32 or not page_table.is_contiguous() or page_table.device != _dev(k_pages):
             raise _invalid("page_table must be a contiguous int32 tensor on the pages' device")
         self.k_pages, self.v_pages, self.page_table = k_pages, v_pages, page_table
-        self.num_pages, self.num_kv_heads, self.page_size, self.head_dim = k_pages.shape
-        self.num_seqs, self.max_pages = page_table.shape
-        self.device, self.dtype = k_pages.device, k_pages.dtype
-        self.c = _lib.PagedKVC(k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr(), self.num_pages,
-                               self.page_size, self.max_pages, self.num_seqs, self.num_kv_heads, self.head_dim)
-        self.address = ctypes.addressof(self.c)
+
+    num_pages = property(lambda self: self.k_pages.shape[0])
+    num_kv_heads = property(lambda self: self.k_pages.shape[1])
+    page_size = property(lambda self: self.k_pages.shape[2])
+    head_dim = property(lambda self: self.k_pages.shape[3])
+    num_seqs = property(lambda self: self.page_table.shape[0])
+    max_pages = property(lambda self: self.page_table.shape[1])
+    device = property(lambda self: self.k_pages.device)
+    dtype = property(lambda self: self.k_pages.dtype)
 
 
 def paged_kv_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, positions: Optional[torch.Tensor],
@@ -527,8 +531,8 @@ def paged_kv_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor,
         tdata, max_pos, rotary_dim = None, 0, 0
     else:
         tdata, max_pos, rotary_dim = table.data, table.max_pos, table.head_dim
-    return _lib.serving_ops().paged_kv_append(q, k, v, positions, slots, seq_ids, cache.address, cache.k_pages, tdata, max_pos,
-                                              rotary_dim, interleaved, q_out, _word(status), _handle(stream))
+    return _lib.serving_ops().paged_kv_append(q, k, v, positions, slots, seq_ids, cache.k_pages, cache.v_pages, cache.page_table,
+                                              tdata, max_pos, rotary_dim, interleaved, q_out, _word(status), _handle(stream))
 
 
 def paged_tree_attention_workspace(q: torch.Tensor, cache: PagedKV, batch: int, max_ctx: int, max_tree: int,
@@ -563,8 +567,8 @@ def paged_tree_attention(q: torch.Tensor, cache: PagedKV, ctx_lens: torch.Tensor
         workspace = paged_tree_attention_workspace(q, cache, ctx_lens.numel(), max_ctx, max_tree, stream)
     if stream is not None and out is None:
         out = _like(q, stream)
-    return _lib.serving_ops().paged_tree_attention(q, cache.address, cache.k_pages, ctx_lens, q_starts, max_ctx, max_tree,
-                                                   tree_mask, seq_ids, scale, out, workspace, _word(status), _handle(stream))
+    return _lib.serving_ops().paged_tree_attention(q, cache.k_pages, cache.v_pages, cache.page_table, ctx_lens, q_starts,
+                                                   max_ctx, max_tree, tree_mask, seq_ids, scale, out, workspace, _word(status), _handle(stream))
 
 
 def sample(logits: torch.Tensor, uniforms: torch.Tensor, temperature: Optional[torch.Tensor] = None,

@@ -154,3 +154,41 @@ def test_another_stream_and_a_captured_graph(cuda):
     torch.cuda.synchronize()
     assert bits_equal(cache.k_pages[1, :, 1], kept[1, :, 1]) and int(torch.count_nonzero(cache.k_pages[1, :, 3])) > 0
     assert int(torch.count_nonzero(cache.k_pages[1, :, 0])) == 0 and bits_equal(out[1:], want[1:])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_a_cache_whose_tensors_are_replaced(cuda, dtype):
+    """Calls go by the tensors that a PagedKV holds at the time: other pages, other page tables,
+    more of either; what no longer fits together is refused."""
+    g = gen(10)
+    cache = paged(cuda, g, 4, 2, 8, 64, dtype, [[2, 0], [3, 1]])
+    old = cache.k_pages, cache.v_pages, cache.page_table
+    kept = [t.clone() for t in old]
+    q, k, v = (randn((3, h, 64), dtype, g).to(cuda) for h in (4, 2, 2))
+    pos, ones = i32([0, 1, 2], cuda), i32([1, 1, 1], cuda)
+    new = paged(cuda, g, 7, 2, 8, 64, dtype, [[0, 1, 2], [6, 5, 4]])
+    want = paged(cuda, g, 7, 2, 8, 64, dtype, [[0, 1, 2], [6, 5, 4]])
+    want.k_pages.copy_(new.k_pages)
+    want.v_pages.copy_(new.v_pages)
+    ops.paged_kv_append(None, k, v, pos, want, seq_ids=ones)
+    cache.k_pages, cache.v_pages, cache.page_table = new.k_pages, new.v_pages, new.page_table
+    assert (cache.num_pages, cache.num_seqs, cache.max_pages) == (7, 2, 3)
+    ops.paged_kv_append(None, k, v, pos, cache, seq_ids=ones)
+    assert bits_equal(cache.k_pages, want.k_pages) and bits_equal(cache.v_pages, want.v_pages)
+    for t, was in zip(old, kept):
+        assert bits_equal(t, was)
+    args = i32([0], cuda), i32([0, 3], cuda), 0, 3
+    ids = i32([1], cuda)
+    assert bits_equal(ops.paged_tree_attention(q, cache, *args, seq_ids=ids),
+                      ops.paged_tree_attention(q, want, *args, seq_ids=ids))
+    for name, bad in (("k_pages", new.k_pages[:6]), ("v_pages", new.v_pages.to(torch.float64)),
+                      ("v_pages", new.v_pages.transpose(0, 1)), ("k_pages", new.k_pages.cpu()), ("page_table", new.page_table.long()),
+                      ("page_table", new.page_table[:, :2]), ("page_table", new.page_table[0]), ("page_table", None)):
+        good = getattr(cache, name)
+        setattr(cache, name, bad)
+        with pytest.raises(_lib.BMError):
+            ops.paged_kv_append(None, k, v, pos, cache, seq_ids=ones)
+        with pytest.raises(_lib.BMError):
+            ops.paged_tree_attention(q, cache, *args, seq_ids=ids, workspace=torch.empty(1 << 20, dtype=torch.uint8, device=cuda))
+        setattr(cache, name, good)
+    assert bits_equal(cache.k_pages, want.k_pages) and bits_equal(cache.v_pages, want.v_pages)
