@@ -5,6 +5,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <initializer_list>
+
 #include "bm_layer_ops.h"
 
 namespace bm {
@@ -76,6 +78,15 @@ int gemm_f32_norm(float* const* c, const float* h, const float* d, const float* 
 int allow_dynamic_smem(const void* kernel, int bytes, const char* what);
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+// NULL, or a multiple of `bytes`: what a kernel's loads of an element need.
+inline bool aligned_to(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p) % static_cast<uintptr_t>(bytes) == 0; }
+inline bool aligned_to(std::initializer_list<const void*> ptrs, int bytes) {
+  for (const void* p : ptrs) {
+    if (!aligned_to(p, bytes)) return false;
+  }
+  return true;
+}
 
 inline int dtype_size(bm_dtype_t dt) { return dt == BM_F32 ? 4 : 2; }
 

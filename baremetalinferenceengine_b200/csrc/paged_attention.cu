@@ -718,6 +718,9 @@ extern "C" int bm_paged_tree_attention(void* out, const void* q, const bm_paged_
   if (!aligned16(out) || !aligned16(q) || !aligned16(c.k_pages) || !aligned16(c.v_pages) || !aligned16(workspace)) {
     return fail(BM_ERR_INVALID_ARGUMENT, "%s: q, out, pages and workspace must be 16-byte aligned", what);
   }
+  if (!aligned_to({seq_ids, ctx_lens, q_starts, c.page_table, d_status}, 4) || !aligned_to(tree_mask, 8)) {
+    return fail(BM_ERR_INVALID_ARGUMENT, "%s: a pointer is not aligned to its elements", what);
+  }
   if (!seq_ids && batch > c.num_seqs) return fail(BM_ERR_INVALID_ARGUMENT, "%s: more sequences than the cache holds", what);
   const uintptr_t o = reinterpret_cast<uintptr_t>(out), i = reinterpret_cast<uintptr_t>(q);
   const uintptr_t bytes = static_cast<uintptr_t>(total_q) * num_q_heads * c.head_dim * dtype_size(dtype);

@@ -406,6 +406,9 @@ extern "C" int bm_rotary(void* q_out, void* k_out, const void* q, const void* k,
   }
   if (!positions && (pos0 < 0 || pos0 + rows > INT32_MAX)) return fail(BM_ERR_INVALID_ARGUMENT, "%s: bad pos0", what);
   const int es = dtype_size(dtype);
+  if (!aligned_to({q, k, q_out, k_out}, es) || !aligned_to({positions, d_status}, 4)) {
+    return fail(BM_ERR_INVALID_ARGUMENT, "%s: a pointer is not aligned to its elements", what);
+  }
   const Rows qi{q, q_stride, qn}, ki{k, k_stride, kn}, qo{q_out, q_out_stride, qn}, ko{k_out, k_out_stride, kn};
   if ((meet(qo, qi, rows, es) && !same(qo, qi, rows)) || (meet(ko, ki, rows, es) && !same(ko, ki, rows)) ||
       meet(qo, ki, rows, es) || meet(ko, qi, rows, es) || meet(qo, ko, rows, es)) {
@@ -457,6 +460,9 @@ extern "C" int bm_paged_kv_append(void* q_out, const void* q, const void* k, con
     return fail(BM_ERR_INVALID_ARGUMENT, "%s: a row stride below heads * head_dim", what);
   }
   const int es = dtype_size(dtype);
+  if (!aligned_to({q, k, v, q_out, c.k_pages, c.v_pages}, es) || !aligned_to({positions, slots, seq_ids, c.page_table, d_status}, 4)) {
+    return fail(BM_ERR_INVALID_ARGUMENT, "%s: a pointer is not aligned to its elements", what);
+  }
   const Rows qi{q, q_stride, qn}, qo{q_out, q_out_stride, qn};
   if ((meet(qo, qi, rows, es) && !same(qo, qi, rows)) || meet(qo, Rows{k, k_stride, kn}, rows, es) ||
       meet(qo, Rows{v, v_stride, kn}, rows, es)) {

@@ -1064,6 +1064,9 @@ extern "C" int bm_sample(int32_t* tokens, const void* logits, const float* unifo
   if (rows == 0) return BM_OK;
   if (!tokens || !logits || !uniforms) return fail(BM_ERR_INVALID_ARGUMENT, "%s: NULL pointer", what);
   const int es = dtype_size(dtype);
+  if (!aligned_to(logits, es) || !aligned_to({tokens, uniforms, temperature, top_k, top_p, min_p, d_status}, 4)) {
+    return fail(BM_ERR_INVALID_ARGUMENT, "%s: a pointer is not aligned to its elements", what);
+  }
   SampleArgs a{};
   a.tokens = tokens;
   a.logits = logits;

@@ -154,3 +154,24 @@ def test_python_layer_rejects_cpu_tensors_and_bad_arguments():
         ops.RopeScaling("stretch", 2.0).c_struct()
     with pytest.raises(_lib.BMError):
         ops.RopeScaling("linear", 2.0, mscale=-1.0).c_struct()
+
+
+MISALIGNED = {
+    "rotary": [dict(q=FAKE + 2), dict(k=FAKE * 2 + 1), dict(qo=FAR + 3), dict(ko=FAR * 2 + 2), dict(pos=FAKE + 2),
+               dict(q=FAKE + 1, dtype=1), dict(ko=FAR * 2 + 1, dtype=1)],
+    "append": [dict(q=FAKE + 2), dict(k=FAKE * 2 + 2), dict(v=FAKE * 3 + 1), dict(qo=FAR + 2), dict(pos=FAKE + 1),
+               dict(slots=FAKE + 2), dict(v=FAKE * 3 + 1, dtype=1), dict(k_pages=FAKE + 2), dict(v_pages=FAKE + 1),
+               dict(v_pages=FAKE + 1, dtype=1), dict(page_table=FAKE + 2)],
+    "attend": [dict(ctx=FAKE + 2), dict(starts=FAKE + 1), dict(mask=FAKE + 4), dict(seqs=FAKE + 2), dict(page_table=FAKE + 2)],
+    "sample": [dict(logits=FAKE + 2), dict(logits=FAKE + 1, dtype=1), dict(tokens=FAKE + 2), dict(u=FAKE + 1)],
+}
+
+
+@pytest.mark.parametrize("name,kw", [(n, kw) for n, all_kw in MISALIGNED.items() for kw in all_kw])
+def test_pointers_below_their_elements_alignment_are_refused(lib, name, kw):
+    """A kernel's scalar loads need it, too: such a pointer would fault there."""
+    kw = dict(kw)
+    in_cache = {f: kw.pop(f) for f in ("k_pages", "v_pages", "page_table") if f in kw}
+    call = {"rotary": rotary, "append": append, "attend": attend, "sample": sample}[name]
+    assert call(lib, **kw, **({"c": cache(**in_cache)} if in_cache else {})) == _lib.BM_ERR_INVALID_ARGUMENT
+    assert b"aligned" in lib.bm_last_error_message()
