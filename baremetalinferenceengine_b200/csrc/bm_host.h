@@ -96,6 +96,8 @@ inline cudaStream_t as_stream(void* s) { return reinterpret_cast<cudaStream_t>(s
 
 // Host checks of a paged cache's description, shared by its entry points.
 int check_paged_kv(const char* what, const bm_paged_kv_t* cache);
+// Whether `bytes` from p on share memory with the pages of a checked cache of es-byte elements.
+bool meets_pages(const bm_paged_kv_t& cache, const void* p, uintptr_t bytes, int es);
 
 // bm_decode_attention with a host-side length for every query (lens == NULL:
 // len0), as the reference's single-token launch_attention needs.

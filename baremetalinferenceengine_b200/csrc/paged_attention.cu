@@ -678,6 +678,16 @@ int check_paged_kv(const char* what, const bm_paged_kv_t* c) {
   return BM_OK;
 }
 
+bool meets_pages(const bm_paged_kv_t& c, const void* p, uintptr_t bytes, int es) {
+  const uintptr_t from = reinterpret_cast<uintptr_t>(p);
+  const uintptr_t all = static_cast<uintptr_t>(c.num_pages) * c.num_kv_heads * c.page_size * c.head_dim * es;
+  for (const void* pages : {c.k_pages, c.v_pages}) {
+    const uintptr_t lo = reinterpret_cast<uintptr_t>(pages);
+    if (from < lo + all && lo < from + bytes) return true;
+  }
+  return false;
+}
+
 }  // namespace bm
 
 extern "C" int bm_paged_tree_attention_workspace_size(int64_t total_q, int64_t batch, int32_t num_q_heads,
@@ -725,6 +735,7 @@ extern "C" int bm_paged_tree_attention(void* out, const void* q, const bm_paged_
   const uintptr_t o = reinterpret_cast<uintptr_t>(out), i = reinterpret_cast<uintptr_t>(q);
   const uintptr_t bytes = static_cast<uintptr_t>(total_q) * num_q_heads * c.head_dim * dtype_size(dtype);
   if (o < i + bytes && i < o + bytes) return fail(BM_ERR_INVALID_ARGUMENT, "%s: out overlaps q", what);
+  if (meets_pages(c, out, bytes, dtype_size(dtype))) return fail(BM_ERR_INVALID_ARGUMENT, "%s: out overlaps the cache's pages", what);
   const size_t simt = paged::simt_workspace_bytes(total_q, batch, num_q_heads, c.num_kv_heads, c.head_dim, max_ctx, max_tree);
   const size_t tc = paged::tc_workspace_bytes(batch, c.num_kv_heads, c.head_dim, num_q_heads / c.num_kv_heads, max_ctx,
                                               max_tree);

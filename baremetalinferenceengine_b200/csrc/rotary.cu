@@ -468,6 +468,9 @@ extern "C" int bm_paged_kv_append(void* q_out, const void* q, const void* k, con
       meet(qo, Rows{v, v_stride, kn}, rows, es)) {
     return fail(BM_ERR_INVALID_ARGUMENT, "%s: q_out overlaps an input", what);
   }
+  if (qn != 0 && meets_pages(c, q_out, static_cast<uintptr_t>((rows - 1) * q_out_stride + qn) * es, es)) {
+    return fail(BM_ERR_INVALID_ARGUMENT, "%s: q_out overlaps the cache's pages", what);
+  }
   RotaryArgs a{};
   a.q_out = q_out;
   a.q = q;

@@ -175,3 +175,16 @@ def test_pointers_below_their_elements_alignment_are_refused(lib, name, kw):
     call = {"rotary": rotary, "append": append, "attend": attend, "sample": sample}[name]
     assert call(lib, **kw, **({"c": cache(**in_cache)} if in_cache else {})) == _lib.BM_ERR_INVALID_ARGUMENT
     assert b"aligned" in lib.bm_last_error_message()
+
+
+# pages of 4 * 2 * 8 * 64 elements: 16 KB in fp32, 8 KB in bf16
+@pytest.mark.parametrize("name,kw", [
+    ("append", dict(k_pages=FAR)), ("append", dict(v_pages=FAR)), ("append", dict(v_pages=FAR - 16380)),
+    ("append", dict(k_pages=FAR + 4 * 4 * 64 * 4 - 4)), ("append", dict(k_pages=FAR - 8190, dtype=1)),
+    ("attend", dict(k_pages=FAR)), ("attend", dict(v_pages=FAR + 4080)), ("attend", dict(v_pages=FAR - 16368))])
+def test_outputs_over_the_cache_are_refused(lib, name, kw):
+    kw = dict(kw)
+    dtype = kw.pop("dtype", 0)
+    call = {"append": append, "attend": attend}[name]
+    assert call(lib, c=cache(**kw), dtype=dtype) == _lib.BM_ERR_INVALID_ARGUMENT
+    assert b"pages" in lib.bm_last_error_message()
