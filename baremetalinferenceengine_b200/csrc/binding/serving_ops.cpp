@@ -117,6 +117,14 @@ void i32(const at::Tensor* t, const char* name, c10::Device device, int64_t nume
   if (t->numel() != numel) invalid("%s must have %lld entries", name, static_cast<long long>(numel));
 }
 
+// A rope table's entries: max_pos rows of rotary_dim / 2 fp32 pairs.
+void rope_table(const at::Tensor& t, c10::Device device, int64_t max_pos, int64_t rotary_dim) {
+  if (t.device() != device) invalid("the rope table is on another device");
+  if (t.scalar_type() != at::kFloat || !t.is_contiguous() || max_pos < 0 || rotary_dim < 0 || t.numel() < max_pos * (rotary_dim / 2) * 2) {
+    invalid("the rope table must be contiguous float32 [max_pos, rotary_dim / 2, 2]");
+  }
+}
+
 int32_t* status_word(PyObject* o, c10::Device device) {
   const at::Tensor* t = tensor(o, "status");
   if (t == nullptr) return nullptr;
@@ -197,11 +205,12 @@ PyObject* rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
     }
     const int64_t rows = q != nullptr ? qr.rows : kr.rows;
     i32(pos, "positions", device, rows);
-    if (table.device() != device) invalid("the rope table is on another device");
+    const int32_t max_pos = integer32(a[5], "max_pos"), rotary_dim = integer32(a[6], "rotary_dim");
+    rope_table(table, device, max_pos, rotary_dim);
     const c10::cuda::CUDAGuard guard(device);
     check(bm_rotary(q ? THPVariable_Unpack(q_out.p).data_ptr() : nullptr, k ? THPVariable_Unpack(k_out.p).data_ptr() : nullptr,
                     data(q), data(k), static_cast<const int32_t*>(data(pos)), integer32(a[3], "positions"),
-                    table.data_ptr(), integer32(a[5], "max_pos"), integer32(a[6], "rotary_dim"), truth(a[7]), rows,
+                    table.data_ptr(), max_pos, rotary_dim, truth(a[7]), rows,
                     static_cast<int32_t>(qr.heads), static_cast<int32_t>(kr.heads), static_cast<int32_t>(hd), qr.stride,
                     kr.stride, qor.stride, kor.stride, dtype, status_word(a[10], device), stream_of(a[11], device)));
     if (q_out.p == nullptr) {
@@ -270,12 +279,13 @@ PyObject* paged_kv_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
     i32(pos, "positions", device, kr.rows);
     i32(slots, "slots", device, kr.rows);
     i32(seqs, "seq_ids", device, kr.rows);
-    if (table != nullptr && table->device() != device) invalid("the rope table is on another device");
+    const int32_t max_pos = integer32(a[10], "max_pos"), rotary_dim = integer32(a[11], "rotary_dim");
+    if (table != nullptr) rope_table(*table, device, max_pos, rotary_dim);
     const c10::cuda::CUDAGuard guard(device);
     check(bm_paged_kv_append(q ? THPVariable_Unpack(q_out.p).data_ptr() : nullptr, data(q), k.data_ptr(), v.data_ptr(),
                              static_cast<const int32_t*>(data(pos)), static_cast<const int32_t*>(data(slots)),
-                             static_cast<const int32_t*>(data(seqs)), &cache.c, data(table), integer32(a[10], "max_pos"),
-                             integer32(a[11], "rotary_dim"), truth(a[12]), kr.rows, static_cast<int32_t>(qr.heads),
+                             static_cast<const int32_t*>(data(seqs)), &cache.c, data(table), max_pos,
+                             rotary_dim, truth(a[12]), kr.rows, static_cast<int32_t>(qr.heads),
                              qr.stride, kr.stride, vr.stride, qor.stride, dtype, status_word(a[14], device),
                              stream_of(a[15], device)));
     if (q_out.p == nullptr) Py_RETURN_NONE;

@@ -125,3 +125,21 @@ def test_no_rows(cuda):
     table = ops.RopeTable(10, 32, 1e4, cuda)
     z = torch.empty(0, 2, 32, device=cuda)
     assert ops.rotary(z, None, torch.empty(0, dtype=torch.int32, device=cuda), table)[0].shape == (0, 2, 32)
+
+
+def test_a_table_smaller_than_it_says_is_refused(cuda):
+    """A table's tensor and its sizes go into a call apart: kernels would read past the
+    tensor where the sizes say more. (Refused on the host; nothing is launched.)"""
+    q = randn((3, 2, 32), torch.float32, gen(3)).to(cuda)
+    pos = torch.zeros(3, dtype=torch.int32, device=cuda)
+    pages = torch.zeros(1, 2, 8, 32, device=cuda)
+    cache = ops.PagedKV(pages, pages.clone(), torch.zeros(1, 1, dtype=torch.int32, device=cuda))
+    for name, value in (("data", torch.zeros(9, 12, 2, device=cuda)), ("data", torch.zeros(10, 12, 2, dtype=torch.float64, device=cuda)),
+                        ("data", torch.zeros(10, 2, 12, device=cuda).transpose(1, 2)), ("max_pos", 11), ("head_dim", 26)):
+        table = ops.RopeTable(10, 24, 1e4, cuda)
+        setattr(table, name, value)
+        with pytest.raises(_lib.BMError):
+            ops.rotary(q, None, pos, table)
+        with pytest.raises(_lib.BMError):
+            ops.paged_kv_append(None, q, q, pos, cache, table=table)
+    assert int(torch.count_nonzero(pages)) == 0
