@@ -1,5 +1,6 @@
 """Tree attention over a paged cache on the GPU against 64-bit softmax attention, one
 row and head at a time; the tolerance is derived where it is computed (serving_ref)."""
+import ctypes
 import math
 
 import numpy as np
@@ -290,3 +291,46 @@ def test_two_streams_at_once(cuda):
     for (args, kw), want in zip(calls, first):
         for k in kw:
             assert bits_equal(k["out"], want)
+
+
+@pytest.mark.parametrize("dtype,hq,hkv,hd", [(BF16, 8, 2, 128), (BF16, 8, 2, 64), (F32, 6, 6, 48), (F32, 8, 2, 128)])
+def test_a_token_alone_and_decode_attention_on_the_static_cache(cuda, dtype, hq, hkv, hd):
+    """One row per sequence and no mask, and bm_decode_attention on the same K and V laid out
+    statically: each within the tolerance of the same 64-bit result."""
+    b = Batch(cuda, [(200, 1), (77, 1), (0, 1), (1300, 1)], hq, hkv, hd, 16, dtype, seed=20, tree=False)
+    b.check()
+    want, tol = b.want()
+    max_seq = b.max_ctx + 1
+    k, v = (torch.zeros(len(b.lens), hkv, max_seq, hd, dtype=dtype) for _ in range(2))
+    for s, (c, n) in enumerate(b.lens):
+        for t in range(c + n):
+            k[s, :, t] = b.k[int(b.table[s, t // 16]), :, t % 16]
+            v[s, :, t] = b.v[int(b.table[s, t // 16]), :, t % 16]
+    lib, need = _lib.load(), ctypes.c_size_t()
+    _lib.check(lib.bm_decode_attention_workspace_size(len(b.lens), hq, hkv, hd, max_seq, ctypes.byref(need)))
+    ws = torch.empty(max(need.value, 1), dtype=torch.uint8, device=cuda)
+    q, k, v, lens = b.q.to(cuda), k.to(cuda), v.to(cuda), i32([c + n for c, n in b.lens], cuda)
+    out, ids = torch.empty_like(q), i32(list(range(len(b.lens))), cuda)
+    _lib.check(lib.bm_decode_attention(out.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), ids.data_ptr(), lens.data_ptr(),
+                                       max_seq, len(b.lens), hq, hkv, hd, max_seq, len(b.lens), 0.0, ws.data_ptr(), need.value,
+                                       ops.bm_dtype(q), None, torch.cuda.current_stream(cuda).cuda_stream))
+    assert np.all(np.abs(out.cpu().double().numpy() - want) <= tol)
+
+
+@pytest.mark.parametrize("dtype,hd", [(BF16, 128), (BF16, 64), (BF16, 256), (F32, 48), (F32, 128)])
+@pytest.mark.parametrize("seqs", [[3, 2, 1, 0], [1, 0, 1, 2], [2, 2, 2, 2]])
+def test_sequence_ids_in_any_order_and_twice(cuda, dtype, hd, seqs):
+    """Entries of the batch on cache sequences of another number, two and more on the same one."""
+    b = Batch(cuda, [(60, 3), (60, 2), (60, 3), (60, 1)], 8, 2, hd, 16, dtype, seed=21)
+    for s in range(4):  # three drafted slots in every cache sequence
+        for t in range(61, 63):
+            page = int(b.table[s, t // 16])
+            b.k[page, :, t % 16] = randn((2, hd), dtype, gen(100 + s + t))
+            b.v[page, :, t % 16] = randn((2, hd), dtype, gen(200 + s + t))
+    b.cache.k_pages.copy_(b.k)
+    b.cache.v_pages.copy_(b.v)
+    st = ops.DeviceStatus(cuda)
+    got = b.run(seq_ids=i32(seqs, cuda), status=st)
+    assert st.read() == 0
+    want, tol = b.want(seqs=seqs)
+    assert np.all(np.abs(got.cpu().double().numpy() - want) <= tol)
