@@ -7,16 +7,19 @@ produces ``baremetalinferenceengine_b200/libbm_layer_ops.so`` from ``csrc/*.cu``
 with nvcc (``-gencode arch=compute_100a,code=sm_100a``), static cudart, C++17.
 Objects go to ``_build/`` at the repository root. A source newer than the
 library (or a changed header) triggers a rebuild. ``_serving_ops.so`` beside it is the
-CPython module of ``csrc/binding/`` (g++ against torch's headers), linked to the library.
+CPython module of ``csrc/binding/`` (g++ against torch's headers), linked to the library;
+it is left out, with a note, where torch or Python's headers are not installed.
 """
 from __future__ import annotations
 
 import argparse
 import concurrent.futures as cf
+import importlib.util
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 REPO_ROOT = os.path.dirname(PKG_DIR)
@@ -71,13 +74,26 @@ def _run(cmd: list[str]) -> None:
         raise RuntimeError("command failed:\n  " + " ".join(cmd) + "\n" + proc.stdout)
 
 
+def _binding_lacks() -> str | None:
+    """What the CPython module needs and this machine has not; None where it has all."""
+    if importlib.util.find_spec("torch") is None:
+        return "torch is not installed"
+    if not os.path.exists(os.path.join(sysconfig.get_paths()["include"], "Python.h")):
+        return "Python's headers are not installed"
+    return None
+
+
 def _build_binding(force: bool) -> None:
     """_serving_ops.so: g++ against torch's headers and libraries, and libbm_layer_ops.so
-    (found beside it at run time)."""
+    (found beside it at run time). Users of the C ABI do without: where torch or Python's
+    headers are missing this says so and builds nothing."""
     if not (force or _stale(BINDING_PATH, [BINDING_SRC, os.path.join(INCLUDE, "bm_layer_ops.h")])):
         return
-    import sysconfig
-
+    lacks = _binding_lacks()
+    if lacks:
+        print(f"{os.path.basename(BINDING_PATH)} not built: {lacks} (only the Python calls of ops.rotary, paged_kv_append, "
+              "paged_tree_attention and sample need it)", file=sys.stderr)
+        return
     import torch
 
     root = os.path.dirname(torch.__file__)
