@@ -62,7 +62,7 @@ def _headers() -> list[str]:
 
 
 def _stale(target: str, deps: list[str]) -> bool:
-    if not os.path.exists(target):
+    if not all(os.path.exists(p) for p in [target] + deps):
         return True
     t = os.path.getmtime(target)
     return any(os.path.getmtime(d) > t for d in deps)
@@ -83,13 +83,24 @@ def _binding_lacks() -> str | None:
     return None
 
 
+def _binding_for() -> str:
+    """The torch and the Python that a module built now is for (torch itself stays unloaded)."""
+    at = os.path.dirname(importlib.util.find_spec("torch").origin)
+    with open(os.path.join(at, "version.py")) as f:
+        return f"{at}\n{sys.implementation.cache_tag}\n{f.read()}"
+
+
 def _build_binding(force: bool) -> None:
     """_serving_ops.so: g++ against torch's headers and libraries, and libbm_layer_ops.so
     (found beside it at run time). Users of the C ABI do without: where torch or Python's
     headers are missing this says so and builds nothing."""
-    if not (force or _stale(BINDING_PATH, [BINDING_SRC, os.path.join(INCLUDE, "bm_layer_ops.h")])):
-        return
+    made_for = os.path.join(BUILD_DIR, "_serving_ops.made_for")
     lacks = _binding_lacks()
+    now = "" if lacks else _binding_for()
+    if not (force or _stale(BINDING_PATH, [BINDING_SRC, os.path.join(INCLUDE, "bm_layer_ops.h"), made_for])):
+        with open(made_for) as f:
+            if lacks or f.read() == now:
+                return
     if lacks:
         print(f"{os.path.basename(BINDING_PATH)} not built: {lacks} (only the Python calls of ops.rotary, paged_kv_append, "
               "paged_tree_attention and sample need it)", file=sys.stderr)
@@ -106,7 +117,10 @@ def _build_binding(force: bool) -> None:
          + [f"-I{i}" for i in includes] + [BINDING_SRC, "-o", tmp, LIB_PATH, f"-L{os.path.join(root, 'lib')}",
                                            "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda",
                                            "-Wl,-rpath,$ORIGIN"])
+    with open(made_for, "w") as f:
+        f.write(now)
     os.replace(tmp, BINDING_PATH)
+    os.utime(BINDING_PATH)  # not older than made_for
 
 
 def build(force: bool = False, verbose: bool = False) -> str:

@@ -32,3 +32,27 @@ def test_without_torch_or_pythons_headers_the_library_is_all(commands, monkeypat
     assert build.build(force=True) == build.LIB_PATH and os.path.exists(build.LIB_PATH)
     assert not [c for c in commands if c[0] == "g++"] and not os.path.exists(build.BINDING_PATH)
     assert missing in capsys.readouterr().err
+
+
+def test_a_module_made_for_another_torch_or_python_is_built_again(commands, monkeypatch, tmp_path):
+    built = lambda: len([c for c in commands if c[0] == "g++"])  # noqa: E731
+    build.build()
+    assert built() == 1
+    build.build()
+    assert built() == 1
+    torch = tmp_path / "torch"
+    torch.mkdir()
+    (torch / "version.py").write_text("__version__ = '0.0.1'\n")
+    real = importlib.util.find_spec
+    monkeypatch.setattr(importlib.util, "find_spec", lambda name, *a: type("Spec", (), {"origin": str(torch / "__init__.py")})
+                        if name == "torch" else real(name, *a))
+    build.build()
+    assert built() == 2
+    (torch / "version.py").write_text("__version__ = '0.0.2'\n")  # another one in its place
+    build.build()
+    assert built() == 3
+    monkeypatch.setattr(build.sys.implementation, "cache_tag", "cpython-399")
+    build.build()
+    assert built() == 4
+    build.build()
+    assert built() == 4
