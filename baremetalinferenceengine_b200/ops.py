@@ -476,6 +476,8 @@ def rotary(q: Optional[torch.Tensor], k: Optional[torch.Tensor], positions, tabl
     outside the table leaves its row unwritten and sets BAD_POSITION."""
     if table is None:
         raise _invalid("rotary needs a table")
+    if positions is None:
+        raise _invalid("rotary needs positions")
     if stream is not None:
         q_out = _like(q, stream) if q is not None and q_out is None else q_out
         k_out = _like(k, stream) if k is not None and k_out is None else k_out

@@ -188,3 +188,10 @@ def test_outputs_over_the_cache_are_refused(lib, name, kw):
     call = {"append": append, "attend": attend}[name]
     assert call(lib, c=cache(**kw), dtype=dtype) == _lib.BM_ERR_INVALID_ARGUMENT
     assert b"pages" in lib.bm_last_error_message()
+
+
+def test_rotary_without_positions_is_refused():
+    """None is no pos0 of 0."""
+    table = type("Table", (), dict(data=torch.zeros(4, 32, 2), max_pos=4, head_dim=64))
+    with pytest.raises(_lib.BMError, match="positions"):
+        ops.rotary(torch.zeros(2, 4, 64), None, None, table)
