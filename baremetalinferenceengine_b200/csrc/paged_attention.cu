@@ -722,7 +722,9 @@ extern "C" int bm_paged_tree_attention(void* out, const void* q, const bm_paged_
   if (tree_mask && (mask_words <= 0 || max_tree > 64 * static_cast<int64_t>(mask_words))) {
     return fail(BM_ERR_INVALID_ARGUMENT, "%s: max_tree %d does not fit %d mask words", what, max_tree, mask_words);
   }
-  if (scale != scale) return fail(BM_ERR_INVALID_ARGUMENT, "%s: scale is NaN", what);
+  const float s = scale > 0.f ? scale : 1.f / std::sqrt(static_cast<float>(c.head_dim));
+  const float qscale = s * 1.4426950408889634f;  // the softmax runs in base 2
+  if (scale != scale || !std::isfinite(qscale)) return fail(BM_ERR_INVALID_ARGUMENT, "%s: scale is not finite", what);
   if (batch == 0 || total_q == 0 || max_tree == 0) return BM_OK;
   if (!out || !q || !ctx_lens || !q_starts) return fail(BM_ERR_INVALID_ARGUMENT, "%s: NULL pointer", what);
   if (!aligned16(out) || !aligned16(q) || !aligned16(c.k_pages) || !aligned16(c.v_pages) || !aligned16(workspace)) {
@@ -767,8 +769,7 @@ extern "C" int bm_paged_tree_attention(void* out, const void* q, const bm_paged_
   a.num_seqs = c.num_seqs;
   a.max_ctx = max_ctx;
   a.max_tree = max_tree;
-  const float s = scale > 0.f ? scale : 1.f / std::sqrt(static_cast<float>(c.head_dim));
-  a.qscale = s * 1.4426950408889634f;
+  a.qscale = qscale;
   a.status = d_status;
   if (paged::tc_takes(a, dtype)) return paged::launch_tc(a, as_stream(stream), what);
   paged::plan(batch, a.hkv, a.group, max_ctx, max_tree, &a.row_tiles, &a.splits, &a.split_len);

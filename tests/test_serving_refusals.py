@@ -195,3 +195,10 @@ def test_rotary_without_positions_is_refused():
     table = type("Table", (), dict(data=torch.zeros(4, 32, 2), max_pos=4, head_dim=64))
     with pytest.raises(_lib.BMError, match="positions"):
         ops.rotary(torch.zeros(2, 4, 64), None, None, table)
+
+
+@pytest.mark.parametrize("scale", [float("inf"), 3.4e38, float("nan")])
+def test_a_scale_that_is_not_finite_is_refused(lib, scale):
+    """Times log2(e), too: every output would be NaN."""
+    assert attend(lib, scale=scale) == _lib.BM_ERR_INVALID_ARGUMENT
+    assert b"scale" in lib.bm_last_error_message()
