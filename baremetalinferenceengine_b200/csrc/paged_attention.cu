@@ -13,7 +13,9 @@
 // (64 rows against 64 slots), and both products run from shared memory in register
 // tiles (4 x 4 scores and 4 x hd/16 outputs per thread), 64 multiply-adds for 8 16-byte
 // shared loads; up to 32 rows have a kernel of their own, bound by its shared loads of Q
-// (8 rows of 128 in fp32 over 16 sequences of 1000 to 2000, 8 heads: 82 us, floor 30). Slots
+// (8 rows of 128 in fp32 over 16 sequences of 1000 to 2000, 8 heads: 84 us, floor 30; of 256 in
+// bf16, which the tensor-core form does not take, 4 rows 72, 32 rows 318, 512 rows 4870 us,
+// floors 27, 28 and 60). Slots
 // are shared out over CTAs when the (sequence, kv head, row tile) triples do not fill the
 // GPU; the shares' partial sums meet in tree_combine_kernel.
 #include <algorithm>

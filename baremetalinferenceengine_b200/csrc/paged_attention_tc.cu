@@ -11,8 +11,13 @@
 // exchange between threads; P overwrites S in TMEM as bf16 and is the A operand of the
 // mix from there. O stays in TMEM; a row whose maximum rises by more than 2^8 (in the
 // exponent's base) is rescaled there, smaller rises leave its weights up to 2^8 (fp32
-// sums, bf16's exponent range: nothing is lost by it). Weights are rounded to bf16 for
-// the mix, the row sums take them before rounding.
+// sums, bf16's exponent range: nothing is lost by it).
+//
+// Weights are rounded to bf16 for the mix, as bm_decode_attention does: both operands of these
+// MMAs have V's type. The row sums take them before rounding. Outputs are off 64 bits by
+// 1.9e-3 to 2.3e-3 in the 2-norm, of which 1.7e-3 is their own rounding. A weight in two bf16 parts
+// (16 MMAs a mix, twice the stores to TMEM) brings that to 1.7e-3 and the three cases measured
+// below to 246, 364 and 27 us; not kept.
 //
 // Bound: memory while group * tokens is below about 200 (two operations per K and V
 // element and row against 2.25 bytes per ns and SM), the tensor cores and the
@@ -21,10 +26,12 @@
 // rows would leave idle is the softmax: a thread walks its row's 128 scores however few
 // rows there are. So with at most 64 (32) rows the row tile holds them twice (four times),
 // and each copy weighs a half (quarter) of the tile's slots, with zero weights elsewhere;
-// the copies' sums meet at the segment's end. Measured on a B200 with both launches: 64
-// sequences of 1 to 8192 and up to 8 drafted tokens, 32 / 8 heads of 128: 181 us (1.03 GB,
-// floor 157; one copy everywhere 197); 16 of 4096 to 8192 and 64, 64 / 8 heads: 241 us (floor
-// 124 by products, 120 by bytes); one of 8000 and 12: 23 us (floor 5).
+// the copies' sums meet at the segment's end. Measured on a B200 with both launches, calls
+// one after the other (in brackets before the power limit lowers the SM clock from 1965 to 1600
+// MHz): 64 sequences of 1 to 8192 and up to 8 drafted tokens, 32 / 8 heads of 128: 214 (189) us
+// (1.03 GB, floor 157; one copy everywhere 16 us more); 16 of 4096 to 8192 and 64, 64 / 8 heads:
+// 285 (241) us (floor 124 by products, 120 by bytes); one of 8000 and 12: 25 us (floor 5); a
+// prompt's 2048 tokens behind 6144 without a mask, 64 / 8 heads: 547 us (floor 290 by products).
 //
 // Split: the host does not see the lengths, so one CTA per SM takes an equal share of
 // all tiles of the batch, counted on the device: items (sequence, kv head, row tile) laid

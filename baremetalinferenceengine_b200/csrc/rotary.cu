@@ -16,9 +16,10 @@
 // or one of `parts` shares of a token's heads when there are few tokens: a decode
 // batch is bound by the chain position -> (cos, sin), sequence -> page -> store, which
 // more warps with one pass each overlap. Data loads are issued before that chain is
-// waited for. Measured on a B200, bf16: 16384 rows of 64 + 8 heads of 128 in 100 us (604 MB,
-// 0.92 of the copy rate), 32768 rows of 64 + 8 appended to pages of 64 in 223 us (0.92), a
-// decode batch of 64 rows in 3.5 us either way.
+// waited for. Measured on a B200, bf16, calls one after the other: 16384 rows of 64 + 8 heads
+// of 128 in 101 to 103 us (604 MB, 0.91 to 0.89 of the copy rate: the power limit), 32768 rows
+// of 64 + 8 appended to pages of 64 in 224 to 227 us (0.92 to 0.90), a decode batch of 64 rows in 4 us
+// either way.
 #include <algorithm>
 #include <cmath>
 

@@ -15,11 +15,12 @@
 //
 // Bound: a row is read from HBM once (the passes below find it in L2), so bytes count
 // only for many rows; there the fp64 operations (eleven a logit where all weigh) cost as
-// much, and one or few rows are bound by the chain of passes. Measured on a B200 with
-// top-p alone: 21 us for one fp32 row of 32000, 28 for one of 128256 and 193 for 256 bf16
-// rows of 128256 (floor 10; 96 without top-p); all settings mixed by row, fp32: 19 us for
-// 8 rows of 128256, 44 for 64 (floor 5). A row of up to 1024 logits stays in one CTA's
-// registers (12 us for 256 rows of 1000; 22 with the passes). A cluster of up to 8 CTAs
+// much, and one or few rows are bound by the chain of passes. Measured on a B200, calls one
+// after the other on changing rows: with top-p alone 9 to 21 us for one fp32 row of 32000 (by
+// the row), 22 for one of 128256 and 202 for 256 bf16 rows of 128256 (floor 10; 100 without
+// a filter, 85 with top-k alone, 17 at temperature 0); all settings mixed by row, fp32: 19 us for
+// 8 rows of 128256, 55 for 64 (floor 5). A row of up to 1024 logits stays in one CTA's
+// registers (11 us for 64 rows of 1000, 22 with the passes; 18 for 256). A cluster of up to 8 CTAs
 // shares a longer row:
 //   1. the largest logit and its first index;
 //   2. for a small top-k: the logits that reach the k-th largest of the maxima of 512 or

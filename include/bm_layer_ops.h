@@ -19,7 +19,7 @@
  *   - Rows are dense and row-major unless a stride argument says otherwise.
  *     16-byte aligned pointers with 16-byte multiple row pitches take the
  *     128-bit vector path; anything else runs a scalar path with the same
- *     results.
+ *     results. Every pointer is aligned to its elements.
  *   - Values that only the device can check (token ids, positions and sequence
  *     ids held in device arrays) are checked by the kernels. A bad row is skipped
  *     (its outputs are left unwritten) and a BM_DEVERR_* bit is OR-ed into
@@ -485,7 +485,8 @@ typedef struct bm_paged_kv {
  * theirs is read or written. Bad positions (outside the table), slots (negative or
  * outside max_pages pages), sequences and page ids flag *d_status; such a row is
  * skipped. The rows of one call name distinct slots: with two rows on one slot either
- * row's values may be kept, chunk by chunk. */
+ * row's values may be kept, chunk by chunk. q_out must not overlap the pages, nor k and v
+ * slots that the call writes. */
 int bm_paged_kv_append(void* q_out, const void* q, const void* k, const void* v, const int32_t* positions,
                        const int32_t* slots, const int32_t* seq_ids, const bm_paged_kv_t* cache, const void* table,
                        int32_t table_len, int32_t rotary_dim, int32_t interleaved, int64_t rows, int32_t num_q_heads,
@@ -502,9 +503,10 @@ int bm_paged_kv_append(void* q_out, const void* q, const void* k, const void* v,
  * over the context and the drafted slots j that it sees: bit j%64 of
  * tree_mask[row][j/64] (uint64 [total_q][mask_words], bits past n_b ignored), or j <= i
  * when tree_mask is NULL. G = num_q_heads / num_kv_heads <= 64, scale <= 0 means
- * 1/sqrt(head_dim), head_dim <= 256 with whole 16-byte rows, and
- * batch * max_tree * num_q_heads <= 2^25. out must not overlap q. A row that sees nothing
- * gets zeros. Rows outside [q_starts[0], q_starts[batch]) are left as they were.
+ * 1/sqrt(head_dim) (a scale that is not finite is refused), head_dim <= 256 with whole 16-byte rows, and
+ * batch * max_tree * num_q_heads <= 2^25. q and out are dense, and out must not overlap
+ * q or the pages. A row that sees nothing gets zeros. With batch, total_q or max_tree 0
+ * nothing runs and nothing is flagged. Rows outside [q_starts[0], q_starts[batch]) are left as they were.
  * max_ctx and max_tree are host-side upper bounds of ctx_lens and n_b that size the
  * work split; with a mask max_tree <= 64 * mask_words. K and V of the ctx + n_b slots
  * must be finite; slots behind them may hold anything. Softmax statistics and sums are
