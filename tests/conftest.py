@@ -18,6 +18,16 @@ def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs a CUDA device (B200) and the built sm_100a library")
 
 
+# These need programs built from the reference's own sources and fail where it is absent.
+NEED_THE_REFERENCE = ("test_gpu_engine.py", "test_gpu_reference.py")
+
+
+def pytest_collection_modifyitems(items):
+    """They run after all others, so that a run that stops at its first failure (-x) has run
+    everything that needs no reference."""
+    items.sort(key=lambda item: item.path.name in NEED_THE_REFERENCE)
+
+
 @pytest.fixture(scope="session")
 def cuda():
     import torch
