@@ -1,4 +1,4 @@
-"""INTEGRATION.md's recipe of a step over a paged cache, compiled as it stands and run against
+"""The integration guide's recipe of a step over a paged cache, compiled as it stands and run against
 stand-ins of the entry points that check how the calls fit together."""
 import os
 import re
