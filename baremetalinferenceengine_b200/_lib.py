@@ -65,6 +65,14 @@ class PagedKVC(ctypes.Structure):
                 ("head_dim", c_int32)]
 
 
+class PagedKV8C(ctypes.Structure):
+    """Mirror of bm_paged_kv8_t."""
+
+    _fields_ = [("k_pages", c_void_p), ("v_pages", c_void_p), ("k_scales", c_void_p), ("v_scales", c_void_p),
+                ("page_table", c_void_p), ("num_pages", c_int32), ("page_size", c_int32), ("block", c_int32),
+                ("max_pages", c_int32), ("num_seqs", c_int32), ("num_kv_heads", c_int32), ("head_dim", c_int32)]
+
+
 # name -> (restype, argtypes). Every symbol include/bm_layer_ops.h declares.
 SIGNATURES = {
     "bm_status_string": (c_char_p, [c_int]),
@@ -130,6 +138,20 @@ SIGNATURES = {
     "bm_paged_tree_attention": (c_int, [c_void_p, c_void_p, ctypes.POINTER(PagedKVC), c_void_p, c_void_p, c_void_p,
                                         c_void_p, c_int32, c_int64, c_int64, c_int32, c_int32, c_int32, c_float,
                                         c_void_p, ctypes.c_size_t, c_int, c_void_p, c_void_p]),
+    "bm_qk_norm_rotary": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_float, c_void_p, c_int32,
+                                  c_void_p, c_int32, c_int32, c_int32, c_int64, c_int32, c_int32, c_int32, c_int64,
+                                  c_int64, c_int64, c_int64, c_int, c_void_p, c_void_p]),
+    "bm_paged_kv8_append": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_float, c_void_p,
+                                    ctypes.POINTER(PagedKV8C), c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int32,
+                                    c_int32, c_int64, c_int64, c_int32, c_int32, c_int64, c_int64, c_int64, c_int64, c_int,
+                                    c_void_p, c_void_p]),
+    "bm_paged_kv8_read": (c_int, [c_void_p, c_void_p, ctypes.POINTER(PagedKV8C), c_void_p, c_void_p, c_void_p, c_int64,
+                                  c_int64, c_int32, c_int, c_void_p, c_void_p]),
+    "bm_paged_kv8_tree_attention_workspace_size": (c_int, [c_int64, c_int64, c_int32, c_int32, c_int32, c_int32, c_int32,
+                                                           ctypes.POINTER(ctypes.c_size_t)]),
+    "bm_paged_kv8_tree_attention": (c_int, [c_void_p, c_void_p, ctypes.POINTER(PagedKV8C), c_void_p, c_void_p, c_void_p,
+                                            c_void_p, c_int32, c_int64, c_int64, c_int32, c_int32, c_int32, c_float,
+                                            c_void_p, ctypes.c_size_t, c_int, c_void_p, c_void_p]),
     "bm_sample": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64,
                           c_int64, c_int, c_void_p, c_void_p]),
     "bm_layer_step": (c_int, [ctypes.POINTER(LayerStepC), c_int, c_void_p, c_void_p]),

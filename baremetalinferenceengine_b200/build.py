@@ -102,8 +102,8 @@ def _build_binding(force: bool) -> None:
             if lacks or f.read() == now:
                 return
     if lacks:
-        print(f"{os.path.basename(BINDING_PATH)} not built: {lacks} (only the Python calls of ops.rotary, paged_kv_append, "
-              "paged_tree_attention and sample need it)", file=sys.stderr)
+        print(f"{os.path.basename(BINDING_PATH)} not built: {lacks} (only the Python calls of ops.rotary, qk_norm_rotary, sample and "
+              "the paged caches' need it)", file=sys.stderr)
         return
     import torch
 

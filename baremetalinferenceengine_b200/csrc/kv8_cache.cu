@@ -1,0 +1,797 @@
+// RMSNorm of every head of Q and K and their rotary positions in one pass
+// (bm_qk_norm_rotary); the same on the way into a paged cache held in 8 bits, which
+// quantises K and V as it writes them (bm_paged_kv8_append); and a stretch of that cache
+// read back as dense rows (bm_paged_kv8_read).
+//
+// Mathematics: per head x of hd elements, with r = rsqrt(mean(x^2) + eps),
+//   y = x r w,  then the pairs (a, b) of its first rd elements become (a c - b s, b c + a s),
+// fp32 throughout, rounded once at the end: to the storage type, or to e4m3 as
+//   code = rne(y 2^-E),  E = max(E before, ceil(log2(max |y| / 448)))
+// over the block's new rows and elements of the head. A block with slots of earlier calls
+// keeps its scale unless it has to grow; then its earlier codes move with it. (A scale left
+// by rows that a later call overwrites is at worst larger than needed, which costs a floating
+// code nothing above 2^-6.)
+//
+// Bound: memory; q, k and v are read once, and q and the codes written once.
+#include <algorithm>
+#include <cmath>
+
+#include "kv8.cuh"
+#include "rotary_device.cuh"
+
+namespace bm {
+namespace {
+
+using namespace bm::rot;
+using namespace bm::kv8;
+
+constexpr int kMaxHeadDim = 256;
+constexpr int kThreads = 128;
+constexpr int kWarps = kThreads / 32;
+constexpr int kU = 4;  // passes whose loads a lane keeps in flight
+
+struct HeadArgs {
+  void* q_out;
+  void* k_out;               // norm_rotary only
+  const void* q;
+  const void* k;
+  const void* v;             // append only
+  const void* q_weight;      // NULL: no norm
+  const void* k_weight;
+  const int32_t* positions;  // norm_rotary: NULL = pos0 + row; append: NULL = the slot
+  const float2* table;       // NULL: no rotation (append only)
+  int64_t rows, q_stride, k_stride, v_stride, q_out_stride, k_out_stride;
+  int32_t pos0, table_len;
+  float eps;
+  int hq, hkv, hd, rd;
+  int units, rest;           // rotated and copied units of a head
+  int heads_per_pass;        // lanes of a warp hold so many heads, or rows of one
+  int parts;                 // warps per row of Q (and K, norm_rotary)
+  int32_t* status;
+  // append
+  bm_paged_kv8_t cache;
+  const int32_t* ctx_lens;
+  const int32_t* starts;
+  const int32_t* seq_ids;
+  int64_t batch, kv_ctas;
+  int max_tokens, blocks, warps_per_job;
+};
+
+// A lane's share of a head: J units of two chunks of N elements.
+template <int N, int J>
+struct Share {
+  int first[J], second[J];
+  bool own[J], pair[J], turns[J];
+  template <bool INTER>
+  __device__ __forceinline__ void place(const HeadArgs& a, int c0, bool live) {
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      const int c = c0 + 32 * j;
+      own[j] = live && c < a.units + a.rest;
+      turns[j] = c < a.units;
+      first[j] = turns[j] ? c * (INTER ? 2 * N : N) : a.rd + (c - a.units) * 2 * N;
+      second[j] = first[j] + (turns[j] && !INTER ? a.rd / 2 : N);
+      pair[j] = own[j] && second[j] < a.hd;  // the last copied unit may have one chunk
+    }
+  }
+};
+
+// The sum over the n lanes of a head (lane = head * n + c), for each of them.
+__device__ __forceinline__ float head_sum(float v, int c, int n, int lane) {
+  if ((n & (n - 1)) == 0) {
+    for (int off = n >> 1; off > 0; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
+    return v;
+  }
+  int region = n;  // the lanes below it hold what is left to add
+  for (int off = 16; off > 0; off >>= 1) {
+    if (off >= n) continue;
+    const float other = __shfl_down_sync(0xffffffffu, v, off);
+    if (c < off && c + off < region) v += other;
+    region = min(region, off);
+  }
+  return __shfl_sync(0xffffffffu, v, lane - c);
+}
+
+template <typename T, int N, int J>
+struct Head {
+  Piece<T, N> p1[J], p2[J];
+
+  __device__ __forceinline__ void load(const T* x, const Share<N, J>& s) {
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      if (s.own[j]) p1[j].load(x + s.first[j]);
+      if (s.pair[j]) p2[j].load(x + s.second[j]);
+    }
+  }
+  __device__ __forceinline__ void get(float (&x)[J][2 * N], const Share<N, J>& s) const {
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+#pragma unroll
+      for (int e = 0; e < 2 * N; ++e) x[j][e] = 0.f;
+      if (s.own[j]) p1[j].get(x[j]);
+      if (s.pair[j]) p2[j].get(x[j] + N);
+    }
+  }
+  __device__ __forceinline__ void set_store(T* to, const float (&x)[J][2 * N], const Share<N, J>& s) {
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      p1[j].set(x[j]);
+      p2[j].set(x[j] + N);
+      if (s.own[j]) p1[j].store(to + s.first[j]);
+      if (s.pair[j]) p2[j].store(to + s.second[j]);
+    }
+  }
+};
+
+// x r w. Every lane of the warp takes part, whether it holds elements or not.
+template <typename T, int N, int J>
+__device__ __forceinline__ void norm(float (&x)[J][2 * N], const Head<T, N, J>& weight, const Share<N, J>& s, const HeadArgs& a,
+                                     int c, int n, int lane) {
+  float sum = 0.f;
+#pragma unroll
+  for (int j = 0; j < J; ++j) {
+#pragma unroll
+    for (int e = 0; e < 2 * N; ++e) sum = fmaf(x[j][e], x[j][e], sum);
+  }
+  const float r = rsqrtf(head_sum(sum, c, n, lane) / a.hd + a.eps);
+  float w[J][2 * N];
+  weight.get(w, s);
+#pragma unroll
+  for (int j = 0; j < J; ++j) {
+#pragma unroll
+    for (int e = 0; e < 2 * N; ++e) x[j][e] = x[j][e] * r * w[j][e];
+  }
+}
+
+template <int N, int J>
+struct Angles {
+  float2 cs[J][N];
+  __device__ __forceinline__ void load(const HeadArgs& a, int pos, int c0, const Share<N, J>& s) {
+    const float2* t = a.table + static_cast<int64_t>(pos) * (a.rd / 2);
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      if (s.own[j] && s.turns[j]) load_angles<N>(t + (c0 + 32 * j) * N, cs[j]);
+    }
+  }
+};
+template <int N, int J, bool INTER>
+__device__ __forceinline__ void turn(float (&x)[J][2 * N], const Angles<N, J>& t, const Share<N, J>& s) {
+#pragma unroll
+  for (int j = 0; j < J; ++j) {
+    if (s.own[j] && s.turns[j]) rotate<N, INTER>(x[j], t.cs[j]);
+  }
+}
+
+// One warp's share of a row's heads: part `part` of a.parts of `heads` heads from src to dst.
+template <typename T, int N, int J, bool INTER>
+__device__ __forceinline__ void turn_heads(const HeadArgs& a, const T* src, T* dst, int heads, int part, const void* weight, int pos,
+                                           int lane) {
+  const int n = min(32, a.units + a.rest), hpi = a.heads_per_pass;
+  const int hl = lane / n, c = lane - hl * n;
+  Share<N, J> s;
+  s.template place<INTER>(a, c, hl < hpi);
+  const int passes = (heads + hpi - 1) / hpi, mine = (passes + a.parts - 1) / a.parts;
+  const int h_end = min(heads, (part + 1) * mine * hpi);
+  if (part * mine * hpi >= h_end) return;
+  Head<T, N, J> w;
+  Angles<N, J> t;
+  bool have = false;
+  for (int hb = part * mine * hpi; hb < h_end; hb += hpi * kU) {  // the same for the warp
+    Head<T, N, J> x[kU];
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      const int h = hb + u * hpi + hl;
+      if (h < h_end) x[u].load(src + static_cast<int64_t>(h) * a.hd, s);
+    }
+    if (!have) {
+      if (weight) w.load(static_cast<const T*>(weight), s);
+      if (a.table) t.load(a, pos, c, s);
+      have = true;
+    }
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      const int h = hb + u * hpi + hl;
+      if (hb + u * hpi >= h_end) break;
+      float y[J][2 * N];
+      x[u].get(y, s);
+      if (weight) norm<T, N, J>(y, w, s, a, c, n, lane);
+      if (a.table) turn<N, J, INTER>(y, t, s);
+      if (h < h_end) x[u].set_store(dst + static_cast<int64_t>(h) * a.hd, y, s);
+    }
+  }
+}
+
+template <typename T, int N, int J, bool INTER>
+__global__ void __launch_bounds__(kThreads) norm_rotary_kernel(const __grid_constant__ HeadArgs a) {
+  grid_dependency_wait();
+  const int lane = threadIdx.x & 31;
+  const int64_t job = static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
+  const int64_t row = job / a.parts;
+  if (row >= a.rows) return;
+  const int part = static_cast<int>(job - row * a.parts);
+  const int32_t pos = a.positions ? __ldg(a.positions + row) : static_cast<int32_t>(a.pos0 + row);
+  if (pos < 0 || pos >= a.table_len) {
+    if (lane == 0) raise_status(a.status, BM_DEVERR_BAD_POSITION);
+    return;
+  }
+  if (a.hq) {
+    turn_heads<T, N, J, INTER>(a, static_cast<const T*>(a.q) + row * a.q_stride, static_cast<T*>(a.q_out) + row * a.q_out_stride,
+                               a.hq, part, a.q_weight, pos, lane);
+  }
+  if (a.hkv) {
+    turn_heads<T, N, J, INTER>(a, static_cast<const T*>(a.k) + row * a.k_stride, static_cast<T*>(a.k_out) + row * a.k_out_stride,
+                               a.hkv, part, a.k_weight, pos, lane);
+  }
+}
+
+// A sequence of the batch: its cache sequence, cached slots, new rows and the first of them.
+struct Span {
+  int seq, ctx, n;
+  int64_t row0;
+};
+// Reads and checks sequence b (starts[b], starts[b + 1], first[b], seq_ids[b]): its rows go
+// to the slots from `first` on. The BM_DEVERR_* bits are 0 when it is sound.
+__device__ __forceinline__ int32_t read_span(const bm_paged_kv8_t& c, const int32_t* starts, const int32_t* first,
+                                             const int32_t* seq_ids, int64_t rows, int most, int64_t b, Span* s) {
+  const int32_t r0 = __ldg(starts + b), r1 = __ldg(starts + b + 1);
+  s->ctx = __ldg(first + b);
+  s->seq = seq_ids ? __ldg(seq_ids + b) : static_cast<int>(b);
+  s->row0 = r0;
+  const int64_t n = static_cast<int64_t>(r1) - r0;
+  s->n = static_cast<int>(n);
+  int32_t bad = 0;
+  if (r0 < 0 || r1 > rows || n < 0 || n > most || s->ctx < 0 || (n > 0 && s->ctx + n > static_cast<int64_t>(c.max_pages) * c.page_size)) {
+    bad |= BM_DEVERR_BAD_POSITION;
+  }
+  if (s->seq < 0 || s->seq >= c.num_seqs) bad |= BM_DEVERR_BAD_SEQUENCE;
+  if (bad) s->n = 0;
+  return bad;
+}
+
+// N codes to memory.
+template <int N>
+__device__ __forceinline__ void store_codes(uint8_t* to, const float* x, float f) {
+  if constexpr (N == 1) {
+    *to = static_cast<uint8_t>(to_codes(x[0] * f, 0.f));
+  } else {
+    uint32_t w[N / 4];
+#pragma unroll
+    for (int e = 0; e < N; e += 4) w[e / 4] = to_codes(x[e] * f, x[e + 1] * f) | to_codes(x[e + 2] * f, x[e + 3] * f) << 16;
+    if constexpr (N == 8) {
+      *reinterpret_cast<uint2*>(to) = make_uint2(w[0], w[1]);
+    } else {
+      *reinterpret_cast<uint32_t*>(to) = w[0];
+    }
+  }
+}
+
+// The first kv_ctas blocks take K and V: one job is K or V of one head in one block of slots,
+// held by warps_per_job warps of a block (16 rows each in registers, at the widest heads 128
+// elements). A lane group holds a row, so the norm is a sum over a group and the scale a
+// maximum over the warp, then over the job's warps. The other blocks rotate Q.
+template <typename T, int N, int J, bool INTER>
+__global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant__ HeadArgs a) {
+  grid_dependency_wait();
+  __shared__ uint32_t tops[kWarps];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const bm_paged_kv8_t& c8 = a.cache;
+  if (blockIdx.x >= a.kv_ctas) {
+    const int64_t job = (static_cast<int64_t>(blockIdx.x) - a.kv_ctas) * kWarps + warp;
+    const int64_t token = job / a.parts;
+    const int part = static_cast<int>(job - token * a.parts);
+    const int64_t b = token / a.max_tokens;
+    const int j = static_cast<int>(token - b * a.max_tokens);
+    if (b >= a.batch) return;
+    Span s;
+    if (read_span(c8, a.starts, a.ctx_lens, a.seq_ids, a.rows, a.max_tokens, b, &s) || j >= s.n) return;
+    const int64_t row = s.row0 + j;
+    const int32_t pos = a.positions ? __ldg(a.positions + row) : s.ctx + j;
+    if (a.table && (pos < 0 || pos >= a.table_len)) return;  // K's and V's jobs tell
+    turn_heads<T, N, J, INTER>(a, static_cast<const T*>(a.q) + row * a.q_stride, static_cast<T*>(a.q_out) + row * a.q_out_stride,
+                               a.hq, part, a.q_weight, pos, lane);
+    return;
+  }
+  // ---------------- K and V ----------------
+  const int wpj = a.warps_per_job, sub = warp % wpj;
+  const int64_t job = static_cast<int64_t>(blockIdx.x) * (kWarps / wpj) + warp / wpj;
+  const int which = static_cast<int>(job % (2 * a.hkv));
+  const int head = which >> 1;
+  const bool is_v = which & 1;
+  const int64_t bj = job / (2 * a.hkv), b = bj / a.blocks;
+  const int jb = static_cast<int>(bj - b * a.blocks);
+  Span s{};
+  int lo = 0, hi = 0, begin = 0;     // the block's new slots; its first slot
+  uint8_t *pages = nullptr, *scale = nullptr;
+  bool active = b < a.batch;
+  if (active) {
+    const int32_t bad = read_span(c8, a.starts, a.ctx_lens, a.seq_ids, a.rows, a.max_tokens, b, &s);
+    if (bad && jb == 0 && which == 0 && lane == 0 && sub == 0) raise_status(a.status, bad);
+    // 64 bits: a block's end may pass the last slot there can be
+    const int64_t from = (static_cast<int64_t>(s.ctx / c8.block) + jb) * c8.block;
+    lo = static_cast<int>(max(static_cast<int64_t>(s.ctx), min(from, static_cast<int64_t>(s.ctx) + s.n)));
+    hi = static_cast<int>(min(static_cast<int64_t>(s.ctx) + s.n, from + c8.block));
+    active = !bad && lo < hi;
+    if (active) {
+      begin = static_cast<int>(from);
+      const int nth = begin / c8.page_size;
+      const int32_t page = __ldg(c8.page_table + static_cast<int64_t>(s.seq) * c8.max_pages + nth);
+      if (page < 0 || page >= c8.num_pages) {
+        if (lane == 0 && sub == 0) raise_status(a.status, BM_DEVERR_BAD_PAGE);
+        active = false;
+      } else {
+        const int64_t ph = static_cast<int64_t>(page) * a.hkv + head;
+        const int off = begin - nth * c8.page_size;
+        pages = static_cast<uint8_t*>(is_v ? c8.v_pages : c8.k_pages) + (ph * c8.page_size + off) * a.hd;
+        scale = static_cast<uint8_t*>(is_v ? c8.v_scales : c8.k_scales) + ph * (c8.page_size / c8.block) + off / c8.block;
+      }
+    }
+  }
+  if (!active) lo = hi = 0;
+  // A block with slots of earlier calls has a scale: read here, since the job's first warp
+  // writes it at its own end, behind the barrier.
+  const bool keeps = active && begin < s.ctx;
+  const int before = keeps ? exponent(*scale) : kLowest;
+  const int n = min(32, a.units + a.rest), rpi = a.heads_per_pass;
+  const int rl = lane / n, c = lane - rl * n;
+  Share<N, J> sh;
+  sh.template place<INTER>(a, c, rl < rpi);
+  const T* src = static_cast<const T*>(is_v ? a.v : a.k) + static_cast<int64_t>(head) * a.hd;
+  const int64_t stride = is_v ? a.v_stride : a.k_stride;
+  const bool normed = !is_v && a.k_weight, turned = !is_v && a.table;
+  Head<T, N, J> w;
+  if (normed && active) w.load(static_cast<const T*>(a.k_weight), sh);
+
+  // Batches of kU passes, of rpi rows each, in turn over the job's warps. One batch stays in
+  // registers until its scale is known; more are read again.
+  const int step = kU * rpi * wpj;
+  float y[kU][J][2 * N];
+  bool good[kU];
+  uint32_t top = 0;
+  int bad_position = 0;
+  auto batch = [&](int from) {
+    Head<T, N, J> x[kU];
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      const int slot = from + (sub * kU + u) * rpi + rl;
+      good[u] = active && slot < hi && rl < rpi;
+      if (good[u]) x[u].load(src + (s.row0 + (slot - s.ctx)) * stride, sh);
+    }
+    int32_t pos[kU];
+    if (a.table) {  // V, too, leaves out the rows whose position is bad
+#pragma unroll
+      for (int u = 0; u < kU; ++u) {
+        const int slot = from + (sub * kU + u) * rpi + rl;
+        pos[u] = !good[u] ? 0 : a.positions ? __ldg(a.positions + s.row0 + (slot - s.ctx)) : slot;
+        if (pos[u] < 0 || pos[u] >= a.table_len) {
+          good[u] = false;
+          bad_position = 1;
+        }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      Angles<N, J> t;
+      if (turned && good[u]) t.load(a, pos[u], c, sh);
+      x[u].get(y[u], sh);
+      if (normed) norm<T, N, J>(y[u], w, sh, a, c, n, lane);
+      if (turned && good[u]) turn<N, J, INTER>(y[u], t, sh);
+    }
+  };
+  const int batches = (hi - lo + step - 1) / step;
+  for (int i = 0; i < batches; ++i) {
+    batch(lo + i * step);
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+#pragma unroll
+        for (int e = 0; e < 2 * N; ++e) top = max(top, good[u] && (e < N ? sh.own[j] : sh.pair[j]) ? magnitude(y[u][j][e]) : 0u);
+      }
+    }
+  }
+  top = __reduce_max_sync(0xffffffffu, top);
+  if (wpj > 1) {
+    if (lane == 0) tops[warp] = top;
+    __syncthreads();
+    for (int i = 0; i < wpj; ++i) top = max(top, tops[warp - sub + i]);
+  }
+  if (bad_position) raise_status(a.status, BM_DEVERR_BAD_POSITION);
+  if (!active) return;
+  const int e = max(exponent_for(top), before);
+  if (keeps && e > before) {
+    const float f = power(before - e);
+    const int chunks = (s.ctx - begin) * (a.hd / 16);
+    for (int i = sub * 32 + lane; i < chunks; i += wpj * 32) {
+      uint4* at = reinterpret_cast<uint4*>(pages) + i;
+      uint4 raw = *at;
+      uint32_t* words = &raw.x;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        float v[4];
+        from_codes(words[k], v);
+        words[k] = to_codes(v[0] * f, v[1] * f) | to_codes(v[2] * f, v[3] * f) << 16;
+      }
+      *at = raw;
+    }
+  }
+  const float f = power(-e);
+  for (int i = 0; i < batches; ++i) {
+    if (batches > 1) batch(lo + i * step);
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      const int slot = lo + i * step + (sub * kU + u) * rpi + rl;
+      uint8_t* to = pages + static_cast<int64_t>(slot - begin) * a.hd;
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+        if (good[u] && sh.own[j]) store_codes<N>(to + sh.first[j], y[u][j], f);
+        if (good[u] && sh.pair[j]) store_codes<N>(to + sh.second[j], y[u][j] + N, f);
+      }
+    }
+  }
+  if (lane == 0 && sub == 0) *scale = static_cast<uint8_t>(e + 127);
+}
+
+struct ReadArgs {
+  void* k_out;
+  void* v_out;
+  bm_paged_kv8_t cache;
+  const int32_t* first;
+  const int32_t* starts;
+  const int32_t* seq_ids;
+  int64_t rows, batch;
+  int max_rows, chunks;  // the most rows of a sequence; jobs of them
+  int32_t* status;
+};
+
+// 16 values to memory.
+template <typename T>
+__device__ __forceinline__ void store16(T* to, const uint4& codes, float f) {
+  float v[16];
+  from_codes(codes.x, v);
+  from_codes(codes.y, v + 4);
+  from_codes(codes.z, v + 8);
+  from_codes(codes.w, v + 12);
+#pragma unroll
+  for (int e = 0; e < 16; ++e) v[e] *= f;
+#pragma unroll
+  for (int e = 0; e < 16; e += VecWidth<T>::value) st_plain(to + e, pack16<T>(v + e));
+}
+
+// A warp takes K and V of one head in kU passes of rows; a lane 16 codes of each.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) read_kernel(const __grid_constant__ ReadArgs a) {
+  grid_dependency_wait();
+  const bm_paged_kv8_t& c8 = a.cache;
+  const int lane = threadIdx.x & 31;
+  const int64_t job = static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
+  const int head = static_cast<int>(job % c8.num_kv_heads);
+  const int64_t rest = job / c8.num_kv_heads, b = rest / a.chunks;
+  const int chunk = static_cast<int>(rest - b * a.chunks);
+  if (b >= a.batch) return;
+  Span s;
+  const int32_t bad = read_span(c8, a.starts, a.first, a.seq_ids, a.rows, a.max_rows, b, &s);
+  if (bad) {
+    if (chunk == 0 && head == 0 && lane == 0) raise_status(a.status, bad);
+    return;
+  }
+  const int n = c8.head_dim / 16, rpi = 32 / n;  // lanes of a row, rows of a pass
+  const int rl = lane / n, c = lane - rl * n;
+  const int i0 = chunk * kU * rpi + rl;
+  if (rl >= rpi) return;
+  uint4 k[kU], v[kU];
+  float kf[kU], vf[kU];
+  bool good[kU];
+#pragma unroll
+  for (int u = 0; u < kU; ++u) {
+    const int i = i0 + u * rpi;
+    good[u] = i < s.n;
+    if (good[u]) {
+      const int slot = s.ctx + i, nth = slot / c8.page_size;
+      const int32_t page = __ldg(c8.page_table + static_cast<int64_t>(s.seq) * c8.max_pages + nth);
+      good[u] = page >= 0 && page < c8.num_pages;
+      if (good[u]) {
+        const int64_t ph = static_cast<int64_t>(page) * c8.num_kv_heads + head;
+        const int off = slot - nth * c8.page_size;
+        const int64_t at = (ph * c8.page_size + off) * c8.head_dim + c * 16;
+        const int64_t sc = ph * (c8.page_size / c8.block) + off / c8.block;
+        k[u] = ld_stream(static_cast<const uint8_t*>(c8.k_pages) + at);
+        v[u] = ld_stream(static_cast<const uint8_t*>(c8.v_pages) + at);
+        kf[u] = power(exponent(static_cast<const uint8_t*>(c8.k_scales)[sc]));
+        vf[u] = power(exponent(static_cast<const uint8_t*>(c8.v_scales)[sc]));
+      } else if (c == 0) {
+        raise_status(a.status, BM_DEVERR_BAD_PAGE);
+      }
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < kU; ++u) {
+    if (!good[u]) continue;
+    const int64_t to = ((s.row0 + i0 + u * rpi) * c8.num_kv_heads + head) * c8.head_dim + c * 16;
+    store16(static_cast<T*>(a.k_out) + to, k[u], kf[u]);
+    store16(static_cast<T*>(a.v_out) + to, v[u], vf[u]);
+  }
+}
+
+// Sets the units of a head and calls go(N, J): the widest chunk that divides every run of
+// elements and suits every pointer and stride, as rotary.cu picks it: 16 bytes, 8 (bf16),
+// else single elements, of which a lane holds up to four pairs.
+template <typename F>
+int with_chunk(HeadArgs* a, bm_dtype_t dtype, F go) {
+  const int es = dtype_size(dtype);
+  auto fits = [&](int n) {
+    if ((a->rd / 2) % n || (a->hd - a->rd) % n || a->hd % n) return false;
+    const uintptr_t bytes = static_cast<uintptr_t>(n) * es;
+    for (const void* p : {a->q, a->k, a->v, static_cast<const void*>(a->q_out), static_cast<const void*>(a->k_out), a->q_weight, a->k_weight}) {
+      if (reinterpret_cast<uintptr_t>(p) % bytes) return false;
+    }
+    for (int64_t s : {a->q_stride, a->k_stride, a->v_stride, a->q_out_stride, a->k_out_stride}) {
+      if (s % n) return false;
+    }
+    return n % 2 != 0 || aligned16(a->table);
+  };
+  int n = 16 / es;
+  if (!fits(n)) n = es == 2 && fits(4) ? 4 : 1;
+  a->units = a->rd / 2 / n;
+  a->rest = (a->hd - a->rd + 2 * n - 1) / (2 * n);
+  a->heads_per_pass = 32 / std::min(32, a->units + a->rest);
+  return go(n);
+}
+
+// Warps of a row of heads: one where the rows fill the GPU (2048 warps: 14 per SM), else up to 8.
+int parts_for(int64_t rows) {
+  return static_cast<int>(std::min<int64_t>(8, std::max<int64_t>(1, 2048 / std::max<int64_t>(1, rows))));
+}
+
+int check_heads(const char* what, int64_t rows, int hq, int hkv, int hd) {
+  if (rows < 0 || rows > INT32_MAX || hq < 0 || hkv < 0 || hq > (1 << 16) || hkv > (1 << 16)) {
+    return fail(BM_ERR_INVALID_ARGUMENT, "%s: bad rows or head count", what);
+  }
+  if (hd <= 0 || hd > kMaxHeadDim) return fail(BM_ERR_INVALID_ARGUMENT, "%s: head_dim %d outside [1, %d]", what, hd, kMaxHeadDim);
+  return BM_OK;
+}
+int check_eps(const char* what, float eps) {
+  if (!(eps >= 0.f) || !std::isfinite(eps)) return fail(BM_ERR_INVALID_ARGUMENT, "%s: eps must be finite and >= 0", what);
+  return BM_OK;
+}
+// Whether the weights of a norm (hd elements, or NULL) meet an output.
+bool meets_weight(const Rows& out, const void* w, int hd, int64_t rows, int es) {
+  if (w == nullptr || out.p == nullptr || out.n == 0) return false;
+  const uintptr_t o = reinterpret_cast<uintptr_t>(out.p), i = reinterpret_cast<uintptr_t>(w);
+  return o < i + static_cast<uintptr_t>(hd) * es && i < o + static_cast<uintptr_t>((rows - 1) * out.stride + out.n) * es;
+}
+
+}  // namespace
+
+int check_paged_kv8(const char* what, const bm_paged_kv8_t* c) {
+  if (!c) return fail(BM_ERR_INVALID_ARGUMENT, "%s: NULL cache", what);
+  if (!c->k_pages || !c->v_pages || !c->k_scales || !c->v_scales || !c->page_table) {
+    return fail(BM_ERR_INVALID_ARGUMENT, "%s: NULL pointer in the cache", what);
+  }
+  if (c->num_pages <= 0 || c->page_size <= 0 || c->block <= 0 || c->max_pages <= 0 || c->num_seqs <= 0 || c->num_kv_heads <= 0 ||
+      c->num_kv_heads > (1 << 16)) {
+    return fail(BM_ERR_INVALID_ARGUMENT, "%s: bad sizes in the cache", what);
+  }
+  if (c->head_dim <= 0 || c->head_dim > kMaxHeadDim || c->head_dim % 16) {
+    return fail(BM_ERR_INVALID_ARGUMENT, "%s: head_dim %d of an 8-bit cache must be a multiple of 16 up to %d", what, c->head_dim, kMaxHeadDim);
+  }
+  if (c->page_size % c->block) return fail(BM_ERR_INVALID_ARGUMENT, "%s: block %d does not divide page_size %d", what, c->block, c->page_size);
+  if (static_cast<int64_t>(c->page_size) * c->max_pages > INT32_MAX) {
+    return fail(BM_ERR_INVALID_ARGUMENT, "%s: page_size * max_pages above 2^31 - 1", what);
+  }
+  if (!aligned16(c->k_pages) || !aligned16(c->v_pages)) return fail(BM_ERR_INVALID_ARGUMENT, "%s: pages must be 16-byte aligned", what);
+  if (!aligned_to(c->page_table, 4)) return fail(BM_ERR_INVALID_ARGUMENT, "%s: a pointer is not aligned to its elements", what);
+  return BM_OK;
+}
+
+bool meets_pages8(const bm_paged_kv8_t& c, const void* p, uintptr_t bytes) {
+  const uintptr_t from = reinterpret_cast<uintptr_t>(p);
+  const uintptr_t slots = static_cast<uintptr_t>(c.num_pages) * c.num_kv_heads * c.page_size;
+  auto meets = [&](const void* q, uintptr_t n) {
+    const uintptr_t lo = reinterpret_cast<uintptr_t>(q);
+    return from < lo + n && lo < from + bytes;
+  };
+  return meets(c.k_pages, slots * c.head_dim) || meets(c.v_pages, slots * c.head_dim) || meets(c.k_scales, slots / c.block) ||
+         meets(c.v_scales, slots / c.block);
+}
+
+}  // namespace bm
+
+extern "C" int bm_qk_norm_rotary(void* q_out, void* k_out, const void* q, const void* k, const void* q_weight, const void* k_weight,
+                                 float eps, const int32_t* positions, int32_t pos0, const void* table, int32_t table_len,
+                                 int32_t rotary_dim, int32_t interleaved, int64_t rows, int32_t num_q_heads, int32_t num_kv_heads,
+                                 int32_t head_dim, int64_t q_stride, int64_t k_stride, int64_t q_out_stride, int64_t k_out_stride,
+                                 bm_dtype_t dtype, int32_t* d_status, void* stream) {
+  using namespace bm;
+  const char* what = "bm_qk_norm_rotary";
+  if (!valid_dtype(dtype)) return fail(BM_ERR_INVALID_ARGUMENT, "%s: bad dtype %d", what, static_cast<int>(dtype));
+  if (int st = check_heads(what, rows, num_q_heads, num_kv_heads, head_dim)) return st;
+  if (int st = check_eps(what, eps)) return st;
+  if (!table) return fail(BM_ERR_INVALID_ARGUMENT, "%s: NULL table", what);
+  if (int st = check_rotation(what, table, table_len, rotary_dim, head_dim)) return st;
+  if (rows == 0 || (num_q_heads == 0 && num_kv_heads == 0)) return BM_OK;
+  if ((num_q_heads > 0 && (!q || !q_out || !q_weight)) || (num_kv_heads > 0 && (!k || !k_out || !k_weight))) {
+    return fail(BM_ERR_INVALID_ARGUMENT, "%s: NULL pointer", what);
+  }
+  const int64_t qn = static_cast<int64_t>(num_q_heads) * head_dim, kn = static_cast<int64_t>(num_kv_heads) * head_dim;
+  if ((qn && (q_stride < qn || q_out_stride < qn)) || (kn && (k_stride < kn || k_out_stride < kn))) {
+    return fail(BM_ERR_INVALID_ARGUMENT, "%s: a row stride below heads * head_dim", what);
+  }
+  if (!positions && (pos0 < 0 || pos0 + rows > INT32_MAX)) return fail(BM_ERR_INVALID_ARGUMENT, "%s: bad pos0", what);
+  const int es = dtype_size(dtype);
+  if (!aligned_to({q, k, q_out, k_out, q_weight, k_weight}, es) || !aligned_to({positions, d_status}, 4)) {
+    return fail(BM_ERR_INVALID_ARGUMENT, "%s: a pointer is not aligned to its elements", what);
+  }
+  const Rows qi{q, q_stride, qn}, ki{k, k_stride, kn}, qo{q_out, q_out_stride, qn}, ko{k_out, k_out_stride, kn};
+  if ((meet(qo, qi, rows, es) && !same(qo, qi, rows)) || (meet(ko, ki, rows, es) && !same(ko, ki, rows)) ||
+      meet(qo, ki, rows, es) || meet(ko, qi, rows, es) || meet(qo, ko, rows, es)) {
+    return fail(BM_ERR_INVALID_ARGUMENT, "%s: an output overlaps an input or the other output", what);
+  }
+  for (const void* w : {num_q_heads ? q_weight : nullptr, num_kv_heads ? k_weight : nullptr}) {
+    if (meets_weight(qo, w, head_dim, rows, es) || meets_weight(ko, w, head_dim, rows, es)) {
+      return fail(BM_ERR_INVALID_ARGUMENT, "%s: an output overlaps a weight", what);
+    }
+  }
+  HeadArgs a{};
+  if (num_q_heads) {
+    a.q_out = q_out;
+    a.q = q;
+    a.q_weight = q_weight;
+    a.q_stride = q_stride;
+    a.q_out_stride = q_out_stride;
+  }
+  if (num_kv_heads) {
+    a.k_out = k_out;
+    a.k = k;
+    a.k_weight = k_weight;
+    a.k_stride = k_stride;
+    a.k_out_stride = k_out_stride;
+  }
+  a.eps = eps;
+  a.positions = positions;
+  a.pos0 = pos0;
+  a.table = static_cast<const float2*>(table);
+  a.table_len = table_len;
+  a.rd = rotary_dim;
+  a.rows = rows;
+  a.hq = num_q_heads;
+  a.hkv = num_kv_heads;
+  a.hd = head_dim;
+  a.status = d_status;
+  a.parts = parts_for(rows);
+  const int64_t blocks = (rows * a.parts + kWarps - 1) / kWarps;
+  return with_chunk(&a, dtype, [&](int n) {
+    auto go = [&](auto kernel) {
+      return launch_kernel(what, kernel, dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0, as_stream(stream), nullptr, a);
+    };
+    if (dtype == BM_F32) {
+      if (n == 4) return interleaved ? go(norm_rotary_kernel<float, 4, 1, true>) : go(norm_rotary_kernel<float, 4, 1, false>);
+      return interleaved ? go(norm_rotary_kernel<float, 1, 4, true>) : go(norm_rotary_kernel<float, 1, 4, false>);
+    }
+    if (n == 8) return interleaved ? go(norm_rotary_kernel<bf16, 8, 1, true>) : go(norm_rotary_kernel<bf16, 8, 1, false>);
+    if (n == 4) return interleaved ? go(norm_rotary_kernel<bf16, 4, 1, true>) : go(norm_rotary_kernel<bf16, 4, 1, false>);
+    return interleaved ? go(norm_rotary_kernel<bf16, 1, 4, true>) : go(norm_rotary_kernel<bf16, 1, 4, false>);
+  });
+}
+
+extern "C" int bm_paged_kv8_append(void* q_out, const void* q, const void* k, const void* v, const void* q_weight,
+                                   const void* k_weight, float eps, const int32_t* positions, const bm_paged_kv8_t* cache,
+                                   const int32_t* seq_ids, const int32_t* ctx_lens, const int32_t* q_starts, const void* table,
+                                   int32_t table_len, int32_t rotary_dim, int32_t interleaved, int64_t rows, int64_t batch,
+                                   int32_t num_q_heads, int32_t max_tokens, int64_t q_stride, int64_t k_stride, int64_t v_stride,
+                                   int64_t q_out_stride, bm_dtype_t dtype, int32_t* d_status, void* stream) {
+  using namespace bm;
+  const char* what = "bm_paged_kv8_append";
+  if (!valid_dtype(dtype)) return fail(BM_ERR_INVALID_ARGUMENT, "%s: bad dtype %d", what, static_cast<int>(dtype));
+  if (int st = check_paged_kv8(what, cache)) return st;
+  const bm_paged_kv8_t& c = *cache;
+  if (int st = check_heads(what, rows, num_q_heads, c.num_kv_heads, c.head_dim)) return st;
+  if (int st = check_eps(what, eps)) return st;
+  if (batch < 0 || batch > INT32_MAX || max_tokens < 0) return fail(BM_ERR_INVALID_ARGUMENT, "%s: bad batch or max_tokens", what);
+  if (table) {
+    if (int st = check_rotation(what, table, table_len, rotary_dim, c.head_dim)) return st;
+  }
+  if (rows == 0 || batch == 0 || max_tokens == 0) return BM_OK;
+  if (!k || !v || !ctx_lens || !q_starts || (num_q_heads > 0 && (!q || !q_out))) return fail(BM_ERR_INVALID_ARGUMENT, "%s: NULL pointer", what);
+  if (!seq_ids && batch > c.num_seqs) return fail(BM_ERR_INVALID_ARGUMENT, "%s: more sequences than the cache holds", what);
+  const int64_t qn = static_cast<int64_t>(num_q_heads) * c.head_dim, kn = static_cast<int64_t>(c.num_kv_heads) * c.head_dim;
+  if ((qn && (q_stride < qn || q_out_stride < qn)) || k_stride < kn || v_stride < kn) {
+    return fail(BM_ERR_INVALID_ARGUMENT, "%s: a row stride below heads * head_dim", what);
+  }
+  const int es = dtype_size(dtype);
+  if (!aligned_to({q, k, v, q_out, q_weight, k_weight}, es) || !aligned_to({positions, seq_ids, ctx_lens, q_starts, d_status}, 4)) {
+    return fail(BM_ERR_INVALID_ARGUMENT, "%s: a pointer is not aligned to its elements", what);
+  }
+  const Rows qi{q, q_stride, qn}, qo{q_out, q_out_stride, qn}, ki{k, k_stride, kn}, vi{v, v_stride, kn};
+  if ((meet(qo, qi, rows, es) && !same(qo, qi, rows)) || meet(qo, ki, rows, es) || meet(qo, vi, rows, es) ||
+      meets_weight(qo, q_weight, c.head_dim, rows, es) || meets_weight(qo, k_weight, c.head_dim, rows, es)) {
+    return fail(BM_ERR_INVALID_ARGUMENT, "%s: q_out overlaps an input", what);
+  }
+  auto in_cache = [&](const Rows& r) { return r.n != 0 && meets_pages8(c, r.p, static_cast<uintptr_t>((rows - 1) * r.stride + r.n) * es); };
+  if (in_cache(qo) || in_cache(qi) || in_cache(ki) || in_cache(vi)) {
+    return fail(BM_ERR_INVALID_ARGUMENT, "%s: q, k, v or q_out overlaps the cache", what);
+  }
+  HeadArgs a{};
+  if (num_q_heads) {
+    a.q_out = q_out;
+    a.q = q;
+    a.q_weight = q_weight;
+    a.q_stride = q_stride;
+    a.q_out_stride = q_out_stride;
+  }
+  a.k = k;
+  a.v = v;
+  a.k_weight = k_weight;
+  a.k_stride = k_stride;
+  a.v_stride = v_stride;
+  a.eps = eps;
+  a.positions = positions;
+  a.table = static_cast<const float2*>(table);
+  a.table_len = table_len;
+  a.rd = table ? rotary_dim : 0;
+  a.rows = rows;
+  a.hq = num_q_heads;
+  a.hkv = c.num_kv_heads;
+  a.hd = c.head_dim;
+  a.status = d_status;
+  a.cache = c;
+  a.ctx_lens = ctx_lens;
+  a.starts = q_starts;
+  a.seq_ids = seq_ids;
+  a.batch = batch;
+  a.max_tokens = max_tokens;
+  a.blocks = static_cast<int>((static_cast<int64_t>(max_tokens) - 1 + c.block - 1) / c.block + 1);  // that max_tokens neighbouring slots can meet
+  a.parts = parts_for(std::min<int64_t>(rows, batch * static_cast<int64_t>(max_tokens)));
+  return with_chunk(&a, dtype, [&](int n) {
+    // 64 slots of a block need the registers of four warps (kU passes of four rows of 128)
+    const int one = kU * a.heads_per_pass;
+    a.warps_per_job = std::min(max_tokens, c.block) <= one ? 1 : std::min(max_tokens, c.block) <= 2 * one ? 2 : kWarps;
+    const int64_t per = kWarps / a.warps_per_job;
+    const double jobs = static_cast<double>(batch) * a.blocks * 2 * a.hkv, q_jobs = static_cast<double>(batch) * max_tokens * a.parts;
+    if (jobs + q_jobs > INT32_MAX) return fail(BM_ERR_INVALID_ARGUMENT, "%s: batch * max_tokens too large", what);
+    a.kv_ctas = (batch * a.blocks * 2 * a.hkv + per - 1) / per;
+    const int64_t q_ctas = num_q_heads ? (batch * max_tokens * a.parts + kWarps - 1) / kWarps : 0;
+    auto go = [&](auto kernel) {
+      return launch_kernel(what, kernel, dim3(static_cast<unsigned>(a.kv_ctas + q_ctas)), dim3(kThreads), 0, as_stream(stream), nullptr, a);
+    };
+    if (dtype == BM_F32) {
+      if (n == 4) return interleaved ? go(append_kernel<float, 4, 1, true>) : go(append_kernel<float, 4, 1, false>);
+      return interleaved ? go(append_kernel<float, 1, 4, true>) : go(append_kernel<float, 1, 4, false>);
+    }
+    if (n == 8) return interleaved ? go(append_kernel<bf16, 8, 1, true>) : go(append_kernel<bf16, 8, 1, false>);
+    if (n == 4) return interleaved ? go(append_kernel<bf16, 4, 1, true>) : go(append_kernel<bf16, 4, 1, false>);
+    return interleaved ? go(append_kernel<bf16, 1, 4, true>) : go(append_kernel<bf16, 1, 4, false>);
+  });
+}
+
+extern "C" int bm_paged_kv8_read(void* k_out, void* v_out, const bm_paged_kv8_t* cache, const int32_t* seq_ids, const int32_t* first,
+                                 const int32_t* starts, int64_t rows, int64_t batch, int32_t max_rows, bm_dtype_t dtype,
+                                 int32_t* d_status, void* stream) {
+  using namespace bm;
+  const char* what = "bm_paged_kv8_read";
+  if (!valid_dtype(dtype)) return fail(BM_ERR_INVALID_ARGUMENT, "%s: bad dtype %d", what, static_cast<int>(dtype));
+  if (int st = check_paged_kv8(what, cache)) return st;
+  const bm_paged_kv8_t& c = *cache;
+  if (rows < 0 || rows > INT32_MAX || batch < 0 || batch > INT32_MAX || max_rows < 0) {
+    return fail(BM_ERR_INVALID_ARGUMENT, "%s: bad rows, batch or max_rows", what);
+  }
+  if (rows == 0 || batch == 0 || max_rows == 0) return BM_OK;
+  if (!k_out || !v_out || !first || !starts) return fail(BM_ERR_INVALID_ARGUMENT, "%s: NULL pointer", what);
+  if (!seq_ids && batch > c.num_seqs) return fail(BM_ERR_INVALID_ARGUMENT, "%s: more sequences than the cache holds", what);
+  if (!aligned16(k_out) || !aligned16(v_out)) return fail(BM_ERR_INVALID_ARGUMENT, "%s: k_out and v_out must be 16-byte aligned", what);
+  if (!aligned_to({seq_ids, first, starts, d_status}, 4)) return fail(BM_ERR_INVALID_ARGUMENT, "%s: a pointer is not aligned to its elements", what);
+  const uintptr_t bytes = static_cast<uintptr_t>(rows) * c.num_kv_heads * c.head_dim * dtype_size(dtype);
+  const uintptr_t ko = reinterpret_cast<uintptr_t>(k_out), vo = reinterpret_cast<uintptr_t>(v_out);
+  if ((ko < vo + bytes && vo < ko + bytes) || meets_pages8(c, k_out, bytes) || meets_pages8(c, v_out, bytes)) {
+    return fail(BM_ERR_INVALID_ARGUMENT, "%s: an output overlaps the other or the cache", what);
+  }
+  ReadArgs a{k_out, v_out, c, first, starts, seq_ids, rows, batch, max_rows, 0, d_status};
+  const int per = kU * (32 / (c.head_dim / 16));
+  a.chunks = static_cast<int>((static_cast<int64_t>(max_rows) + per - 1) / per);
+  const double jobs = static_cast<double>(batch) * a.chunks * c.num_kv_heads;
+  if (jobs > INT32_MAX) return fail(BM_ERR_INVALID_ARGUMENT, "%s: batch * max_rows too large", what);
+  const int64_t blocks = (batch * a.chunks * c.num_kv_heads + kWarps - 1) / kWarps;
+  auto go = [&](auto kernel) {
+    return launch_kernel(what, kernel, dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0, as_stream(stream), nullptr, a);
+  };
+  return dtype == BM_F32 ? go(read_kernel<float>) : go(read_kernel<bf16>);
+}

@@ -1,6 +1,7 @@
-// Attention of a tree of drafted tokens per sequence over a paged KV cache: the entry
-// points (bm_paged_tree_attention), and the CUDA-core kernels that serve fp32, every
-// head_dim and every page size. The tensor-core form is paged_attention_tc.cu.
+// Attention of a tree of drafted tokens per sequence over a paged KV cache, of the storage
+// type or in 8 bits: the entry points (bm_paged_tree_attention, bm_paged_kv8_tree_attention),
+// and the CUDA-core kernels that serve fp32, every head_dim and every page size. The
+// tensor-core form of the first is paged_attention_tc.cu.
 //
 // Mathematics: for row r = (token i, head) of a sequence, over the slots t that it sees,
 //   out = sum_t 2^(s_t - m) v_t / sum_t 2^(s_t - m),  s_t = q . k_t * scale * log2(e),
@@ -22,18 +23,40 @@
 #include <cmath>
 #include <type_traits>
 
+#include "kv8.cuh"
 #include "paged_attention.cuh"
 
 namespace bm {
 namespace paged {
 namespace {
 
+using Code = uint8_t;  // the cache's element where it is held in 8 bits, else T
+
 constexpr int kThreads = 256;
 constexpr int BM = 64;   // query rows of a CTA
 constexpr int kBN = 64;  // slots per tile
 
+// A 16-byte chunk of the cache as floats (codes without their scale).
+template <typename C>
+__device__ __forceinline__ void unpack_cache(const uint4& raw, float* f) {
+  if constexpr (sizeof(C) == 1) {
+    kv8::from_codes(raw.x, f);
+    kv8::from_codes(raw.y, f + 4);
+    kv8::from_codes(raw.z, f + 8);
+    kv8::from_codes(raw.w, f + 12);
+  } else {
+    unpack16<C>(raw, f);
+  }
+}
+// The scales of K and V at slot `off` of page and head ph of an 8-bit cache.
+__device__ __forceinline__ void slot_scales(const TreeArgs& a, int64_t ph, int off, float* k, float* v) {
+  const int64_t at = ph * (a.page_size / a.block) + off / a.block;
+  *k = kv8::power(kv8::exponent(__ldg(a.k_scales + at)));
+  *v = kv8::power(kv8::exponent(__ldg(a.v_scales + at)));
+}
+
 // NJ: 16-byte groups of four outputs a thread owns per row, ceil(hd / 64).
-template <typename T, int NJ>
+template <typename T, typename C, int NJ>
 __global__ void __launch_bounds__(kThreads) tree_attention_kernel(const TreeArgs a) {
   grid_dependency_wait();
   constexpr int MR = BM / 16;
@@ -92,35 +115,47 @@ __global__ void __launch_bounds__(kThreads) tree_attention_kernel(const TreeArgs
 #pragma unroll
     for (int j = 0; j < NJ; ++j) acc[r][j][0] = acc[r][j][1] = acc[r][j][2] = acc[r][j][3] = 0.f;
   }
-  const T* kp = static_cast<const T*>(a.k_pages);
-  const T* vp = static_cast<const T*>(a.v_pages);
+  const C* kp = static_cast<const C*>(a.k_pages);
+  const C* vp = static_cast<const C*>(a.v_pages);
   const int32_t* pages = a.page_table + static_cast<int64_t>(s.seq) * a.max_pages;
   const int nchunks = hd / 4;
+  constexpr int CV = 16 / sizeof(C);  // elements of a chunk of the cache
+  const int ccr = hd / CV;
 
   for (int t0 = start; t0 < end; t0 += kBN) {
     __syncthreads();  // the last tile has been read
-    for (int c = tid; c < kBN * cpr; c += kThreads) {
-      const int r = c / cpr, col = (c - r * cpr) * VEC;
+    for (int c = tid; c < kBN * ccr; c += kThreads) {
+      const int r = c / ccr, col = (c - r * ccr) * CV;
       const int slot = t0 + r;
-      float kf[VEC], vf[VEC];
+      float kf[CV], vf[CV];
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) kf[e] = vf[e] = 0.f;
+      for (int e = 0; e < CV; ++e) kf[e] = vf[e] = 0.f;
       bool ok = slot < end;
       if (ok) {
         const int nth = slot / a.page_size;
         const int32_t page = __ldg(pages + nth);
         ok = page >= 0 && page < a.num_pages;
         if (ok) {
-          const int64_t at = ((static_cast<int64_t>(page) * a.hkv + kvh) * a.page_size + (slot - nth * a.page_size)) * hd + col;
-          unpack16<T>(ld_stream(kp + at), kf);
-          unpack16<T>(ld_stream(vp + at), vf);
+          const int64_t ph = static_cast<int64_t>(page) * a.hkv + kvh;
+          const int64_t at = (ph * a.page_size + (slot - nth * a.page_size)) * hd + col;
+          unpack_cache<C>(ld_stream(kp + at), kf);
+          unpack_cache<C>(ld_stream(vp + at), vf);
+          if constexpr (sizeof(C) == 1) {
+            float ks, vs;
+            slot_scales(a, ph, slot - nth * a.page_size, &ks, &vs);
+#pragma unroll
+            for (int e = 0; e < CV; ++e) {
+              kf[e] *= ks;
+              vf[e] *= vs;
+            }
+          }
         } else if (col == 0) {
           raise_status(a.status, BM_DEVERR_BAD_PAGE);
         }
       }
       if (col == 0) valid[r] = ok;
 #pragma unroll
-      for (int e = 0; e < VEC; e += 4) {
+      for (int e = 0; e < CV; e += 4) {
         *reinterpret_cast<float4*>(Ks + r * ld + col + e) = make_float4(kf[e], kf[e + 1], kf[e + 2], kf[e + 3]);
         *reinterpret_cast<float4*>(Vs + r * ld + col + e) = make_float4(vf[e], vf[e + 1], vf[e + 2], vf[e + 3]);
       }
@@ -250,8 +285,8 @@ __global__ void __launch_bounds__(kThreads) tree_attention_kernel(const TreeArgs
 // share a slot: each makes a quarter of all its scores, then, these summed up, weighs a
 // quarter of the rows; and a lane owns 16-byte chunks of every row of V. Multiply-adds go
 // two to an instruction. The four warps' sums meet at the end. The tiled kernel above would
-// read its shared K and V eight times over for a few rows. J: 16-byte chunks of a row of V
-// per lane.
+// read its shared K and V eight times over for a few rows. J: chunks of a row of V per lane,
+// 16 bytes of it or four codes; the scales of 8-bit slots go to their scores and weights.
 constexpr int kRowThreads = 128;
 constexpr int kGroup = 8;   // slots of a warp's step
 constexpr int kStages = 2;  // groups of a warp in flight or in use
@@ -272,7 +307,12 @@ __device__ __forceinline__ void copy16_async(void* to, const void* from, bool re
 // A 16-byte chunk as pairs of fp32.
 template <typename T>
 __device__ __forceinline__ void unpack_pairs(const uint4& raw, uint64_t* f) {
-  if constexpr (sizeof(T) == 4) {
+  if constexpr (sizeof(T) == 1) {
+    float x[16];
+    unpack_cache<T>(raw, x);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = pair(x[2 * e], x[2 * e + 1]);
+  } else if constexpr (sizeof(T) == 4) {
     f[0] = pair(raw.x, raw.y);
     f[1] = pair(raw.z, raw.w);
   } else {
@@ -283,10 +323,13 @@ __device__ __forceinline__ void unpack_pairs(const uint4& raw, uint64_t* f) {
   }
 }
 
-template <typename T, int MR, int J>
+template <typename T, typename C, int MR, int J>
 __global__ void __launch_bounds__(kRowThreads) tree_rows_kernel(const TreeArgs a) {
   grid_dependency_wait();
   constexpr int VEC = VecWidth<T>::value;
+  constexpr bool k8 = sizeof(C) == 1;
+  constexpr int KV = 16 / sizeof(C);  // elements of a chunk of the ring
+  constexpr int VV = k8 ? 4 : KV;     // and of a lane's chunk of V
   constexpr int kWarps = kRowThreads / 32;
   const int hd = a.hd, cpr = hd / VEC;
   int64_t id = blockIdx.x;
@@ -311,26 +354,39 @@ __global__ void __launch_bounds__(kRowThreads) tree_rows_kernel(const TreeArgs a
   const int start = split * a.split_len, end = min(seen, start + a.split_len);
 
   extern __shared__ __align__(16) float smem[];
-  T* ring = reinterpret_cast<T*>(smem) + warp * kStages * 2 * kGroup * hd;
-  float* Qs = smem + ring_bytes(hd, sizeof(T)) / 4;       // [MR][hd]
+  C* ring = reinterpret_cast<C*>(smem) + warp * kStages * 2 * kGroup * hd;
+  float* Qs = smem + ring_bytes(hd, sizeof(C)) / 4;    // [MR][hd]
   float* Ps = Qs + MR * hd + warp * kGroup * MR;          // this warp's weights [kGroup][MR]
   float* ml = Qs + MR * (hd + kWarps * kGroup);           // [kWarps][MR] maxima, then sums
-  const T* kp = static_cast<const T*>(a.k_pages);
-  const T* vp = static_cast<const T*>(a.v_pages);
+  const C* kp = static_cast<const C*>(a.k_pages);
+  const C* vp = static_cast<const C*>(a.v_pages);
   const int32_t* pages = a.page_table + static_cast<int64_t>(s.seq) * a.max_pages;
+  const int ccr = hd / KV;  // chunks of the ring's rows
   const int own = lane >> 2, sub = lane & 3;  // this lane's slot of the group, its quarter of K's chunks
   // Neighbouring rows' chunks lie 64 bytes apart in the banks, by the pitch or by a swap.
-  const int swap = cpr % 8 == 0 ? 4 : 0;
+  const int swap = ccr % 8 == 0 ? 4 : 0;
 
   uint32_t sound = 0;  // bit i: this lane's slot in stage i has a sound page
+  float k_next[kStages], v_next[kStages];  // and its scales, in the order of the stages' use
+#pragma unroll
+  for (int i = 0; i < kStages; ++i) k_next[i] = v_next[i] = 1.f;
   auto fetch = [&](int g0, int stage) {
     const int slot = g0 + own;
     int64_t at = -1;  // the slot's row of the pages
+    if constexpr (k8) {
+#pragma unroll
+      for (int i = 0; i + 1 < kStages; ++i) {
+        k_next[i] = k_next[i + 1];
+        v_next[i] = v_next[i + 1];
+      }
+    }
     if (slot < end) {
       const int nth = slot / a.page_size;
       const int32_t page = __ldg(pages + nth);
       if (page >= 0 && page < a.num_pages) {
-        at = ((static_cast<int64_t>(page) * a.hkv + kvh) * a.page_size + (slot - nth * a.page_size)) * hd;
+        const int64_t ph = static_cast<int64_t>(page) * a.hkv + kvh;
+        at = (ph * a.page_size + (slot - nth * a.page_size)) * hd;
+        if constexpr (k8) slot_scales(a, ph, slot - nth * a.page_size, &k_next[kStages - 1], &v_next[kStages - 1]);
       } else if (sub == 0) {
         raise_status(a.status, BM_DEVERR_BAD_PAGE);
       }
@@ -338,12 +394,12 @@ __global__ void __launch_bounds__(kRowThreads) tree_rows_kernel(const TreeArgs a
     const bool real = at >= 0;
     sound = (sound & ~(1u << stage)) | (real ? 1u << stage : 0u);
     if (g0 < end) {
-      const T* k_from = kp + (real ? at : 0);
-      const T* v_from = vp + (real ? at : 0);
-      T* k_to = ring + (stage * 2 * kGroup + own) * hd;
-      T* v_to = k_to + kGroup * hd;
-      for (int c = sub; c < cpr; c += 4) copy16_async(k_to + (c ^ (own & 1 ? swap : 0)) * VEC, k_from + c * VEC, real);
-      for (int c = sub; c < cpr; c += 4) copy16_async(v_to + (c ^ (own & 1 ? swap : 0)) * VEC, v_from + c * VEC, real);
+      const C* k_from = kp + (real ? at : 0);
+      const C* v_from = vp + (real ? at : 0);
+      C* k_to = ring + (stage * 2 * kGroup + own) * hd;
+      C* v_to = k_to + kGroup * hd;
+      for (int c = sub; c < ccr; c += 4) copy16_async(k_to + (c ^ (own & 1 ? swap : 0)) * KV, k_from + c * KV, real);
+      for (int c = sub; c < ccr; c += 4) copy16_async(v_to + (c ^ (own & 1 ? swap : 0)) * KV, v_from + c * KV, real);
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
@@ -367,7 +423,7 @@ __global__ void __launch_bounds__(kRowThreads) tree_rows_kernel(const TreeArgs a
 
   constexpr int RL = MR / 4;        // rows that a lane weighs for its slot, from
   const int r_own = sub * RL;       // this one on
-  constexpr int P2 = J * VEC / 2;   // pairs of a row's dims that a lane owns
+  constexpr int P2 = J * VV / 2;    // pairs of a row's dims that a lane owns
   float m[RL], l[RL];
   uint64_t acc[MR][P2];
 #pragma unroll
@@ -384,20 +440,20 @@ __global__ void __launch_bounds__(kRowThreads) tree_rows_kernel(const TreeArgs a
   for (int g0 = first; g0 < end; g0 += kWarps * kGroup) {
     asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
     __syncwarp();  // all lanes' copies of this group are there
-    const T* ks = ring + (stage * 2 * kGroup + own) * hd;
-    const T* vs = ring + (stage * 2 + 1) * kGroup * hd;
+    const C* ks = ring + (stage * 2 * kGroup + own) * hd;
+    const C* vs = ring + (stage * 2 + 1) * kGroup * hd;
     uint64_t s2[MR];
 #pragma unroll
     for (int r = 0; r < MR; ++r) s2[r] = 0;
 #pragma unroll 4
-    for (int c = sub; c < cpr; c += 4) {
-      uint64_t k2[VEC / 2];
-      unpack_pairs<T>(*reinterpret_cast<const uint4*>(ks + (c ^ (own & 1 ? swap : 0)) * VEC), k2);
+    for (int c = sub; c < ccr; c += 4) {
+      uint64_t k2[KV / 2];
+      unpack_pairs<C>(*reinterpret_cast<const uint4*>(ks + (c ^ (own & 1 ? swap : 0)) * KV), k2);
 #pragma unroll
       for (int r = 0; r < MR; ++r) {
 #pragma unroll
-        for (int e = 0; e < VEC; e += 4) {
-          const ulonglong2 q4 = *reinterpret_cast<const ulonglong2*>(Qs + r * hd + c * VEC + e);
+        for (int e = 0; e < KV; e += 4) {
+          const ulonglong2 q4 = *reinterpret_cast<const ulonglong2*>(Qs + r * hd + c * KV + e);
           s2[r] = fma2(q4.x, k2[e / 2], s2[r]);
           s2[r] = fma2(q4.y, k2[e / 2 + 1], s2[r]);
         }
@@ -422,6 +478,10 @@ __global__ void __launch_bounds__(kRowThreads) tree_rows_kernel(const TreeArgs a
       }
     }
     const bool real = (sound >> stage) & 1;
+    if constexpr (k8) {
+#pragma unroll
+      for (int r = 0; r < RL; ++r) sc[r] *= k_next[0];
+    }
     const int j0 = g0 + own - s.ctx;
     float alpha[RL], p[RL];
     bool rise = false;
@@ -438,7 +498,7 @@ __global__ void __launch_bounds__(kRowThreads) tree_rows_kernel(const TreeArgs a
       p[r] = exp2f(sc[r] - base);
       m[r] = m_new;
       l[r] = l[r] * alpha[r] + p[r];  // this slot's share
-      Ps[own * MR + r_own + r] = p[r];
+      Ps[own * MR + r_own + r] = k8 ? p[r] * v_next[0] : p[r];
     }
     if (__any_sync(0xffffffffu, rise)) {
 #pragma unroll
@@ -462,13 +522,20 @@ __global__ void __launch_bounds__(kRowThreads) tree_rows_kernel(const TreeArgs a
       }
 #pragma unroll
       for (int j = 0; j < J; ++j) {
-        if (lane + 32 * j >= cpr) continue;
-        uint64_t v2[VEC / 2];
-        unpack_pairs<T>(*reinterpret_cast<const uint4*>(vs + i * hd + ((lane + 32 * j) ^ (i & 1 ? swap : 0)) * VEC), v2);
+        if ((lane + 32 * j) * VV >= hd) continue;
+        uint64_t v2[VV / 2];
+        if constexpr (k8) {  // word k of a row is in chunk k / 4
+          float x[4];
+          kv8::from_codes(*reinterpret_cast<const uint32_t*>(vs + i * hd + ((lane + 32 * j) ^ (i & 1 ? 4 * swap : 0)) * 4), x);
+          v2[0] = pair(x[0], x[1]);
+          v2[1] = pair(x[2], x[3]);
+        } else {
+          unpack_pairs<C>(*reinterpret_cast<const uint4*>(vs + i * hd + ((lane + 32 * j) ^ (i & 1 ? swap : 0)) * VV), v2);
+        }
 #pragma unroll
         for (int r = 0; r < MR; ++r) {
 #pragma unroll
-          for (int e = 0; e < VEC / 2; ++e) acc[r][j * VEC / 2 + e] = fma2(w[r], v2[e], acc[r][j * VEC / 2 + e]);
+          for (int e = 0; e < VV / 2; ++e) acc[r][j * VV / 2 + e] = fma2(w[r], v2[e], acc[r][j * VV / 2 + e]);
         }
       }
     }
@@ -492,11 +559,11 @@ __global__ void __launch_bounds__(kRowThreads) tree_rows_kernel(const TreeArgs a
   for (int r = 0; r < MR; ++r) {
 #pragma unroll
     for (int j = 0; j < J; ++j) {
-      if (lane + 32 * j < cpr) {
+      if ((lane + 32 * j) * VV < hd) {
 #pragma unroll
-        for (int e = 0; e < VEC; e += 4) {
-          *reinterpret_cast<ulonglong2*>(smem + (warp * MR + r) * hd + (lane + 32 * j) * VEC + e) =
-              make_ulonglong2(acc[r][(j * VEC + e) / 2], acc[r][(j * VEC + e) / 2 + 1]);
+        for (int e = 0; e < VV; e += 4) {
+          *reinterpret_cast<ulonglong2*>(smem + (warp * MR + r) * hd + (lane + 32 * j) * VV + e) =
+              make_ulonglong2(acc[r][(j * VV + e) / 2], acc[r][(j * VV + e) / 2 + 1]);
         }
       }
     }
@@ -601,26 +668,26 @@ void plan(int64_t batch, int hkv, int group, int max_ctx, int max_tree, int* row
   *splits = (len + *split_len - 1) / *split_len;
 }
 
-template <typename T, int NJ>
+template <typename T, typename C, int NJ>
 int launch_one(const TreeArgs& a, cudaStream_t stream, const char* what) {
   const int ld = a.hd + 4;
   const int smem = ((BM + 2 * kBN) * ld + BM * (kBN + 4) + kBN) * 4;
-  auto kernel = tree_attention_kernel<T, NJ>;
+  auto kernel = tree_attention_kernel<T, C, NJ>;
   if (int st = allow_dynamic_smem(reinterpret_cast<const void*>(kernel), smem, what)) return st;
   const int64_t grid = a.batch * a.hkv * a.row_tiles * a.splits;
   return launch_kernel(what, kernel, dim3(static_cast<unsigned>(grid)), dim3(kThreads), smem, stream, nullptr, a);
 }
 
-template <typename T>
+template <typename T, typename C>
 int launch(TreeArgs a, cudaStream_t stream, const char* what) {
   const int nj = (a.hd + 63) / 64;
   auto few = [&](auto mr) {
     constexpr int MR = decltype(mr)::value;
-    const int smem = rows_smem(a.hd, sizeof(T), MR);
+    const int smem = rows_smem(a.hd, sizeof(C), MR);
     const int64_t grid = a.batch * a.hkv * a.row_tiles * a.splits;
-    auto kernel = tree_rows_kernel<T, MR, 1>;
-    if constexpr (sizeof(T) == 4) {
-      if (a.hd > 128) kernel = tree_rows_kernel<T, MR, 2>;
+    auto kernel = tree_rows_kernel<T, C, MR, 1>;
+    if constexpr (sizeof(C) != 2) {
+      if (a.hd > 128) kernel = tree_rows_kernel<T, C, MR, 2>;
     }
     if (int st = allow_dynamic_smem(reinterpret_cast<const void*>(kernel), smem, what)) return st;
     return launch_kernel(what, kernel, dim3(static_cast<unsigned>(grid)), dim3(kRowThreads), smem, stream, nullptr, a);
@@ -628,9 +695,9 @@ int launch(TreeArgs a, cudaStream_t stream, const char* what) {
   const int rows = rows_per_tile(a.group * a.max_tree);
   const int st = rows == 4   ? few(std::integral_constant<int, 4>{})
                  : rows == 8 ? few(std::integral_constant<int, 8>{})
-                 : nj == 1   ? launch_one<T, 1>(a, stream, what)
-                 : nj == 2   ? launch_one<T, 2>(a, stream, what)
-                             : launch_one<T, 4>(a, stream, what);
+                 : nj == 1   ? launch_one<T, C, 1>(a, stream, what)
+                 : nj == 2   ? launch_one<T, C, 2>(a, stream, what)
+                             : launch_one<T, C, 4>(a, stream, what);
   if (st != BM_OK || a.splits == 1) return st;
   const int64_t warps = a.batch * a.max_tree * a.hq;
   const int64_t grid = (warps + kThreads / 32 - 1) / (kThreads / 32);
@@ -664,6 +731,90 @@ size_t simt_workspace_bytes(int64_t total_q, int64_t batch, int hq, int hkv, int
   return splits == 1 ? 0 : static_cast<size_t>(total_q) * hq * splits * (hd + 4) * sizeof(float);
 }
 
+int workspace_size(const char* what, int64_t total_q, int64_t batch, int hq, int hkv, int hd, int max_ctx, int max_tree, size_t* bytes_out) {
+  if (!bytes_out) return fail(BM_ERR_INVALID_ARGUMENT, "%s: NULL bytes_out", what);
+  *bytes_out = 0;
+  if (int st = check_sizes(what, total_q, batch, hq, hkv, hd, max_ctx, max_tree)) return st;
+  if (batch == 0 || max_tree == 0) return BM_OK;
+  *bytes_out = std::max(simt_workspace_bytes(total_q, batch, hq, hkv, hd, max_ctx, max_tree),
+                        tc_workspace_bytes(batch, hkv, hd, hq / hkv, max_ctx, max_tree));
+  return BM_OK;
+}
+
+// The rest of both entry points: `a` holds a checked cache and the call's other arguments.
+// `meets(p, bytes)`: whether memory overlaps the cache's.
+template <typename Meets>
+int attend(const char* what, TreeArgs a, float scale, size_t workspace_bytes, bm_dtype_t dtype, bool k8, Meets meets, void* stream) {
+  if (int st = check_sizes(what, a.total_q, a.batch, a.hq, a.hkv, a.hd, a.max_ctx, a.max_tree)) return st;
+  if (a.hd * dtype_size(dtype) % 16) {
+    return fail(BM_ERR_INVALID_ARGUMENT, "%s: head_dim %d is not whole 16-byte rows", what, a.hd);
+  }
+  if (a.mask && (a.words <= 0 || a.max_tree > 64 * static_cast<int64_t>(a.words))) {
+    return fail(BM_ERR_INVALID_ARGUMENT, "%s: max_tree %d does not fit %d mask words", what, a.max_tree, a.words);
+  }
+  const float s = scale > 0.f ? scale : 1.f / std::sqrt(static_cast<float>(a.hd));
+  a.qscale = s * 1.4426950408889634f;  // the softmax runs in base 2
+  if (scale != scale || !std::isfinite(a.qscale)) return fail(BM_ERR_INVALID_ARGUMENT, "%s: scale is not finite", what);
+  if (a.batch == 0 || a.total_q == 0 || a.max_tree == 0) return BM_OK;
+  if (!a.out || !a.q || !a.ctx_lens || !a.q_starts) return fail(BM_ERR_INVALID_ARGUMENT, "%s: NULL pointer", what);
+  if (!aligned16(a.out) || !aligned16(a.q) || !aligned16(a.k_pages) || !aligned16(a.v_pages) || !aligned16(a.ws)) {
+    return fail(BM_ERR_INVALID_ARGUMENT, "%s: q, out, pages and workspace must be 16-byte aligned", what);
+  }
+  if (!aligned_to({a.seq_ids, a.ctx_lens, a.q_starts, a.page_table, a.status}, 4) || !aligned_to(a.mask, 8)) {
+    return fail(BM_ERR_INVALID_ARGUMENT, "%s: a pointer is not aligned to its elements", what);
+  }
+  if (!a.seq_ids && a.batch > a.num_seqs) return fail(BM_ERR_INVALID_ARGUMENT, "%s: more sequences than the cache holds", what);
+  const uintptr_t o = reinterpret_cast<uintptr_t>(a.out), i = reinterpret_cast<uintptr_t>(a.q);
+  const uintptr_t bytes = static_cast<uintptr_t>(a.total_q) * a.hq * a.hd * dtype_size(dtype);
+  if (o < i + bytes && i < o + bytes) return fail(BM_ERR_INVALID_ARGUMENT, "%s: out overlaps q", what);
+  if (meets(a.out, bytes)) return fail(BM_ERR_INVALID_ARGUMENT, "%s: out overlaps the cache's pages", what);
+  a.group = a.hq / a.hkv;
+  size_t need = 0;
+  if (int st = workspace_size(what, a.total_q, a.batch, a.hq, a.hkv, a.hd, a.max_ctx, a.max_tree, &need)) return st;
+  if (need > 0 && (!a.ws || workspace_bytes < need)) {
+    return fail(BM_ERR_INVALID_ARGUMENT, "%s: workspace of %zu bytes is smaller than %zu", what, workspace_bytes, need);
+  }
+  const cudaStream_t st = as_stream(stream);
+  if (!k8 && tc_takes(a, dtype)) return launch_tc(a, st, what);
+  plan(a.batch, a.hkv, a.group, a.max_ctx, a.max_tree, &a.row_tiles, &a.splits, &a.split_len);
+  if (k8) return dtype == BM_F32 ? launch<float, Code>(a, st, what) : launch<bf16, Code>(a, st, what);
+  return dtype == BM_F32 ? launch<float, float>(a, st, what) : launch<bf16, bf16>(a, st, what);
+}
+
+// The arguments that both entry points take; the cache is the caller's to fill in.
+TreeArgs tree_args(void* out, const void* q, const int32_t* seq_ids, const int32_t* ctx_lens, const int32_t* q_starts,
+                   const uint64_t* tree_mask, int32_t mask_words, int64_t total_q, int64_t batch, int32_t num_q_heads,
+                   int32_t max_ctx, int32_t max_tree, void* workspace, int32_t* d_status) {
+  TreeArgs a{};
+  a.out = out;
+  a.q = q;
+  a.seq_ids = seq_ids;
+  a.ctx_lens = ctx_lens;
+  a.q_starts = q_starts;
+  a.mask = tree_mask;
+  a.words = mask_words;
+  a.ws = static_cast<float*>(workspace);
+  a.total_q = total_q;
+  a.batch = batch;
+  a.hq = num_q_heads;
+  a.max_ctx = max_ctx;
+  a.max_tree = max_tree;
+  a.status = d_status;
+  return a;
+}
+template <typename Cache>
+void set_cache(TreeArgs* a, const Cache& c) {
+  a->k_pages = c.k_pages;
+  a->v_pages = c.v_pages;
+  a->page_table = c.page_table;
+  a->hkv = c.num_kv_heads;
+  a->hd = c.head_dim;
+  a->num_pages = c.num_pages;
+  a->page_size = c.page_size;
+  a->max_pages = c.max_pages;
+  a->num_seqs = c.num_seqs;
+}
+
 }  // namespace
 }  // namespace paged
 
@@ -695,16 +846,8 @@ bool meets_pages(const bm_paged_kv_t& c, const void* p, uintptr_t bytes, int es)
 extern "C" int bm_paged_tree_attention_workspace_size(int64_t total_q, int64_t batch, int32_t num_q_heads,
                                                       int32_t num_kv_heads, int32_t head_dim, int32_t max_ctx,
                                                       int32_t max_tree, size_t* bytes_out) {
-  using namespace bm;
-  const char* what = "bm_paged_tree_attention_workspace_size";
-  if (!bytes_out) return fail(BM_ERR_INVALID_ARGUMENT, "%s: NULL bytes_out", what);
-  *bytes_out = 0;
-  if (int st = paged::check_sizes(what, total_q, batch, num_q_heads, num_kv_heads, head_dim, max_ctx, max_tree)) return st;
-  if (batch == 0 || max_tree == 0) return BM_OK;
-  *bytes_out = std::max(paged::simt_workspace_bytes(total_q, batch, num_q_heads, num_kv_heads, head_dim, max_ctx, max_tree),
-                        paged::tc_workspace_bytes(batch, num_kv_heads, head_dim, num_q_heads / num_kv_heads,
-                                                  max_ctx, max_tree));
-  return BM_OK;
+  return bm::paged::workspace_size("bm_paged_tree_attention_workspace_size", total_q, batch, num_q_heads, num_kv_heads, head_dim,
+                                   max_ctx, max_tree, bytes_out);
 }
 
 extern "C" int bm_paged_tree_attention(void* out, const void* q, const bm_paged_kv_t* cache, const int32_t* seq_ids,
@@ -716,64 +859,35 @@ extern "C" int bm_paged_tree_attention(void* out, const void* q, const bm_paged_
   const char* what = "bm_paged_tree_attention";
   if (!valid_dtype(dtype)) return fail(BM_ERR_INVALID_ARGUMENT, "%s: bad dtype %d", what, static_cast<int>(dtype));
   if (int st = check_paged_kv(what, cache)) return st;
-  const bm_paged_kv_t& c = *cache;
-  if (int st = paged::check_sizes(what, total_q, batch, num_q_heads, c.num_kv_heads, c.head_dim, max_ctx, max_tree)) return st;
-  if (c.head_dim * dtype_size(dtype) % 16) {
-    return fail(BM_ERR_INVALID_ARGUMENT, "%s: head_dim %d is not whole 16-byte rows", what, c.head_dim);
-  }
-  if (tree_mask && (mask_words <= 0 || max_tree > 64 * static_cast<int64_t>(mask_words))) {
-    return fail(BM_ERR_INVALID_ARGUMENT, "%s: max_tree %d does not fit %d mask words", what, max_tree, mask_words);
-  }
-  const float s = scale > 0.f ? scale : 1.f / std::sqrt(static_cast<float>(c.head_dim));
-  const float qscale = s * 1.4426950408889634f;  // the softmax runs in base 2
-  if (scale != scale || !std::isfinite(qscale)) return fail(BM_ERR_INVALID_ARGUMENT, "%s: scale is not finite", what);
-  if (batch == 0 || total_q == 0 || max_tree == 0) return BM_OK;
-  if (!out || !q || !ctx_lens || !q_starts) return fail(BM_ERR_INVALID_ARGUMENT, "%s: NULL pointer", what);
-  if (!aligned16(out) || !aligned16(q) || !aligned16(c.k_pages) || !aligned16(c.v_pages) || !aligned16(workspace)) {
-    return fail(BM_ERR_INVALID_ARGUMENT, "%s: q, out, pages and workspace must be 16-byte aligned", what);
-  }
-  if (!aligned_to({seq_ids, ctx_lens, q_starts, c.page_table, d_status}, 4) || !aligned_to(tree_mask, 8)) {
-    return fail(BM_ERR_INVALID_ARGUMENT, "%s: a pointer is not aligned to its elements", what);
-  }
-  if (!seq_ids && batch > c.num_seqs) return fail(BM_ERR_INVALID_ARGUMENT, "%s: more sequences than the cache holds", what);
-  const uintptr_t o = reinterpret_cast<uintptr_t>(out), i = reinterpret_cast<uintptr_t>(q);
-  const uintptr_t bytes = static_cast<uintptr_t>(total_q) * num_q_heads * c.head_dim * dtype_size(dtype);
-  if (o < i + bytes && i < o + bytes) return fail(BM_ERR_INVALID_ARGUMENT, "%s: out overlaps q", what);
-  if (meets_pages(c, out, bytes, dtype_size(dtype))) return fail(BM_ERR_INVALID_ARGUMENT, "%s: out overlaps the cache's pages", what);
-  const size_t simt = paged::simt_workspace_bytes(total_q, batch, num_q_heads, c.num_kv_heads, c.head_dim, max_ctx, max_tree);
-  const size_t tc = paged::tc_workspace_bytes(batch, c.num_kv_heads, c.head_dim, num_q_heads / c.num_kv_heads, max_ctx,
-                                              max_tree);
-  if (std::max(simt, tc) > 0 && (!workspace || workspace_bytes < std::max(simt, tc))) {
-    return fail(BM_ERR_INVALID_ARGUMENT, "%s: workspace of %zu bytes is smaller than %zu", what, workspace_bytes,
-                std::max(simt, tc));
-  }
-  paged::TreeArgs a{};
-  a.out = out;
-  a.q = q;
-  a.k_pages = c.k_pages;
-  a.v_pages = c.v_pages;
-  a.page_table = c.page_table;
-  a.seq_ids = seq_ids;
-  a.ctx_lens = ctx_lens;
-  a.q_starts = q_starts;
-  a.mask = tree_mask;
-  a.words = mask_words;
-  a.ws = static_cast<float*>(workspace);
-  a.total_q = total_q;
-  a.batch = batch;
-  a.hq = num_q_heads;
-  a.hkv = c.num_kv_heads;
-  a.hd = c.head_dim;
-  a.group = num_q_heads / c.num_kv_heads;
-  a.num_pages = c.num_pages;
-  a.page_size = c.page_size;
-  a.max_pages = c.max_pages;
-  a.num_seqs = c.num_seqs;
-  a.max_ctx = max_ctx;
-  a.max_tree = max_tree;
-  a.qscale = qscale;
-  a.status = d_status;
-  if (paged::tc_takes(a, dtype)) return paged::launch_tc(a, as_stream(stream), what);
-  paged::plan(batch, a.hkv, a.group, max_ctx, max_tree, &a.row_tiles, &a.splits, &a.split_len);
-  return dtype == BM_F32 ? paged::launch<float>(a, as_stream(stream), what) : paged::launch<bf16>(a, as_stream(stream), what);
+  paged::TreeArgs a = paged::tree_args(out, q, seq_ids, ctx_lens, q_starts, tree_mask, mask_words, total_q, batch, num_q_heads,
+                                       max_ctx, max_tree, workspace, d_status);
+  paged::set_cache(&a, *cache);
+  return paged::attend(what, a, scale, workspace_bytes, dtype, false,
+                       [&](const void* p, uintptr_t n) { return meets_pages(*cache, p, n, dtype_size(dtype)); }, stream);
+}
+
+extern "C" int bm_paged_kv8_tree_attention_workspace_size(int64_t total_q, int64_t batch, int32_t num_q_heads,
+                                                          int32_t num_kv_heads, int32_t head_dim, int32_t max_ctx,
+                                                          int32_t max_tree, size_t* bytes_out) {
+  return bm::paged::workspace_size("bm_paged_kv8_tree_attention_workspace_size", total_q, batch, num_q_heads, num_kv_heads,
+                                   head_dim, max_ctx, max_tree, bytes_out);
+}
+
+extern "C" int bm_paged_kv8_tree_attention(void* out, const void* q, const bm_paged_kv8_t* cache, const int32_t* seq_ids,
+                                           const int32_t* ctx_lens, const int32_t* q_starts, const uint64_t* tree_mask,
+                                           int32_t mask_words, int64_t total_q, int64_t batch, int32_t num_q_heads,
+                                           int32_t max_ctx, int32_t max_tree, float scale, void* workspace,
+                                           size_t workspace_bytes, bm_dtype_t dtype, int32_t* d_status, void* stream) {
+  using namespace bm;
+  const char* what = "bm_paged_kv8_tree_attention";
+  if (!valid_dtype(dtype)) return fail(BM_ERR_INVALID_ARGUMENT, "%s: bad dtype %d", what, static_cast<int>(dtype));
+  if (int st = check_paged_kv8(what, cache)) return st;
+  paged::TreeArgs a = paged::tree_args(out, q, seq_ids, ctx_lens, q_starts, tree_mask, mask_words, total_q, batch, num_q_heads,
+                                       max_ctx, max_tree, workspace, d_status);
+  paged::set_cache(&a, *cache);
+  a.k_scales = static_cast<const uint8_t*>(cache->k_scales);
+  a.v_scales = static_cast<const uint8_t*>(cache->v_scales);
+  a.block = cache->block;
+  return paged::attend(what, a, scale, workspace_bytes, dtype, true,
+                       [&](const void* p, uintptr_t n) { return meets_pages8(*cache, p, n); }, stream);
 }

@@ -13,6 +13,9 @@ struct TreeArgs {
   const void* q;
   const void* k_pages;        // [num_pages][hkv][page_size][hd]
   const void* v_pages;
+  const uint8_t* k_scales;    // an 8-bit cache's: [num_pages][hkv][page_size / block]
+  const uint8_t* v_scales;
+  int block;
   const int32_t* page_table;  // [num_seqs][max_pages]
   const int32_t* seq_ids;     // NULL: b
   const int32_t* ctx_lens;

@@ -25,9 +25,12 @@
 
 #include "bm_common.cuh"
 #include "bm_host.h"
+#include "rotary_device.cuh"
 
 namespace bm {
 namespace {
+
+using namespace bm::rot;
 
 constexpr int kMaxHeadDim = 1024;
 constexpr int kThreads = 128;  // 256: 1 to 3 % slower on prompts
@@ -54,60 +57,6 @@ struct RotaryArgs {
   int units, rest;          // rotated and copied units of a head
   int32_t* status;
 };
-
-// N consecutive elements of T held between load and store.
-template <typename T>
-struct Piece16 {
-  uint4 raw;
-  __device__ __forceinline__ void load(const T* p) { raw = ld_stream(p); }
-  __device__ __forceinline__ void store(T* p) const { st_plain(p, raw); }
-  __device__ __forceinline__ void get(float* f) const { unpack16<T>(raw, f); }
-  __device__ __forceinline__ void set(const float* f) { raw = pack16<T>(f); }
-};
-template <typename T, int N>
-struct Piece;
-template <>
-struct Piece<float, 4> : Piece16<float> {};
-template <>
-struct Piece<bf16, 8> : Piece16<bf16> {};
-template <>
-struct Piece<bf16, 4> {
-  uint2 raw;
-  __device__ __forceinline__ void load(const bf16* p) { raw = __ldcs(reinterpret_cast<const uint2*>(p)); }
-  __device__ __forceinline__ void store(bf16* p) const { *reinterpret_cast<uint2*>(p) = raw; }
-  __device__ __forceinline__ void get(float* f) const {
-    f[0] = bf16_lo(raw.x);
-    f[1] = bf16_hi(raw.x);
-    f[2] = bf16_lo(raw.y);
-    f[3] = bf16_hi(raw.y);
-  }
-  __device__ __forceinline__ void set(const float* f) {
-    raw.x = pack_bf16x2(f[0], f[1]);
-    raw.y = pack_bf16x2(f[2], f[3]);
-  }
-};
-template <typename T>
-struct Piece<T, 1> {
-  T raw;
-  __device__ __forceinline__ void load(const T* p) { raw = *p; }
-  __device__ __forceinline__ void store(T* p) const { *p = raw; }
-  __device__ __forceinline__ void get(float* f) const { f[0] = load1<T>(&raw); }
-  __device__ __forceinline__ void set(const float* f) { store1<T>(&raw, f[0]); }
-};
-
-template <typename T, int N, bool INTER>
-__device__ __forceinline__ void rotate(Piece<T, N>& p1, Piece<T, N>& p2, const float2* cs) {
-  float x[2 * N];
-  p1.get(x);
-  p2.get(x + N);
-#pragma unroll
-  for (int e = 0; e < N; ++e) {
-    const int a = INTER ? 2 * e : e, b = INTER ? 2 * e + 1 : N + e;
-    rope_rotate(x[a], x[b], cs[e], &x[a], &x[b]);
-  }
-  p1.set(x);
-  p2.set(x + N);
-}
 
 // PAGED: k goes into the cache's pages and v with it; otherwise k into k_out.
 template <typename T, int N, bool INTER, bool PAGED>
@@ -200,17 +149,7 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(RotaryArgs a) {
         }
         if (turns && !have) {
           const float2* t = a.table + static_cast<int64_t>(pos) * (a.rd / 2) + c * N;
-          if constexpr (N % 2 == 0) {  // 16-byte loads: the host checked the table's alignment
-#pragma unroll
-            for (int e = 0; e < N; e += 2) {
-              const float4 two = __ldg(reinterpret_cast<const float4*>(t + e));
-              cs[e] = make_float2(two.x, two.y);
-              cs[e + 1] = make_float2(two.z, two.w);
-            }
-          } else {
-#pragma unroll
-            for (int e = 0; e < N; ++e) cs[e] = __ldg(t + e);
-          }
+          load_angles<N>(t, cs);
           have = true;
         }
 #pragma unroll
@@ -261,37 +200,6 @@ int launch(RotaryArgs a, bool interleaved, bm_dtype_t dtype, cudaStream_t stream
   if (n == 8) return interleaved ? go(rotary_kernel<bf16, 8, true, PAGED>) : go(rotary_kernel<bf16, 8, false, PAGED>);
   if (n == 4) return interleaved ? go(rotary_kernel<bf16, 4, true, PAGED>) : go(rotary_kernel<bf16, 4, false, PAGED>);
   return interleaved ? go(rotary_kernel<bf16, 1, true, PAGED>) : go(rotary_kernel<bf16, 1, false, PAGED>);
-}
-
-// Rows of `n` elements, `stride` apart.
-struct Rows {
-  const void* p;
-  int64_t stride, n;
-};
-
-// Whether two runs of rows share memory. Slices of one buffer's rows (q, k and v of a
-// fused projection) interleave without meeting.
-bool meet(const Rows& a, const Rows& b, int64_t rows, int es) {
-  if (a.p == nullptr || b.p == nullptr || a.n == 0 || b.n == 0) return false;
-  const uintptr_t pa = reinterpret_cast<uintptr_t>(a.p), pb = reinterpret_cast<uintptr_t>(b.p);
-  if (pa + static_cast<uintptr_t>((rows - 1) * a.stride + a.n) * es <= pb) return false;
-  if (pb + static_cast<uintptr_t>((rows - 1) * b.stride + b.n) * es <= pa) return false;
-  if (rows > 1 && a.stride == b.stride) {
-    const int64_t pitch = a.stride * es;
-    const int64_t d = ((static_cast<int64_t>(pa - pb) % pitch) + pitch) % pitch;  // a's offset behind b in a row
-    return !(d >= b.n * es && d + a.n * es <= pitch);
-  }
-  return true;
-}
-bool same(const Rows& a, const Rows& b, int64_t rows) { return a.p == b.p && (rows == 1 || a.stride == b.stride); }
-
-int check_rotation(const char* what, const void* table, int32_t table_len, int rd, int hd) {
-  if (table_len <= 0) return fail(BM_ERR_INVALID_ARGUMENT, "%s: table_len must be > 0", what);
-  if (reinterpret_cast<uintptr_t>(table) & 7u) return fail(BM_ERR_INVALID_ARGUMENT, "%s: table not 8-byte aligned", what);
-  if (rd <= 0 || rd % 2 || rd > hd) {
-    return fail(BM_ERR_INVALID_ARGUMENT, "%s: rotary_dim %d must be even, positive and at most head_dim %d", what, rd, hd);
-  }
-  return BM_OK;
 }
 
 struct Frequencies {

@@ -573,6 +573,147 @@ def paged_tree_attention(q: torch.Tensor, cache: PagedKV, ctx_lens: torch.Tensor
                                                    max_ctx, max_tree, tree_mask, seq_ids, scale, out, workspace, _word(status), _handle(stream))
 
 
+def qk_norm_rotary(q: Optional[torch.Tensor], k: Optional[torch.Tensor], q_weight: Optional[torch.Tensor],
+                   k_weight: Optional[torch.Tensor], positions, table: RopeTable, eps: float = 1e-5,
+                   interleaved: bool = False, q_out: Optional[torch.Tensor] = None, k_out: Optional[torch.Tensor] = None,
+                   status: Optional[DeviceStatus] = None, stream=None):
+    """rotary of heads that are normed first: every head x of q and k becomes x * rsqrt(mean(x^2) +
+    eps) * its weight [head_dim] and is rotated, in one pass, with one rounding. Everything else as
+    rotary has it; either of q and k may be None, with its weight. head_dim <= 256."""
+    if table is None:
+        raise _invalid("qk_norm_rotary needs a table")
+    if positions is None:
+        raise _invalid("qk_norm_rotary needs positions")
+    if stream is not None:
+        q_out = _like(q, stream) if q is not None and q_out is None else q_out
+        k_out = _like(k, stream) if k is not None and k_out is None else k_out
+    pos, pos0 = (None, positions) if isinstance(positions, int) else (positions, 0)
+    return _lib.serving_ops().qk_norm_rotary(q, k, q_weight, k_weight, eps, pos, pos0, table.data, table.max_pos, table.head_dim,
+                                             interleaved, q_out, k_out, _word(status), _handle(stream))
+
+
+class PagedKV8:
+    """A paged KV cache in 8 bits over the caller's tensors: k_pages and v_pages float8_e4m3fn
+    [num_pages, Hkv, page_size, hd], k_scales and v_scales float8_e8m0fnu [num_pages, Hkv,
+    page_size // block] (powers of two: the value of a slot's elements is code times the scale
+    of its block of slots) and page_table int32 [num_seqs, max_pages], all contiguous on one
+    device; hd a multiple of 16 up to 256. Like a PagedKV's, its tensors are read by each call."""
+
+    def __init__(self, k_pages: torch.Tensor, v_pages: torch.Tensor, k_scales: torch.Tensor, v_scales: torch.Tensor,
+                 page_table: torch.Tensor):
+        if k_pages.dim() != 4 or k_pages.shape != v_pages.shape:
+            raise _invalid("k_pages and v_pages must be [num_pages, kv_heads, page_size, head_dim]")
+        if k_pages.dtype != torch.float8_e4m3fn or v_pages.dtype != torch.float8_e4m3fn:
+            raise _invalid("k_pages and v_pages must be float8_e4m3fn")
+        if k_pages.shape[3] % 16 or not 16 <= k_pages.shape[3] <= 256:
+            raise _invalid("head_dim of an 8-bit cache must be a multiple of 16 up to 256")
+        if (k_scales.dim() != 3 or k_scales.shape != v_scales.shape or k_scales.shape[:2] != k_pages.shape[:2]
+                or k_scales.shape[2] == 0 or k_pages.shape[2] % k_scales.shape[2]):
+            raise _invalid("k_scales and v_scales must be [num_pages, kv_heads, page_size / block]")
+        if k_scales.dtype != torch.float8_e8m0fnu or v_scales.dtype != torch.float8_e8m0fnu:
+            raise _invalid("k_scales and v_scales must be float8_e8m0fnu")
+        for t, n in ((k_pages, "k_pages"), (v_pages, "v_pages"), (k_scales, "k_scales"), (v_scales, "v_scales")):
+            _dense(t, n)
+            if t.device != _dev(k_pages):
+                raise _invalid("tensors must share device")
+        if page_table.dim() != 2:
+            raise _invalid("page_table must be [num_seqs, max_pages]")
+        if page_table.dtype != torch.int32 or not page_table.is_contiguous() or page_table.device != _dev(k_pages):
+            raise _invalid("page_table must be a contiguous int32 tensor on the pages' device")
+        self.k_pages, self.v_pages, self.k_scales, self.v_scales = k_pages, v_pages, k_scales, v_scales
+        self.page_table = page_table
+
+    num_pages = property(lambda self: self.k_pages.shape[0])
+    num_kv_heads = property(lambda self: self.k_pages.shape[1])
+    page_size = property(lambda self: self.k_pages.shape[2])
+    block = property(lambda self: self.k_pages.shape[2] // self.k_scales.shape[2])
+    head_dim = property(lambda self: self.k_pages.shape[3])
+    num_seqs = property(lambda self: self.page_table.shape[0])
+    max_pages = property(lambda self: self.page_table.shape[1])
+    device = property(lambda self: self.k_pages.device)
+
+
+def paged_kv8_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, cache: PagedKV8, ctx_lens: torch.Tensor,
+                     q_starts: torch.Tensor, max_tokens: int, positions: Optional[torch.Tensor] = None,
+                     table: Optional[RopeTable] = None, q_weight: Optional[torch.Tensor] = None,
+                     k_weight: Optional[torch.Tensor] = None, eps: float = 1e-5, seq_ids: Optional[torch.Tensor] = None,
+                     interleaved: bool = False, q_out: Optional[torch.Tensor] = None,
+                     status: Optional[DeviceStatus] = None, stream=None) -> Optional[torch.Tensor]:
+    """Appends sequence b's rows q_starts[b]:q_starts[b + 1] of k and v [rows, Hkv, hd] (at most
+    max_tokens) to its slots from ctx_lens[b] on, quantised, and returns q [rows, Hq, hd]
+    (``q_out``, made when not given; ``q_out=q`` in place; None without q): q and k normed with
+    q_weight and k_weight [hd] (None: not) and rotated by ``table`` (None: not) at ``positions``
+    (None: their slots). A block's scale is the power of two that its largest value needs; it
+    grows, and earlier codes of the block with it, where new rows are larger, and is set afresh
+    where a call writes the block's first slot. ctx_lens, q_starts and seq_ids are
+    paged_kv8_tree_attention's. Rows of ``q_out`` outside every sequence are left as they were.
+    A call must not name a sequence twice."""
+    if stream is not None and q is not None and q_out is None:
+        q_out = _like(q, stream)
+    if table is None:
+        tdata, max_pos, rotary_dim = None, 0, 0
+    else:
+        tdata, max_pos, rotary_dim = table.data, table.max_pos, table.head_dim
+    return _lib.serving_ops().paged_kv8_append(q, k, v, cache.k_pages, cache.v_pages, cache.k_scales, cache.v_scales, cache.page_table,
+                                               ctx_lens, q_starts, max_tokens, positions, tdata, max_pos, rotary_dim, q_weight,
+                                               k_weight, eps, seq_ids, interleaved, q_out, _word(status), _handle(stream))
+
+
+def paged_kv8_read(cache: PagedKV8, first: torch.Tensor, starts: torch.Tensor, rows: int, max_rows: int,
+                   dtype: torch.dtype = torch.bfloat16, seq_ids: Optional[torch.Tensor] = None,
+                   k_out: Optional[torch.Tensor] = None, v_out: Optional[torch.Tensor] = None,
+                   status: Optional[DeviceStatus] = None, stream=None):
+    """Cached slots as dense values: rows starts[b]:starts[b + 1] (at most max_rows) of k and v
+    [rows, Hkv, hd] are sequence b's slots from first[b] on; exact in bf16 and fp32. Returns
+    (k_out, v_out), made when not given, of ``dtype``; rows outside every sequence are left as
+    they were."""
+    shape = (rows, cache.num_kv_heads, cache.head_dim)
+    if rows < 0:
+        raise _invalid("rows must be >= 0")
+    for out in (k_out, v_out):
+        if out is not None and out.shape != shape:
+            raise _invalid("k_out and v_out must be [rows, kv_heads, head_dim]")
+    given = k_out if k_out is not None else v_out
+    if given is not None:
+        dtype = given.dtype
+    if k_out is None:
+        k_out = _empty(shape, dtype, cache.device, stream)
+    if v_out is None:
+        v_out = _empty(shape, dtype, cache.device, stream)
+    return _lib.serving_ops().paged_kv8_read(cache.k_pages, cache.v_pages, cache.k_scales, cache.v_scales, cache.page_table, first,
+                                             starts, max_rows, seq_ids, k_out, v_out, _word(status), _handle(stream))
+
+
+def paged_kv8_tree_attention_workspace(q: torch.Tensor, cache: PagedKV8, batch: int, max_ctx: int, max_tree: int,
+                                       stream=None) -> torch.Tensor:
+    """Device scratch for paged_kv8_tree_attention calls of these sizes (q's rows, batch and
+    bounds). Calls that overlap on the GPU need one each."""
+    if q.dim() != 3:
+        raise _invalid("q must be [rows, heads, head_dim]")
+    _dev(q)
+    n = ctypes.c_size_t()
+    with torch.cuda.device(cache.device):
+        check(load().bm_paged_kv8_tree_attention_workspace_size(q.shape[0], batch, q.shape[1], cache.num_kv_heads,
+                                                                cache.head_dim, max_ctx, max_tree, ctypes.byref(n)))
+    return _empty((n.value,), torch.uint8, cache.device, stream)
+
+
+def paged_kv8_tree_attention(q: torch.Tensor, cache: PagedKV8, ctx_lens: torch.Tensor, q_starts: torch.Tensor,
+                             max_ctx: int, max_tree: int, tree_mask: Optional[torch.Tensor] = None,
+                             seq_ids: Optional[torch.Tensor] = None, scale: float = 0.0,
+                             out: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None,
+                             status: Optional[DeviceStatus] = None, stream=None) -> torch.Tensor:
+    """paged_tree_attention over an 8-bit cache: the same arguments and rules, with q and out of
+    bf16 or fp32. ``workspace``: paged_kv8_tree_attention_workspace's, made for the call when None."""
+    if workspace is None:
+        workspace = paged_kv8_tree_attention_workspace(q, cache, ctx_lens.numel(), max_ctx, max_tree, stream)
+    if stream is not None and out is None:
+        out = _like(q, stream)
+    return _lib.serving_ops().paged_kv8_tree_attention(q, cache.k_pages, cache.v_pages, cache.k_scales, cache.v_scales,
+                                                       cache.page_table, ctx_lens, q_starts, max_ctx, max_tree, tree_mask, seq_ids,
+                                                       scale, out, workspace, _word(status), _handle(stream))
+
+
 def sample(logits: torch.Tensor, uniforms: torch.Tensor, temperature: Optional[torch.Tensor] = None,
            top_k: Optional[torch.Tensor] = None, top_p: Optional[torch.Tensor] = None,
            min_p: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,

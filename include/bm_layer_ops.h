@@ -530,6 +530,86 @@ int bm_paged_tree_attention(void* out, const void* q, const bm_paged_kv_t* cache
                             int32_t* d_status, void* stream);
 
 /* ---------------------------------------------------------------------------
+ * RMSNorm of every head of Q and K, then rotary positions, in one pass. No counterpart in
+ * the reference, whose heads are rotated as they are (src/kernels.cu:126-140). For each head
+ * x of q and k, with w its norm's weight [head_dim] (of the storage type):
+ *   y = x * rsqrt(mean(x^2) + eps) * w, then bm_rotary's rotation of y,
+ * in fp32 throughout, rounded once. Every argument that bm_rotary has means what it means
+ * there (strides, positions, outputs that may be their inputs, bad positions);
+ * head_dim <= 256. A head of zeros stays one (with eps 0: NaN). */
+int bm_qk_norm_rotary(void* q_out, void* k_out, const void* q, const void* k, const void* q_weight, const void* k_weight,
+                      float eps, const int32_t* positions, int32_t pos0, const void* table, int32_t table_len,
+                      int32_t rotary_dim, int32_t interleaved, int64_t rows, int32_t num_q_heads, int32_t num_kv_heads,
+                      int32_t head_dim, int64_t q_stride, int64_t k_stride, int64_t q_out_stride, int64_t k_out_stride,
+                      bm_dtype_t dtype, int32_t* d_status, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Paged KV cache held in 8 bits. bm_paged_kv_t with pages of e4m3 codes (sign, four bits of
+ * exponent, three of mantissa; largest 448) and a scale for each block of `block`
+ * neighbouring slots of a page (block divides page_size) and head:
+ *   K[t] = k_pages[p][h][o][:] * k_scales[p][h][o / block],  p = page_table[s][t / page_size],
+ *   o = t % page_size;  V alike.
+ * A scale is a power of two in one byte, 2^(byte - 127) (e8m0), from 2^-40 to 2^40; a byte
+ * outside these counts as the nearest. k_scales and v_scales are
+ * [num_pages][num_kv_heads][page_size / block]. head_dim is a multiple of 16 up to 256. */
+typedef struct bm_paged_kv8 {
+  void* k_pages;
+  void* v_pages;
+  void* k_scales;
+  void* v_scales;
+  const int32_t* page_table;
+  int32_t num_pages, page_size, block, max_pages, num_seqs, num_kv_heads, head_dim;
+} bm_paged_kv8_t;
+
+/* Norm, RoPE and K/V store into an 8-bit paged cache. Sequence b (cache sequence seq_ids[b],
+ * b when NULL) appends the rows [q_starts[b], q_starts[b+1]) of k and v, n_b of them, as its
+ * slots ctx_lens[b] + i: the arguments of bm_paged_kv8_tree_attention, which reads them.
+ *   q_out[r] = q[r], K = k[r]: each head normed (q_weight, k_weight; NULL: not) and rotated
+ *   (table; NULL: not) as bm_qk_norm_rotary does, at positions[r] (NULL: the row's slot);
+ *   V = v[r] as it is.
+ * K and V are quantised from fp32, one rounding to the nearest (even) code. The scale of a
+ * block is 2^E, E = ceil(log2(a / 448)) with a its largest new magnitude, at least 2^-40 and at
+ * most 2^40 (larger values end at 448 * 2^40). A block that has slots before ctx_lens[b] keeps
+ * its scale where that is larger; else its earlier codes are moved to the new scale (exactly,
+ * unless they fall below 2^-6). Slots behind the new ones keep their codes, which mean nothing under another
+ * scale. A value that is not finite becomes NaN and sets no scale.
+ * q, k, v and q_out rows are *_stride elements apart; num_q_heads may be 0 (q, q_out NULL);
+ * q_out may be q and must not overlap anything else. max_tokens is a host-side upper bound of
+ * n_b. Rows outside [q_starts[0], q_starts[batch]) are neither read nor written. A call names
+ * no block twice: with one sequence in it twice, or one page under two of its sequences,
+ * where both append, the codes and scale of the blocks they share are either one's, or mixed.
+ * A sequence with n_b outside [0, max_tokens], slots outside its max_pages pages or rows
+ * outside [0, rows) flags BM_DEVERR_BAD_POSITION, a bad sequence id BM_DEVERR_BAD_SEQUENCE: it
+ * is skipped. A bad page id flags BM_DEVERR_BAD_PAGE: K and V of its slots are skipped. A
+ * position outside the table flags BM_DEVERR_BAD_POSITION: its row is skipped. */
+int bm_paged_kv8_append(void* q_out, const void* q, const void* k, const void* v, const void* q_weight,
+                        const void* k_weight, float eps, const int32_t* positions, const bm_paged_kv8_t* cache,
+                        const int32_t* seq_ids, const int32_t* ctx_lens, const int32_t* q_starts, const void* table,
+                        int32_t table_len, int32_t rotary_dim, int32_t interleaved, int64_t rows, int64_t batch,
+                        int32_t num_q_heads, int32_t max_tokens, int64_t q_stride, int64_t k_stride, int64_t v_stride,
+                        int64_t q_out_stride, bm_dtype_t dtype, int32_t* d_status, void* stream);
+
+/* Reads cached slots back: rows [starts[b], starts[b+1]) of k_out and v_out
+ * [rows][num_kv_heads][head_dim] (dense, 16-byte aligned) get slots first[b] + i of sequence b
+ * (seq_ids[b], b when NULL) as values of dtype: exact in fp32 and in bf16. max_rows bounds a
+ * sequence's rows; other rows of the outputs are left as they were. Bad sequences are
+ * skipped as bm_paged_kv8_append does, and rows whose page id is bad. */
+int bm_paged_kv8_read(void* k_out, void* v_out, const bm_paged_kv8_t* cache, const int32_t* seq_ids,
+                      const int32_t* first, const int32_t* starts, int64_t rows, int64_t batch, int32_t max_rows,
+                      bm_dtype_t dtype, int32_t* d_status, void* stream);
+
+/* bm_paged_tree_attention over an 8-bit paged cache: every argument and every rule as there, with
+ * q and out of dtype, K and V the values that the cache stands for. Those of the ctx + n slots
+ * must be finite (no NaN code). Runs on the CUDA cores, fp32 throughout. */
+int bm_paged_kv8_tree_attention_workspace_size(int64_t total_q, int64_t batch, int32_t num_q_heads, int32_t num_kv_heads,
+                                               int32_t head_dim, int32_t max_ctx, int32_t max_tree, size_t* bytes_out);
+int bm_paged_kv8_tree_attention(void* out, const void* q, const bm_paged_kv8_t* cache, const int32_t* seq_ids,
+                                const int32_t* ctx_lens, const int32_t* q_starts, const uint64_t* tree_mask,
+                                int32_t mask_words, int64_t total_q, int64_t batch, int32_t num_q_heads, int32_t max_ctx,
+                                int32_t max_tree, float scale, void* workspace, size_t workspace_bytes, bm_dtype_t dtype,
+                                int32_t* d_status, void* stream);
+
+/* ---------------------------------------------------------------------------
  * Sampling: one token per row of logits [rows][vocab], rows row_stride elements apart,
  * from given uniform numbers in [0, 1). The reference leaves this to its callers (an
  * argmax on the host, src/benchmark.cpp). For each row, in this order:
