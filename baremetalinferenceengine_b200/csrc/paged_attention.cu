@@ -1,7 +1,7 @@
 // Attention of a tree of drafted tokens per sequence over a paged KV cache, of the storage
 // type or in 8 bits: the entry points (bm_paged_tree_attention, bm_paged_kv8_tree_attention),
 // and the CUDA-core kernels that serve fp32, every head_dim and every page size. The
-// tensor-core form of the first is paged_attention_tc.cu.
+// tensor-core forms are paged_attention_tc.cu and paged_attention8_tc.cu.
 //
 // Mathematics: for row r = (token i, head) of a sequence, over the slots t that it sees,
 //   out = sum_t 2^(s_t - m) v_t / sum_t 2^(s_t - m),  s_t = q . k_t * scale * log2(e),
@@ -775,7 +775,7 @@ int attend(const char* what, TreeArgs a, float scale, size_t workspace_bytes, bm
     return fail(BM_ERR_INVALID_ARGUMENT, "%s: workspace of %zu bytes is smaller than %zu", what, workspace_bytes, need);
   }
   const cudaStream_t st = as_stream(stream);
-  if (!k8 && tc_takes(a, dtype)) return launch_tc(a, st, what);
+  if (k8 ? tc8_takes(a, dtype) : tc_takes(a, dtype)) return k8 ? launch_tc8(a, st, what) : launch_tc(a, st, what);
   plan(a.batch, a.hkv, a.group, a.max_ctx, a.max_tree, &a.row_tiles, &a.splits, &a.split_len);
   if (k8) return dtype == BM_F32 ? launch<float, Code>(a, st, what) : launch<bf16, Code>(a, st, what);
   return dtype == BM_F32 ? launch<float, float>(a, st, what) : launch<bf16, bf16>(a, st, what);
