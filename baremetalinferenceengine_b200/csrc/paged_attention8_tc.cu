@@ -19,11 +19,10 @@
 // Bound: memory while group * tokens is below about 100 (a slot is half the bytes of a bf16
 // cache's, for the same tensor time), above it the softmax: exponentials, and the conversions of P.
 //
-// Split and roles are paged_attention_tc.cu's, but for the query warp: warp 2 converts each
-// segment's queries into two operands in shared memory (all idle warps together for a CTA's first, so
-// that a short call does not wait for one warp's loads), a segment ahead where shared memory has room, and
-// looks up the scales of each tile's slots, eight neighbouring ones of which share one: a tile whose
-// scores may be issued has its K (TMA) and its scales (one arrival of warp 2) in shared memory.
+// Split and roles are paged_attention_tc.cu's, but for the queries and the scales: warp 2 converts a
+// segment's queries into two operands in shared memory while the segment before is computed (all
+// warps but those of TMA together for a CTA's first, which all wait for), and the warp that fetches K looks up
+// the scales of its tile's slots, eight neighbouring ones of which share one.
 #include <cuda.h>
 
 #include "kv8.cuh"
@@ -45,17 +44,17 @@ struct Layout8 : RowLayout<HD, COPIES> {
   using Rows = RowLayout<HD, COPIES>;
   static constexpr int kOperand = kTile * HD;               // a tile of K or V, one part of Q
   static constexpr int kQTile = 2 * kOperand;               // both parts of a row tile
-  static constexpr int kQBufs = Rows::kTwo ? 1 : 2;
-  static constexpr int kKS = HD == 128 ? 4 : 6;             // K ring: freed by the scores
-  static constexpr int kVS = HD == 128 ? (Rows::kCopies > 1 ? 4 : 5) : 8;  // V ring: freed by the mix
-  static constexpr int kOffK = kQBufs * Rows::kTiles * kQTile;
+  static constexpr int kQBuf = Rows::kTiles * kQTile;       // of two: a segment's, and the next one's
+  static constexpr int kKS = HD == 64 ? 6 : Rows::kTwo ? 2 : 4;                          // K ring: freed by the scores
+  static constexpr int kVS = HD == 64 ? 8 : Rows::kTwo ? 3 : Rows::kCopies > 1 ? 4 : 5;  // V ring: freed by the mix
+  static constexpr int kOffK = 2 * kQBuf;
   static constexpr int kOffV = kOffK + kKS * kOperand;
   static constexpr int kOffMl = kOffV + kVS * kOperand;
   static constexpr int kOffSum = kOffMl + Rows::kMlBytes;
   static constexpr int kOffScale = kOffSum + Rows::kSumBytes;  // [kBadRing][kGroups] (f of K, e_v, 2^-e_v, -)
   static constexpr int kOffFactor = kOffScale + kBadRing * kGroups * 16;  // [kQRing][rows]
   static constexpr int kOffBar = kOffFactor + kQRing * Rows::kRows * 4;
-  static constexpr int kBars = 2 * kKS + 2 * kVS + 6 + 2 * kQBufs + 2;
+  static constexpr int kBars = 2 * kKS + 2 * kVS + 6 + 6;
   static constexpr int kOffPlan = kOffBar + kBars * 8;      // Plan, scan, bad-page ring
   static constexpr int kBytes = kOffPlan + 96 + 16 * 8 + kBadRing * 4 + 16 + 1024 /* alignment slack */;
   static_assert(kBytes <= 232448, "shared memory of a CTA");
@@ -99,6 +98,10 @@ __device__ __forceinline__ void tmem_store8(uint32_t taddr, const uint32_t (&r)[
       "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(taddr)
       : "memory");
 }
+// The phase's bytes to come, without an arrival.
+__device__ __forceinline__ void mbar_expect_only(uint64_t* bar, uint32_t bytes) {
+  asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
+}
 __device__ __forceinline__ void mbar_arrive_n(uint64_t* bar, uint32_t count) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(count) : "memory");
 }
@@ -128,35 +131,43 @@ __device__ __forceinline__ void weight_parts(float lo, float hi, uint32_t* part,
 template <typename L, int HD>
 __device__ __forceinline__ void convert_queries(const TreeArgs& a, const Seq& s, int kvh, int p, int tpt, unsigned char* to, float* factor,
                                                 int worker, int workers) {
-  constexpr int kBatch = 8;  // pairs of rows whose loads are in flight
+  constexpr int kBatch = 4;  // pairs of rows that are converted side by side
   const int lane = threadIdx.x & 31, half = lane >> 4, c = lane & 15;
   const int i_first = p * tpt * L::kTiles;
-  const bf16* q = static_cast<const bf16*>(a.q);
+  const uint32_t by_group = (65536u + a.group - 1) / a.group;  // r / group = r * by_group >> 16 for r < 128
+  const bf16* q = static_cast<const bf16*>(a.q) + (s.row0 * a.hq + static_cast<int64_t>(kvh) * a.group) * a.hd + c * 8;
+  const int64_t token_step = static_cast<int64_t>(a.hq) * a.hd;
   for (int pair0 = worker; pair0 < L::kRows / 2; pair0 += workers * kBatch) {
     uint4 raw[kBatch];
 #pragma unroll
     for (int k = 0; k < kBatch; ++k) {
-      const int row = 2 * (pair0 + k * workers) + half, tile = row / L::kCopyRows, r = row % L::kCopyRows;
-      const int i = i_first + tile * tpt + r / a.group;
+      const int row = 2 * (pair0 + k * workers) + half, r = row % L::kCopyRows;
+      const int token = static_cast<int>(r * by_group >> 16), i = i_first + row / L::kCopyRows * tpt + token;
       raw[k] = make_uint4(0u, 0u, 0u, 0u);
-      if (row < L::kRows && r < tpt * a.group && i < s.n && c * 8 < a.hd) {
-        raw[k] = ld_keep(q + ((s.row0 + i) * a.hq + kvh * a.group + r % a.group) * a.hd + c * 8);
-      }
+      if (row < L::kRows && token < tpt && i < s.n && c * 8 < a.hd) raw[k] = ld_keep(q + i * token_step + (r - token * a.group) * a.hd);
+    }
+    uint32_t top[kBatch];
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      // the larger of two neighbours' magnitudes, as bf16 in either half of a word
+      const uint32_t m01 = __vmaxu2(raw[k].x & 0x7fff7fffu, raw[k].y & 0x7fff7fffu), m23 = __vmaxu2(raw[k].z & 0x7fff7fffu, raw[k].w & 0x7fff7fffu);
+      const uint32_t m = __vmaxu2(m01, m23);
+      top[k] = max(m & 0xffffu, m >> 16);
+    }
+#pragma unroll
+    for (int off = 8; off > 0; off >>= 1) {
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) top[k] = max(top[k], __shfl_xor_sync(0xffffffffu, top[k], off));
     }
 #pragma unroll
     for (int k = 0; k < kBatch; ++k) {
-      const int row = 2 * (pair0 + k * workers) + half, tile = row / L::kCopyRows, r = row % L::kCopyRows;
-      if (2 * (pair0 + k * workers) >= L::kRows) break;  // the same for the warp
-      float x[8];
-      unpack16<bf16>(raw[k], x);
-      uint32_t top = 0;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
-#pragma unroll
-      for (int off = 8; off > 0; off >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, off));
-      const int e = min(max(static_cast<int>(top >> 23) - 127, -60), 127);
+      const int row = 2 * (pair0 + k * workers) + half, r = row % L::kCopyRows;
+      if (row >= L::kRows) continue;
+      const int e = min(max(static_cast<int>(top[k] >> 7) - 127, -60), 127);
       const float f = kv8::power(7 - e);
       if (c * 8 < HD) {
+        float x[8];
+        unpack16<bf16>(raw[k], x);
         uint32_t hi[2], lo[2];
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
@@ -171,13 +182,13 @@ __device__ __forceinline__ void convert_queries(const TreeArgs& a, const Seq& s,
         for (int copy = 0; copy < L::kCopies; ++copy) {
           const int at = copy * L::kCopyRows + r;
           const int chunk = (c >> 1) ^ (HD == 128 ? at & 7 : (at >> 1) & 3);  // the swizzle of 16-byte chunks
-          unsigned char* dst = to + tile * L::kQTile + at * HD + chunk * 16 + (c & 1) * 8;
+          unsigned char* dst = to + row / L::kCopyRows * L::kQTile + at * HD + chunk * 16 + (c & 1) * 8;
           *reinterpret_cast<uint2*>(dst) = make_uint2(hi[0], hi[1]);
           *reinterpret_cast<uint2*>(dst + L::kOperand) = make_uint2(lo[0], lo[1]);
         }
       }
       // a query that is not finite spoils its row
-      if (c == 0) factor[row] = top >= 0x7f800000u ? __int_as_float(0x7fffffff) : a.qscale * kv8::power(e - 7);
+      if (c == 0) factor[row] = top[k] >= 0x7f80u ? __int_as_float(0x7fffffff) : a.qscale * kv8::power(e - 7);
     }
   }
   fence_proxy_async_smem();
@@ -201,7 +212,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
   const int tpt = L::kCopyRows / a.group;  // tokens of a row tile
   const int per = tpt * L::kTiles;         // and of an item
 
-  uint64_t* kfull = reinterpret_cast<uint64_t*>(smem + L::kOffBar);  // K (TMA) and its tile's scales (warp 2)
+  uint64_t* kfull = reinterpret_cast<uint64_t*>(smem + L::kOffBar);  // K, and its tile's scales
   uint64_t* kempty = kfull + L::kKS;
   uint64_t* vfull = kempty + L::kKS;
   uint64_t* vempty = vfull + L::kVS;
@@ -209,8 +220,8 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
   uint64_t* pfull = sfull + 2;          // weights in TMEM      (one arrival per warp of the group)
   uint64_t* pvdone = pfull + 2;         // mix done             (commit)
   uint64_t* qfull = pvdone + 2;         // queries converted    (kQWarps arrivals)
-  uint64_t* qempty = qfull + L::kQBufs; // the segment's last scores are done (commit)
-  uint64_t* ofree = qempty + L::kQBufs; // the segment's O has been read (one arrival per softmax warp)
+  uint64_t* qempty = qfull + 2;         // the segment's last scores are done (commit)
+  uint64_t* ofree = qempty + 2;         // the segment's O has been read (one arrival per softmax warp)
   uint64_t* mma_done = ofree + 1;
   Plan* plan = reinterpret_cast<Plan*>(smem + L::kOffPlan);
   int64_t* scan = reinterpret_cast<int64_t*>(smem + L::kOffPlan + 96);
@@ -229,7 +240,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
     // barriers and TMEM come up while the lengths are read
     if (tid == 0) {
       for (int i = 0; i < L::kKS; ++i) {
-        mbar_init(&kfull[i], 2);
+        mbar_init(&kfull[i], 1);
         mbar_init(&kempty[i], 1);
       }
       for (int i = 0; i < L::kVS; ++i) {
@@ -240,8 +251,6 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
         mbar_init(&sfull[i], 1);
         mbar_init(&pfull[i], 4);
         mbar_init(&pvdone[i], 1);
-      }
-      for (int i = 0; i < L::kQBufs; ++i) {
         mbar_init(&qfull[i], kQWarps);
         mbar_init(&qempty[i], 1);
       }
@@ -278,7 +287,9 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
   }
 
   if (warp == 0 || warp == 3) {
-    // ---------------- K (warp 0) and V (warp 3) ----------------
+    // ---------------- K with the scales (warp 0) and V (warp 3) ----------------
+    // Lanes 0 to 15 each fetch a box of the tile; warp 0's others look up the scales of eight slots
+    // each, one step ahead, and their pages two.
     const bool is_v = warp == 3;
     const CUtensorMap* map = is_v ? &tv : &tk;
     uint64_t* full = is_v ? vfull : kfull;
@@ -286,102 +297,92 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
     unsigned char* ring = smem + (is_v ? L::kOffV : L::kOffK);
     const int stages = is_v ? L::kVS : L::kKS;
     const int boxes = a.tile / a.box;    // of a tile: at most 16
+    const bool scaler = !is_v && lane >= 16;
+    const int first_slot = lane < 16 ? lane * a.box : (lane - 16) * kGroupSlots;  // of this lane in a tile
     int kt = 0, stage = 0;               // tiles asked for; the next one's ring slot
     uint32_t phase = 1;
     bool ok = true;
     for (; ok && walk.left > 0; walk.next(a, per)) {
       const int n = walk.segment();
       const int32_t* pages = a.page_table + static_cast<int64_t>(walk.s.seq) * a.max_pages;
-      const int total = walk.s.ctx + walk.s.n;
-      auto row_of = [&](int t) {  // this lane's box of tile t: its row in the tensor map, -1 bad, -2 none
-        const int slot = t * a.tile + lane * a.box;
-        if (lane >= boxes || slot >= total) return -2;
+      const int total = walk.s.ctx + walk.s.n, t0 = walk.t, kvh = walk.kvh;
+      const bool mine = lane < 16 ? lane < boxes : scaler && first_slot < a.tile;
+      // This lane's slot of tile i of the segment: its row in the tensor map, -1 bad, -2 none.
+      auto row_of = [&](int i) {
+        const int slot = (t0 + i) * a.tile + first_slot;
+        if (!mine || i >= n || slot >= total) return -2;
         const int nth = slot / a.page_size;
         const int32_t page = __ldg(pages + nth);
         if (page < 0 || page >= a.num_pages) return -1;
-        return (page * a.hkv + walk.kvh) * a.page_size + (slot - nth * a.page_size);
+        return (page * a.hkv + kvh) * a.page_size + (slot - nth * a.page_size);
       };
-      int row = row_of(walk.t);
+      // The scales of a row, as bytes; 127 (2^0) where there are none.
+      auto scales_of = [&](int row, uint32_t* k, uint32_t* v) {
+        *k = *v = 127;
+        if (!scaler || row < 0) return;
+        const int at = row / a.block;  // blocks divide pages
+        *k = __ldg(a.k_scales + at);
+        *v = __ldg(a.v_scales + at);
+      };
+      int row = row_of(0), row1 = scaler ? row_of(1) : -2;
+      uint32_t k, v;
+      scales_of(row, &k, &v);
       for (int i = 0; i < n; ++i) {
-        const int next_row = i + 1 < n ? row_of(walk.t + i + 1) : -2;  // looked up while this tile waits
-        const uint32_t have = __ballot_sync(0xffffffffu, row >= 0);
-        const uint32_t bad = __ballot_sync(0xffffffffu, row == -1);
+        // looked up while this tile waits
+        const int next = row_of(i + (scaler ? 2 : 1));
+        uint32_t k1 = 127, v1 = 127;
+        scales_of(row1, &k1, &v1);
+        const uint32_t have = __ballot_sync(0xffffffffu, lane < 16 && row >= 0);
+        const uint32_t bad = __ballot_sync(0xffffffffu, lane < 16 && row == -1);
         if (!(ok = warp_wait(&empty[stage], phase, abort_flag, a.status))) break;
         if (lane == 0) {
-          if (!is_v) {
+          const uint32_t bytes = __popc(have) * a.box * HD;
+          if (is_v) {
+            mbar_expect_tx(&full[stage], bytes);
+          } else {
+            mbar_expect_only(&full[stage], bytes);  // the arrival follows the scales
             bad_ring[kt % kBadRing] = bad;
             if (bad) raise_status(a.status, BM_DEVERR_BAD_PAGE);
           }
-          mbar_expect_tx(&full[stage], __popc(have) * a.box * HD);
         }
         __syncwarp();
-        if (row >= 0) tma_load_2d(ring + stage * L::kOperand + lane * a.box * HD, map, &full[stage], 0, row);
+        if (lane < 16 && row >= 0) tma_load_2d(ring + stage * L::kOperand + lane * a.box * HD, map, &full[stage], 0, row);
+        if (!is_v) {
+          if (scaler) {
+            const int ev = kv8::exponent(static_cast<uint8_t>(v));
+            scales[kt % kBadRing * kGroups + lane - 16] =
+                make_float4(kv8::power(kv8::exponent(static_cast<uint8_t>(k))), static_cast<float>(ev), kv8::power(-ev), 0.f);
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&full[stage]);
+        }
         ++kt;
         if (++stage == stages) {
           stage = 0;
           phase ^= 1;
         }
-        row = next_row;
+        row = scaler ? row1 : next;
+        row1 = next;
+        k = k1;
+        v = v1;
       }
     }
-    // Copies still in flight land before the CTA ends. (Past an abort warp 2's arrivals of the last tiles may be
-    // missing: then the wait ends by its limit, long after the copies.)
-    if (lane == 0) {
+    if (lane == 0) {  // copies still in flight land before the CTA ends
       for (int i = max(0, kt - stages); i < kt; ++i) {
         wait_phase(&full[i % stages], (i / stages) & 1, abort_flag, a.status, kDrainNs, false);
       }
     }
     __syncwarp();
   } else if (warp == 2) {
-    // ---------------- scales, and the queries of the segments behind the first ----------------
-    const int half = lane >> 4, g = lane & 15;  // two tiles at a time, a lane for eight slots of one
-    int kt = 0, stage = 0;
-    uint32_t phase = 1;
-    bool ok = true;
-    for (int seg = 0; ok && walk.left > 0; walk.next(a, per), ++seg) {
-      const int n = walk.segment();
-      const int32_t* pages = a.page_table + static_cast<int64_t>(walk.s.seq) * a.max_pages;
-      const int total = walk.s.ctx + walk.s.n, kvh = walk.kvh, t0 = walk.t;
-      // The scales of this lane's slots of tile i of the segment, as bytes (k, v); 127 (2^0) where there are none.
-      auto fetch = [&](int i, uint32_t* k, uint32_t* v) {
-        *k = *v = 127;
-        const int slot = (t0 + i) * a.tile + g * kGroupSlots;
-        if (i >= n || g * kGroupSlots >= a.tile || slot >= total) return;
-        const int nth = slot / a.page_size;
-        const int32_t page = __ldg(pages + nth);
-        if (page < 0 || page >= a.num_pages) return;
-        const int64_t at = (static_cast<int64_t>(page) * a.hkv + kvh) * (a.page_size / a.block) + (slot - nth * a.page_size) / a.block;
-        *k = __ldg(a.k_scales + at);
-        *v = __ldg(a.v_scales + at);
-      };
-      uint32_t k, v;
-      fetch(half, &k, &v);
-      if (seg > 0) {
-        const int buf = seg % L::kQBufs;
-        if (!(ok = warp_wait(&qempty[buf], ((seg / L::kQBufs) & 1) ^ 1u, abort_flag, a.status))) break;
-        convert_queries<L, HD>(a, walk.s, walk.kvh, walk.p, tpt, smem + buf * L::kTiles * L::kQTile, factors + seg % kQRing * L::kRows, 0, 1);
-        if (lane == 0) mbar_arrive_n(&qfull[buf], kQWarps);
-        __syncwarp();
-      }
-      for (int i = 0; ok && i < n; i += 2) {
-        uint32_t k_next, v_next;
-        fetch(i + 2 + half, &k_next, &v_next);  // on their way while these tiles wait
-        const int ev = kv8::exponent(static_cast<uint8_t>(v));
-        const float4 mine = make_float4(kv8::power(kv8::exponent(static_cast<uint8_t>(k))), static_cast<float>(ev), kv8::power(-ev), 0.f);
-        for (int h = 0; h < min(2, n - i); ++h) {
-          if (!(ok = warp_wait(&kempty[stage], phase, abort_flag, a.status))) break;
-          if (half == h) scales[kt % kBadRing * kGroups + g] = mine;
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&kfull[stage]);
-          ++kt;
-          if (++stage == L::kKS) {
-            stage = 0;
-            phase ^= 1;
-          }
-        }
-        k = k_next;
-        v = v_next;
-      }
+    // ---------------- the queries of the segments behind the first, one ahead ----------------
+    int seg = 0;
+    for (walk.next(a, per); walk.left > 0; walk.next(a, per)) {
+      ++seg;
+      const int buf = seg & 1;
+      if (!warp_wait(&qempty[buf], ((seg >> 1) & 1) ^ 1u, abort_flag, a.status)) break;
+      convert_queries<L, HD>(a, walk.s, walk.kvh, walk.p, tpt, smem + buf * L::kQBuf, factors + seg % kQRing * L::kRows, 0, 1);
+      if (lane == 0) mbar_arrive_n(&qfull[buf], kQWarps);
+      __syncwarp();
     }
   } else if (warp == 1) {
     // ---------------- MMA issuer ----------------
@@ -430,14 +431,14 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
         }
       }
       if (left > 0) {
-        const int buf = seg % L::kQBufs;
-        if (first) ok = warp_wait(&qfull[buf], (seg / L::kQBufs) & 1, abort_flag, a.status);
+        const int buf = seg & 1;
+        if (first) ok = warp_wait(&qfull[buf], (seg >> 1) & 1, abort_flag, a.status);
         if (ok) ok = warp_wait(&kfull[ks], k_phase, abort_flag, a.status);
         if (ok && x >= 2) ok = warp_wait(&pvdone[w], ((x - 2) >> 1) & 1, abort_flag, a.status);
         if (!ok) break;
         tc_fence_after();
         if (elect_one()) {
-          const uint64_t q_at = q_desc + ((buf * L::kTiles + (DUAL ? w : 0)) * L::kQTile >> 4);
+          const uint64_t q_at = q_desc + ((buf * L::kQBuf + (DUAL ? w * L::kQTile : 0)) >> 4);
 #pragma unroll
           for (int kk = 0; kk < HD / 32; ++kk) {
             mma_f8(tmem + w * kTile, q_at + kk * 2, k_desc + ks * kStage + kk * 2, kIdescS, kk > 0 ? 1u : 0u);
