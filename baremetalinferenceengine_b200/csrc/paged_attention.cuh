@@ -95,13 +95,15 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   return r;
 }
 
-// The tensor-core forms (paged_attention_tc.cu; tc8: paged_attention8_tc.cu): whether they take
-// these arguments, the scratch they need (the same), and their launches.
+// The tensor-core forms (paged_attention_tc.cu; tc8: paged_attention8_tc.cu and
+// paged_attention8_few.cu): whether they take these arguments, the scratch they need, and their
+// launches.
 bool tc_takes(const TreeArgs& a, bm_dtype_t dtype);
 size_t tc_workspace_bytes(int64_t batch, int hkv, int hd, int group, int max_ctx, int max_tree);
 int launch_tc(const TreeArgs& a, cudaStream_t stream, const char* what);
 bool tc8_takes(const TreeArgs& a, bm_dtype_t dtype);
-int launch_tc8(const TreeArgs& a, cudaStream_t stream, const char* what);
+size_t tc8_workspace_bytes(int64_t batch, int hkv, int hd, int group, int max_ctx, int max_tree);
+int launch_tc8(TreeArgs a, cudaStream_t stream, const char* what);
 
 }  // namespace paged
 }  // namespace bm

@@ -490,7 +490,7 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(const TreeArgs a, int c
   const int skip = border(k - 1) != first;  // in the first CTA the item is not the first segment
   auto part = [&](int c) { return slots + (2 * static_cast<int64_t>(c) + (c == k - 1 ? skip : 0)) * L::kSlotFloats; };
   for (int r = static_cast<int>(blockIdx.y) * 8 + threadIdx.x / 32; r < L::kRows; r += 8 * gridDim.y) {
-    const int tile = r / kTile, rr = r - tile * kTile;
+    const int tile = r / L::kCopyRows, rr = r - tile * L::kCopyRows;
     const int i0 = rec.p * tpt * L::kTiles + tile * tpt;
     if (rr >= max(0, min(tpt, s.n - i0)) * a.group) continue;
     // the first parts' maxima, sums and values at once: two parts are all there is, mostly
@@ -583,13 +583,15 @@ inline bool tile_of(int page_size, int* tile, int* box) {
   return *tile >= kTile / 2;
 }
 
-// CTAs for the bounds: one per SM, no more than the tiles there can be (a tile holds at
+// CTAs for the bounds and items of `per` tokens: one per SM, no more than the tiles there can be (a tile holds at
 // least half of 128 slots).
-inline int ctas_for(int64_t batch, int hkv, int group, int max_ctx, int max_tree) {
-  const int per = tokens_of(copies_for(group, max_tree), group);
+inline int ctas_of(int64_t batch, int hkv, int per, int max_ctx, int max_tree) {
   const int64_t tiles = batch * hkv * ((max_tree + per - 1) / per) *
                         ((static_cast<int64_t>(max_ctx) + max_tree + kTile / 2 - 1) / (kTile / 2));
   return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(sm_count(), tiles)));
+}
+inline int ctas_for(int64_t batch, int hkv, int group, int max_ctx, int max_tree) {
+  return ctas_of(batch, hkv, tokens_of(copies_for(group, max_tree), group), max_ctx, max_tree);
 }
 
 // Whole items up to kWholeTiles tiles where they make CTAs for a quarter of the SMs or more

@@ -26,17 +26,18 @@ def i32(values, cuda):
     return torch.tensor(values, dtype=torch.int32, device=cuda)
 
 
-def on_tensor_cores(dtype, hd, page, block):
+def on_tensor_cores(dtype, hd, page, block, group, max_tree):
     """Whether the header says so: bf16, heads up to 128, pages up to 128 that are multiples of 8
-    or at least 64, or with an equal part of 64 to 128 slots; eight neighbouring slots of a
-    tile with one scale."""
+    or at least 64, or with an equal part of 64 to 128 slots; and few rows (two tiles of 32 hold a
+    sequence's), or eight neighbouring slots of a tile with one scale."""
     if page <= 128:
         tile, box = (128 // page * page, page) if page % 8 == 0 else (page, page)
     else:
         parts = next(n for n in range(-(-page // 128), page + 1) if page % n == 0)
         tile = box = page // parts
+    few = group <= 32 and max_tree <= 2 * (32 // group)
     return (dtype == BF16 and hd <= 128 and tile >= 64
-            and ((block % 8 == 0 and box % 8 == 0) or (tile == box and block % box == 0)))
+            and (few or (block % 8 == 0 and box % 8 == 0) or (tile == box and block % box == 0)))
 
 
 class Batch:
@@ -77,7 +78,7 @@ class Batch:
                 self.mask[self.starts[b]:self.starts[b + 1]] = ref.tree_bits(self.parents[b], self.words)
         self.tree = tree
         self.table = torch.tensor(table, dtype=torch.int32)
-        self.tc = on_tensor_cores(dtype, hd, page, block)
+        self.tc = on_tensor_cores(dtype, hd, page, block, self.group, self.max_tree)
         self.upload()
 
     def upload(self):
@@ -155,9 +156,10 @@ LENS = {
 
 def test_which_cores():
     """The shapes below reach both."""
-    takes = [on_tensor_cores(*s) for s in ((BF16, 128, 16, 16), (BF16, 48, 16, 8), (BF16, 128, 100, 100), (BF16, 64, 200, 200),
+    takes = [on_tensor_cores(*s, 8, 16) for s in ((BF16, 128, 16, 16), (BF16, 48, 16, 8), (BF16, 128, 100, 100), (BF16, 64, 200, 200),
                                            (BF16, 128, 256, 8), (BF16, 128, 512, 64))]
-    lacks = [on_tensor_cores(*s) for s in ((F32, 128, 16, 16), (BF16, 256, 16, 16), (BF16, 128, 16, 4), (BF16, 128, 100, 20),
+    assert on_tensor_cores(BF16, 128, 16, 4, 8, 8) and not on_tensor_cores(BF16, 128, 16, 4, 8, 9)
+    lacks = [on_tensor_cores(*s, 8, 16) for s in ((F32, 128, 16, 16), (BF16, 256, 16, 16), (BF16, 128, 16, 4), (BF16, 128, 100, 20),
                                            (BF16, 128, 136, 8), (BF16, 128, 7, 7))]
     assert all(takes) and not any(lacks)
 
@@ -180,6 +182,16 @@ def test_many_uneven_sequences(cuda, dtype, hd):
     rng = np.random.RandomState(3)
     lens = [(int(rng.randint(0, 600)), int(rng.randint(0, 12))) for _ in range(70)]
     Batch(cuda, lens, 4, 2, hd, 16, 16, dtype, seed=4).check()
+
+
+@pytest.mark.parametrize("hq,hkv,hd,page,block", [
+    (8, 2, 128, 16, 16), (8, 2, 64, 32, 1), (4, 4, 48, 24, 3), (32, 1, 128, 64, 64), (20, 1, 112, 128, 2), (7, 7, 16, 8, 8),
+    (5, 1, 80, 100, 50), (3, 1, 128, 256, 128), (11, 1, 96, 200, 25), (64, 1, 128, 16, 16), (33, 1, 64, 16, 8)])
+@pytest.mark.parametrize("rows", [1, 8, 9, 31, 32, 33, 48, 64, 65, 127, 128, 129, 256, 257])
+def test_rows_about_every_form(cuda, hq, hkv, hd, page, block, rows):
+    """Trees whose rows (tokens times group) fill, and pass, the tiles of 32, 64, 128 and 256 rows."""
+    n = max(1, rows // (hq // hkv))
+    Batch(cuda, [(700, n), (0, n), (131, max(1, n - 1)), (40, 1)], hq, hkv, hd, page, block, BF16, seed=rows + hd).check()
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])

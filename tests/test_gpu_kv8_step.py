@@ -71,7 +71,7 @@ class Server:
                     assert np.all(np.abs(got_[p, :, o] - x) <= step + dx)
         seen = (lambda row, i, j: j <= i) if mask is None else (lambda row, i, j: bool((int(mask[row, 0]) >> j) & 1))
         k, v = (torch.from_numpy(np.nan_to_num(x)) for x in (k, v))
-        tc = on_tensor_cores(self.dtype, HD, PAGE, BLOCK)
+        tc = on_tensor_cores(self.dtype, HD, PAGE, BLOCK, HQ // HKV, max(np.diff(starts)))
         want, tol = ref.attention(q, k, v, self.ids, list(range(SEQS)), ctx, starts, seen, 1 / math.sqrt(HD), self.dtype, tc)
         if tc:  # the parts of queries and weights: 2^-17 of a score's terms, 2^-11 and 2^-18 of weights
             size = q.cpu().double().abs().amax(-1, keepdim=True).numpy() * HD * float(k.abs().max()) / math.sqrt(HD)
