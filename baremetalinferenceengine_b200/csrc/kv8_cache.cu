@@ -15,6 +15,7 @@
 // Bound: memory; q, k and v are read once, and q and the codes written once.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "kv8.cuh"
 #include "rotary_device.cuh"
@@ -28,7 +29,13 @@ using namespace bm::kv8;
 constexpr int kMaxHeadDim = 256;
 constexpr int kThreads = 128;
 constexpr int kWarps = kThreads / 32;
-constexpr int kU = 4;  // passes whose loads a lane keeps in flight
+constexpr int kAppendThreads = 256;
+constexpr int kAppendWarps = kAppendThreads / 32;
+// Passes whose loads a lane keeps in flight, of Q's (and norm_rotary's) heads and of K's and V's rows; and the blocks
+// that an SM has room for at the registers these take. A prompt's 16384 rows of 64 + 8 heads of 128, us: 4 and 5 blocks
+// 114, 4 and 4 123, 2 and 6 116. K and V of 32768 tokens, 8 heads: 2 and 2 blocks 118, 1 and 3 154, 4 and 1 146.
+constexpr int kUQ = 4, kUK = 2;
+constexpr int kQBlocks = 5, kKvBlocks = 2;
 
 struct HeadArgs {
   void* q_out;
@@ -57,21 +64,25 @@ struct HeadArgs {
   int max_tokens, blocks, warps_per_job;
 };
 
-// A lane's share of a head: J units of two chunks of N elements.
-template <int N, int J>
+// A lane's share of a head: J units of two chunks of N elements. FULL: every lane of a warp has a rotated
+// unit (heads of 32, 64, 128 or 256 elements in a power of two of units, all of them rotated), so that nothing of it is asked.
+template <int N, int J, bool FULL>
 struct Share {
   int first[J], second[J];
-  bool own[J], pair[J], turns[J];
+  bool own_[J], pair_[J], turns_[J];
+  __device__ __forceinline__ bool own(int j) const { return FULL || own_[j]; }
+  __device__ __forceinline__ bool pair(int j) const { return FULL || pair_[j]; }
+  __device__ __forceinline__ bool turns(int j) const { return FULL || turns_[j]; }
   template <bool INTER>
   __device__ __forceinline__ void place(const HeadArgs& a, int c0, bool live) {
 #pragma unroll
     for (int j = 0; j < J; ++j) {
       const int c = c0 + 32 * j;
-      own[j] = live && c < a.units + a.rest;
-      turns[j] = c < a.units;
-      first[j] = turns[j] ? c * (INTER ? 2 * N : N) : a.rd + (c - a.units) * 2 * N;
-      second[j] = first[j] + (turns[j] && !INTER ? a.rd / 2 : N);
-      pair[j] = own[j] && second[j] < a.hd;  // the last copied unit may have one chunk
+      own_[j] = live && c < a.units + a.rest;
+      turns_[j] = c < a.units;
+      first[j] = turns(j) ? c * (INTER ? 2 * N : N) : a.rd + (c - a.units) * 2 * N;
+      second[j] = first[j] + (turns(j) && !INTER ? a.rd / 2 : N);
+      pair_[j] = own(j) && second[j] < a.hd;  // the last copied unit may have one chunk
     }
   }
 };
@@ -92,136 +103,168 @@ __device__ __forceinline__ float head_sum(float v, int c, int n, int lane) {
   return __shfl_sync(0xffffffffu, v, lane - c);
 }
 
-template <typename T, int N, int J>
+template <typename T, int N, int J, bool FULL>
 struct Head {
   Piece<T, N> p1[J], p2[J];
 
-  __device__ __forceinline__ void load(const T* x, const Share<N, J>& s) {
+  __device__ __forceinline__ void load(const T* x, const Share<N, J, FULL>& s) {
 #pragma unroll
     for (int j = 0; j < J; ++j) {
-      if (s.own[j]) p1[j].load(x + s.first[j]);
-      if (s.pair[j]) p2[j].load(x + s.second[j]);
+      if (s.own(j)) p1[j].load(x + s.first[j]);
+      if (s.pair(j)) p2[j].load(x + s.second[j]);
     }
   }
-  __device__ __forceinline__ void get(float (&x)[J][2 * N], const Share<N, J>& s) const {
+  __device__ __forceinline__ void get(float (&x)[J][2 * N], const Share<N, J, FULL>& s) const {
 #pragma unroll
     for (int j = 0; j < J; ++j) {
 #pragma unroll
       for (int e = 0; e < 2 * N; ++e) x[j][e] = 0.f;
-      if (s.own[j]) p1[j].get(x[j]);
-      if (s.pair[j]) p2[j].get(x[j] + N);
+      if (s.own(j)) p1[j].get(x[j]);
+      if (s.pair(j)) p2[j].get(x[j] + N);
     }
   }
-  __device__ __forceinline__ void set_store(T* to, const float (&x)[J][2 * N], const Share<N, J>& s) {
+  __device__ __forceinline__ void set_store(T* to, const float (&x)[J][2 * N], const Share<N, J, FULL>& s) {
 #pragma unroll
     for (int j = 0; j < J; ++j) {
       p1[j].set(x[j]);
       p2[j].set(x[j] + N);
-      if (s.own[j]) p1[j].store(to + s.first[j]);
-      if (s.pair[j]) p2[j].store(to + s.second[j]);
+      if (s.own(j)) p1[j].store(to + s.first[j]);
+      if (s.pair(j)) p2[j].store(to + s.second[j]);
     }
   }
 };
 
-// x r w. Every lane of the warp takes part, whether it holds elements or not.
-template <typename T, int N, int J>
-__device__ __forceinline__ void norm(float (&x)[J][2 * N], const Head<T, N, J>& weight, const Share<N, J>& s, const HeadArgs& a,
-                                     int c, int n, int lane) {
-  float sum = 0.f;
+// x r w, w unpacked. Every lane of the warp takes part, whether it holds elements or not.
+template <int N, int J>
+__device__ __forceinline__ void norm(float (&x)[J][2 * N], const float (&w)[J][2 * N], const HeadArgs& a, int c, int n, int lane) {
+  uint64_t sum2 = 0;
 #pragma unroll
   for (int j = 0; j < J; ++j) {
 #pragma unroll
-    for (int e = 0; e < 2 * N; ++e) sum = fmaf(x[j][e], x[j][e], sum);
+    for (int e = 0; e < 2 * N; e += 2) sum2 = fma2(pair(x[j][e], x[j][e + 1]), pair(x[j][e], x[j][e + 1]), sum2);
   }
-  const float r = rsqrtf(head_sum(sum, c, n, lane) / a.hd + a.eps);
-  float w[J][2 * N];
-  weight.get(w, s);
+  const float2 sums = unpair(sum2);
+  const float r = rsqrtf(head_sum(sums.x + sums.y, c, n, lane) / a.hd + a.eps);
+  const uint64_t r2 = pair(r, r);
 #pragma unroll
   for (int j = 0; j < J; ++j) {
 #pragma unroll
-    for (int e = 0; e < 2 * N; ++e) x[j][e] = x[j][e] * r * w[j][e];
+    for (int e = 0; e < 2 * N; e += 2) {
+      const float2 y = unpair(mul2(mul2(pair(x[j][e], x[j][e + 1]), r2), pair(w[j][e], w[j][e + 1])));
+      x[j][e] = y.x;
+      x[j][e + 1] = y.y;
+    }
   }
 }
+// The lane's share of a norm's weights, from global or shared memory (Piece::load streams from global memory only).
+template <typename T, int N, int J, bool FULL>
+__device__ __forceinline__ void load_weight(float (&w)[J][2 * N], const T* weight, const Share<N, J, FULL>& s) {
+  using Raw = decltype(Piece<T, N>::raw);
+  Head<T, N, J, FULL> raw;
+#pragma unroll
+  for (int j = 0; j < J; ++j) {
+    if (s.own(j)) raw.p1[j].raw = *reinterpret_cast<const Raw*>(weight + s.first[j]);
+    if (s.pair(j)) raw.p2[j].raw = *reinterpret_cast<const Raw*>(weight + s.second[j]);
+  }
+  raw.get(w, s);
+}
 
-template <int N, int J>
+template <int N, int J, bool FULL>
 struct Angles {
   float2 cs[J][N];
-  __device__ __forceinline__ void load(const HeadArgs& a, int pos, int c0, const Share<N, J>& s) {
+  __device__ __forceinline__ void load(const HeadArgs& a, int pos, int c0, const Share<N, J, FULL>& s) {
     const float2* t = a.table + static_cast<int64_t>(pos) * (a.rd / 2);
 #pragma unroll
     for (int j = 0; j < J; ++j) {
-      if (s.own[j] && s.turns[j]) load_angles<N>(t + (c0 + 32 * j) * N, cs[j]);
+      if (s.own(j) && s.turns(j)) load_angles<N>(t + (c0 + 32 * j) * N, cs[j]);
     }
   }
 };
-template <int N, int J, bool INTER>
-__device__ __forceinline__ void turn(float (&x)[J][2 * N], const Angles<N, J>& t, const Share<N, J>& s) {
+template <int N, int J, bool INTER, bool FULL>
+__device__ __forceinline__ void turn(float (&x)[J][2 * N], const Angles<N, J, FULL>& t, const Share<N, J, FULL>& s) {
 #pragma unroll
   for (int j = 0; j < J; ++j) {
-    if (s.own[j] && s.turns[j]) rotate<N, INTER>(x[j], t.cs[j]);
+    if (s.own(j) && s.turns(j)) {
+      if constexpr (!INTER && N % 2 == 0) {
+        rotate2<N>(x[j], t.cs[j]);
+      } else {
+        rotate<N, INTER>(x[j], t.cs[j]);
+      }
+    }
   }
 }
 
-// One warp's share of a row's heads: part `part` of a.parts of `heads` heads from src to dst.
-template <typename T, int N, int J, bool INTER>
-__device__ __forceinline__ void turn_heads(const HeadArgs& a, const T* src, T* dst, int heads, int part, const void* weight, int pos,
-                                           int lane) {
-  const int n = min(32, a.units + a.rest), hpi = a.heads_per_pass;
+// The weights of Q's and K's norms as a block keeps them, in shared memory (a lane's share of either would take
+// a dozen registers): q's hd elements, then k's.
+template <typename T>
+__device__ __forceinline__ void stage_weights(T* to, const HeadArgs& a, int threads) {
+  for (int i = threadIdx.x; i < 2 * a.hd; i += threads) {
+    const T* w = static_cast<const T*>(i < a.hd ? a.q_weight : a.k_weight);
+    if (w != nullptr) to[i < a.hd ? i : i - a.hd + kMaxHeadDim] = w[i < a.hd ? i : i - a.hd];
+  }
+  __syncthreads();
+}
+
+// One warp's share of a row's heads: part `part` of a.parts of Q's heads and, behind them, `hkv` of K's.
+template <typename T, int N, int J, bool INTER, bool FULL>
+__device__ __forceinline__ void turn_heads(const HeadArgs& a, int64_t row, int hkv, int part, bool normed, const T* weights, int pos, int lane) {
+  const int n = min(32, a.units + a.rest), hpi = a.heads_per_pass, heads = a.hq + hkv;
   const int hl = lane / n, c = lane - hl * n;
-  Share<N, J> s;
+  Share<N, J, FULL> s;
   s.template place<INTER>(a, c, hl < hpi);
   const int passes = (heads + hpi - 1) / hpi, mine = (passes + a.parts - 1) / a.parts;
   const int h_end = min(heads, (part + 1) * mine * hpi);
   if (part * mine * hpi >= h_end) return;
-  Head<T, N, J> w;
-  Angles<N, J> t;
+  const T* q = static_cast<const T*>(a.q) + row * a.q_stride;
+  const T* k = static_cast<const T*>(a.k) + row * a.k_stride;
+  T* q_out = static_cast<T*>(a.q_out) + row * a.q_out_stride;
+  T* k_out = static_cast<T*>(a.k_out) + row * a.k_out_stride;
+  Angles<N, J, FULL> t;
   bool have = false;
-  for (int hb = part * mine * hpi; hb < h_end; hb += hpi * kU) {  // the same for the warp
-    Head<T, N, J> x[kU];
+  for (int hb = part * mine * hpi; hb < h_end; hb += hpi * kUQ) {  // the same for the warp
+    Head<T, N, J, FULL> x[kUQ];
 #pragma unroll
-    for (int u = 0; u < kU; ++u) {
+    for (int u = 0; u < kUQ; ++u) {
       const int h = hb + u * hpi + hl;
-      if (h < h_end) x[u].load(src + static_cast<int64_t>(h) * a.hd, s);
+      if (h < h_end) x[u].load(h < a.hq ? q + h * a.hd : k + (h - a.hq) * a.hd, s);
     }
     if (!have) {
-      if (weight) w.load(static_cast<const T*>(weight), s);
       if (a.table) t.load(a, pos, c, s);
       have = true;
     }
 #pragma unroll
-    for (int u = 0; u < kU; ++u) {
+    for (int u = 0; u < kUQ; ++u) {
       const int h = hb + u * hpi + hl;
       if (hb + u * hpi >= h_end) break;
       float y[J][2 * N];
       x[u].get(y, s);
-      if (weight) norm<T, N, J>(y, w, s, a, c, n, lane);
-      if (a.table) turn<N, J, INTER>(y, t, s);
-      if (h < h_end) x[u].set_store(dst + static_cast<int64_t>(h) * a.hd, y, s);
+      if (normed) {
+        float w[J][2 * N];
+        load_weight<T, N, J, FULL>(w, weights + (h < a.hq ? 0 : kMaxHeadDim), s);
+        norm<N, J>(y, w, a, c, n, lane);
+      }
+      if (a.table) turn<N, J, INTER, FULL>(y, t, s);
+      if (h < h_end) x[u].set_store(h < a.hq ? q_out + h * a.hd : k_out + (h - a.hq) * a.hd, y, s);
     }
   }
 }
 
-template <typename T, int N, int J, bool INTER>
-__global__ void __launch_bounds__(kThreads) norm_rotary_kernel(const __grid_constant__ HeadArgs a) {
+template <typename T, int N, int J, bool INTER, bool FULL>
+__global__ void __launch_bounds__(kThreads, kQBlocks) norm_rotary_kernel(const __grid_constant__ HeadArgs a) {
   grid_dependency_wait();
+  __shared__ __align__(16) T weights[2 * kMaxHeadDim];
   const int lane = threadIdx.x & 31;
   const int64_t job = static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
   const int64_t row = job / a.parts;
-  if (row >= a.rows) return;
   const int part = static_cast<int>(job - row * a.parts);
-  const int32_t pos = a.positions ? __ldg(a.positions + row) : static_cast<int32_t>(a.pos0 + row);
+  const int32_t pos = row >= a.rows ? 0 : a.positions ? __ldg(a.positions + row) : static_cast<int32_t>(a.pos0 + row);
+  stage_weights(weights, a, kThreads);
+  if (row >= a.rows) return;
   if (pos < 0 || pos >= a.table_len) {
     if (lane == 0) raise_status(a.status, BM_DEVERR_BAD_POSITION);
     return;
   }
-  if (a.hq) {
-    turn_heads<T, N, J, INTER>(a, static_cast<const T*>(a.q) + row * a.q_stride, static_cast<T*>(a.q_out) + row * a.q_out_stride,
-                               a.hq, part, a.q_weight, pos, lane);
-  }
-  if (a.hkv) {
-    turn_heads<T, N, J, INTER>(a, static_cast<const T*>(a.k) + row * a.k_stride, static_cast<T*>(a.k_out) + row * a.k_out_stride,
-                               a.hkv, part, a.k_weight, pos, lane);
-  }
+  turn_heads<T, N, J, INTER, FULL>(a, row, a.hkv, part, true, weights, pos, lane);
 }
 
 // A sequence of the batch: its cache sequence, cached slots, new rows and the first of them.
@@ -265,35 +308,47 @@ __device__ __forceinline__ void store_codes(uint8_t* to, const float* x, float f
   }
 }
 
-// The first kv_ctas blocks take K and V: one job is K or V of one head in one block of slots,
-// held by warps_per_job warps of a block (16 rows each in registers, at the widest heads 128
-// elements). A lane group holds a row, so the norm is a sum over a group and the scale a
-// maximum over the warp, then over the job's warps. The other blocks rotate Q.
-template <typename T, int N, int J, bool INTER>
-__global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant__ HeadArgs a) {
+// One warp's share of a token's Q on the way of an append.
+template <typename T, int N, int J, bool INTER, bool FULL>
+__device__ __forceinline__ void append_q(const HeadArgs& a, int64_t job, const T* weights, int lane) {
+  const int64_t token = job / a.parts;
+  const int part = static_cast<int>(job - token * a.parts);
+  const int64_t b = token / a.max_tokens;
+  const int j = static_cast<int>(token - b * a.max_tokens);
+  if (b >= a.batch) return;
+  Span s;
+  if (read_span(a.cache, a.starts, a.ctx_lens, a.seq_ids, a.rows, a.max_tokens, b, &s) || j >= s.n) return;
+  const int64_t row = s.row0 + j;
+  const int32_t pos = a.positions ? __ldg(a.positions + row) : s.ctx + j;
+  if (a.table && (pos < 0 || pos >= a.table_len)) return;  // K's and V's jobs tell
+  turn_heads<T, N, J, INTER, FULL>(a, row, 0, part, a.q_weight != nullptr, weights, pos, lane);
+}
+template <typename T, int N, int J, bool INTER, bool FULL>
+__global__ void __launch_bounds__(kThreads, kQBlocks) append_q_kernel(const __grid_constant__ HeadArgs a) {
   grid_dependency_wait();
-  __shared__ uint32_t tops[kWarps];
+  __shared__ __align__(16) T weights[2 * kMaxHeadDim];
+  if (a.q_weight) stage_weights(weights, a, kThreads);
+  append_q<T, N, J, INTER, FULL>(a, static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5), weights, threadIdx.x & 31);
+}
+
+// The first kv_ctas blocks take K and V: one job is K or V of one head in one block of slots,
+// held by warps_per_job warps of a block. A lane group holds a row, so the norm is a sum over a group and the scale a
+// maximum over the warp, then over the job's warps. The other blocks rotate Q.
+template <typename T, int N, int J, bool INTER, bool FULL>
+__global__ void __launch_bounds__(kAppendThreads, kKvBlocks) append_kernel(const __grid_constant__ HeadArgs a) {
+  grid_dependency_wait();
+  __shared__ uint32_t tops[kAppendWarps];
+  __shared__ __align__(16) T weights[2 * kMaxHeadDim];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const bm_paged_kv8_t& c8 = a.cache;
   if (blockIdx.x >= a.kv_ctas) {
-    const int64_t job = (static_cast<int64_t>(blockIdx.x) - a.kv_ctas) * kWarps + warp;
-    const int64_t token = job / a.parts;
-    const int part = static_cast<int>(job - token * a.parts);
-    const int64_t b = token / a.max_tokens;
-    const int j = static_cast<int>(token - b * a.max_tokens);
-    if (b >= a.batch) return;
-    Span s;
-    if (read_span(c8, a.starts, a.ctx_lens, a.seq_ids, a.rows, a.max_tokens, b, &s) || j >= s.n) return;
-    const int64_t row = s.row0 + j;
-    const int32_t pos = a.positions ? __ldg(a.positions + row) : s.ctx + j;
-    if (a.table && (pos < 0 || pos >= a.table_len)) return;  // K's and V's jobs tell
-    turn_heads<T, N, J, INTER>(a, static_cast<const T*>(a.q) + row * a.q_stride, static_cast<T*>(a.q_out) + row * a.q_out_stride,
-                               a.hq, part, a.q_weight, pos, lane);
+    if (a.q_weight) stage_weights(weights, a, kAppendThreads);
+    append_q<T, N, J, INTER, FULL>(a, (static_cast<int64_t>(blockIdx.x) - a.kv_ctas) * kAppendWarps + warp, weights, lane);
     return;
   }
   // ---------------- K and V ----------------
   const int wpj = a.warps_per_job, sub = warp % wpj;
-  const int64_t job = static_cast<int64_t>(blockIdx.x) * (kWarps / wpj) + warp / wpj;
+  const int64_t job = static_cast<int64_t>(blockIdx.x) * (kAppendWarps / wpj) + warp / wpj;
   const int which = static_cast<int>(job % (2 * a.hkv));
   const int head = which >> 1;
   const bool is_v = which & 1;
@@ -311,81 +366,85 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant_
     lo = static_cast<int>(max(static_cast<int64_t>(s.ctx), min(from, static_cast<int64_t>(s.ctx) + s.n)));
     hi = static_cast<int>(min(static_cast<int64_t>(s.ctx) + s.n, from + c8.block));
     active = !bad && lo < hi;
-    if (active) {
-      begin = static_cast<int>(from);
-      const int nth = begin / c8.page_size;
-      const int32_t page = __ldg(c8.page_table + static_cast<int64_t>(s.seq) * c8.max_pages + nth);
-      if (page < 0 || page >= c8.num_pages) {
-        if (lane == 0 && sub == 0) raise_status(a.status, BM_DEVERR_BAD_PAGE);
-        active = false;
-      } else {
-        const int64_t ph = static_cast<int64_t>(page) * a.hkv + head;
-        const int off = begin - nth * c8.page_size;
-        pages = static_cast<uint8_t*>(is_v ? c8.v_pages : c8.k_pages) + (ph * c8.page_size + off) * a.hd;
-        scale = static_cast<uint8_t*>(is_v ? c8.v_scales : c8.k_scales) + ph * (c8.page_size / c8.block) + off / c8.block;
-      }
-    }
+    begin = static_cast<int>(active ? from : 0);
   }
   if (!active) lo = hi = 0;
-  // A block with slots of earlier calls has a scale: read here, since the job's first warp
-  // writes it at its own end, behind the barrier.
-  const bool keeps = active && begin < s.ctx;
-  const int before = keeps ? exponent(*scale) : kLowest;
   const int n = min(32, a.units + a.rest), rpi = a.heads_per_pass;
   const int rl = lane / n, c = lane - rl * n;
-  Share<N, J> sh;
+  Share<N, J, FULL> sh;
   sh.template place<INTER>(a, c, rl < rpi);
   const T* src = static_cast<const T*>(is_v ? a.v : a.k) + static_cast<int64_t>(head) * a.hd;
   const int64_t stride = is_v ? a.v_stride : a.k_stride;
   const bool normed = !is_v && a.k_weight, turned = !is_v && a.table;
-  Head<T, N, J> w;
-  if (normed && active) w.load(static_cast<const T*>(a.k_weight), sh);
 
-  // Batches of kU passes, of rpi rows each, in turn over the job's warps. One batch stays in
-  // registers until its scale is known; more are read again.
-  const int step = kU * rpi * wpj;
-  float y[kU][J][2 * N];
-  bool good[kU];
+  // Batches of kUK passes, of rpi rows each, in turn over the job's warps. One batch stays in
+  // registers until its scale is known; more are read again. The first one's loads are on their way before
+  // the chain of page and scale is walked.
+  const int step = kUK * rpi * wpj;
+  Head<T, N, J, FULL> x[kUK];
+  int32_t pos[kUK];
+  float y[kUK][J][2 * N];
+  bool good[kUK];
+  auto fetch = [&](int from) {
+#pragma unroll
+    for (int u = 0; u < kUK; ++u) {
+      const int slot = from + (sub * kUK + u) * rpi + rl;
+      good[u] = active && slot < hi && (FULL || rl < rpi);
+      const int64_t r = s.row0 + (slot - s.ctx);
+      if (good[u]) x[u].load(src + r * stride, sh);
+      pos[u] = good[u] && a.table && a.positions ? __ldg(a.positions + r) : slot;
+    }
+  };
+  fetch(lo);
+  float w[J][2 * N];
+  if (normed && active) load_weight<T, N, J, FULL>(w, static_cast<const T*>(a.k_weight), sh);
+  if (active) {
+    const int nth = begin / c8.page_size;
+    const int32_t page = __ldg(c8.page_table + static_cast<int64_t>(s.seq) * c8.max_pages + nth);
+    if (page < 0 || page >= c8.num_pages) {
+      if (lane == 0 && sub == 0) raise_status(a.status, BM_DEVERR_BAD_PAGE);
+      active = false;
+      lo = hi = 0;
+#pragma unroll
+      for (int u = 0; u < kUK; ++u) good[u] = false;
+    } else {
+      const int64_t ph = static_cast<int64_t>(page) * a.hkv + head;
+      const int off = begin - nth * c8.page_size;
+      pages = static_cast<uint8_t*>(is_v ? c8.v_pages : c8.k_pages) + (ph * c8.page_size + off) * a.hd;
+      scale = static_cast<uint8_t*>(is_v ? c8.v_scales : c8.k_scales) + ph * (c8.page_size / c8.block) + off / c8.block;
+    }
+  }
+  // A block with slots of earlier calls has a scale: read here, since the job's first warp
+  // writes it at its own end, behind the barrier.
+  const bool keeps = active && begin < s.ctx;
+  const int before = keeps ? exponent(*scale) : kLowest;
+
   uint32_t top = 0;
   int bad_position = 0;
-  auto batch = [&](int from) {
-    Head<T, N, J> x[kU];
+  auto compute = [&]() {
 #pragma unroll
-    for (int u = 0; u < kU; ++u) {
-      const int slot = from + (sub * kU + u) * rpi + rl;
-      good[u] = active && slot < hi && rl < rpi;
-      if (good[u]) x[u].load(src + (s.row0 + (slot - s.ctx)) * stride, sh);
-    }
-    int32_t pos[kU];
-    if (a.table) {  // V, too, leaves out the rows whose position is bad
-#pragma unroll
-      for (int u = 0; u < kU; ++u) {
-        const int slot = from + (sub * kU + u) * rpi + rl;
-        pos[u] = !good[u] ? 0 : a.positions ? __ldg(a.positions + s.row0 + (slot - s.ctx)) : slot;
-        if (pos[u] < 0 || pos[u] >= a.table_len) {
-          good[u] = false;
-          bad_position = 1;
-        }
+    for (int u = 0; u < kUK; ++u) {
+      if (a.table && good[u] && (pos[u] < 0 || pos[u] >= a.table_len)) {  // V, too, leaves out the rows whose position is bad
+        good[u] = false;
+        bad_position = 1;
       }
-    }
-#pragma unroll
-    for (int u = 0; u < kU; ++u) {
-      Angles<N, J> t;
+      Angles<N, J, FULL> t;
       if (turned && good[u]) t.load(a, pos[u], c, sh);
       x[u].get(y[u], sh);
-      if (normed) norm<T, N, J>(y[u], w, sh, a, c, n, lane);
-      if (turned && good[u]) turn<N, J, INTER>(y[u], t, sh);
+      if (normed) norm<N, J>(y[u], w, a, c, n, lane);
+      if (turned && good[u]) turn<N, J, INTER, FULL>(y[u], t, sh);
     }
   };
   const int batches = (hi - lo + step - 1) / step;
   for (int i = 0; i < batches; ++i) {
-    batch(lo + i * step);
+    if (i > 0) fetch(lo + i * step);
+    compute();
 #pragma unroll
-    for (int u = 0; u < kU; ++u) {
+    for (int u = 0; u < kUK; ++u) {
 #pragma unroll
       for (int j = 0; j < J; ++j) {
 #pragma unroll
-        for (int e = 0; e < 2 * N; ++e) top = max(top, good[u] && (e < N ? sh.own[j] : sh.pair[j]) ? magnitude(y[u][j][e]) : 0u);
+        for (int e = 0; e < 2 * N; ++e) top = max(top, good[u] && (e < N ? sh.own(j) : sh.pair(j)) ? magnitude(y[u][j][e]) : 0u);
       }
     }
   }
@@ -416,15 +475,18 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant_
   }
   const float f = power(-e);
   for (int i = 0; i < batches; ++i) {
-    if (batches > 1) batch(lo + i * step);
+    if (batches > 1) {
+      fetch(lo + i * step);
+      compute();
+    }
 #pragma unroll
-    for (int u = 0; u < kU; ++u) {
-      const int slot = lo + i * step + (sub * kU + u) * rpi + rl;
+    for (int u = 0; u < kUK; ++u) {
+      const int slot = lo + i * step + (sub * kUK + u) * rpi + rl;
       uint8_t* to = pages + static_cast<int64_t>(slot - begin) * a.hd;
 #pragma unroll
       for (int j = 0; j < J; ++j) {
-        if (good[u] && sh.own[j]) store_codes<N>(to + sh.first[j], y[u][j], f);
-        if (good[u] && sh.pair[j]) store_codes<N>(to + sh.second[j], y[u][j] + N, f);
+        if (good[u] && sh.own(j)) store_codes<N>(to + sh.first[j], y[u][j], f);
+        if (good[u] && sh.pair(j)) store_codes<N>(to + sh.second[j], y[u][j] + N, f);
       }
     }
   }
@@ -443,9 +505,10 @@ struct ReadArgs {
   int32_t* status;
 };
 
-// 16 values to memory.
+// A lane's 16 values to memory. In bf16 they are 32 bytes, two stores: where neighbouring lanes hold
+// neighbours of a row (paired), they swap halves, so that a store of both fills a 32-byte sector.
 template <typename T>
-__device__ __forceinline__ void store16(T* to, const uint4& codes, float f) {
+__device__ __forceinline__ void store16(T* to, const uint4& codes, float f, bool paired, bool odd, bool good) {
   float v[16];
   from_codes(codes.x, v);
   from_codes(codes.y, v + 4);
@@ -453,11 +516,32 @@ __device__ __forceinline__ void store16(T* to, const uint4& codes, float f) {
   from_codes(codes.w, v + 12);
 #pragma unroll
   for (int e = 0; e < 16; ++e) v[e] *= f;
+  if constexpr (sizeof(T) == 2) {
+    uint4 lo = pack16<T>(v), hi = pack16<T>(v + 8);
+    if (paired) {
+      const uint4 give = odd ? lo : hi;
+      uint4 got;
+      got.x = __shfl_xor_sync(0xffffffffu, give.x, 1);
+      got.y = __shfl_xor_sync(0xffffffffu, give.y, 1);
+      got.z = __shfl_xor_sync(0xffffffffu, give.z, 1);
+      got.w = __shfl_xor_sync(0xffffffffu, give.w, 1);
+      // even: its first half and the neighbour's; odd: the neighbour's second half and its own
+      if (good) {
+        st_plain(to - (odd ? 8 : 0), odd ? got : lo);
+        st_plain(to + (odd ? 8 : 16), odd ? hi : got);
+      }
+    } else {
+      st_plain(to, lo);
+      st_plain(to + 8, hi);
+    }
+  } else {
 #pragma unroll
-  for (int e = 0; e < 16; e += VecWidth<T>::value) st_plain(to + e, pack16<T>(v + e));
+    for (int e = 0; e < 16; e += 4) st_plain(to + e, pack16<T>(v + e));
+  }
 }
 
-// A warp takes K and V of one head in kU passes of rows; a lane 16 codes of each.
+constexpr int kReadU = 4;
+// A warp takes K and V of one head in kReadU passes of rows; a lane 16 codes of each.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) read_kernel(const __grid_constant__ ReadArgs a) {
   grid_dependency_wait();
@@ -476,15 +560,15 @@ __global__ void __launch_bounds__(kThreads) read_kernel(const __grid_constant__ 
   }
   const int n = c8.head_dim / 16, rpi = 32 / n;  // lanes of a row, rows of a pass
   const int rl = lane / n, c = lane - rl * n;
-  const int i0 = chunk * kU * rpi + rl;
-  if (rl >= rpi) return;
-  uint4 k[kU], v[kU];
-  float kf[kU], vf[kU];
-  bool good[kU];
+  const int i0 = chunk * kReadU * rpi + rl;
+  const bool paired = sizeof(T) == 2 && n % 2 == 0;
+  uint4 k[kReadU], v[kReadU];
+  float kf[kReadU], vf[kReadU];
+  bool good[kReadU];
 #pragma unroll
-  for (int u = 0; u < kU; ++u) {
+  for (int u = 0; u < kReadU; ++u) {
     const int i = i0 + u * rpi;
-    good[u] = i < s.n;
+    good[u] = rl < rpi && i < s.n;
     if (good[u]) {
       const int slot = s.ctx + i, nth = slot / c8.page_size;
       const int32_t page = __ldg(c8.page_table + static_cast<int64_t>(s.seq) * c8.max_pages + nth);
@@ -504,11 +588,11 @@ __global__ void __launch_bounds__(kThreads) read_kernel(const __grid_constant__ 
     }
   }
 #pragma unroll
-  for (int u = 0; u < kU; ++u) {
-    if (!good[u]) continue;
+  for (int u = 0; u < kReadU; ++u) {
+    if (!paired && !good[u]) continue;  // where lanes are paired, all of them swap, and good ones store
     const int64_t to = ((s.row0 + i0 + u * rpi) * c8.num_kv_heads + head) * c8.head_dim + c * 16;
-    store16(static_cast<T*>(a.k_out) + to, k[u], kf[u]);
-    store16(static_cast<T*>(a.v_out) + to, v[u], vf[u]);
+    store16(static_cast<T*>(a.k_out) + to, k[u], kf[u], paired, c & 1, good[u]);
+    store16(static_cast<T*>(a.v_out) + to, v[u], vf[u], paired, c & 1, good[u]);
   }
 }
 
@@ -660,16 +744,21 @@ extern "C" int bm_qk_norm_rotary(void* q_out, void* k_out, const void* q, const 
   a.parts = parts_for(rows);
   const int64_t blocks = (rows * a.parts + kWarps - 1) / kWarps;
   return with_chunk(&a, dtype, [&](int n) {
+    const bool full = a.rest == 0 && 32 % a.units == 0;
     auto go = [&](auto kernel) {
       return launch_kernel(what, kernel, dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0, as_stream(stream), nullptr, a);
     };
-    if (dtype == BM_F32) {
-      if (n == 4) return interleaved ? go(norm_rotary_kernel<float, 4, 1, true>) : go(norm_rotary_kernel<float, 4, 1, false>);
-      return interleaved ? go(norm_rotary_kernel<float, 1, 4, true>) : go(norm_rotary_kernel<float, 1, 4, false>);
-    }
-    if (n == 8) return interleaved ? go(norm_rotary_kernel<bf16, 8, 1, true>) : go(norm_rotary_kernel<bf16, 8, 1, false>);
-    if (n == 4) return interleaved ? go(norm_rotary_kernel<bf16, 4, 1, true>) : go(norm_rotary_kernel<bf16, 4, 1, false>);
-    return interleaved ? go(norm_rotary_kernel<bf16, 1, 4, true>) : go(norm_rotary_kernel<bf16, 1, 4, false>);
+    auto pick = [&](auto inter) {
+      constexpr bool I = decltype(inter)::value;
+      if (dtype == BM_F32) {
+        if (n == 4) return full ? go(norm_rotary_kernel<float, 4, 1, I, true>) : go(norm_rotary_kernel<float, 4, 1, I, false>);
+        return go(norm_rotary_kernel<float, 1, 4, I, false>);
+      }
+      if (n == 8) return full ? go(norm_rotary_kernel<bf16, 8, 1, I, true>) : go(norm_rotary_kernel<bf16, 8, 1, I, false>);
+      if (n == 4) return go(norm_rotary_kernel<bf16, 4, 1, I, false>);
+      return go(norm_rotary_kernel<bf16, 1, 4, I, false>);
+    };
+    return interleaved ? pick(std::true_type{}) : pick(std::false_type{});
   });
 }
 
@@ -742,24 +831,37 @@ extern "C" int bm_paged_kv8_append(void* q_out, const void* q, const void* k, co
   a.blocks = static_cast<int>((static_cast<int64_t>(max_tokens) - 1 + c.block - 1) / c.block + 1);  // that max_tokens neighbouring slots can meet
   a.parts = parts_for(std::min<int64_t>(rows, batch * static_cast<int64_t>(max_tokens)));
   return with_chunk(&a, dtype, [&](int n) {
-    // 64 slots of a block need the registers of four warps (kU passes of four rows of 128)
-    const int one = kU * a.heads_per_pass;
-    a.warps_per_job = std::min(max_tokens, c.block) <= one ? 1 : std::min(max_tokens, c.block) <= 2 * one ? 2 : kWarps;
-    const int64_t per = kWarps / a.warps_per_job;
+    // A warp holds kUK passes of a block's rows in registers (of 128 elements in bf16: 8 rows); the widest blocks are
+    // read twice.
+    const int rows_at_once = std::min(max_tokens, c.block);
+    a.warps_per_job = 1;
+    while (a.warps_per_job < kAppendWarps && a.warps_per_job * kUK * a.heads_per_pass < rows_at_once) a.warps_per_job *= 2;
+    const int64_t per = kAppendWarps / a.warps_per_job;
     const double jobs = static_cast<double>(batch) * a.blocks * 2 * a.hkv, q_jobs = static_cast<double>(batch) * max_tokens * a.parts;
     if (jobs + q_jobs > INT32_MAX) return fail(BM_ERR_INVALID_ARGUMENT, "%s: batch * max_tokens too large", what);
     a.kv_ctas = (batch * a.blocks * 2 * a.hkv + per - 1) / per;
-    const int64_t q_ctas = num_q_heads ? (batch * max_tokens * a.parts + kWarps - 1) / kWarps : 0;
-    auto go = [&](auto kernel) {
-      return launch_kernel(what, kernel, dim3(static_cast<unsigned>(a.kv_ctas + q_ctas)), dim3(kThreads), 0, as_stream(stream), nullptr, a);
+    // Few tokens go in one launch; where they fill the GPU, Q's warps are better off in a kernel of their own, since
+    // K's and V's registers leave room for only 16 warps on an SM (32768 tokens of 64 + 8 heads: 335 us in one).
+    const bool apart = num_q_heads > 0 && a.parts == 1;
+    const int64_t q_warps = num_q_heads ? batch * max_tokens * a.parts : 0;
+    const int64_t q_ctas = apart ? 0 : (q_warps + kAppendWarps - 1) / kAppendWarps;
+    const bool full = a.rest == 0 && 32 % a.units == 0;
+    auto go = [&](auto kernel, auto q_kernel) {
+      const int st = launch_kernel(what, kernel, dim3(static_cast<unsigned>(a.kv_ctas + q_ctas)), dim3(kAppendThreads), 0, as_stream(stream), nullptr, a);
+      if (st != BM_OK || !apart) return st;
+      return launch_kernel(what, q_kernel, dim3(static_cast<unsigned>((q_warps + kWarps - 1) / kWarps)), dim3(kThreads), 0, as_stream(stream), nullptr, a);
     };
-    if (dtype == BM_F32) {
-      if (n == 4) return interleaved ? go(append_kernel<float, 4, 1, true>) : go(append_kernel<float, 4, 1, false>);
-      return interleaved ? go(append_kernel<float, 1, 4, true>) : go(append_kernel<float, 1, 4, false>);
-    }
-    if (n == 8) return interleaved ? go(append_kernel<bf16, 8, 1, true>) : go(append_kernel<bf16, 8, 1, false>);
-    if (n == 4) return interleaved ? go(append_kernel<bf16, 4, 1, true>) : go(append_kernel<bf16, 4, 1, false>);
-    return interleaved ? go(append_kernel<bf16, 1, 4, true>) : go(append_kernel<bf16, 1, 4, false>);
+    auto pick = [&](auto inter) {
+      constexpr bool I = decltype(inter)::value;
+      if (dtype == BM_F32) {
+        if (n == 4) return full ? go(append_kernel<float, 4, 1, I, true>, append_q_kernel<float, 4, 1, I, true>) : go(append_kernel<float, 4, 1, I, false>, append_q_kernel<float, 4, 1, I, false>);
+        return go(append_kernel<float, 1, 4, I, false>, append_q_kernel<float, 1, 4, I, false>);
+      }
+      if (n == 8) return full ? go(append_kernel<bf16, 8, 1, I, true>, append_q_kernel<bf16, 8, 1, I, true>) : go(append_kernel<bf16, 8, 1, I, false>, append_q_kernel<bf16, 8, 1, I, false>);
+      if (n == 4) return go(append_kernel<bf16, 4, 1, I, false>, append_q_kernel<bf16, 4, 1, I, false>);
+      return go(append_kernel<bf16, 1, 4, I, false>, append_q_kernel<bf16, 1, 4, I, false>);
+    };
+    return interleaved ? pick(std::true_type{}) : pick(std::false_type{});
   });
 }
 
@@ -785,7 +887,7 @@ extern "C" int bm_paged_kv8_read(void* k_out, void* v_out, const bm_paged_kv8_t*
     return fail(BM_ERR_INVALID_ARGUMENT, "%s: an output overlaps the other or the cache", what);
   }
   ReadArgs a{k_out, v_out, c, first, starts, seq_ids, rows, batch, max_rows, 0, d_status};
-  const int per = kU * (32 / (c.head_dim / 16));
+  const int per = kReadU * (32 / (c.head_dim / 16));
   a.chunks = static_cast<int>((static_cast<int64_t>(max_rows) + per - 1) / per);
   const double jobs = static_cast<double>(batch) * a.chunks * c.num_kv_heads;
   if (jobs > INT32_MAX) return fail(BM_ERR_INVALID_ARGUMENT, "%s: batch * max_rows too large", what);

@@ -1,7 +1,7 @@
 // Attention of a tree of drafted tokens per sequence over a paged KV cache, of the storage
 // type or in 8 bits: the entry points (bm_paged_tree_attention, bm_paged_kv8_tree_attention),
 // and the CUDA-core kernels that serve fp32, every head_dim and every page size. The
-// tensor-core forms are paged_attention_tc.cu, paged_attention8_tc.cu and paged_attention8_few.cu.
+// tensor-core forms are paged_attention_tc.cu and paged_attention8_tc.cu.
 //
 // Mathematics: for row r = (token i, head) of a sequence, over the slots t that it sees,
 //   out = sum_t 2^(s_t - m) v_t / sum_t 2^(s_t - m),  s_t = q . k_t * scale * log2(e),
@@ -731,14 +731,13 @@ size_t simt_workspace_bytes(int64_t total_q, int64_t batch, int hq, int hkv, int
   return splits == 1 ? 0 : static_cast<size_t>(total_q) * hq * splits * (hd + 4) * sizeof(float);
 }
 
-int workspace_size(const char* what, int64_t total_q, int64_t batch, int hq, int hkv, int hd, int max_ctx, int max_tree, bool k8,
-                   size_t* bytes_out) {
+int workspace_size(const char* what, int64_t total_q, int64_t batch, int hq, int hkv, int hd, int max_ctx, int max_tree, size_t* bytes_out) {
   if (!bytes_out) return fail(BM_ERR_INVALID_ARGUMENT, "%s: NULL bytes_out", what);
   *bytes_out = 0;
   if (int st = check_sizes(what, total_q, batch, hq, hkv, hd, max_ctx, max_tree)) return st;
   if (batch == 0 || max_tree == 0) return BM_OK;
   *bytes_out = std::max(simt_workspace_bytes(total_q, batch, hq, hkv, hd, max_ctx, max_tree),
-                        (k8 ? tc8_workspace_bytes : tc_workspace_bytes)(batch, hkv, hd, hq / hkv, max_ctx, max_tree));
+                        tc_workspace_bytes(batch, hkv, hd, hq / hkv, max_ctx, max_tree));
   return BM_OK;
 }
 
@@ -771,7 +770,7 @@ int attend(const char* what, TreeArgs a, float scale, size_t workspace_bytes, bm
   if (meets(a.out, bytes)) return fail(BM_ERR_INVALID_ARGUMENT, "%s: out overlaps the cache's pages", what);
   a.group = a.hq / a.hkv;
   size_t need = 0;
-  if (int st = workspace_size(what, a.total_q, a.batch, a.hq, a.hkv, a.hd, a.max_ctx, a.max_tree, k8, &need)) return st;
+  if (int st = workspace_size(what, a.total_q, a.batch, a.hq, a.hkv, a.hd, a.max_ctx, a.max_tree, &need)) return st;
   if (need > 0 && (!a.ws || workspace_bytes < need)) {
     return fail(BM_ERR_INVALID_ARGUMENT, "%s: workspace of %zu bytes is smaller than %zu", what, workspace_bytes, need);
   }
@@ -848,7 +847,7 @@ extern "C" int bm_paged_tree_attention_workspace_size(int64_t total_q, int64_t b
                                                       int32_t num_kv_heads, int32_t head_dim, int32_t max_ctx,
                                                       int32_t max_tree, size_t* bytes_out) {
   return bm::paged::workspace_size("bm_paged_tree_attention_workspace_size", total_q, batch, num_q_heads, num_kv_heads, head_dim,
-                                   max_ctx, max_tree, false, bytes_out);
+                                   max_ctx, max_tree, bytes_out);
 }
 
 extern "C" int bm_paged_tree_attention(void* out, const void* q, const bm_paged_kv_t* cache, const int32_t* seq_ids,
@@ -871,7 +870,7 @@ extern "C" int bm_paged_kv8_tree_attention_workspace_size(int64_t total_q, int64
                                                           int32_t num_kv_heads, int32_t head_dim, int32_t max_ctx,
                                                           int32_t max_tree, size_t* bytes_out) {
   return bm::paged::workspace_size("bm_paged_kv8_tree_attention_workspace_size", total_q, batch, num_q_heads, num_kv_heads,
-                                   head_dim, max_ctx, max_tree, true, bytes_out);
+                                   head_dim, max_ctx, max_tree, bytes_out);
 }
 
 extern "C" int bm_paged_kv8_tree_attention(void* out, const void* q, const bm_paged_kv8_t* cache, const int32_t* seq_ids,

@@ -67,43 +67,13 @@ __device__ __forceinline__ bool sees(const TreeArgs& a, int64_t row0, int i, int
   return (__ldg(a.mask + (row0 + i) * a.words + (j >> 6)) >> (j & 63)) & 1;
 }
 
-// Pairs of fp32 in one register pair: one instruction for two multiply-adds or adds.
-__device__ __forceinline__ uint64_t pair(float a, float b) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ uint64_t pair(uint32_t a, uint32_t b) { return static_cast<uint64_t>(b) << 32 | a; }
-__device__ __forceinline__ float2 unpair(uint64_t p) {
-  float2 r;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(p));
-  return r;
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-
-// The tensor-core forms (paged_attention_tc.cu; tc8: paged_attention8_tc.cu and
-// paged_attention8_few.cu): whether they take these arguments, the scratch they need, and their
-// launches.
+// The tensor-core forms (paged_attention_tc.cu; tc8: paged_attention8_tc.cu): whether they take
+// these arguments, the scratch they need (the same), and their launches.
 bool tc_takes(const TreeArgs& a, bm_dtype_t dtype);
 size_t tc_workspace_bytes(int64_t batch, int hkv, int hd, int group, int max_ctx, int max_tree);
 int launch_tc(const TreeArgs& a, cudaStream_t stream, const char* what);
 bool tc8_takes(const TreeArgs& a, bm_dtype_t dtype);
-size_t tc8_workspace_bytes(int64_t batch, int hkv, int hd, int group, int max_ctx, int max_tree);
-int launch_tc8(TreeArgs a, cudaStream_t stream, const char* what);
+int launch_tc8(const TreeArgs& a, cudaStream_t stream, const char* what);
 
 }  // namespace paged
 }  // namespace bm

@@ -8,12 +8,12 @@
 // Qh is the query times a power of two that puts its largest element in [128, 256), rounded to
 // e4m3, and Ql what that leaves: together all 8 bits of a bf16 element down to 2^-9 of the largest, and
 // 2^-17 of the largest below. Scales are powers of two, so they meet the softmax as exponents:
-//   t = S f + e_v,  f = 2^(e_k - e_q) scale log2(e),  P = 2^(t - m + 4),  l += P 2^(-e_v)
+//   t = S f + e_v,  f = 2^(e_k - e_q) scale log2(e),  P = 2^(t - m + 2),  l += P 2^(-e_v)
 // with e_k and e_v the exponents of K's and V's scale at the slot, e_q the query's and m the running maximum
 // of t: the weight times V's scale is what the mix takes, so its rounding is relative to the
-// largest term of the sum, however far blocks' scales lie apart. P is at most 2^8 (a row is rescaled when m rises by more than 2^4); as
+// largest term of the sum, however far blocks' scales lie apart. P is at most 2^8 (a row is rescaled when m rises by more than 6); as
 // fp16 it splits into Ph (e4m3) and Pl = P - Ph (e5m2, whose exponents reach down to 2^-16): off by 2^-8 of itself
-// at most, by 2^-18 of the largest where it is small: the precision of bf16 weights, for two products of
+// at most, by 2^-16 of the largest where it is small: the precision of bf16 weights, for two products of
 // twice bf16's rate.
 //
 // Bound: memory while group * tokens is below about 100 (a slot is half the bytes of a bf16
@@ -25,14 +25,19 @@
 // the scales of its tile's slots, eight neighbouring ones of which share one.
 #include <cuda.h>
 
-#include "paged_attention8_tc.cuh"
+#include "kv8.cuh"
+#include "paged_attention_tc.cuh"
 
 namespace bm {
 namespace paged {
 namespace {
 
+constexpr float kRescaleAt8 = 6.f;  // rise of the maximum (log2) that a row's sums are rescaled at
+constexpr float kLift = 2.f;        // P is 2^2 at the running maximum, so at most 2^8
 constexpr int kGroupSlots = 8;      // slots of a tile that share a scale
 constexpr int kGroups = kTile / kGroupSlots;
+constexpr int kQRing = 4;           // segments whose queries' factors are kept
+constexpr int kQWarps = 10;         // warps that convert a CTA's first queries: all but the two of TMA
 
 template <int HD, int COPIES>
 struct Layout8 : RowLayout<HD, COPIES> {
@@ -62,6 +67,21 @@ __host__ __device__ constexpr uint32_t instr_desc_e4m3(bool a_e5m2, bool b_mn_ma
   return (1u << 4) | ((a_e5m2 ? 1u : 0u) << 7) | ((b_mn_major ? 1u : 0u) << 16) | (static_cast<uint32_t>(n >> 3) << 17) |
          (static_cast<uint32_t>(m >> 4) << 24);
 }
+// The matrix descriptor of rows of HD bytes, 8-row groups HD * 8 bytes apart, with the swizzle
+// of such rows (128 or 64 bytes). Both operands' tiles are one swizzle atom wide.
+template <int HD>
+__device__ __forceinline__ uint64_t byte_desc(uint32_t addr) {
+  return static_cast<uint64_t>((addr >> 4) & 0x3FFFu) | (1ull << 16) | (static_cast<uint64_t>((HD * 8) >> 4) << 32) | (1ull << 46) |
+         ((HD == 128 ? 2ull : 4ull) << 61);
+}
+__device__ __forceinline__ void mma_f8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
 // A's rows are TMEM lanes, four codes a column.
 __device__ __forceinline__ void mma_f8_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
@@ -81,6 +101,98 @@ __device__ __forceinline__ void tmem_store8(uint32_t taddr, const uint32_t (&r)[
 // The phase's bytes to come, without an arrival.
 __device__ __forceinline__ void mbar_expect_only(uint64_t* bar, uint32_t bytes) {
   asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive_n(uint64_t* bar, uint32_t count) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(count) : "memory");
+}
+
+// Two values as e4m3 (lo in the low byte); ends at +-448.
+__device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+// Two weights: e4m3 of their fp16 values, and e5m2 of what that leaves.
+__device__ __forceinline__ void weight_parts(float lo, float hi, uint32_t* part, uint32_t* rest) {
+  uint32_t p, back;
+  uint16_t h, l;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(p) : "f"(hi), "f"(lo));
+  asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(h) : "r"(p));
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(back) : "h"(h));
+  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(back) : "r"(p), "r"(back));
+  asm("cvt.rn.satfinite.e5m2x2.f16x2 %0, %1;" : "=h"(l) : "r"(back));
+  *part = h;
+  *rest = l;
+}
+
+// Converts the queries of an item into its two parts in the buffer at `to`, row tile after row
+// tile, copies and all, and their factors scale * log2(e) * 2^-e_q into factor[row]. Warp
+// `worker` of `workers` takes every workers-th pair of rows, half a warp a row; rows of no token are zero.
+template <typename L, int HD>
+__device__ __forceinline__ void convert_queries(const TreeArgs& a, const Seq& s, int kvh, int p, int tpt, unsigned char* to, float* factor,
+                                                int worker, int workers) {
+  constexpr int kBatch = 4;  // pairs of rows that are converted side by side
+  const int lane = threadIdx.x & 31, half = lane >> 4, c = lane & 15;
+  const int i_first = p * tpt * L::kTiles;
+  const uint32_t by_group = (65536u + a.group - 1) / a.group;  // r / group = r * by_group >> 16 for r < 128
+  const bf16* q = static_cast<const bf16*>(a.q) + (s.row0 * a.hq + static_cast<int64_t>(kvh) * a.group) * a.hd + c * 8;
+  const int64_t token_step = static_cast<int64_t>(a.hq) * a.hd;
+  for (int pair0 = worker; pair0 < L::kRows / 2; pair0 += workers * kBatch) {
+    uint4 raw[kBatch];
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      const int row = 2 * (pair0 + k * workers) + half, r = row % L::kCopyRows;
+      const int token = static_cast<int>(r * by_group >> 16), i = i_first + row / L::kCopyRows * tpt + token;
+      raw[k] = make_uint4(0u, 0u, 0u, 0u);
+      if (row < L::kRows && token < tpt && i < s.n && c * 8 < a.hd) raw[k] = ld_keep(q + i * token_step + (r - token * a.group) * a.hd);
+    }
+    uint32_t top[kBatch];
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      // the larger of two neighbours' magnitudes, as bf16 in either half of a word
+      const uint32_t m01 = __vmaxu2(raw[k].x & 0x7fff7fffu, raw[k].y & 0x7fff7fffu), m23 = __vmaxu2(raw[k].z & 0x7fff7fffu, raw[k].w & 0x7fff7fffu);
+      const uint32_t m = __vmaxu2(m01, m23);
+      top[k] = max(m & 0xffffu, m >> 16);
+    }
+#pragma unroll
+    for (int off = 8; off > 0; off >>= 1) {
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) top[k] = max(top[k], __shfl_xor_sync(0xffffffffu, top[k], off));
+    }
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      const int row = 2 * (pair0 + k * workers) + half, r = row % L::kCopyRows;
+      if (row >= L::kRows) continue;
+      const int e = min(max(static_cast<int>(top[k] >> 7) - 127, -60), 127);
+      const float f = kv8::power(7 - e);
+      if (c * 8 < HD) {
+        float x[8];
+        unpack16<bf16>(raw[k], x);
+        uint32_t hi[2], lo[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          float back[4];
+          hi[j] = e4m3x2(x[4 * j] * f, x[4 * j + 1] * f) | e4m3x2(x[4 * j + 2] * f, x[4 * j + 3] * f) << 16;
+          kv8::from_codes(hi[j], back);
+#pragma unroll
+          for (int d = 0; d < 4; ++d) back[d] = fmaf(x[4 * j + d], f, -back[d]);
+          lo[j] = e4m3x2(back[0], back[1]) | e4m3x2(back[2], back[3]) << 16;
+        }
+#pragma unroll
+        for (int copy = 0; copy < L::kCopies; ++copy) {
+          const int at = copy * L::kCopyRows + r;
+          const int chunk = (c >> 1) ^ (HD == 128 ? at & 7 : (at >> 1) & 3);  // the swizzle of 16-byte chunks
+          unsigned char* dst = to + row / L::kCopyRows * L::kQTile + at * HD + chunk * 16 + (c & 1) * 8;
+          *reinterpret_cast<uint2*>(dst) = make_uint2(hi[0], hi[1]);
+          *reinterpret_cast<uint2*>(dst + L::kOperand) = make_uint2(lo[0], lo[1]);
+        }
+      }
+      // a query that is not finite spoils its row
+      if (c == 0) factor[row] = top[k] >= 0x7f80u ? __int_as_float(0x7fffffff) : a.qscale * kv8::power(e - 7);
+    }
+  }
+  fence_proxy_async_smem();
+  __syncwarp();
 }
 
 template <int HD, int COPIES>
@@ -410,7 +522,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
               for (int c = 0; c < kHeld / 32; ++c) {
                 const int at = copy * NC + col + 32 * c;
                 uint32_t see = r < live ? seen32(a, s, token, slot0 + at) & low_bits(a.tile - at) : 0xffffffffu;
-                if (bad) see &= sound32(bad, at / 32, a.box);
+                if (bad) see &= sound32(bad, at, a.box);
                 if (__all_sync(0xffffffffu, see == 0xffffffffu)) continue;  // a prompt's chunks are mostly seen
 #pragma unroll
                 for (int e = 0; e < 32; ++e) {
@@ -532,7 +644,15 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
         if (lane == 0) mbar_arrive(&pfull[w]);
       }
 
-      finish_segment<L, HD>(a, smem, walk, s, slots, pvdone, abort_flag, tmem, w, copy, r, x, units, seg, i0, live, m, l);
+      // the groups' last mixes of the segment: of both where finish_segment reads both O, else of this one's
+      const int end = x + units;
+      const int last0 = end - 1 - ((end - 1) & 1), last1 = end - 1 - (~(end - 1) & 1);
+      const bool had0 = last0 >= x, had1 = last1 >= x;
+      constexpr bool kOwnOnly = DUAL || L::kCopies > 1;
+      if (had0 && (!kOwnOnly || w == 0)) warp_wait(&pvdone[0], (last0 >> 1) & 1, abort_flag, a.status);
+      if (had1 && (!kOwnOnly || w == 1)) warp_wait(&pvdone[1], (last1 >> 1) & 1, abort_flag, a.status);
+      tc_fence_after();
+      finish_segment<L, HD>(a, smem, walk, s, slots, tmem, w, copy, r, had0, had1, seg, i0, live, m, l);
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(ofree);
@@ -548,56 +668,49 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
 }
 
 template <int HD, int COPIES>
-int launch_form(TreeArgs a, int nc, cudaStream_t stream, const char* what) {
+int launch_form(TreeArgs a, cudaStream_t stream, const char* what) {
   using L = Layout8<HD, COPIES>;
+  tile_of(a.page_size, &a.tile, &a.box);
   const uint64_t rows = static_cast<uint64_t>(a.num_pages) * a.hkv * a.page_size;
   CUtensorMap tk, tv;
   if (int st = make_tensor_map_bytes(&tk, a.k_pages, a.hd, rows, HD, a.box, what)) return st;
   if (int st = make_tensor_map_bytes(&tv, a.v_pages, a.hd, rows, HD, a.box, what)) return st;
   auto kernel = tree_tc8_kernel<HD, COPIES>;
   if (int st = allow_dynamic_smem(reinterpret_cast<const void*>(kernel), L::kBytes, what)) return st;
-  a.whole = whole_items(a, L::kTiles * (kTile / a.group));
+  a.whole = whole_items(a, tokens_of(COPIES, a.group));
+  const int nc = ctas_for(a.batch, a.hkv, a.group, a.max_ctx, a.max_tree);
   if (int st = launch_kernel(what, kernel, dim3(nc), dim3(kThreadsTc), L::kBytes, stream, nullptr, tk, tv, a)) return st;
   if (nc == 1 || a.whole) return BM_OK;  // no item is cut
   return launch_kernel(what, tree_merge_kernel<L, HD>, dim3(nc - 1, std::min(L::kRows / 8, 8)), dim3(256), 0, stream, nullptr, a, nc);
 }
 
-// Whether the rows that the bounds allow fit one row tile of 128.
-bool one_tile(int group, int max_tree) { return max_tree <= kTile / group; }
-// Rows, and tokens, of an item in the form for the bounds.
-int rows8(int group, int max_tree) {
-  if (few8_takes(group, max_tree)) return max_tree <= 32 / group ? 32 : 64;
-  return one_tile(group, max_tree) ? kTile : 2 * kTile;
-}
-int tokens8(int group, int max_tree) {
-  if (few8_takes(group, max_tree)) return (max_tree <= 32 / group ? 1 : 2) * (32 / group);
-  return (one_tile(group, max_tree) ? 1 : 2) * (kTile / group);
+template <int HD>
+int launch_hd(const TreeArgs& a, cudaStream_t stream, const char* what) {
+  switch (copies_for(a.group, a.max_tree)) {
+    case 4:
+      return launch_form<HD, 4>(a, stream, what);
+    case 2:
+      return launch_form<HD, 2>(a, stream, what);
+    case 1:
+      return launch_form<HD, 1>(a, stream, what);
+    default:
+      return launch_form<HD, kDual>(a, stream, what);
+  }
 }
 
 }  // namespace
 
-// The few-row form takes blocks of any size. The other one wants eight neighbouring slots of a tile,
-// from its beginning on, to share a scale: blocks and boxes of whole eights, or a tile that is one
-// part of a page inside one block.
+// Eight neighbouring slots of a tile, from its beginning on, share a scale: blocks and boxes of whole
+// eights, or a tile that is one part of a page inside one block.
 bool tc8_takes(const TreeArgs& a, bm_dtype_t dtype) {
   const int64_t rows = static_cast<int64_t>(a.num_pages) * a.hkv * a.page_size;
   int tile, box;
-  if (dtype != BM_BF16 || a.hd > 128 || !tile_of(a.page_size, &tile, &box) || rows + kTile >= (int64_t{1} << 31)) return false;
-  return few8_takes(a.group, a.max_tree) || (a.block % kGroupSlots == 0 && box % kGroupSlots == 0) || (tile == box && a.block % box == 0);
+  return dtype == BM_BF16 && a.hd <= 128 && tile_of(a.page_size, &tile, &box) && rows + kTile < (int64_t{1} << 31) &&
+         ((a.block % kGroupSlots == 0 && box % kGroupSlots == 0) || (tile == box && a.block % box == 0));
 }
 
-size_t tc8_workspace_bytes(int64_t batch, int hkv, int hd, int group, int max_ctx, int max_tree) {
-  if (hd > 128 || hd % 16) return 0;
-  const int nc = ctas_of(batch, hkv, tokens8(group, max_tree), max_ctx, max_tree);
-  return records_bytes(nc) + 2 * static_cast<size_t>(nc) * rows8(group, max_tree) * ((hd <= 64 ? 64 : 128) + 2) * sizeof(float);
-}
-
-int launch_tc8(TreeArgs a, cudaStream_t stream, const char* what) {
-  tile_of(a.page_size, &a.tile, &a.box);
-  const int nc = ctas_of(a.batch, a.hkv, tokens8(a.group, a.max_tree), a.max_ctx, a.max_tree);
-  if (few8_takes(a.group, a.max_tree)) return launch_few8(a, nc, stream, what);
-  if (one_tile(a.group, a.max_tree)) return a.hd > 64 ? launch_form<128, 1>(a, nc, stream, what) : launch_form<64, 1>(a, nc, stream, what);
-  return a.hd > 64 ? launch_form<128, kDual>(a, nc, stream, what) : launch_form<64, kDual>(a, nc, stream, what);
+int launch_tc8(const TreeArgs& a, cudaStream_t stream, const char* what) {
+  return a.hd > 64 ? launch_hd<128>(a, stream, what) : launch_hd<64>(a, stream, what);
 }
 
 }  // namespace paged

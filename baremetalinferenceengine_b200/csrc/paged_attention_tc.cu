@@ -389,7 +389,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
               for (int c = 0; c < kHeld / 32; ++c) {
                 const int at = copy * NC + col + 32 * c;
                 uint32_t see = r < live ? seen32(a, s, token, slot0 + at) & low_bits(a.tile - at) : 0xffffffffu;
-                if (bad) see &= sound32(bad, at / 32, a.box);
+                if (bad) see &= sound32(bad, at, a.box);
                 if (__all_sync(0xffffffffu, see == 0xffffffffu)) continue;  // a prompt's chunks are mostly seen
 #pragma unroll
                 for (int e = 0; e < 32; ++e) {
@@ -489,7 +489,15 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
         if (lane == 0) mbar_arrive(&pfull[w]);
       }
 
-      finish_segment<L, HD>(a, smem, walk, s, slots, pvdone, abort_flag, tmem, w, copy, r, x, units, seg, i0, live, m, l);
+      // the groups' last mixes of the segment: of both where finish_segment reads both O, else of this one's
+      const int end = x + units;
+      const int last0 = end - 1 - ((end - 1) & 1), last1 = end - 1 - (~(end - 1) & 1);
+      const bool had0 = last0 >= x, had1 = last1 >= x;
+      constexpr bool kOwnOnly = DUAL || L::kCopies > 1;
+      if (had0 && (!kOwnOnly || w == 0)) warp_wait(&pvdone[0], (last0 >> 1) & 1, abort_flag, a.status);
+      if (had1 && (!kOwnOnly || w == 1)) warp_wait(&pvdone[1], (last1 >> 1) & 1, abort_flag, a.status);
+      tc_fence_after();
+      finish_segment<L, HD>(a, smem, walk, s, slots, tmem, w, copy, r, had0, had1, seg, i0, live, m, l);
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(ofree);

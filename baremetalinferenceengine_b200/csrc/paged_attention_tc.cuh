@@ -195,12 +195,12 @@ __device__ __forceinline__ uint32_t seen32(const TreeArgs& a, const Seq& s, int 
   return v;
 }
 
-// Which of the 32 slots at column 32c of a tile have a sound page (bit b of bad: the
+// Which of the 32 slots from slot `at` of a tile on have a sound page (bit b of bad: the
 // tile's box b has not). Two boxes or more hold whole groups of 8 slots each.
-__device__ __forceinline__ uint32_t sound32(uint32_t bad, int c, int box_rows) {
+__device__ __forceinline__ uint32_t sound32(uint32_t bad, int at, int box_rows) {
   uint32_t v = 0xffffffffu;
   for (int e = 0; e < 32; e += 8) {
-    if ((bad >> min((32 * c + e) / box_rows, 31)) & 1) v &= ~(0xffu << e);
+    if ((bad >> min((at + e) / box_rows, 31)) & 1) v &= ~(0xffu << e);
   }
   return v;
 }
@@ -289,11 +289,12 @@ __device__ __forceinline__ bool plan_share(const TreeArgs& a, int per, int64_t* 
 
 // A segment's end, by the softmax threads: sums out of TMEM, to out (whole item) or to a
 // partial. Group w's thread for row r of the row tile (and copy) has the running maximum m and sum
-// l of its units among [x, x + units); L is the kernel's layout.
+// l of its units; had0 and had1 tell which groups had some (O of the other is stale), and their mixes are
+// done. L is the kernel's layout.
 template <typename L, int HD>
 __device__ __forceinline__ void finish_segment(const TreeArgs& a, unsigned char* smem, const Walk& walk, const Seq& s, float* slots,
-                                               uint64_t* pvdone, volatile int* abort_flag, uint32_t tmem, int w, int copy, int r,
-                                               int x, int units, int seg, int i0, int live, float m, float l) {
+                                               uint32_t tmem, int w, int copy, int r, bool had0, bool had1, int seg, int i0,
+                                               int live, float m, float l) {
   const int tid = threadIdx.x, lane = tid & 31, quarter = (tid >> 5) & 3;
   const bool warp_live = r - lane < live;
   const int token = i0 + r / a.group;
@@ -302,12 +303,9 @@ __device__ __forceinline__ void finish_segment(const TreeArgs& a, unsigned char*
   float2* ml = reinterpret_cast<float2*>(smem + L::kOffMl);
   const bool whole = walk.t == 0 && walk.segment() == walk.tiles;
   float* slot = slots + (2 * static_cast<int64_t>(blockIdx.x) + (seg > 0)) * L::kSlotFloats;
-  const int end = x + units;
   const int h = r - (r / a.group) * a.group;
   bf16* out = static_cast<bf16*>(a.out) + ((s.row0 + token) * a.hq + walk.kvh * a.group + h) * a.hd;
   if constexpr (L::kTwo) {
-    warp_wait(&pvdone[w], ((end - 2 + w) >> 1) & 1, abort_flag, a.status);
-    tc_fence_after();
     const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
     if (warp_live) {
 #pragma unroll
@@ -352,10 +350,7 @@ __device__ __forceinline__ void finish_segment(const TreeArgs& a, unsigned char*
       sum = fmaf(part.y, ex2(part.x - base), sum);  // a maximum of -inf: 0
     }
     const float inv = !whole ? 1.f : sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
-    const int last = end - 1 - ((end - 1 - w) & 1);  // this group's last unit; none: its O is stale
-    const bool had = last >= x && warp_live;
-    if (last >= x) warp_wait(&pvdone[w], (last >> 1) & 1, abort_flag, a.status);
-    tc_fence_after();
+    const bool had = (w == 0 ? had0 : had1) && warp_live;
     const float f = m == -INFINITY || r >= live ? 0.f : ex2(m - base) * inv;
     float* acc = reinterpret_cast<float*>(smem + L::kOffSum);
     for (int d0 = 0; d0 < HD; d0 += L::kDims) {
@@ -417,25 +412,21 @@ __device__ __forceinline__ void finish_segment(const TreeArgs& a, unsigned char*
     ml[((seg & 1) * 2 + w) * kTile + r] = make_float2(m, l);
     both_groups_sync();
     const float2 other = ml[((seg & 1) * 2 + (w ^ 1)) * kTile + r];
-    const int last0 = end - 1 - ((end - 1) & 1), last1 = end - 1 - (~(end - 1) & 1);  // last units of groups 0, 1
-    if (last0 >= x) warp_wait(&pvdone[0], (last0 >> 1) & 1, abort_flag, a.status);
-    if (last1 >= x) warp_wait(&pvdone[1], (last1 >> 1) & 1, abort_flag, a.status);
-    tc_fence_after();
     if (warp_live) {
       const float top = fmaxf(m, other.x), base = top == -INFINITY ? 0.f : top;
       const float own_f = m == -INFINITY ? 0.f : ex2(m - base), other_f = other.x == -INFINITY ? 0.f : ex2(other.x - base);
       const float sum = l * own_f + other.y * other_f;
       const float inv = !whole ? 1.f : sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
       const float f0 = (w == 0 ? own_f : other_f) * inv, f1 = (w == 0 ? other_f : own_f) * inv;
-      const bool two = last0 >= x && last1 >= x;  // otherwise one group had no unit and its O is stale
+      const bool two = had0 && had1;
 #pragma unroll
       for (int c = 0; c < HD / 64; ++c) {
         const int col = w * (HD / 2) + 32 * c;
         uint32_t v[32];
         float f[32];
-        tmem_load32(tmem + lane_addr + L::kColO + (last0 >= x ? 0 : HD) + col, v);
+        tmem_load32(tmem + lane_addr + L::kColO + (had0 ? 0 : HD) + col, v);
         tmem_wait_ld();
-        const float fa = last0 >= x ? f0 : f1;
+        const float fa = had0 ? f0 : f1;
 #pragma unroll
         for (int e = 0; e < 32; ++e) f[e] = fa == 0.f ? 0.f : __uint_as_float(v[e]) * fa;
         if (two) {
@@ -490,7 +481,7 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(const TreeArgs a, int c
   const int skip = border(k - 1) != first;  // in the first CTA the item is not the first segment
   auto part = [&](int c) { return slots + (2 * static_cast<int64_t>(c) + (c == k - 1 ? skip : 0)) * L::kSlotFloats; };
   for (int r = static_cast<int>(blockIdx.y) * 8 + threadIdx.x / 32; r < L::kRows; r += 8 * gridDim.y) {
-    const int tile = r / L::kCopyRows, rr = r - tile * L::kCopyRows;
+    const int tile = r / kTile, rr = r - tile * kTile;
     const int i0 = rec.p * tpt * L::kTiles + tile * tpt;
     if (rr >= max(0, min(tpt, s.n - i0)) * a.group) continue;
     // the first parts' maxima, sums and values at once: two parts are all there is, mostly
@@ -583,15 +574,13 @@ inline bool tile_of(int page_size, int* tile, int* box) {
   return *tile >= kTile / 2;
 }
 
-// CTAs for the bounds and items of `per` tokens: one per SM, no more than the tiles there can be (a tile holds at
+// CTAs for the bounds: one per SM, no more than the tiles there can be (a tile holds at
 // least half of 128 slots).
-inline int ctas_of(int64_t batch, int hkv, int per, int max_ctx, int max_tree) {
+inline int ctas_for(int64_t batch, int hkv, int group, int max_ctx, int max_tree) {
+  const int per = tokens_of(copies_for(group, max_tree), group);
   const int64_t tiles = batch * hkv * ((max_tree + per - 1) / per) *
                         ((static_cast<int64_t>(max_ctx) + max_tree + kTile / 2 - 1) / (kTile / 2));
   return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(sm_count(), tiles)));
-}
-inline int ctas_for(int64_t batch, int hkv, int group, int max_ctx, int max_tree) {
-  return ctas_of(batch, hkv, tokens_of(copies_for(group, max_tree), group), max_ctx, max_tree);
 }
 
 // Whole items up to kWholeTiles tiles where they make CTAs for a quarter of the SMs or more

@@ -61,6 +61,21 @@ __device__ __forceinline__ void rotate(float* x, const float2* cs) {
     rope_rotate(x[a], x[b], cs[e], &x[a], &x[b]);
   }
 }
+// The same for half pairs, two to an instruction (N even): rope_rotate's roundings, since a product with -s is
+// the negative of the one with s.
+template <int N>
+__device__ __forceinline__ void rotate2(float* x, const float2* cs) {
+#pragma unroll
+  for (int e = 0; e < N; e += 2) {
+    const uint64_t a = pair(x[e], x[e + 1]), b = pair(x[N + e], x[N + e + 1]), c = pair(cs[e].x, cs[e + 1].x);
+    const float2 first = unpair(fma2(a, c, mul2(b, pair(-cs[e].y, -cs[e + 1].y))));
+    const float2 second = unpair(fma2(b, c, mul2(a, pair(cs[e].y, cs[e + 1].y))));
+    x[e] = first.x;
+    x[e + 1] = first.y;
+    x[N + e] = second.x;
+    x[N + e + 1] = second.y;
+  }
+}
 template <typename T, int N, bool INTER>
 __device__ __forceinline__ void rotate(Piece<T, N>& p1, Piece<T, N>& p2, const float2* cs) {
   float x[2 * N];
