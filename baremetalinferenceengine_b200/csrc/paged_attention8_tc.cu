@@ -4,25 +4,33 @@
 // Mathematics: the running softmax of paged_attention.cu on tiles of 128 slots, K and V as the
 // codes they are held in: nothing is widened on its way to the tensor cores.
 //   scores  S[row][slot] = (Qh + Ql)[row][:] . Kc[slot][:]    two e4m3 x e4m3 products
-//   mix     O[row][:]   += (Ph + Pl)[row][slot] Vc[slot][:]   e4m3 x e4m3 and e5m2 x e4m3
+//   mix     O[row][:]   += (Ph + Pl)[row][slot] Vc[slot][:]   e5m2 x e4m3 and e4m3 x e4m3
 // Qh is the query times a power of two that puts its largest element in [128, 256), rounded to
 // e4m3, and Ql what that leaves: together all 8 bits of a bf16 element down to 2^-9 of the largest, and
 // 2^-17 of the largest below. Scales are powers of two, so they meet the softmax as exponents:
-//   t = S f + e_v,  f = 2^(e_k - e_q) scale log2(e),  P = 2^(t - m + 2),  l += P 2^(-e_v)
+//   t = S f + e_v,  f = 2^(e_k - e_q) scale log2(e),  P = 2^(t - m + 6),  l += P 2^(-e_v)
 // with e_k and e_v the exponents of K's and V's scale at the slot, e_q the query's and m the running maximum
 // of t: the weight times V's scale is what the mix takes, so its rounding is relative to the
-// largest term of the sum, however far blocks' scales lie apart. P is at most 2^8 (a row is rescaled when m rises by more than 6); as
-// fp16 it splits into Ph (e4m3) and Pl = P - Ph (e5m2, whose exponents reach down to 2^-16): off by 2^-8 of itself
-// at most, by 2^-16 of the largest where it is small: the precision of bf16 weights, for two products of
-// twice bf16's rate.
+// largest term of the sum, however far blocks' scales lie apart. P is at most 2^12 (a row is rescaled when m rises by
+// more than 6). As fp16 it splits into Ph, e5m2 and so the upper byte of the fp16 value, rounded, and Pl = P - Ph as
+// e4m3, at most 2^8 and in steps of 2^-9 at least: off by 2^-8 of itself at most, by 2^-16 of the largest where it is
+// small. That is the precision of bf16 weights, for two products of twice bf16's rate. (The other way round, e4m3
+// first, takes two conversions more.)
 //
-// Bound: memory while group * tokens is below about 100 (a slot is half the bytes of a bf16
-// cache's, for the same tensor time), above it the softmax: exponentials, and the conversions of P.
+// Bound: memory while group * tokens is below about 100 (a slot is half the bytes of a bf16 cache's, for the same
+// tensor time), above it the products. What it takes is neither: it is the chain scores, softmax, weights, mix of each
+// row tile, whose waits two groups of warps leave open (counters of 64 tokens at group 8: tensor pipe 20 % of its
+// cycles, conversions and exponentials 21 %, issue slots 35 %), and for few rows the ends of segments.
+// Measured, heads of 128, 8 kv heads: 1 sequence, 12 tokens at group 4 over 8000 slots 31 us; 64 ragged sequences of up
+// to 8192 slots, 8 tokens at group 4 207 us (2.5 TB/s of codes); 16 sequences of 4096 to 8192 slots, 64 tokens at group 8
+// 361 us (553 TFLOP/s of the formula's products; with one issuer for both groups and whole tiles 402, with parts for
+// few rows too 217 and 34 in the first two).
 //
-// Split and roles are paged_attention_tc.cu's, but for the queries and the scales: warp 2 converts a
-// segment's queries into two operands in shared memory while the segment before is computed (all
-// warps but those of TMA together for a CTA's first, which all wait for), and the warp that fetches K looks up
-// the scales of its tile's slots, eight neighbouring ones of which share one.
+// Split and roles are paged_attention_tc.cu's, but for the queries, the scales and the MMAs. The warp that fetches V
+// converts a segment's queries into two operands in shared memory, some rows between two tiles, while the segment before
+// is computed (all warps but those of TMA together for a CTA's first, which all wait for). The warp that fetches K
+// looks up the scales of its tile's slots, eight neighbouring ones of which share one. Each softmax group has an MMA
+// issuer of its own (warps 1 and 2).
 #include <cuda.h>
 
 #include "kv8.cuh"
@@ -33,15 +41,20 @@ namespace paged {
 namespace {
 
 constexpr float kRescaleAt8 = 6.f;  // rise of the maximum (log2) that a row's sums are rescaled at
-constexpr float kLift = 2.f;        // P is 2^2 at the running maximum, so at most 2^8
+constexpr float kLift = 6.f;        // P is 2^6 at the running maximum, so at most 2^12: Pl ends at 2^8
 constexpr int kGroupSlots = 8;      // slots of a tile that share a scale
 constexpr int kGroups = kTile / kGroupSlots;
+constexpr int kConvert = 8;         // pairs of rows of the next queries that are converted between two tiles
 constexpr int kQRing = 4;           // segments whose queries' factors are kept
 constexpr int kQWarps = 10;         // warps that convert a CTA's first queries: all but the two of TMA
 
 template <int HD, int COPIES>
 struct Layout8 : RowLayout<HD, COPIES> {
   using Rows = RowLayout<HD, COPIES>;
+  // Scores and mixes are issued for parts of a tile, each with TMEM columns of its own: where rows fill a tile a group
+  // weighs one part while the other's mix and the next unit's scores are computed; copies' tiles wait for memory.
+  static constexpr int kParts = Rows::kCopies > 1 ? 1 : 2;
+  static constexpr int kPart = kTile / kParts;              // slots
   static constexpr int kOperand = kTile * HD;               // a tile of K or V, one part of Q
   static constexpr int kQTile = 2 * kOperand;               // both parts of a row tile
   static constexpr int kQBuf = Rows::kTiles * kQTile;       // of two: a segment's, and the next one's
@@ -54,12 +67,12 @@ struct Layout8 : RowLayout<HD, COPIES> {
   static constexpr int kOffScale = kOffSum + Rows::kSumBytes;  // [kBadRing][kGroups] (f of K, e_v, 2^-e_v, -)
   static constexpr int kOffFactor = kOffScale + kBadRing * kGroups * 16;  // [kQRing][rows]
   static constexpr int kOffBar = kOffFactor + kQRing * Rows::kRows * 4;
-  static constexpr int kBars = 2 * kKS + 2 * kVS + 6 + 6;
+  static constexpr int kBars = 2 * kKS + 2 * kVS + 12 + 7;
   static constexpr int kOffPlan = kOffBar + kBars * 8;      // Plan, scan, bad-page ring
   static constexpr int kBytes = kOffPlan + 96 + 16 * 8 + kBadRing * 4 + 16 + 1024 /* alignment slack */;
   static_assert(kBytes <= 232448, "shared memory of a CTA");
   // Tiles between the one whose scores are issued next and the one a softmax group may still read.
-  static_assert(kKS + 4 <= kBadRing, "rings by tile");
+  static_assert(kKS + 6 <= kBadRing, "rings by tile");
 };
 
 // Instruction descriptors for kind::f8f6f4 with an fp32 accumulator: A e4m3 or e5m2, B e4m3.
@@ -91,12 +104,30 @@ __device__ __forceinline__ void mma_f8_ts(uint32_t d_tmem, uint32_t a_tmem, uint
       ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
-// 8 consecutive 32-bit columns of this thread's TMEM lane.
-__device__ __forceinline__ void tmem_store8(uint32_t taddr, const uint32_t (&r)[8]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};" ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]),
-      "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(taddr)
-      : "memory");
+// N consecutive 32-bit columns of this thread's TMEM lane.
+template <int N>
+__device__ __forceinline__ void tmem_load_n(uint32_t taddr, uint32_t (&r)[N]) {
+  if constexpr (N == 32) {
+    tmem_load32(taddr, r);
+  } else {
+    static_assert(N == 16, "columns");
+    tmem_load16(taddr, r);
+  }
+}
+template <int N>
+__device__ __forceinline__ void tmem_store_n(uint32_t taddr, const uint32_t (&r)[N]) {
+  if constexpr (N == 16) {
+    tmem_store16(taddr, r);
+  } else if constexpr (N == 8) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};" ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]),
+        "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(taddr)
+        : "memory");
+  } else {
+    static_assert(N == 4, "columns");
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%4], {%0, %1, %2, %3};" ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(taddr)
+                 : "memory");
+  }
 }
 // The phase's bytes to come, without an arrival.
 __device__ __forceinline__ void mbar_expect_only(uint64_t* bar, uint32_t bytes) {
@@ -112,39 +143,43 @@ __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
   return r;
 }
-// Two weights: e4m3 of their fp16 values, and e5m2 of what that leaves.
-__device__ __forceinline__ void weight_parts(float lo, float hi, uint32_t* part, uint32_t* rest) {
-  uint32_t p, back;
-  uint16_t h, l;
-  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(p) : "f"(hi), "f"(lo));
-  asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(h) : "r"(p));
-  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(back) : "h"(h));
-  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(back) : "r"(p), "r"(back));
-  asm("cvt.rn.satfinite.e5m2x2.f16x2 %0, %1;" : "=h"(l) : "r"(back));
-  *part = h;
-  *rest = l;
+// Four weights: e5m2 of their fp16 values, which is the upper byte of such a value, rounded, and e4m3 of what that
+// leaves. Weights are not negative; one that is NaN leaves NaN.
+__device__ __forceinline__ void weight_parts(float p0, float p1, float p2, float p3, uint32_t* part, uint32_t* rest) {
+  uint32_t p01, p23, r01, r23;
+  uint16_t l01, l23;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(p01) : "f"(p1), "f"(p0));
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(p23) : "f"(p3), "f"(p2));
+  const uint32_t h01 = p01 + 0x00800080u, h23 = p23 + 0x00800080u;
+  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r01) : "r"(p01), "r"(h01 & 0xff00ff00u));
+  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r23) : "r"(p23), "r"(h23 & 0xff00ff00u));
+  asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(l01) : "r"(r01));
+  asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(l23) : "r"(r23));
+  *part = __byte_perm(h01, h23, 0x7531);
+  *rest = l01 | static_cast<uint32_t>(l23) << 16;
 }
 
 // Converts the queries of an item into its two parts in the buffer at `to`, row tile after row
 // tile, copies and all, and their factors scale * log2(e) * 2^-e_q into factor[row]. Warp
-// `worker` of `workers` takes every workers-th pair of rows, half a warp a row; rows of no token are zero.
+// `worker` of `workers` takes every workers-th pair of rows of [from, until), half a warp a row; rows of no
+// token are zero.
 template <typename L, int HD>
 __device__ __forceinline__ void convert_queries(const TreeArgs& a, const Seq& s, int kvh, int p, int tpt, unsigned char* to, float* factor,
-                                                int worker, int workers) {
+                                                int worker, int workers, int from, int until) {
   constexpr int kBatch = 4;  // pairs of rows that are converted side by side
   const int lane = threadIdx.x & 31, half = lane >> 4, c = lane & 15;
   const int i_first = p * tpt * L::kTiles;
   const uint32_t by_group = (65536u + a.group - 1) / a.group;  // r / group = r * by_group >> 16 for r < 128
   const bf16* q = static_cast<const bf16*>(a.q) + (s.row0 * a.hq + static_cast<int64_t>(kvh) * a.group) * a.hd + c * 8;
   const int64_t token_step = static_cast<int64_t>(a.hq) * a.hd;
-  for (int pair0 = worker; pair0 < L::kRows / 2; pair0 += workers * kBatch) {
+  for (int pair0 = from + worker; pair0 < until; pair0 += workers * kBatch) {
     uint4 raw[kBatch];
 #pragma unroll
     for (int k = 0; k < kBatch; ++k) {
       const int row = 2 * (pair0 + k * workers) + half, r = row % L::kCopyRows;
       const int token = static_cast<int>(r * by_group >> 16), i = i_first + row / L::kCopyRows * tpt + token;
       raw[k] = make_uint4(0u, 0u, 0u, 0u);
-      if (row < L::kRows && token < tpt && i < s.n && c * 8 < a.hd) raw[k] = ld_keep(q + i * token_step + (r - token * a.group) * a.hd);
+      if (row < 2 * until && token < tpt && i < s.n && c * 8 < a.hd) raw[k] = ld_keep(q + i * token_step + (r - token * a.group) * a.hd);
     }
     uint32_t top[kBatch];
 #pragma unroll
@@ -162,7 +197,7 @@ __device__ __forceinline__ void convert_queries(const TreeArgs& a, const Seq& s,
 #pragma unroll
     for (int k = 0; k < kBatch; ++k) {
       const int row = 2 * (pair0 + k * workers) + half, r = row % L::kCopyRows;
-      if (row >= L::kRows) continue;
+      if (row >= 2 * until) continue;
       const int e = min(max(static_cast<int>(top[k] >> 7) - 127, -60), 127);
       const float f = kv8::power(7 - e);
       if (c * 8 < HD) {
@@ -201,9 +236,9 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
   grid_dependency_wait();
   using L = Layout8<HD, COPIES>;
   constexpr bool DUAL = L::kTwo;
-  constexpr uint32_t kIdescS = instr_desc_e4m3(false, false, kTile, kTile);
-  constexpr uint32_t kIdescH = instr_desc_e4m3(false, true, HD, kTile);
-  constexpr uint32_t kIdescL = instr_desc_e4m3(true, true, HD, kTile);
+  constexpr uint32_t kIdescS = instr_desc_e4m3(false, false, L::kPart, kTile);
+  constexpr uint32_t kIdescH = instr_desc_e4m3(true, true, HD, kTile);
+  constexpr uint32_t kIdescL = instr_desc_e4m3(false, true, HD, kTile);
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                                          ~static_cast<uintptr_t>(1023));
@@ -216,13 +251,14 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
   uint64_t* kempty = kfull + L::kKS;
   uint64_t* vfull = kempty + L::kKS;
   uint64_t* vempty = vfull + L::kVS;
+  // of group w's part h of a unit, at kParts w + h:
   uint64_t* sfull = vempty + L::kVS;    // scores in TMEM       (commit)
-  uint64_t* pfull = sfull + 2;          // weights in TMEM      (one arrival per warp of the group)
-  uint64_t* pvdone = pfull + 2;         // mix done             (commit)
-  uint64_t* qfull = pvdone + 2;         // queries converted    (kQWarps arrivals)
-  uint64_t* qempty = qfull + 2;         // the segment's last scores are done (commit)
+  uint64_t* pfull = sfull + 4;          // weights in TMEM      (one arrival per warp of the group)
+  uint64_t* pvdone = pfull + 4;         // mix done             (commit)
+  uint64_t* qfull = pvdone + 4;         // queries converted    (kQWarps arrivals)
+  uint64_t* qempty = qfull + 2;         // each group's last scores of the segment are done (two commits)
   uint64_t* ofree = qempty + 2;         // the segment's O has been read (one arrival per softmax warp)
-  uint64_t* mma_done = ofree + 1;
+  uint64_t* mma_done = ofree + 1;      // of each issuer
   Plan* plan = reinterpret_cast<Plan*>(smem + L::kOffPlan);
   int64_t* scan = reinterpret_cast<int64_t*>(smem + L::kOffPlan + 96);
   volatile uint32_t* bad_ring = reinterpret_cast<volatile uint32_t*>(scan + 16);
@@ -241,21 +277,23 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
     if (tid == 0) {
       for (int i = 0; i < L::kKS; ++i) {
         mbar_init(&kfull[i], 1);
-        mbar_init(&kempty[i], 1);
+        mbar_init(&kempty[i], L::kTiles);  // read for each row tile
       }
       for (int i = 0; i < L::kVS; ++i) {
         mbar_init(&vfull[i], 1);
-        mbar_init(&vempty[i], 1);
+        mbar_init(&vempty[i], L::kTiles);
       }
-      for (int i = 0; i < 2; ++i) {
+      for (int i = 0; i < 4; ++i) {
         mbar_init(&sfull[i], 1);
         mbar_init(&pfull[i], 4);
         mbar_init(&pvdone[i], 1);
+      }
+      for (int i = 0; i < 2; ++i) {
         mbar_init(&qfull[i], kQWarps);
-        mbar_init(&qempty[i], 1);
+        mbar_init(&qempty[i], 2);
+        mbar_init(&mma_done[i], 1);
       }
       mbar_init(ofree, 8);
-      mbar_init(mma_done, 1);
       *abort_flag = 0;
       fence_barrier_init();
     }
@@ -281,13 +319,13 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
   }
   if (warp != 0 && warp != 3) {
     const int worker = warp < 3 ? warp - 1 : warp - 2;
-    convert_queries<L, HD>(a, walk.s, walk.kvh, walk.p, tpt, smem, factors, worker, kQWarps);
+    convert_queries<L, HD>(a, walk.s, walk.kvh, walk.p, tpt, smem, factors, worker, kQWarps, 0, L::kRows / 2);
     if (lane == 0) mbar_arrive(&qfull[0]);
     __syncwarp();
   }
 
   if (warp == 0 || warp == 3) {
-    // ---------------- K with the scales (warp 0) and V (warp 3) ----------------
+    // ---------------- K with the scales (warp 0), V and the next segment's queries (warp 3) ----------------
     // Lanes 0 to 15 each fetch a box of the tile; warp 0's others look up the scales of eight slots
     // each, one step ahead, and their pages two.
     const bool is_v = warp == 3;
@@ -302,7 +340,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
     int kt = 0, stage = 0;               // tiles asked for; the next one's ring slot
     uint32_t phase = 1;
     bool ok = true;
-    for (; ok && walk.left > 0; walk.next(a, per)) {
+    for (int seg = 0; ok && walk.left > 0; walk.next(a, per), ++seg) {
       const int n = walk.segment();
       const int32_t* pages = a.page_table + static_cast<int64_t>(walk.s.seq) * a.max_pages;
       const int total = walk.s.ctx + walk.s.n, t0 = walk.t, kvh = walk.kvh;
@@ -324,6 +362,11 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
         *k = __ldg(a.k_scales + at);
         *v = __ldg(a.v_scales + at);
       };
+      // the next segment's queries, whose buffer is the segment before's
+      Walk ahead = walk;
+      if (is_v) ahead.next(a, per);
+      const bool converts = is_v && ahead.left > 0;
+      int pairs = 0;  // of their rows converted
       int row = row_of(0), row1 = scaler ? row_of(1) : -2;
       uint32_t k, v;
       scales_of(row, &k, &v);
@@ -365,6 +408,17 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
         row1 = next;
         k = k1;
         v = v1;
+        if (converts) {  // a few rows at a time, so that V's ring stays full
+          if (pairs == 0 && !(ok = warp_wait(&qempty[(seg + 1) & 1], (((seg + 1) >> 1) & 1) ^ 1u, abort_flag, a.status))) break;
+          const int until = i + 1 < n ? min(pairs + kConvert, L::kRows / 2) : L::kRows / 2;
+          if (pairs < until) {
+            convert_queries<L, HD>(a, ahead.s, ahead.kvh, ahead.p, tpt, smem + ((seg + 1) & 1) * L::kQBuf,
+                                   factors + (seg + 1) % kQRing * L::kRows, 0, 1, pairs, until);
+            if (until == L::kRows / 2 && lane == 0) mbar_arrive_n(&qfull[(seg + 1) & 1], kQWarps);
+            __syncwarp();
+          }
+          pairs = until;
+        }
       }
     }
     if (lane == 0) {  // copies still in flight land before the CTA ends
@@ -373,121 +427,113 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
       }
     }
     __syncwarp();
-  } else if (warp == 2) {
-    // ---------------- the queries of the segments behind the first, one ahead ----------------
-    int seg = 0;
-    for (walk.next(a, per); walk.left > 0; walk.next(a, per)) {
-      ++seg;
-      const int buf = seg & 1;
-      if (!warp_wait(&qempty[buf], ((seg >> 1) & 1) ^ 1u, abort_flag, a.status)) break;
-      convert_queries<L, HD>(a, walk.s, walk.kvh, walk.p, tpt, smem + buf * L::kQBuf, factors + seg % kQRing * L::kRows, 0, 1);
-      if (lane == 0) mbar_arrive_n(&qfull[buf], kQWarps);
-      __syncwarp();
-    }
-  } else if (warp == 1) {
-    // ---------------- MMA issuer ----------------
-    // Step x: the mix of unit x - 2, then the scores of unit x into the TMEM buffer that
-    // mix has done with. The whole warp walks, one thread issues.
+  } else if (warp == 1 || warp == 2) {
+    // ---------------- MMA issuers, one for each group ----------------
+    // Of a segment's units group w has every other one, from unit w on. The whole warp walks, one thread issues.
+    const int w = warp == 1 ? 0 : 1;
     const uint64_t q_desc = byte_desc<HD>(smem_u32(smem));
     const uint64_t k_desc = byte_desc<HD>(smem_u32(smem + L::kOffK));
     const uint64_t v_desc = byte_desc<HD>(smem_u32(smem + L::kOffV));
-    constexpr uint32_t kStage = L::kOperand >> 4;
-    bool issued = false, ok = true, first = true;
-    int seg = 0, mix_seg = -1, end = -1;  // segments of the scores and of the mix; units in all, once known
-    int ks = 0, vs = 0;                   // ring slots of the next scores and mix
-    uint32_t k_phase = 0, v_phase = 0;
-    uint32_t firsts = 0;                  // bit i: unit x - 1 - i is its segment's first
-    int left = __shfl_sync(0xffffffffu, walk.segment(), 0) * L::kTiles;
-    for (int x = 0; ok; ++x) {
-      const int w = x & 1;
-      if (x >= 2) {
-        const bool opens = (firsts & 2) != 0;
-        if (opens) ++mix_seg;
-        ok = warp_wait(&pfull[w], ((x - 2) >> 1) & 1, abort_flag, a.status);
+    constexpr uint32_t kStage = L::kOperand >> 4, kPartRows = L::kPart * HD >> 4;
+    struct Place {
+      int u, units, tiles, seg;  // unit of the segment, units of it, tiles and segments before
+      uint32_t parity;           // of the group's units so far
+    };
+    auto tile_of_place = [&](const Place& p) { return p.tiles + (DUAL ? p.u >> 1 : p.u); };
+    // Moves on to the group's next unit from its segment on; false when there is none. `scores`: the walk of the
+    // scores, which owes an arrival for each segment without a unit of the group.
+    auto settle = [&](Place& p, Walk& at, bool scores) {
+      while (p.u >= p.units) {
+        if (scores && p.units <= w && lane == 0) mbar_arrive(&qempty[p.seg & 1]);
+        __syncwarp();
+        p.tiles += p.units / L::kTiles;
+        at.next(a, per);
+        if (__shfl_sync(0xffffffffu, at.left > 0 ? 1 : 0, 0) == 0) return false;
+        p.units = __shfl_sync(0xffffffffu, at.segment(), 0) * L::kTiles;
+        p.u = w;
+        ++p.seg;
+      }
+      return true;
+    };
+    bool ok = true;
+    auto score = [&](const Place& p, int h) {
+      const int buf = L::kParts * w + h, kt = tile_of_place(p), ks = kt % L::kKS, qbuf = p.seg & 1;
+      if (h == 0) {
+        if (p.u == w && !(ok = warp_wait(&qfull[qbuf], (p.seg >> 1) & 1, abort_flag, a.status))) return;
+        if (!(ok = warp_wait(&kfull[ks], (kt / L::kKS) & 1, abort_flag, a.status))) return;
+      }
+      // the last weights in these columns have been mixed (before the first: passes)
+      if (!(ok = warp_wait(&pvdone[buf], p.parity ^ 1u, abort_flag, a.status))) return;
+      tc_fence_after();
+      if (elect_one()) {
+        const uint64_t q_at = q_desc + ((qbuf * L::kQBuf + (DUAL ? w * L::kQTile : 0)) >> 4), k_at = k_desc + ks * kStage + h * kPartRows;
+#pragma unroll
+        for (int kk = 0; kk < HD / 32; ++kk) mma_f8(tmem + buf * L::kPart, q_at + kk * 2, k_at + kk * 2, kIdescS, kk > 0 ? 1u : 0u);
+#pragma unroll
+        for (int kk = 0; kk < HD / 32; ++kk) mma_f8(tmem + buf * L::kPart, q_at + kStage + kk * 2, k_at + kk * 2, kIdescS, 1u);
+        mma_commit(&sfull[buf]);
+        if (h == L::kParts - 1) {
+          mma_commit(&kempty[ks]);
+          if (p.u + 2 >= p.units) mma_commit(&qempty[qbuf]);
+        }
+      }
+      __syncwarp();
+    };
+    auto mix = [&](const Place& p, int h) {
+      const int buf = L::kParts * w + h, kt = tile_of_place(p), vs = kt % L::kVS;
+      if (!(ok = warp_wait(&pfull[buf], p.parity, abort_flag, a.status))) return;
+      if (h == 0) {
         // the segment's first mix overwrites O: its last reader was the previous segment's end
-        if (ok && opens && mix_seg > 0) ok = warp_wait(ofree, (mix_seg - 1) & 1, abort_flag, a.status);
-        if (ok) ok = warp_wait(&vfull[vs], v_phase, abort_flag, a.status);
-        if (!ok) break;
-        tc_fence_after();
-        if (elect_one()) {
-          const uint32_t fresh = (firsts & 6) != 0 ? 0u : 1u;  // the group's first unit of the segment
-          constexpr uint32_t kStep = 32 * HD >> 4;             // 32 slots of V
-#pragma unroll
-          for (int kk = 0; kk < kTile / 32; ++kk) {
-            mma_f8_ts(tmem + L::kColO + w * HD, tmem + w * kTile + kk * 8, v_desc + vs * kStage + kk * kStep, kIdescH, kk > 0 ? 1u : fresh);
-          }
-#pragma unroll
-          for (int kk = 0; kk < kTile / 32; ++kk) {
-            mma_f8_ts(tmem + L::kColO + w * HD, tmem + w * kTile + 32 + kk * 8, v_desc + vs * kStage + kk * kStep, kIdescL, 1u);
-          }
-          mma_commit(&pvdone[w]);
-          if (!DUAL || w == 1) mma_commit(&vempty[vs]);
-        }
-        __syncwarp();
-        issued = true;
-        if ((!DUAL || w == 1) && ++vs == L::kVS) {
-          vs = 0;
-          v_phase ^= 1;
-        }
+        if (p.u == w && p.seg > 0 && !(ok = warp_wait(ofree, (p.seg - 1) & 1, abort_flag, a.status))) return;
+        if (!(ok = warp_wait(&vfull[vs], (kt / L::kVS) & 1, abort_flag, a.status))) return;
       }
-      if (left > 0) {
-        const int buf = seg & 1;
-        if (first) ok = warp_wait(&qfull[buf], (seg >> 1) & 1, abort_flag, a.status);
-        if (ok) ok = warp_wait(&kfull[ks], k_phase, abort_flag, a.status);
-        if (ok && x >= 2) ok = warp_wait(&pvdone[w], ((x - 2) >> 1) & 1, abort_flag, a.status);
-        if (!ok) break;
-        tc_fence_after();
-        if (elect_one()) {
-          const uint64_t q_at = q_desc + ((buf * L::kQBuf + (DUAL ? w * L::kQTile : 0)) >> 4);
+      tc_fence_after();
+      if (elect_one()) {
+        const uint32_t o = tmem + L::kColO + w * HD, at = tmem + buf * L::kPart, fresh = p.u == w && h == 0 ? 0u : 1u;
+        const uint64_t v_at = v_desc + vs * kStage + h * kPartRows;
+        constexpr uint32_t kStep = 32 * HD >> 4;  // 32 slots of V
 #pragma unroll
-          for (int kk = 0; kk < HD / 32; ++kk) {
-            mma_f8(tmem + w * kTile, q_at + kk * 2, k_desc + ks * kStage + kk * 2, kIdescS, kk > 0 ? 1u : 0u);
-          }
+        for (int kk = 0; kk < L::kPart / 32; ++kk) mma_f8_ts(o, at + kk * 8, v_at + kk * kStep, kIdescH, kk > 0 ? 1u : fresh);
 #pragma unroll
-          for (int kk = 0; kk < HD / 32; ++kk) {
-            mma_f8(tmem + w * kTile, q_at + kStage + kk * 2, k_desc + ks * kStage + kk * 2, kIdescS, 1u);
-          }
-          mma_commit(&sfull[w]);
-          if (!DUAL || w == 1) mma_commit(&kempty[ks]);
-          if (left == 1) mma_commit(&qempty[buf]);
-        }
-        __syncwarp();
-        issued = true;
-        firsts = firsts << 1 | (first ? 1u : 0u);
-        first = false;
-        if ((!DUAL || w == 1) && ++ks == L::kKS) {
-          ks = 0;
-          k_phase ^= 1;
-        }
-        if (--left == 0) {
-          walk.next(a, per);
-          ++seg;
-          left = __shfl_sync(0xffffffffu, walk.left > 0 ? walk.segment() : 0, 0) * L::kTiles;
-          first = left > 0;
-          if (left == 0) end = x + 1;
-        }
-      } else {
-        firsts <<= 1;
-        if (x == end + 1) break;  // the last unit's mix is issued
+        for (int kk = 0; kk < L::kPart / 32; ++kk) mma_f8_ts(o, at + L::kPart / 4 + kk * 8, v_at + kk * kStep, kIdescL, 1u);
+        mma_commit(&pvdone[buf]);
+        if (h == L::kParts - 1) mma_commit(&vempty[vs]);
       }
-    }
-    if (issued) {
-      if (elect_one()) mma_commit(mma_done);
       __syncwarp();
-      if (lane == 0) wait_phase(mma_done, 0, abort_flag, a.status, kDrainNs, false);
-      __syncwarp();
+    };
+    Place sc{w, __shfl_sync(0xffffffffu, walk.segment(), 0) * L::kTiles, 0, 0, 0}, mx = sc;
+    Walk mix_walk = walk;
+    bool more = settle(sc, walk, true);
+    bool any = more;
+    if (any) settle(mx, mix_walk, false);
+    for (int h = 0; ok && more && h < L::kParts; ++h) score(sc, h);
+    while (ok && any) {
+      sc.u += 2;
+      sc.parity ^= 1;
+      if (more) more = settle(sc, walk, true);
+      for (int h = 0; ok && h < L::kParts; ++h) {
+        mix(mx, h);
+        if (ok && more) score(sc, h);
+      }
+      mx.u += 2;
+      mx.parity ^= 1;
+      any = settle(mx, mix_walk, false);
     }
+    if (elect_one()) mma_commit(&mma_done[w]);
+    __syncwarp();
+    if (lane == 0) wait_phase(&mma_done[w], 0, abort_flag, a.status, kDrainNs, false);
+    __syncwarp();
   } else {
     // ---------------- softmax ----------------
-    constexpr int NC = L::kCols;
+    constexpr int NC = L::kPart / L::kCopies;  // slots of a part that a copy weighs
     const int w = (warp - 4) >> 2;      // group
     const int quarter = warp & 3;
     const int copy = quarter * 32 / L::kCopyRows;
     const int r = quarter * 32 % L::kCopyRows + lane;  // row of the row tile; lane quarter * 32 + lane of TMEM is its
     const uint32_t lane_addr = static_cast<uint32_t>(quarter * 32) << 16;
-    const uint32_t s_addr = tmem + lane_addr + w * kTile;
     const uint32_t o_addr = tmem + lane_addr + L::kColO + w * HD;
-    int x = 0;  // the segment's first unit
+    int tiles = 0;         // before this segment
+    uint32_t parity = 0, other = 0;  // of the group's units, and of the other's
     for (int seg = 0; walk.left > 0; walk.next(a, per), ++seg) {
       const int n = walk.segment();
       const int units = n * L::kTiles;
@@ -498,52 +544,51 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
       const int token = i0 + r / a.group;  // a row past `live` computes on zeros and is not stored
       const int total = s.ctx + s.n;
       float m = -INFINITY, l = 0.f, factor = 0.f;
-      const int u0 = x + ((x & 1) == w ? 0 : 1);
-      for (int u = u0; u < x + units; u += 2) {
-        const int kt = DUAL ? u >> 1 : u;
-        const int t = walk.t + (DUAL ? (u - x) >> 1 : u - x);  // tile of the item
-        warp_wait(&sfull[w], (u >> 1) & 1, abort_flag, a.status);
-        tc_fence_after();
-        const int slot0 = t * a.tile;
-        const uint32_t bad = bad_ring[kt % kBadRing];
-        if (u == u0) factor = factors[seg % kQRing * L::kRows + (DUAL ? w * kTile : 0) + r];
-        if (warp_live) {
-          // This copy's scores of the row: at most 64 are held, of 128 the second half is
-          // loaded twice (its weights go where the first half's scores were).
-          constexpr int kHeld = NC < 64 ? NC : 64;
-          const float4* group = scales + kt % kBadRing * kGroups + copy * (NC / kGroupSlots);
-          uint32_t v[kHeld / 32][32];
-          auto load = [&](int col) {
+      for (int u = w; u < units; u += 2, parity ^= 1) {
+        const int kt = tiles + (DUAL ? u >> 1 : u);
+        const int slot0 = (walk.t + (DUAL ? u >> 1 : u)) * a.tile;
+#pragma unroll 1
+        for (int h = 0; h < L::kParts; ++h) {
+          const int buf = L::kParts * w + h;
+          const uint32_t s_addr = tmem + lane_addr + buf * L::kPart;
+          warp_wait(&sfull[buf], parity, abort_flag, a.status);
+          tc_fence_after();
+          const uint32_t bad = bad_ring[kt % kBadRing];
+          if (u == w && h == 0) factor = factors[seg % kQRing * L::kRows + (DUAL ? w * kTile : 0) + r];
+          if (warp_live) {
+            const int first = h * L::kPart + copy * NC;  // this copy's first slot of the tile
+            const float4* group = scales + kt % kBadRing * kGroups + first / kGroupSlots;
+            constexpr int kChunk = NC < 32 ? NC : 32;
+            uint32_t v[NC / kChunk][kChunk];
 #pragma unroll
-            for (int c = 0; c < kHeld / 32; ++c) tmem_load32(s_addr + copy * NC + col + 32 * c, v[c]);
+            for (int c = 0; c < NC / kChunk; ++c) tmem_load_n<kChunk>(s_addr + copy * NC + kChunk * c, v[c]);
             tmem_wait_ld();
             if (slot0 + a.tile > s.ctx || a.tile < kTile || bad != 0) {
 #pragma unroll
-              for (int c = 0; c < kHeld / 32; ++c) {
-                const int at = copy * NC + col + 32 * c;
+              for (int c = 0; c < NC / kChunk; ++c) {
+                const int at = first + kChunk * c;
                 uint32_t see = r < live ? seen32(a, s, token, slot0 + at) & low_bits(a.tile - at) : 0xffffffffu;
                 if (bad) see &= sound32(bad, at, a.box);
+                if (kChunk < 32) see |= 0xffffffffu << (kChunk & 31);
                 if (__all_sync(0xffffffffu, see == 0xffffffffu)) continue;  // a prompt's chunks are mostly seen
 #pragma unroll
-                for (int e = 0; e < 32; ++e) {
+                for (int e = 0; e < kChunk; ++e) {
                   if (!((see >> e) & 1)) v[c][e] = 0xff800000u;  // -inf: no weight
                 }
               }
               __syncwarp();
             }
-          };
-          // what a group's scores are multiplied by: never 0, since -inf times it has to stay
-          auto times = [&](float k) {
-            const float f = k * factor;
-            return f < 1.17549435e-38f ? 1.17549435e-38f : f;
-          };
-          float top = -INFINITY;
-          auto highest = [&](int col) {
+            // what a group's scores are multiplied by: never 0, since -inf times it has to stay
+            auto times = [&](float k) {
+              const float f = k * factor;
+              return f < 1.17549435e-38f ? 1.17549435e-38f : f;
+            };
+            float top = -INFINITY;
 #pragma unroll
-            for (int c = 0; c < kHeld / 32; ++c) {
+            for (int c = 0; c < NC / kChunk; ++c) {
 #pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                const float4 sc = group[col / kGroupSlots + 4 * c + j];
+              for (int j = 0; j < kChunk / 8; ++j) {
+                const float4 sc = group[4 * c + j];
                 float most = __uint_as_float(v[c][8 * j]);
 #pragma unroll
                 for (int e = 1; e < 7; e += 2) most = max3(most, __uint_as_float(v[c][8 * j + e]), __uint_as_float(v[c][8 * j + e + 1]));
@@ -551,40 +596,35 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
                 top = fmaxf(top, fmaf(most, times(sc.x), sc.y));
               }
             }
-          };
-          if constexpr (NC == 128) {
-            load(64);
-            highest(64);
-          }
-          load(0);
-          highest(0);
-          if (r >= live) top = -INFINITY;
-          if (factor != factor) top = 0.f;  // a row of NaN stays one through its merges
-          const bool rise = top > m + kRescaleAt8 || (m == -INFINITY && top > -INFINITY);
-          const float m_new = rise ? top : m;
-          const float alpha = rise ? ex2(m - m_new) : 1.f;  // m = -inf: 0
-          if (u != u0 && __any_sync(0xffffffffu, rise)) {
-            // the group's previous mix is done: these scores were issued after it
-            l *= alpha;
+            if (r >= live) top = -INFINITY;
+            if (factor != factor) top = 0.f;  // a row of NaN stays one through its merges
+            const bool rise = top > m + kRescaleAt8 || (m == -INFINITY && top > -INFINITY);
+            const float m_new = rise ? top : m;
+            const float alpha = rise ? ex2(m - m_new) : 1.f;  // m = -inf: 0
+            if ((u != w || h > 0) && __any_sync(0xffffffffu, rise)) {
+              // the group's previous mix
+              const int last = h > 0 ? buf - 1 : buf + L::kParts - 1;
+              warp_wait(&pvdone[last], h > 0 ? parity : parity ^ 1, abort_flag, a.status);
+              tc_fence_after();
+              l *= alpha;
 #pragma unroll 1
-            for (int c = 0; c < HD / 16; ++c) {
-              uint32_t o[16];
-              tmem_load16(o_addr + 16 * c, o);
-              tmem_wait_ld();
+              for (int c = 0; c < HD / 16; ++c) {
+                uint32_t o[16];
+                tmem_load16(o_addr + 16 * c, o);
+                tmem_wait_ld();
 #pragma unroll
-              for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-              tmem_store16(o_addr + 16 * c, o);
+                for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+                tmem_store16(o_addr + 16 * c, o);
+              }
             }
-          }
-          m = m_new;
-          const float base = m == -INFINITY ? 0.f : m - kLift;
-          auto weigh = [&](int col) {
+            m = m_new;
+            const float base = m == -INFINITY ? 0.f : m - kLift;
 #pragma unroll
-            for (int c = 0; c < kHeld / 32; ++c) {
-              uint32_t part[8], rest[8];
+            for (int c = 0; c < NC / kChunk; ++c) {
+              uint32_t part[kChunk / 4], rest[kChunk / 4];
 #pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                const float4 sc = group[col / kGroupSlots + 4 * c + j];
+              for (int j = 0; j < kChunk / 8; ++j) {
+                const float4 sc = group[4 * c + j];
                 const float f = times(sc.x), up = sc.y - base;
                 const uint64_t f2 = pair(f, f), up2 = pair(up, up);
                 uint64_t sum = 0;
@@ -594,69 +634,60 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
                   const float2 y1 = unpair(fma2(pair(v[c][8 * j + e + 2], v[c][8 * j + e + 3]), f2, up2));
                   const float p0 = ex2(y0.x), p1 = ex2(y0.y), p2 = ex2(y1.x), p3 = ex2(y1.y);
                   sum = add2(sum, add2(pair(p0, p1), pair(p2, p3)));
-                  uint32_t h0, h1, l0, l1;
-                  weight_parts(p0, p1, &h0, &l0);
-                  weight_parts(p2, p3, &h1, &l1);
-                  part[2 * j + e / 4] = h0 | h1 << 16;
-                  rest[2 * j + e / 4] = l0 | l1 << 16;
+                  weight_parts(p0, p1, p2, p3, &part[2 * j + e / 4], &rest[2 * j + e / 4]);
                 }
                 const float2 two = unpair(sum);
                 l = fmaf(two.x + two.y, sc.z, l);
               }
-              const uint32_t to = s_addr + (copy * NC + col) / 4 + 8 * c;
-              tmem_store8(to, part);
-              tmem_store8(to + 32, rest);
+              const uint32_t to = s_addr + copy * (NC / 4) + kChunk / 4 * c;
+              tmem_store_n<kChunk / 4>(to, part);
+              tmem_store_n<kChunk / 4>(to + L::kPart / 4, rest);
             }
-          };
-          weigh(0);
-          if constexpr (NC == 128) {
-            load(64);
-            weigh(64);
-          }
-          if constexpr (L::kCopies > 1) {  // no weights for the slots of the other copies
-            uint32_t zero[8];
+            if constexpr (L::kCopies > 1) {  // no weights for the slots of the other copies
+              uint32_t zero[NC / 4];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) zero[e] = 0;
+              for (int e = 0; e < NC / 4; ++e) zero[e] = 0;
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              if (c / (NC / 32) != copy) {
-                tmem_store8(s_addr + 8 * c, zero);
-                tmem_store8(s_addr + 32 + 8 * c, zero);
+              for (int c = 0; c < L::kCopies; ++c) {
+                if (c != copy) {
+                  tmem_store_n<NC / 4>(s_addr + c * (NC / 4), zero);
+                  tmem_store_n<NC / 4>(s_addr + L::kPart / 4 + c * (NC / 4), zero);
+                }
               }
             }
+            tmem_wait_st();
           }
-          tmem_wait_st();
-        }
-        if (slot0 + a.tile > total || bad != 0) {
-          // V rows that no copy filled, or stale slots behind the last token: zero
-          const int vs = kt % L::kVS;
-          warp_wait(&vfull[vs], (kt / L::kVS) & 1, abort_flag, a.status);
-          const int vr = quarter * 32 + lane;
-          if (slot0 + vr >= total || (vr < a.tile && ((bad >> (vr / a.box)) & 1))) {
-            unsigned char* row = smem + L::kOffV + vs * L::kOperand + vr * HD;
+          if ((slot0 + a.tile > total || bad != 0) && quarter * L::kParts >> 2 == h) {
+            // V rows that no copy filled, or stale slots behind the last token: zero
+            const int vs = kt % L::kVS;
+            warp_wait(&vfull[vs], (kt / L::kVS) & 1, abort_flag, a.status);
+            const int vr = quarter * 32 + lane;
+            if (slot0 + vr >= total || (vr < a.tile && ((bad >> (vr / a.box)) & 1))) {
+              unsigned char* row = smem + L::kOffV + vs * L::kOperand + vr * HD;
 #pragma unroll
-            for (int c = 0; c < HD / 16; ++c) *reinterpret_cast<uint4*>(row + c * 16) = make_uint4(0u, 0u, 0u, 0u);
+              for (int c = 0; c < HD / 16; ++c) *reinterpret_cast<uint4*>(row + c * 16) = make_uint4(0u, 0u, 0u, 0u);
+            }
+            fence_proxy_async_smem();
           }
-          fence_proxy_async_smem();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&pfull[buf]);
         }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&pfull[w]);
       }
 
       // the groups' last mixes of the segment: of both where finish_segment reads both O, else of this one's
-      const int end = x + units;
-      const int last0 = end - 1 - ((end - 1) & 1), last1 = end - 1 - (~(end - 1) & 1);
-      const bool had0 = last0 >= x, had1 = last1 >= x;
-      constexpr bool kOwnOnly = DUAL || L::kCopies > 1;
-      if (had0 && (!kOwnOnly || w == 0)) warp_wait(&pvdone[0], (last0 >> 1) & 1, abort_flag, a.status);
-      if (had1 && (!kOwnOnly || w == 1)) warp_wait(&pvdone[1], (last1 >> 1) & 1, abort_flag, a.status);
+      const bool had1 = units > 1;
+      if (w == 0 || had1) warp_wait(&pvdone[L::kParts * (w + 1) - 1], parity ^ 1, abort_flag, a.status);
+      if (!DUAL && L::kCopies == 1) {
+        other ^= (units + w) >> 1 & 1;  // the other group had (units + w) / 2
+        if (w == 1 || had1) warp_wait(&pvdone[L::kParts * ((w ^ 1) + 1) - 1], other ^ 1, abort_flag, a.status);
+      }
       tc_fence_after();
-      finish_segment<L, HD>(a, smem, walk, s, slots, tmem, w, copy, r, had0, had1, seg, i0, live, m, l);
+      finish_segment<L, HD>(a, smem, walk, s, slots, tmem, w, copy, r, true, had1, seg, i0, live, m, l);
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(ofree);
-      x += units;
+      tiles += n;
     }
   }
   tc_fence_before();

@@ -1,12 +1,12 @@
 """Tree attention over an 8-bit paged cache on the GPU against 64-bit softmax attention over the
 values that the cache stands for. On the CUDA cores the tolerance is serving_ref's. On the tensor
-cores a query is two e4m3 parts and a weight an e4m3 and an e5m2 part of its fp16 value, which
+cores a query is two e4m3 parts and a weight an e5m2 and an e4m3 part of its fp16 value, which
 adds (the kernel's own scaling puts a row's largest query in [128, 256), and its largest weight
-times V's scale at 2^2 or more):
+times V's scale at 2^6 or more):
 * a query element off by at most 2^-10 of the 128 that its row's largest exceeds, 2^-17 of that;
-* a weight off by 2^-11 + 2^-8 of itself (the first part leaves at most 2^-4 of it, of which
-  the second loses at most 2^-4: its steps are 2^-7 up to 2^-4), or, where it is below the parts' normal
-  range, by 2^-14, which is 2^-16 of the largest weight times scale."""
+* a weight off by 2^-11 + 2^-8 of itself (the first part leaves at most 2^-3 of its power of two, of
+  which the second loses at most 2^-5: its steps are 2^-7 up to 2^-3), or, where what is left is below the
+  second part's normal range, by 2^-10, which is 2^-16 of the largest weight times scale."""
 import math
 
 import numpy as np
