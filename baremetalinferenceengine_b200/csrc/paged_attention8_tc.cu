@@ -21,10 +21,10 @@
 // tensor time), above it the products. What it takes is neither: it is the chain scores, softmax, weights, mix of each
 // row tile, whose waits two groups of warps leave open (counters of 64 tokens at group 8: tensor pipe 20 % of its
 // cycles, conversions and exponentials 21 %, issue slots 35 %), and for few rows the ends of segments.
-// Measured, heads of 128, 8 kv heads: 1 sequence, 12 tokens at group 4 over 8000 slots 31 us; 64 ragged sequences of up
-// to 8192 slots, 8 tokens at group 4 207 us (2.5 TB/s of codes); 16 sequences of 4096 to 8192 slots, 64 tokens at group 8
-// 361 us (553 TFLOP/s of the formula's products; with one issuer for both groups and whole tiles 402, with parts for
-// few rows too 217 and 34 in the first two).
+// Measured, heads of 128, 8 kv heads: 1 sequence, 12 tokens at group 4 over 8000 slots 24 us; 64 ragged sequences of up
+// to 8192 slots, 8 tokens at group 4 179 us (2.9 TB/s of codes); 16 sequences of 4096 to 8192 slots, 64 tokens at group 8
+// 344 us (582 TFLOP/s of the formula's products). Before items had a cost 31, 207 and 361; then with one issuer for
+// both groups and whole tiles 31, 201 and 402; with parts for few rows too 34, 217 and 360.
 //
 // Split and roles are paged_attention_tc.cu's, but for the queries, the scales and the MMAs. The warp that fetches V
 // converts a segment's queries into two operands in shared memory, some rows between two tiles, while the segment before
@@ -44,6 +44,9 @@ constexpr float kRescaleAt8 = 6.f;  // rise of the maximum (log2) that a row's s
 constexpr float kLift = 6.f;        // P is 2^6 at the running maximum, so at most 2^12: Pl ends at 2^8
 constexpr int kGroupSlots = 8;      // slots of a tile that share a scale
 constexpr int kGroups = kTile / kGroupSlots;
+// What beginning and ending an item costs a CTA, in tiles: of 0, 1, 2, 4, 6, 8 the cases above take 31, 24, 24, 24, 24, 23;
+// 213, 208, 196, 186, 179, 182 and 361, 356, 351, 347, 344, 343 us.
+constexpr int kItemCost = 6;
 constexpr int kConvert = 8;         // pairs of rows of the next queries that are converted between two tiles
 constexpr int kQRing = 4;           // segments whose queries' factors are kept
 constexpr int kQWarps = 10;         // warps that convert a CTA's first queries: all but the two of TMA
@@ -709,6 +712,7 @@ int launch_form(TreeArgs a, cudaStream_t stream, const char* what) {
   auto kernel = tree_tc8_kernel<HD, COPIES>;
   if (int st = allow_dynamic_smem(reinterpret_cast<const void*>(kernel), L::kBytes, what)) return st;
   a.whole = whole_items(a, tokens_of(COPIES, a.group));
+  a.item_cost = kItemCost;
   const int nc = ctas_for(a.batch, a.hkv, a.group, a.max_ctx, a.max_tree);
   if (int st = launch_kernel(what, kernel, dim3(nc), dim3(kThreadsTc), L::kBytes, stream, nullptr, tk, tv, a)) return st;
   if (nc == 1 || a.whole) return BM_OK;  // no item is cut

@@ -47,9 +47,11 @@ struct RowLayout {
   static constexpr int kSlotFloats = kRows * (HD + 2);      // a partial: sums, then maxima, then weight sums
 };
 
+// CTAs share out places: a.item_cost of them for each item, ahead of one for each of its tiles.
+
 // What a CTA left of its first segment, for the merge.
 struct Record {
-  int64_t lo, total;   // its first tile, and all tiles
+  int64_t lo, total;   // its first place, and all places
   int32_t b, kvh, p;   // the item
   int32_t t0, tiles;   // the segment's first tile in it (-1: no segment), the item's tiles
   int32_t nc;          // CTAs with tiles
@@ -63,59 +65,69 @@ __device__ __forceinline__ int item_tiles(const TreeArgs& a, const Seq& s, int p
   const int seen = s.ctx + (a.mask ? s.n : min(s.n, (p + 1) * per));
   return (seen + a.tile - 1) / a.tile;
 }
-// All tiles of one kv head of a sequence, and its items.
-__device__ __forceinline__ int64_t head_tiles(const TreeArgs& a, const Seq& s, int per, int* items) {
+// Its places.
+__device__ __forceinline__ int item_places(const TreeArgs& a, const Seq& s, int p, int per) { return a.item_cost + item_tiles(a, s, p, per); }
+// All places of one kv head of a sequence, and its items.
+__device__ __forceinline__ int64_t head_places(const TreeArgs& a, const Seq& s, int per, int* items) {
   *items = (s.n + per - 1) / per;
-  if (a.mask) return static_cast<int64_t>(*items) * item_tiles(a, s, 0, per);
+  if (a.mask) return static_cast<int64_t>(*items) * item_places(a, s, 0, per);
   int64_t t = 0;
-  for (int p = 0; p < *items; ++p) t += item_tiles(a, s, p, per);
+  for (int p = 0; p < *items; ++p) t += item_places(a, s, p, per);
   return t;
 }
 
-// Tiles from tile `off` of a sequence to the next beginning of an item (0: it is one).
-__device__ __forceinline__ int64_t to_next_item(const TreeArgs& a, const Seq& s, int64_t off, int64_t head, int per) {
+// From place `off` of a sequence to where a CTA's part may begin or end: back to an item's beginning
+// from the places ahead of its first tile; with a.whole on to the next beginning. 0: it may here.
+__device__ __forceinline__ int64_t to_border(const TreeArgs& a, const Seq& s, int64_t off, int64_t head, int per) {
   off %= head;
   for (int p = 0;; ++p) {
-    const int tiles = item_tiles(a, s, p, per);
-    if (off < tiles) return off == 0 ? 0 : tiles - off;
-    off -= tiles;
+    const int places = item_places(a, s, p, per);
+    if (off < places) return off == 0 ? 0 : a.whole ? places - off : off <= a.item_cost ? -off : 0;
+    off -= places;
   }
 }
 
 // The walk over a CTA's segments: every role runs its own, with the same results.
 struct Walk {
-  int64_t b, left;
+  int64_t b, left;                // places left
   int items, kvh, p, t, tiles;
   Seq s;
 
-  // Tile `off` of sequence b is the CTA's first, and `n` tiles are its own.
+  // Place `off` of sequence b is the CTA's first, and `n` places are its own.
   __device__ void start(const TreeArgs& a, const Seq& sequence, int64_t b0, int64_t off, int64_t n, int per) {
     b = b0;
     left = n;
     s = sequence;
-    int64_t head = head_tiles(a, s, per, &items);
+    int64_t head = head_places(a, s, per, &items);
     if (off >= a.hkv * head) {  // behind the sequence's last item: the next one with tiles
       do {
         ++b;
         read_seq(a, b, &s);
       } while (s.n == 0);
-      head = head_tiles(a, s, per, &items);
+      head = head_places(a, s, per, &items);
       off = 0;
     }
     kvh = static_cast<int>(off / head);
     off -= kvh * head;
     p = 0;
-    while (off >= (tiles = item_tiles(a, s, p, per))) {
+    while (off >= (tiles = item_places(a, s, p, per))) {
       off -= tiles;
       ++p;
     }
+    tiles -= a.item_cost;
     t = static_cast<int>(off);
+    if (t == 0) {
+      left -= a.item_cost;
+    } else {
+      t -= a.item_cost;  // behind the places ahead of its first tile
+    }
   }
   // Tiles of the current segment (0 when the walk is over).
   __device__ int segment() const { return static_cast<int>(left < tiles - t ? left : tiles - t); }
   __device__ void next(const TreeArgs& a, int per) {
     left -= segment();
     if (left == 0) return;
+    left -= a.item_cost;
     t = 0;
     if (++p == items) {
       p = 0;
@@ -133,7 +145,7 @@ struct Walk {
 };
 
 struct Plan {
-  int64_t lo, hi, b, off;  // this CTA's tiles; the first is tile `off` of sequence b
+  int64_t lo, hi, b, off;  // this CTA's places; the first is place `off` of sequence b
   Seq s;                   // sequence b
 };
 static_assert(sizeof(Plan) <= 96, "room in the layout");
@@ -215,7 +227,7 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-// Shares the tiles of the batch out: this CTA's into *plan, and the number of all tiles and
+// Shares the places of the batch out: this CTA's into *plan, and the number of all places and
 // of the CTAs that have some. False (with the CTA's empty record written) where it has none.
 // All threads of the CTA call it; barriers and TMEM that they set up before are visible behind it.
 __device__ __forceinline__ bool plan_share(const TreeArgs& a, int per, int64_t* scan, Plan* plan, Record* records, int64_t* total_out,
@@ -229,7 +241,7 @@ __device__ __forceinline__ bool plan_share(const TreeArgs& a, int per, int64_t* 
     const int32_t bad = read_seq(a, b, &s);
     if (bad && cta == 0) raise_status(a.status, bad);
     int items;
-    mine += a.hkv * head_tiles(a, s, per, &items);
+    mine += a.hkv * head_places(a, s, per, &items);
   }
   int64_t incl = mine;
 #pragma unroll
@@ -251,8 +263,7 @@ __device__ __forceinline__ bool plan_share(const TreeArgs& a, int per, int64_t* 
     if (tid == 0) records[cta] = Record{0, total, -1, 0, 0, -1, 0, nc};
     return false;
   }
-  // Tile x lies in one thread's sequences; a.whole moves both ends on to the next beginning
-  // of an item.
+  // Place x lies in one thread's sequences.
   const int64_t lo = total * cta / nc, hi = total * (cta + 1) / nc;
   auto locate = [&](int64_t x, bool first) {
     if (x < before || x >= before + mine) return;
@@ -260,9 +271,9 @@ __device__ __forceinline__ bool plan_share(const TreeArgs& a, int per, int64_t* 
     for (int64_t b = b_lo; b < b_hi; ++b) {
       if (share > 1) read_seq(a, b, &s);
       int items;
-      const int64_t head = head_tiles(a, s, per, &items), n = a.hkv * head;
+      const int64_t head = head_places(a, s, per, &items), n = a.hkv * head;
       if (x < at + n) {
-        const int64_t on = a.whole ? to_next_item(a, s, x - at, head, per) : 0;
+        const int64_t on = a.whole || a.item_cost > 0 ? to_border(a, s, x - at, head, per) : 0;
         if (first) {
           plan->lo = x + on;
           plan->b = b;
@@ -468,7 +479,8 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(const TreeArgs a, int c
   const int k = static_cast<int>(blockIdx.x) + 1;
   const Record rec = records[k];
   if (rec.t0 <= 0) return;  // no tiles, or its first tile begins an item
-  const int64_t first = rec.lo - rec.t0;  // the item's first tile
+  const int64_t first = rec.lo - rec.t0;  // the place of the item's first tile
+  const int64_t begin = first - a.item_cost;
   auto border = [&](int c) { return rec.total * c / rec.nc; };
   if (border(k - 1) > first) return;  // an earlier border is inside it, too
   Seq s;
@@ -478,7 +490,7 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(const TreeArgs a, int c
   const int lane = threadIdx.x & 31;
   // one past the last CTA with a part: the one that holds the item's last tile
   const int last = static_cast<int>(((first + rec.tiles) * rec.nc - 1) / rec.total) + 1;
-  const int skip = border(k - 1) != first;  // in the first CTA the item is not the first segment
+  const int skip = border(k - 1) < begin;  // in the first CTA the item is not the first segment
   auto part = [&](int c) { return slots + (2 * static_cast<int64_t>(c) + (c == k - 1 ? skip : 0)) * L::kSlotFloats; };
   for (int r = static_cast<int>(blockIdx.y) * 8 + threadIdx.x / 32; r < L::kRows; r += 8 * gridDim.y) {
     const int tile = r / kTile, rr = r - tile * kTile;
