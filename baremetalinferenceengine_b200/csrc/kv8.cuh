@@ -32,18 +32,14 @@ __device__ __forceinline__ int exponent_for(uint32_t amax_bits) {
   return min(max(e, kLowest), kHighest);
 }
 
-// |x| as bits, which order as the values do; 0 where x is not finite, which sets no scale.
-__device__ __forceinline__ uint32_t magnitude(float x) {
-  const uint32_t b = __float_as_uint(x) & 0x7fffffffu;
-  return b < 0x7f800000u ? b : 0u;
-}
+// |x| as bits, which order as the values do, from kNotFinite on the infinities and NaN.
+constexpr uint32_t kNotFinite = 0x7f800000u;
+__device__ __forceinline__ uint32_t magnitude(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 
-// Two values to two codes (lo in the low byte): nearest even, ends at +-448. An infinity
-// would end there, too: it is made NaN.
+// Two values to two codes (lo in the low byte): nearest even, ends at +-448, NaN stays one. (An infinity would end at
+// 448, too: it is made NaN before.)
 __device__ __forceinline__ uint32_t to_codes(float lo, float hi) {
   uint16_t r;
-  if (isinf(lo)) lo = __int_as_float(0x7fffffff);
-  if (isinf(hi)) hi = __int_as_float(0x7fffffff);
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
   return r;
 }

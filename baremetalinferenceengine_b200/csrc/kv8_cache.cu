@@ -435,18 +435,42 @@ __global__ void __launch_bounds__(kAppendThreads, kKvBlocks) append_kernel(const
       if (turned && good[u]) turn<N, J, INTER, FULL>(y[u], t, sh);
     }
   };
+  // The lane's largest finite magnitude (elements that it does not own are 0); what is not finite becomes NaN and
+  // sets no scale.
+  auto examine = [&]() {
+    uint32_t most = 0;
+#pragma unroll
+    for (int u = 0; u < kUK; ++u) {
+      uint32_t m = 0;
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+#pragma unroll
+        for (int e = 0; e < 2 * N; ++e) m = max(m, magnitude(y[u][j][e]));
+      }
+      if (!good[u]) m = 0;
+      if (m >= kNotFinite) {
+        m = 0;
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+#pragma unroll
+          for (int e = 0; e < 2 * N; ++e) {
+            if (magnitude(y[u][j][e]) >= kNotFinite) {
+              y[u][j][e] = __int_as_float(0x7fffffff);
+            } else {
+              m = max(m, magnitude(y[u][j][e]));
+            }
+          }
+        }
+      }
+      most = max(most, m);
+    }
+    return most;
+  };
   const int batches = (hi - lo + step - 1) / step;
   for (int i = 0; i < batches; ++i) {
     if (i > 0) fetch(lo + i * step);
     compute();
-#pragma unroll
-    for (int u = 0; u < kUK; ++u) {
-#pragma unroll
-      for (int j = 0; j < J; ++j) {
-#pragma unroll
-        for (int e = 0; e < 2 * N; ++e) top = max(top, good[u] && (e < N ? sh.own(j) : sh.pair(j)) ? magnitude(y[u][j][e]) : 0u);
-      }
-    }
+    top = max(top, examine());
   }
   top = __reduce_max_sync(0xffffffffu, top);
   if (wpj > 1) {
@@ -478,6 +502,7 @@ __global__ void __launch_bounds__(kAppendThreads, kKvBlocks) append_kernel(const
     if (batches > 1) {
       fetch(lo + i * step);
       compute();
+      examine();
     }
 #pragma unroll
     for (int u = 0; u < kUK; ++u) {
