@@ -33,9 +33,10 @@ constexpr int kAppendThreads = 256;
 constexpr int kAppendWarps = kAppendThreads / 32;
 // Passes whose loads a lane keeps in flight, of Q's (and norm_rotary's) heads and of K's and V's rows; and the blocks
 // that an SM has room for at the registers these take. A prompt's 16384 rows of 64 + 8 heads of 128, us: 4 and 5 blocks
-// 114, 4 and 4 123, 2 and 6 116. K and V of 32768 tokens, 8 heads: 2 and 2 blocks 118, 1 and 3 154, 4 and 1 146.
+// 114, 4 and 4 123, 2 and 6 116. K and V of 32768 tokens, 8 heads, in one
+// kernel: 2 and 2 blocks 118, 1 and 3 154, 4 and 1 146; jobs of several heads, the next one's rows asked for early: no gain.
 constexpr int kUQ = 4, kUK = 2;
-constexpr int kQBlocks = 5, kKvBlocks = 2;
+constexpr int kQBlocks = 5, kKvBlocks = 2, kVBlocks = 3;
 
 struct HeadArgs {
   void* q_out;
@@ -331,17 +332,20 @@ __global__ void __launch_bounds__(kThreads, kQBlocks) append_q_kernel(const __gr
   append_q<T, N, J, INTER, FULL>(a, static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5), weights, threadIdx.x & 31);
 }
 
+// What a launch appends: all of a call, or K or V alone.
+enum class Jobs { kAll, kK, kV };
+
 // The first kv_ctas blocks take K and V: one job is K or V of one head in one block of slots,
 // held by warps_per_job warps of a block. A lane group holds a row, so the norm is a sum over a group and the scale a
 // maximum over the warp, then over the job's warps. The other blocks rotate Q.
-template <typename T, int N, int J, bool INTER, bool FULL>
-__global__ void __launch_bounds__(kAppendThreads, kKvBlocks) append_kernel(const __grid_constant__ HeadArgs a) {
+template <typename T, int N, int J, bool INTER, bool FULL, Jobs JOBS>
+__global__ void __launch_bounds__(kAppendThreads, JOBS == Jobs::kV ? kVBlocks : kKvBlocks) append_kernel(const __grid_constant__ HeadArgs a) {
   grid_dependency_wait();
   __shared__ uint32_t tops[kAppendWarps];
   __shared__ __align__(16) T weights[2 * kMaxHeadDim];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const bm_paged_kv8_t& c8 = a.cache;
-  if (blockIdx.x >= a.kv_ctas) {
+  if (JOBS == Jobs::kAll && blockIdx.x >= a.kv_ctas) {
     if (a.q_weight) stage_weights(weights, a, kAppendThreads);
     append_q<T, N, J, INTER, FULL>(a, (static_cast<int64_t>(blockIdx.x) - a.kv_ctas) * kAppendWarps + warp, weights, lane);
     return;
@@ -349,10 +353,11 @@ __global__ void __launch_bounds__(kAppendThreads, kKvBlocks) append_kernel(const
   // ---------------- K and V ----------------
   const int wpj = a.warps_per_job, sub = warp % wpj;
   const int64_t job = static_cast<int64_t>(blockIdx.x) * (kAppendWarps / wpj) + warp / wpj;
-  const int which = static_cast<int>(job % (2 * a.hkv));
-  const int head = which >> 1;
-  const bool is_v = which & 1;
-  const int64_t bj = job / (2 * a.hkv), b = bj / a.blocks;
+  const int kinds = JOBS == Jobs::kAll ? 2 * a.hkv : a.hkv;
+  const int which = static_cast<int>(job % kinds);
+  const int head = JOBS == Jobs::kAll ? which >> 1 : which;
+  const bool is_v = JOBS == Jobs::kAll ? which & 1 : JOBS == Jobs::kV;
+  const int64_t bj = job / kinds, b = bj / a.blocks;
   const int jb = static_cast<int>(bj - b * a.blocks);
   Span s{};
   int lo = 0, hi = 0, begin = 0;     // the block's new slots; its first slot
@@ -360,7 +365,7 @@ __global__ void __launch_bounds__(kAppendThreads, kKvBlocks) append_kernel(const
   bool active = b < a.batch;
   if (active) {
     const int32_t bad = read_span(c8, a.starts, a.ctx_lens, a.seq_ids, a.rows, a.max_tokens, b, &s);
-    if (bad && jb == 0 && which == 0 && lane == 0 && sub == 0) raise_status(a.status, bad);
+    if (bad && jb == 0 && which == 0 && !is_v && lane == 0 && sub == 0) raise_status(a.status, bad);
     // 64 bits: a block's end may pass the last slot there can be
     const int64_t from = (static_cast<int64_t>(s.ctx / c8.block) + jb) * c8.block;
     lo = static_cast<int>(max(static_cast<int64_t>(s.ctx), min(from, static_cast<int64_t>(s.ctx) + s.n)));
@@ -844,27 +849,38 @@ extern "C" int bm_paged_kv8_append(void* q_out, const void* q, const void* k, co
     const int64_t per = kAppendWarps / a.warps_per_job;
     const double jobs = static_cast<double>(batch) * a.blocks * 2 * a.hkv, q_jobs = static_cast<double>(batch) * max_tokens * a.parts;
     if (jobs + q_jobs > INT32_MAX) return fail(BM_ERR_INVALID_ARGUMENT, "%s: batch * max_tokens too large", what);
-    a.kv_ctas = (batch * a.blocks * 2 * a.hkv + per - 1) / per;
-    // Few tokens go in one launch; where they fill the GPU, Q's warps are better off in a kernel of their own, since
-    // K's and V's registers leave room for only 16 warps on an SM (32768 tokens of 64 + 8 heads: 335 us in one).
-    const bool apart = num_q_heads > 0 && a.parts == 1;
+    // Few tokens go in one launch; where they fill the GPU, Q, K and V are better off in kernels of their own, since
+    // K's registers leave room for only 16 warps on an SM (32768 tokens of 64 + 8 heads, appended and read back: 512 us
+    // with all in one, 351 with K and V in one, 343).
+    const bool apart = a.parts == 1;
+    a.kv_ctas = (batch * a.blocks * (apart ? 1 : 2) * a.hkv + per - 1) / per;
     const int64_t q_warps = num_q_heads ? batch * max_tokens * a.parts : 0;
     const int64_t q_ctas = apart ? 0 : (q_warps + kAppendWarps - 1) / kAppendWarps;
     const bool full = a.rest == 0 && 32 % a.units == 0;
-    auto go = [&](auto kernel, auto q_kernel) {
-      const int st = launch_kernel(what, kernel, dim3(static_cast<unsigned>(a.kv_ctas + q_ctas)), dim3(kAppendThreads), 0, as_stream(stream), nullptr, a);
-      if (st != BM_OK || !apart) return st;
-      return launch_kernel(what, q_kernel, dim3(static_cast<unsigned>((q_warps + kWarps - 1) / kWarps)), dim3(kThreads), 0, as_stream(stream), nullptr, a);
+    auto go = [&](auto inter, auto whole, auto type, auto width) {
+      constexpr bool I = decltype(inter)::value, F = decltype(whole)::value;
+      using T = decltype(type);
+      constexpr int N = decltype(width)::value, J = N == 1 ? 4 : 1;
+      auto launch = [&](auto kernel, int64_t ctas, int threads) {
+        return launch_kernel(what, kernel, dim3(static_cast<unsigned>(ctas)), dim3(threads), 0, as_stream(stream), nullptr, a);
+      };
+      if (!apart) return launch(append_kernel<T, N, J, I, F, Jobs::kAll>, a.kv_ctas + q_ctas, kAppendThreads);
+      if (int st = launch(append_kernel<T, N, J, I, F, Jobs::kK>, a.kv_ctas, kAppendThreads)) return st;
+      if (int st = launch(append_kernel<T, N, J, I, F, Jobs::kV>, a.kv_ctas, kAppendThreads)) return st;
+      return num_q_heads ? launch(append_q_kernel<T, N, J, I, F>, (q_warps + kWarps - 1) / kWarps, kThreads) : BM_OK;
     };
     auto pick = [&](auto inter) {
-      constexpr bool I = decltype(inter)::value;
+      const std::true_type yes;
+      const std::false_type no;
+      const std::integral_constant<int, 1> one;
+      const std::integral_constant<int, 4> four;
+      const std::integral_constant<int, 8> eight;
       if (dtype == BM_F32) {
-        if (n == 4) return full ? go(append_kernel<float, 4, 1, I, true>, append_q_kernel<float, 4, 1, I, true>) : go(append_kernel<float, 4, 1, I, false>, append_q_kernel<float, 4, 1, I, false>);
-        return go(append_kernel<float, 1, 4, I, false>, append_q_kernel<float, 1, 4, I, false>);
+        if (n == 4) return full ? go(inter, yes, 0.f, four) : go(inter, no, 0.f, four);
+        return go(inter, no, 0.f, one);
       }
-      if (n == 8) return full ? go(append_kernel<bf16, 8, 1, I, true>, append_q_kernel<bf16, 8, 1, I, true>) : go(append_kernel<bf16, 8, 1, I, false>, append_q_kernel<bf16, 8, 1, I, false>);
-      if (n == 4) return go(append_kernel<bf16, 4, 1, I, false>, append_q_kernel<bf16, 4, 1, I, false>);
-      return go(append_kernel<bf16, 1, 4, I, false>, append_q_kernel<bf16, 1, 4, I, false>);
+      if (n == 8) return full ? go(inter, yes, bf16{}, eight) : go(inter, no, bf16{}, eight);
+      return n == 4 ? go(inter, no, bf16{}, four) : go(inter, no, bf16{}, one);
     };
     return interleaved ? pick(std::true_type{}) : pick(std::false_type{});
   });
