@@ -192,6 +192,17 @@ def test_rows_about_every_form(cuda, hq, hkv, hd, page, block, rows):
     Batch(cuda, [(700, n), (0, n), (131, max(1, n - 1)), (40, 1)], hq, hkv, hd, page, block, BF16, seed=rows + hd).check()
 
 
+@pytest.mark.parametrize("hq,hkv,most", [(8, 2, 4), (6, 3, 24), (8, 1, 16), (16, 2, 40)])
+@pytest.mark.parametrize("seed", range(4))
+def test_cuts_anywhere_about_short_items(cuda, hq, hkv, most, seed):
+    """One long context among many short ones: shares of the work begin and end in items of one
+    tile, at their borders, and in what an item's beginning counts for."""
+    rng = np.random.RandomState(seed)
+    lens = [(int(rng.choice([0, 1, 100, 128, 129, 300])), int(rng.randint(0, most + 1))) for _ in range(45 + seed)]
+    lens[int(rng.randint(len(lens)))] = (2000 + 300 * seed, most)
+    Batch(cuda, lens, hq, hkv, 64, 16, 16, BF16, seed=seed, tree=seed != 2).check()
+
+
 @pytest.mark.parametrize("dtype", [BF16, F32])
 def test_wide_groups(cuda, dtype):
     Batch(cuda, [(200, 3), (9, 30)], 64, 1, 128, 32, 32, dtype, seed=5).check()
