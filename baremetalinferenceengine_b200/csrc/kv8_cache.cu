@@ -570,17 +570,17 @@ __global__ void __launch_bounds__(kThreads) read_kernel(const __grid_constant__ 
   }
   const int n = c8.head_dim / 16, rpi = 32 / n;  // lanes of a row, rows of a pass
   const int rl = lane / n, c = lane - rl * n;
-  const int i0 = chunk * kReadU * rpi + rl;
+  const int64_t i0 = static_cast<int64_t>(chunk) * (kReadU * rpi) + rl;
   if (rl >= rpi) return;
   uint4 k[kReadU], v[kReadU];
   float kf[kReadU], vf[kReadU];
   bool good[kReadU];
 #pragma unroll
   for (int u = 0; u < kReadU; ++u) {
-    const int i = i0 + u * rpi;
+    const int64_t i = i0 + u * rpi;
     good[u] = i < s.n;
     if (good[u]) {
-      const int slot = s.ctx + i, nth = slot / c8.page_size;
+      const int slot = static_cast<int>(s.ctx + i), nth = slot / c8.page_size;
       const int32_t page = __ldg(c8.page_table + static_cast<int64_t>(s.seq) * c8.max_pages + nth);
       good[u] = page >= 0 && page < c8.num_pages;
       if (good[u]) {
@@ -669,8 +669,8 @@ int check_paged_kv8(const char* what, const bm_paged_kv8_t* c) {
     return fail(BM_ERR_INVALID_ARGUMENT, "%s: head_dim %d of an 8-bit cache must be a multiple of 16 up to %d", what, c->head_dim, kMaxHeadDim);
   }
   if (c->page_size % c->block) return fail(BM_ERR_INVALID_ARGUMENT, "%s: block %d does not divide page_size %d", what, c->block, c->page_size);
-  if (static_cast<int64_t>(c->page_size) * c->max_pages > INT32_MAX) {
-    return fail(BM_ERR_INVALID_ARGUMENT, "%s: page_size * max_pages above 2^31 - 1", what);
+  if (static_cast<int64_t>(c->page_size) * c->max_pages > INT32_MAX - 4095) {  // a pass may look past a sequence's last slot
+    return fail(BM_ERR_INVALID_ARGUMENT, "%s: page_size * max_pages above 2^31 - 4096", what);
   }
   if (!aligned16(c->k_pages) || !aligned16(c->v_pages)) return fail(BM_ERR_INVALID_ARGUMENT, "%s: pages must be 16-byte aligned", what);
   if (!aligned_to(c->page_table, 4)) return fail(BM_ERR_INVALID_ARGUMENT, "%s: a pointer is not aligned to its elements", what);
@@ -809,6 +809,7 @@ extern "C" int bm_paged_kv8_append(void* q_out, const void* q, const void* k, co
   if (in_cache(qo) || in_cache(qi) || in_cache(ki) || in_cache(vi)) {
     return fail(BM_ERR_INVALID_ARGUMENT, "%s: q, k, v or q_out overlaps the cache", what);
   }
+  max_tokens = static_cast<int32_t>(std::min<int64_t>(max_tokens, rows));  // no sequence has more
   HeadArgs a{};
   if (num_q_heads) {
     a.q_out = q_out;
@@ -907,6 +908,7 @@ extern "C" int bm_paged_kv8_read(void* k_out, void* v_out, const bm_paged_kv8_t*
   if ((ko < vo + bytes && vo < ko + bytes) || meets_pages8(c, k_out, bytes) || meets_pages8(c, v_out, bytes)) {
     return fail(BM_ERR_INVALID_ARGUMENT, "%s: an output overlaps the other or the cache", what);
   }
+  max_rows = static_cast<int32_t>(std::min<int64_t>(max_rows, rows));  // no sequence has more
   ReadArgs a{k_out, v_out, c, first, starts, seq_ids, rows, batch, max_rows, 0, d_status};
   const int per = kReadU * (32 / (c.head_dim / 16));
   a.chunks = static_cast<int>((static_cast<int64_t>(max_rows) + per - 1) / per);

@@ -551,7 +551,8 @@ int bm_qk_norm_rotary(void* q_out, void* k_out, const void* q, const void* k, co
  *   o = t % page_size;  V alike.
  * A scale is a power of two in one byte, 2^(byte - 127) (e8m0), from 2^-40 to 2^40; a byte
  * outside these counts as the nearest. k_scales and v_scales are
- * [num_pages][num_kv_heads][page_size / block]. head_dim is a multiple of 16 up to 256. */
+ * [num_pages][num_kv_heads][page_size / block]. head_dim is a multiple of 16 up to 256, and
+ * page_size * max_pages at most 2^31 - 4096. */
 typedef struct bm_paged_kv8 {
   void* k_pages;
   void* v_pages;

@@ -367,3 +367,21 @@ def test_offsets_past_32_bits(cuda):
     q = randn((3, 16, hd), BF16, gen(4)).to(cuda)
     outs = [ops.paged_kv8_tree_attention(q, c, i32([102], cuda), i32([0, 3], cuda), 102, 3) for c in (cache, small)]
     assert bits_equal(*outs) and bool(torch.isfinite(outs[0].float()).all())
+
+
+def test_bounds_far_above_the_rows(cuda):
+    """max_tokens and max_rows that bound nothing: the same codes and rows as with close ones."""
+    hkv, hd, most = 2, 64, 2 ** 31 - 1
+    x = randn((45, 2 * hkv + 4, hd), BF16, gen(8)).to(cuda)
+    ctx, starts = i32([7, 0, 30], cuda), i32([0, 20, 21, 45], cuda)
+    got = []
+    for tokens, rows in ((24, 24), (most, most), (45, most)):
+        s = State(cuda, 3, 70, hkv, hd, 16, 8, BF16, seed=9, rd=hd, norm=True)
+        st = ops.DeviceStatus(cuda)
+        q = ops.paged_kv8_append(x[:, :4], x[:, 4:4 + hkv], x[:, 4 + hkv:], s.cache, ctx, starts, tokens, table=s.rope,
+                                 q_weight=s.wq.to(cuda), k_weight=s.wk.to(cuda), status=st)
+        k, v = ops.paged_kv8_read(s.cache, ctx, starts, 45, rows, status=st)
+        assert st.read() == 0
+        got.append((q, k, v))
+    for other in got[1:]:
+        assert all(bits_equal(a, b) for a, b in zip(got[0], other))

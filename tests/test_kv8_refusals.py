@@ -59,7 +59,7 @@ def size(L, total=4, batch=2, hq=4, hkv=2, hd=64, max_ctx=8, max_tree=4, out=Tru
 BAD_CACHES = [dict(k_pages=None), dict(v_pages=None), dict(k_scales=None), dict(v_scales=None), dict(page_table=None), dict(num_pages=0),
               dict(page_size=0), dict(block=0), dict(block=-4), dict(block=3), dict(block=16), dict(max_pages=-1), dict(num_seqs=0),
               dict(num_kv_heads=0), dict(num_kv_heads=(1 << 16) + 1), dict(head_dim=0), dict(head_dim=8), dict(head_dim=72),
-              dict(head_dim=272), dict(page_size=1 << 20, max_pages=1 << 12), dict(k_pages=W * 2 + 8), dict(v_pages=W * 3 + 4),
+              dict(head_dim=272), dict(page_size=1 << 20, max_pages=1 << 12), dict(page_size=8, block=8, max_pages=(1 << 28) - 1), dict(k_pages=W * 2 + 8), dict(v_pages=W * 3 + 4),
               dict(page_table=W * 6 + 2)]
 
 
