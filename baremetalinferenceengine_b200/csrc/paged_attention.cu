@@ -16,7 +16,8 @@
 // shared loads; up to 32 rows have a kernel of their own, bound by its shared loads of Q
 // (8 rows of 128 in fp32 over 16 sequences of 1000 to 2000, 8 heads: 84 us, floor 30; of 256 in
 // bf16, which the tensor-core form does not take, 4 rows 72, 32 rows 318, 512 rows 4870 us,
-// floors 27, 28 and 60). Slots
+// floors 27, 28 and 60; 32 sequences of up to 230 + 25, 6 heads of 48, fp32 over an 8-bit cache, whose codes
+// are widened as they are read from the staged tile: 26 us, over an fp32 one 22). Slots
 // are shared out over CTAs when the (sequence, kv head, row tile) triples do not fill the
 // GPU; the shares' partial sums meet in tree_combine_kernel.
 #include <algorithm>

@@ -17,7 +17,7 @@ using namespace bm::tc;
 
 constexpr int kTile = 128;      // slots per tile, rows per row tile
 constexpr int kThreadsTc = 384;
-constexpr int kMinTiles = 2;    // tiles that make a CTA worth starting, where items are cut
+constexpr int kMinTiles = 2;    // places (tiles, and items' costs) that make a CTA worth starting, where items are cut
 constexpr int kWholeTiles = 8;  // of the longest item, up to which items stay whole
 constexpr int kBadRing = 16;    // tiles whose bad-page bits are kept
 constexpr uint64_t kWaitNs = 2000000000ull;
