@@ -22,15 +22,15 @@
 // row tile, whose waits two groups of warps leave open (counters of 64 tokens at group 8: tensor pipe 20 % of its
 // cycles, conversions and exponentials 21 %, issue slots 35 %), and for few rows the ends of segments.
 // Measured, heads of 128, 8 kv heads: 1 sequence, 12 tokens at group 4 over 8000 slots 24 us; 64 ragged sequences of up
-// to 8192 slots, 8 tokens at group 4 179 us (2.9 TB/s of codes); 16 sequences of 4096 to 8192 slots, 64 tokens at group 8
-// 344 us (582 TFLOP/s of the formula's products). Before items had a cost 31, 207 and 361; then with one issuer for
-// both groups and whole tiles 31, 201 and 402; with parts for few rows too 34, 217 and 360.
+// to 8192 slots, 8 tokens at group 4 171 us (3.0 TB/s of codes); 16 sequences of 4096 to 8192 slots, 64 tokens at group 8
+// 337 us (594 TFLOP/s of the formula's products). Before items had a cost 31, 207 and 361; then with one issuer for
+// two row tiles' groups and whole tiles 402 for the last, with parts for few rows too 34 and 217 for the others.
 //
 // Split and roles are paged_attention_tc.cu's, but for the queries, the scales and the MMAs. The warp that fetches V
 // converts a segment's queries into two operands in shared memory, some rows between two tiles, while the segment before
 // is computed (all warps but those of TMA together for a CTA's first, which all wait for). The warp that fetches K
-// looks up the scales of its tile's slots, eight neighbouring ones of which share one. Each softmax group has an MMA
-// issuer of its own (warps 1 and 2).
+// looks up the scales of its tile's slots, eight neighbouring ones of which share one. With two row tiles each softmax
+// group has an MMA issuer of its own (warps 1 and 2), else one has both.
 #include <cuda.h>
 
 #include "kv8.cuh"
@@ -58,6 +58,8 @@ struct Layout8 : RowLayout<HD, COPIES> {
   // weighs one part while the other's mix and the next unit's scores are computed; copies' tiles wait for memory.
   static constexpr int kParts = Rows::kCopies > 1 ? 1 : 2;
   static constexpr int kPart = kTile / kParts;              // slots
+  // Warps that issue MMAs: with two row tiles each group has one of its own.
+  static constexpr int kIssuers = Rows::kTiles;
   static constexpr int kOperand = kTile * HD;               // a tile of K or V, one part of Q
   static constexpr int kQTile = 2 * kOperand;               // both parts of a row tile
   static constexpr int kQBuf = Rows::kTiles * kQTile;       // of two: a segment's, and the next one's
@@ -259,7 +261,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
   uint64_t* pfull = sfull + 4;          // weights in TMEM      (one arrival per warp of the group)
   uint64_t* pvdone = pfull + 4;         // mix done             (commit)
   uint64_t* qfull = pvdone + 4;         // queries converted    (kQWarps arrivals)
-  uint64_t* qempty = qfull + 2;         // each group's last scores of the segment are done (two commits)
+  uint64_t* qempty = qfull + 2;         // the segment's last scores are done (a commit of each issuer)
   uint64_t* ofree = qempty + 2;         // the segment's O has been read (one arrival per softmax warp)
   uint64_t* mma_done = ofree + 1;      // of each issuer
   Plan* plan = reinterpret_cast<Plan*>(smem + L::kOffPlan);
@@ -293,7 +295,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
       }
       for (int i = 0; i < 2; ++i) {
         mbar_init(&qfull[i], kQWarps);
-        mbar_init(&qempty[i], 2);
+        mbar_init(&qempty[i], L::kIssuers);
         mbar_init(&mma_done[i], 1);
       }
       mbar_init(ofree, 8);
@@ -430,43 +432,41 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
       }
     }
     __syncwarp();
-  } else if (warp == 1 || warp == 2) {
-    // ---------------- MMA issuers, one for each group ----------------
-    // Of a segment's units group w has every other one, from unit w on. The whole warp walks, one thread issues.
-    const int w = warp == 1 ? 0 : 1;
+  } else if (warp < 1 + L::kIssuers) {
+    // ---------------- MMA issuers ----------------
+    // Units number through the CTA's segments, group x & 1 has unit x. An issuer has all of them, or with two row tiles
+    // those of its group. Either way it passes through every phase of every barrier that it waits for, as a wait by
+    // parity asks: a group that a segment of one tile passes by would lose count of the segments' queries and the tiles.
+    // Scores go one unit of each group ahead of the mixes. The whole warp walks, one thread issues.
     const uint64_t q_desc = byte_desc<HD>(smem_u32(smem));
     const uint64_t k_desc = byte_desc<HD>(smem_u32(smem + L::kOffK));
     const uint64_t v_desc = byte_desc<HD>(smem_u32(smem + L::kOffV));
     constexpr uint32_t kStage = L::kOperand >> 4, kPartRows = L::kPart * HD >> 4;
     struct Place {
-      int u, units, tiles, seg;  // unit of the segment, units of it, tiles and segments before
-      uint32_t parity;           // of the group's units so far
+      int x, u, units, seg;  // unit, its number in its segment, units of that, segments before
     };
-    auto tile_of_place = [&](const Place& p) { return p.tiles + (DUAL ? p.u >> 1 : p.u); };
-    // Moves on to the group's next unit from its segment on; false when there is none. `scores`: the walk of the
-    // scores, which owes an arrival for each segment without a unit of the group.
-    auto settle = [&](Place& p, Walk& at, bool scores) {
-      while (p.u >= p.units) {
-        if (scores && p.units <= w && lane == 0) mbar_arrive(&qempty[p.seg & 1]);
-        __syncwarp();
-        p.tiles += p.units / L::kTiles;
-        at.next(a, per);
-        if (__shfl_sync(0xffffffffu, at.left > 0 ? 1 : 0, 0) == 0) return false;
-        p.units = __shfl_sync(0xffffffffu, at.segment(), 0) * L::kTiles;
-        p.u = w;
-        ++p.seg;
-      }
+    const int first = warp - 1;  // of the issuer's units in a segment
+    // Moves on to the issuer's next unit; false when there is none.
+    auto advance = [&](Place& p, Walk& at) {
+      p.x += L::kIssuers;
+      p.u += L::kIssuers;
+      if (p.u < p.units) return true;
+      at.next(a, per);
+      if (__shfl_sync(0xffffffffu, at.left > 0 ? 1 : 0, 0) == 0) return false;
+      p.units = __shfl_sync(0xffffffffu, at.segment(), 0) * L::kTiles;
+      p.u = first;
+      ++p.seg;
       return true;
     };
     bool ok = true;
     auto score = [&](const Place& p, int h) {
-      const int buf = L::kParts * w + h, kt = tile_of_place(p), ks = kt % L::kKS, qbuf = p.seg & 1;
+      const int w = p.x & 1, buf = L::kParts * w + h, kt = p.x / L::kTiles, ks = kt % L::kKS, qbuf = p.seg & 1;
       if (h == 0) {
-        if (p.u == w && !(ok = warp_wait(&qfull[qbuf], (p.seg >> 1) & 1, abort_flag, a.status))) return;
+        if (p.u == first && !(ok = warp_wait(&qfull[qbuf], (p.seg >> 1) & 1, abort_flag, a.status))) return;
         if (!(ok = warp_wait(&kfull[ks], (kt / L::kKS) & 1, abort_flag, a.status))) return;
       }
       // the last weights in these columns have been mixed (before the first: passes)
-      if (!(ok = warp_wait(&pvdone[buf], p.parity ^ 1u, abort_flag, a.status))) return;
+      if (!(ok = warp_wait(&pvdone[buf], ((p.x >> 1) & 1) ^ 1u, abort_flag, a.status))) return;
       tc_fence_after();
       if (elect_one()) {
         const uint64_t q_at = q_desc + ((qbuf * L::kQBuf + (DUAL ? w * L::kQTile : 0)) >> 4), k_at = k_desc + ks * kStage + h * kPartRows;
@@ -477,22 +477,23 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
         mma_commit(&sfull[buf]);
         if (h == L::kParts - 1) {
           mma_commit(&kempty[ks]);
-          if (p.u + 2 >= p.units) mma_commit(&qempty[qbuf]);
+          if (p.u + L::kIssuers >= p.units) mma_commit(&qempty[qbuf]);
         }
       }
       __syncwarp();
     };
     auto mix = [&](const Place& p, int h) {
-      const int buf = L::kParts * w + h, kt = tile_of_place(p), vs = kt % L::kVS;
-      if (!(ok = warp_wait(&pfull[buf], p.parity, abort_flag, a.status))) return;
+      const int w = p.x & 1, buf = L::kParts * w + h, kt = p.x / L::kTiles, vs = kt % L::kVS;
+      if (!(ok = warp_wait(&pfull[buf], (p.x >> 1) & 1, abort_flag, a.status))) return;
       if (h == 0) {
         // the segment's first mix overwrites O: its last reader was the previous segment's end
-        if (p.u == w && p.seg > 0 && !(ok = warp_wait(ofree, (p.seg - 1) & 1, abort_flag, a.status))) return;
+        if (p.u == first && p.seg > 0 && !(ok = warp_wait(ofree, (p.seg - 1) & 1, abort_flag, a.status))) return;
         if (!(ok = warp_wait(&vfull[vs], (kt / L::kVS) & 1, abort_flag, a.status))) return;
       }
       tc_fence_after();
       if (elect_one()) {
-        const uint32_t o = tmem + L::kColO + w * HD, at = tmem + buf * L::kPart, fresh = p.u == w && h == 0 ? 0u : 1u;
+        // fresh: the group's first of the segment
+        const uint32_t o = tmem + L::kColO + w * HD, at = tmem + buf * L::kPart, fresh = p.u < 2 && h == 0 ? 0u : 1u;
         const uint64_t v_at = v_desc + vs * kStage + h * kPartRows;
         constexpr uint32_t kStep = 32 * HD >> 4;  // 32 slots of V
 #pragma unroll
@@ -504,29 +505,26 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
       }
       __syncwarp();
     };
-    Place sc{w, __shfl_sync(0xffffffffu, walk.segment(), 0) * L::kTiles, 0, 0, 0}, mx = sc;
+    Place mx{first, first, __shfl_sync(0xffffffffu, walk.segment(), 0) * L::kTiles, 0}, sc = mx;
     Walk mix_walk = walk;
-    bool more = settle(sc, walk, true);
-    bool any = more;
-    if (any) settle(mx, mix_walk, false);
-    for (int h = 0; ok && more && h < L::kParts; ++h) score(sc, h);
+    bool more = true, any = true;
+    for (int lead = 0; more && lead < 2; lead += L::kIssuers) {
+      for (int h = 0; ok && h < L::kParts; ++h) score(sc, h);
+      more = ok && advance(sc, walk);
+    }
     while (ok && any) {
-      sc.u += 2;
-      sc.parity ^= 1;
-      if (more) more = settle(sc, walk, true);
       for (int h = 0; ok && h < L::kParts; ++h) {
         mix(mx, h);
         if (ok && more) score(sc, h);
       }
-      mx.u += 2;
-      mx.parity ^= 1;
-      any = settle(mx, mix_walk, false);
+      if (more) more = advance(sc, walk);
+      any = advance(mx, mix_walk);
     }
-    if (elect_one()) mma_commit(&mma_done[w]);
+    if (elect_one()) mma_commit(&mma_done[first]);
     __syncwarp();
-    if (lane == 0) wait_phase(&mma_done[w], 0, abort_flag, a.status, kDrainNs, false);
+    if (lane == 0) wait_phase(&mma_done[first], 0, abort_flag, a.status, kDrainNs, false);
     __syncwarp();
-  } else {
+  } else if (warp >= 4) {
     // ---------------- softmax ----------------
     constexpr int NC = L::kPart / L::kCopies;  // slots of a part that a copy weighs
     const int w = (warp - 4) >> 2;      // group
@@ -536,7 +534,6 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
     const uint32_t lane_addr = static_cast<uint32_t>(quarter * 32) << 16;
     const uint32_t o_addr = tmem + lane_addr + L::kColO + w * HD;
     int tiles = 0;         // before this segment
-    uint32_t parity = 0, other = 0;  // of the group's units, and of the other's
     for (int seg = 0; walk.left > 0; walk.next(a, per), ++seg) {
       const int n = walk.segment();
       const int units = n * L::kTiles;
@@ -547,8 +544,10 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
       const int token = i0 + r / a.group;  // a row past `live` computes on zeros and is not stored
       const int total = s.ctx + s.n;
       float m = -INFINITY, l = 0.f, factor = 0.f;
-      for (int u = w; u < units; u += 2, parity ^= 1) {
+      const int x0 = tiles * L::kTiles, first_u = (x0 ^ w) & 1;  // the segment's first unit; this group's first of them
+      for (int u = first_u; u < units; u += 2) {
         const int kt = tiles + (DUAL ? u >> 1 : u);
+        const uint32_t parity = (x0 + u) >> 1 & 1;
         const int slot0 = (walk.t + (DUAL ? u >> 1 : u)) * a.tile;
 #pragma unroll 1
         for (int h = 0; h < L::kParts; ++h) {
@@ -557,7 +556,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
           warp_wait(&sfull[buf], parity, abort_flag, a.status);
           tc_fence_after();
           const uint32_t bad = bad_ring[kt % kBadRing];
-          if (u == w && h == 0) factor = factors[seg % kQRing * L::kRows + (DUAL ? w * kTile : 0) + r];
+          if (u == first_u && h == 0) factor = factors[seg % kQRing * L::kRows + (DUAL ? w * kTile : 0) + r];
           if (warp_live) {
             const int first = h * L::kPart + copy * NC;  // this copy's first slot of the tile
             const float4* group = scales + kt % kBadRing * kGroups + first / kGroupSlots;
@@ -604,7 +603,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
             const bool rise = top > m + kRescaleAt8 || (m == -INFINITY && top > -INFINITY);
             const float m_new = rise ? top : m;
             const float alpha = rise ? ex2(m - m_new) : 1.f;  // m = -inf: 0
-            if ((u != w || h > 0) && __any_sync(0xffffffffu, rise)) {
+            if ((u != first_u || h > 0) && __any_sync(0xffffffffu, rise)) {
               // the group's previous mix
               const int last = h > 0 ? buf - 1 : buf + L::kParts - 1;
               warp_wait(&pvdone[last], h > 0 ? parity : parity ^ 1, abort_flag, a.status);
@@ -679,14 +678,15 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
       }
 
       // the groups' last mixes of the segment: of both where finish_segment reads both O, else of this one's
-      const bool had1 = units > 1;
-      if (w == 0 || had1) warp_wait(&pvdone[L::kParts * (w + 1) - 1], parity ^ 1, abort_flag, a.status);
-      if (!DUAL && L::kCopies == 1) {
-        other ^= (units + w) >> 1 & 1;  // the other group had (units + w) / 2
-        if (w == 1 || had1) warp_wait(&pvdone[L::kParts * ((w ^ 1) + 1) - 1], other ^ 1, abort_flag, a.status);
+      const bool had0 = units > 1 || (x0 & 1) == 0, had1 = units > 1 || (x0 & 1) == 1;
+      constexpr bool kOwnOnly = DUAL || L::kCopies > 1;
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        const int last = x0 + units - 1 - ((x0 + units - 1 - g) & 1);  // group g's
+        if ((g == 0 ? had0 : had1) && (!kOwnOnly || g == w)) warp_wait(&pvdone[L::kParts * (g + 1) - 1], (last >> 1) & 1, abort_flag, a.status);
       }
       tc_fence_after();
-      finish_segment<L, HD>(a, smem, walk, s, slots, tmem, w, copy, r, true, had1, seg, i0, live, m, l);
+      finish_segment<L, HD>(a, smem, walk, s, slots, tmem, w, copy, r, had0, had1, seg, i0, live, m, l);
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(ofree);

@@ -203,6 +203,22 @@ def test_cuts_anywhere_about_short_items(cuda, hq, hkv, most, seed):
     Batch(cuda, lens, hq, hkv, 64, 16, 16, BF16, seed=seed, tree=seed != 2).check()
 
 
+@pytest.mark.parametrize("group,most,batch", [(4, 8, 256), (4, 16, 128), (8, 16, 128), (8, 40, 64)])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("mixed", [False, True])
+def test_many_short_items_in_every_form(cuda, group, most, batch, hd, mixed):
+    """Items by far more than CTAs: runs of segments of one tile, between longer ones when mixed,
+    in the forms of 32, 64, 128 and 256 rows. Twice over with the same bits."""
+    rng = np.random.RandomState(batch + most)
+    lens = [(int(rng.randint(300, 601) if mixed and rng.rand() < 0.2 else rng.randint(0, 121)), int(rng.randint(1, most + 1)))
+            for _ in range(batch)]
+    lens[0] = (lens[0][0], most)
+    b = Batch(cuda, lens, 8 * group, 8, hd, 16, 16, BF16, seed=most + hd)
+    first = b.check()
+    for _ in range(3):
+        assert bits_equal(b.run(), first)
+
+
 @pytest.mark.parametrize("dtype", [BF16, F32])
 def test_wide_groups(cuda, dtype):
     Batch(cuda, [(200, 3), (9, 30)], 64, 1, 128, 32, 32, dtype, seed=5).check()
