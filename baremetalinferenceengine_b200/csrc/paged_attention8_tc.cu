@@ -4,27 +4,27 @@
 // Mathematics: the running softmax of paged_attention.cu on tiles of 128 slots, K and V as the
 // codes they are held in: nothing is widened on its way to the tensor cores.
 //   scores  S[row][slot] = (Qh + Ql)[row][:] . Kc[slot][:]    two e4m3 x e4m3 products
-//   mix     O[row][:]   += (Ph + Pl)[row][slot] Vc[slot][:]   e5m2 x e4m3 and e4m3 x e4m3
+//   mix     O[row][:]   += (P1 + P2 + P3)[row][slot] Vc[slot][:]   three e5m2 x e4m3
 // Qh is the query times a power of two that puts its largest element in [128, 256), rounded to
 // e4m3, and Ql what that leaves: together all 8 bits of a bf16 element down to 2^-9 of the largest, and
 // 2^-17 of the largest below. Scales are powers of two, so they meet the softmax as exponents:
-//   t = S f + e_v,  f = 2^(e_k - e_q) scale log2(e),  P = 2^(t - m + 6),  l += P 2^(-e_v)
+//   t = S f + e_v,  f = 2^(e_k - e_q) scale log2(e),  P = 2^(t - m + 12),  l += P 2^(-e_v)
 // with e_k and e_v the exponents of K's and V's scale at the slot, e_q the query's and m the running maximum
 // of t: the weight times V's scale is what the mix takes, so its rounding is relative to the
-// largest term of the sum, however far blocks' scales lie apart. P is at most 2^12 (a row is rescaled when m rises by
-// more than 6). As fp16 it splits into Ph, e5m2 and so the upper byte of the fp16 value, rounded, and Pl = P - Ph as
-// e4m3, at most 2^8 and in steps of 2^-9 at least: off by 2^-8 of itself at most, by 2^-16 of the largest where it is
-// small. That is the precision of bf16 weights, for two products of twice bf16's rate. (The other way round, e4m3
-// first, takes two conversions more.)
+// largest term of the sum, however far blocks' scales lie apart. P is at most 2^15 (a row is rescaled when m rises by
+// more than 3). Its fp16 value has 11 bits, of which each e5m2 part takes three, the first two a bit more by the next
+// one's sign: together all 11, down to steps of 2^-16, the smallest that e5m2 has. So a weight is off by 2^-11 of itself at
+// most, or by 2^-17 of 2^12 where it is small, which 2^17 slots cannot add up to 2^-11 of the sum. (Two parts do not hold
+// that: e5m2 and e4m3 leave 2^-10, which thousands of small weights next to a large one made up to a tenth of the
+// output.)
 //
 // Bound: memory while group * tokens is below about 100 (a slot is half the bytes of a bf16 cache's, for the same
 // tensor time), above it the products. What it takes is neither: it is the chain scores, softmax, weights, mix of each
 // row tile, whose waits two groups of warps leave open (counters of 64 tokens at group 8: tensor pipe 20 % of its
 // cycles, conversions and exponentials 21 %, issue slots 35 %), and for few rows the ends of segments.
-// Measured, heads of 128, 8 kv heads: 1 sequence, 12 tokens at group 4 over 8000 slots 24 us; 64 ragged sequences of up
-// to 8192 slots, 8 tokens at group 4 171 us (3.0 TB/s of codes); 16 sequences of 4096 to 8192 slots, 64 tokens at group 8
-// 337 us (594 TFLOP/s of the formula's products). Before items had a cost 31, 207 and 361; then with one issuer for
-// two row tiles' groups and whole tiles 402 for the last, with parts for few rows too 34 and 217 for the others.
+// Measured, heads of 128, 8 kv heads: 1 sequence, 12 tokens at group 4 over 8000 slots 25 us; 64 ragged sequences of up
+// to 8192 slots, 8 tokens at group 4 188 us (2.7 TB/s of codes); 16 sequences of 4096 to 8192 slots, 64 tokens at group 8
+// 369 us (542 TFLOP/s of the formula's products). With weights of two parts 24, 171 and 337.
 //
 // Split and roles are paged_attention_tc.cu's, but for the queries, the scales and the MMAs. The warp that fetches V
 // converts a segment's queries into two operands in shared memory, some rows between two tiles, while the segment before
@@ -40,8 +40,8 @@ namespace bm {
 namespace paged {
 namespace {
 
-constexpr float kRescaleAt8 = 6.f;  // rise of the maximum (log2) that a row's sums are rescaled at
-constexpr float kLift = 6.f;        // P is 2^6 at the running maximum, so at most 2^12: Pl ends at 2^8
+constexpr float kRescaleAt8 = 3.f;  // rise of the maximum (log2) that a row's sums are rescaled at (4 and 6: no faster; 2: 4 % slower)
+constexpr float kLift = 12.f;       // P is 2^12 at the running maximum, so at most 2^15: e5m2 ends at 1.75 * 2^15
 constexpr int kGroupSlots = 8;      // slots of a tile that share a scale
 constexpr int kGroups = kTile / kGroupSlots;
 // What beginning and ending an item costs a CTA, in tiles: of 0, 1, 2, 4, 6, 8 the cases above take 31, 24, 24, 24, 24, 23;
@@ -148,20 +148,22 @@ __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
   return r;
 }
-// Four weights: e5m2 of their fp16 values, which is the upper byte of such a value, rounded, and e4m3 of what that
-// leaves. Weights are not negative; one that is NaN leaves NaN.
-__device__ __forceinline__ void weight_parts(float p0, float p1, float p2, float p3, uint32_t* part, uint32_t* rest) {
-  uint32_t p01, p23, r01, r23;
-  uint16_t l01, l23;
-  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(p01) : "f"(p1), "f"(p0));
-  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(p23) : "f"(p3), "f"(p2));
-  const uint32_t h01 = p01 + 0x00800080u, h23 = p23 + 0x00800080u;
-  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r01) : "r"(p01), "r"(h01 & 0xff00ff00u));
-  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r23) : "r"(p23), "r"(h23 & 0xff00ff00u));
-  asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(l01) : "r"(r01));
-  asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(l23) : "r"(r23));
-  *part = __byte_perm(h01, h23, 0x7531);
-  *rest = l01 | static_cast<uint32_t>(l23) << 16;
+// Four weights' fp16 values as three e5m2 parts: the upper byte of an fp16 value, rounded, is its e5m2 value, so each part
+// is taken off what the last one leaves. Weights are not negative. (Of a NaN the parts are zeros; its row's sum
+// is one.)
+__device__ __forceinline__ void weight_parts(float p0, float p1, float p2, float p3, uint32_t* first, uint32_t* second, uint32_t* third) {
+  uint32_t a, b;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(a) : "f"(p1), "f"(p0));
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(b) : "f"(p3), "f"(p2));
+  auto part = [&](uint32_t* to) {
+    const uint32_t ha = a + 0x00800080u, hb = b + 0x00800080u;
+    *to = __byte_perm(ha, hb, 0x7531);
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(a) : "r"(a), "r"(ha & 0xff00ff00u));
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(b) : "r"(b), "r"(hb & 0xff00ff00u));
+  };
+  part(first);
+  part(second);
+  part(third);
 }
 
 // Converts the queries of an item into its two parts in the buffer at `to`, row tile after row
@@ -242,8 +244,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
   using L = Layout8<HD, COPIES>;
   constexpr bool DUAL = L::kTwo;
   constexpr uint32_t kIdescS = instr_desc_e4m3(false, false, L::kPart, kTile);
-  constexpr uint32_t kIdescH = instr_desc_e4m3(true, true, HD, kTile);
-  constexpr uint32_t kIdescL = instr_desc_e4m3(false, true, HD, kTile);
+  constexpr uint32_t kIdescO = instr_desc_e4m3(true, true, HD, kTile);
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                                          ~static_cast<uintptr_t>(1023));
@@ -497,9 +498,12 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
         const uint64_t v_at = v_desc + vs * kStage + h * kPartRows;
         constexpr uint32_t kStep = 32 * HD >> 4;  // 32 slots of V
 #pragma unroll
-        for (int kk = 0; kk < L::kPart / 32; ++kk) mma_f8_ts(o, at + kk * 8, v_at + kk * kStep, kIdescH, kk > 0 ? 1u : fresh);
+        for (int i = 0; i < 3; ++i) {  // the weights' parts
 #pragma unroll
-        for (int kk = 0; kk < L::kPart / 32; ++kk) mma_f8_ts(o, at + L::kPart / 4 + kk * 8, v_at + kk * kStep, kIdescL, 1u);
+          for (int kk = 0; kk < L::kPart / 32; ++kk) {
+            mma_f8_ts(o, at + i * (L::kPart / 4) + kk * 8, v_at + kk * kStep, kIdescO, i > 0 || kk > 0 ? 1u : fresh);
+          }
+        }
         mma_commit(&pvdone[buf]);
         if (h == L::kParts - 1) mma_commit(&vempty[vs]);
       }
@@ -623,7 +627,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
             const float base = m == -INFINITY ? 0.f : m - kLift;
 #pragma unroll
             for (int c = 0; c < NC / kChunk; ++c) {
-              uint32_t part[kChunk / 4], rest[kChunk / 4];
+              uint32_t part[3][kChunk / 4];
 #pragma unroll
               for (int j = 0; j < kChunk / 8; ++j) {
                 const float4 sc = group[4 * c + j];
@@ -636,14 +640,14 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
                   const float2 y1 = unpair(fma2(pair(v[c][8 * j + e + 2], v[c][8 * j + e + 3]), f2, up2));
                   const float p0 = ex2(y0.x), p1 = ex2(y0.y), p2 = ex2(y1.x), p3 = ex2(y1.y);
                   sum = add2(sum, add2(pair(p0, p1), pair(p2, p3)));
-                  weight_parts(p0, p1, p2, p3, &part[2 * j + e / 4], &rest[2 * j + e / 4]);
+                  weight_parts(p0, p1, p2, p3, &part[0][2 * j + e / 4], &part[1][2 * j + e / 4], &part[2][2 * j + e / 4]);
                 }
                 const float2 two = unpair(sum);
                 l = fmaf(two.x + two.y, sc.z, l);
               }
               const uint32_t to = s_addr + copy * (NC / 4) + kChunk / 4 * c;
-              tmem_store_n<kChunk / 4>(to, part);
-              tmem_store_n<kChunk / 4>(to + L::kPart / 4, rest);
+#pragma unroll
+              for (int i = 0; i < 3; ++i) tmem_store_n<kChunk / 4>(to + i * (L::kPart / 4), part[i]);
             }
             if constexpr (L::kCopies > 1) {  // no weights for the slots of the other copies
               uint32_t zero[NC / 4];
@@ -652,8 +656,8 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
 #pragma unroll
               for (int c = 0; c < L::kCopies; ++c) {
                 if (c != copy) {
-                  tmem_store_n<NC / 4>(s_addr + c * (NC / 4), zero);
-                  tmem_store_n<NC / 4>(s_addr + L::kPart / 4 + c * (NC / 4), zero);
+#pragma unroll
+                  for (int i = 0; i < 3; ++i) tmem_store_n<NC / 4>(s_addr + i * (L::kPart / 4) + c * (NC / 4), zero);
                 }
               }
             }

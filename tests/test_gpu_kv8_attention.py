@@ -265,6 +265,47 @@ def test_scores_far_apart(cuda, dtype):
     Batch(cuda, [(700, 2), (300, 1)], 4, 2, 128, 16, 16, dtype, seed=11, spread=60.0).check()
 
 
+@pytest.mark.parametrize("group,tokens", [(4, 1), (4, 12), (8, 16), (8, 40)])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("slots,below,spread", [(8192, 12.83, 0.0), (8192, 13.0, 0.1), (8192, 13.0, 0.3), (8192, 13.0, 1.0),
+                                                (8192, 14.83, 0.0), (131072, 17.3, 0.0), (131072, 18.0, 0.2)])
+def test_one_heavy_slot_before_a_long_flat_context(cuda, group, tokens, hd, slots, below, spread):
+    """The first slot's score is `below` (base 2) above those of all others, which lie within `spread` of
+    each other: every weight is small, and their sum is not. As many sequences (of the same pages) as there are SMs, so
+    that a CTA walks one from its first slot to its last. A weight may be off by its fp16 value's half step, 2^-11 of
+    itself, so the output by that part of the sum of weights times |v|. Another half of it is for the rest:
+    scores in fp32 (a few 2^-19 of a weight) and the parts' least step, 2^-17 under a lift of 2^12, which
+    2^17 slots of |v| up to twice the first's make 2^-11 of that sum at the very most, and 2^-12 at random."""
+    g = gen(slots + tokens)
+    page, ctx = 64, slots - tokens
+    pages, batch = slots // page, torch.cuda.get_device_properties(cuda).multi_processor_count
+    k = torch.zeros(pages * page, hd)
+    k[:, 1] = (torch.rand(pages * page, generator=g) * 2 - 1) * 16
+    k[0, 0], k[0, 1] = 16.0, 0.0
+    v = 64.0 * (1 + torch.rand(pages * page, hd, generator=g))
+    v[0] = -v[0]  # the first slot and the others pull apart
+    codes = [x.to(torch.float8_e4m3fn) for x in (k, v)]
+    scales = [torch.full((pages, 1, 2), 127, dtype=torch.uint8, device=cuda).view(torch.float8_e8m0fnu) for _ in range(2)]
+    cache = ops.PagedKV8(*(x.to(cuda).view(pages, 1, page, hd) for x in codes), *scales,
+                         torch.arange(pages, dtype=torch.int32, device=cuda).repeat(batch, 1))
+    q = torch.zeros(batch * tokens, group, hd, dtype=BF16)
+    q[..., 0], q[..., 1] = 2.0, spread / below
+    scale = below * math.log(2.0) / 32
+    st = ops.DeviceStatus(cuda)
+    got = ops.paged_kv8_tree_attention(q.to(cuda), cache, i32([ctx] * batch, cuda), i32(range(0, batch * tokens + 1, tokens), cuda), ctx,
+                                       tokens, scale=scale, status=st)
+    assert st.read() == 0
+    got = got.view(batch, tokens, group, hd)
+    kd, vd = (x.double() for x in codes)
+    s = (kd @ q[0, 0].double()) * float(np.float32(scale))
+    for i in {0, tokens - 1}:
+        p = torch.exp(s[:ctx + i + 1] - s[0])
+        p /= p.sum()
+        want, size = p @ vd[:ctx + i + 1], p @ vd[:ctx + i + 1].abs()
+        err = (got[:, i].cpu().double() - want).abs()
+        assert torch.all(err <= 1.5 * 2.0 ** -11 * size + 1.01 * ref.HALF[BF16] * want.abs()), (err / size).max()
+
+
 @pytest.mark.parametrize("dtype", [BF16, F32])
 def test_queries_of_every_size(cuda, dtype):
     """Heads of zeros, of tiny and of large elements, and one element far above the others."""
