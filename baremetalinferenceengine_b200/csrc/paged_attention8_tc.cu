@@ -3,11 +3,11 @@
 //
 // Mathematics: the running softmax of paged_attention.cu on tiles of 128 slots, K and V as the
 // codes they are held in: nothing is widened on its way to the tensor cores.
-//   scores  S[row][slot] = (Qh + Ql)[row][:] . Kc[slot][:]    two e4m3 x e4m3 products
+//   scores  S[row][slot] = (Qh + Ql)[row][:] . Kc[slot][:]         e4m3 x e4m3 and e5m2 x e4m3
 //   mix     O[row][:]   += (P1 + P2 + P3)[row][slot] Vc[slot][:]   three e5m2 x e4m3
 // Qh is the query times a power of two that puts its largest element in [128, 256), rounded to
-// e4m3, and Ql what that leaves: together all 8 bits of a bf16 element down to 2^-9 of the largest, and
-// 2^-17 of the largest below. Scales are powers of two, so they meet the softmax as exponents:
+// e4m3, and Ql what that leaves, e5m2: together all 8 bits of a bf16 element down to 2^-13 of the largest, and off by
+// 2^-21 of the largest at most below. Scales are powers of two, so they meet the softmax as exponents:
 //   t = S f + e_v,  f = 2^(e_k - e_q) scale log2(e),  P = 2^(t - m + 12),  l += P 2^(-e_v)
 // with e_k and e_v the exponents of K's and V's scale at the slot, e_q the query's and m the running maximum
 // of t: the weight times V's scale is what the mix takes, so its rounding is relative to the
@@ -15,8 +15,8 @@
 // more than 3). Its fp16 value has 11 bits, of which each e5m2 part takes three, the first two a bit more by the next
 // one's sign: together all 11, down to steps of 2^-16, the smallest that e5m2 has. So a weight is off by 2^-11 of itself at
 // most, or by 2^-17 of 2^12 where it is small, which 2^17 slots cannot add up to 2^-11 of the sum. (Two parts do not hold
-// that: e5m2 and e4m3 leave 2^-10, which thousands of small weights next to a large one made up to a tenth of the
-// output.)
+// that: e5m2 and e4m3 leave 2^-10, which for thousands of small weights next to a large one came to 7 % of the sum of
+// weights times |v|.)
 //
 // Bound: memory while group * tokens is below about 100 (a slot is half the bytes of a bf16 cache's, for the same
 // tensor time), above it the products. What it takes is neither: it is the chain scores, softmax, weights, mix of each
@@ -148,6 +148,12 @@ __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
   return r;
 }
+// And as e5m2.
+__device__ __forceinline__ uint32_t e5m2x2(float lo, float hi) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e5m2x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  return r;
+}
 // Four weights' fp16 values as three e5m2 parts: the upper byte of an fp16 value, rounded, is its e5m2 value, so each part
 // is taken off what the last one leaves. Weights are not negative. (Of a NaN the parts are zeros; its row's sum
 // is one.)
@@ -218,7 +224,7 @@ __device__ __forceinline__ void convert_queries(const TreeArgs& a, const Seq& s,
           kv8::from_codes(hi[j], back);
 #pragma unroll
           for (int d = 0; d < 4; ++d) back[d] = fmaf(x[4 * j + d], f, -back[d]);
-          lo[j] = e4m3x2(back[0], back[1]) | e4m3x2(back[2], back[3]) << 16;
+          lo[j] = e5m2x2(back[0], back[1]) | e5m2x2(back[2], back[3]) << 16;
         }
 #pragma unroll
         for (int copy = 0; copy < L::kCopies; ++copy) {
@@ -243,7 +249,8 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
   grid_dependency_wait();
   using L = Layout8<HD, COPIES>;
   constexpr bool DUAL = L::kTwo;
-  constexpr uint32_t kIdescS = instr_desc_e4m3(false, false, L::kPart, kTile);
+  constexpr uint32_t kIdescH = instr_desc_e4m3(false, false, L::kPart, kTile);
+  constexpr uint32_t kIdescL = instr_desc_e4m3(true, false, L::kPart, kTile);
   constexpr uint32_t kIdescO = instr_desc_e4m3(true, true, HD, kTile);
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
@@ -472,9 +479,9 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
       if (elect_one()) {
         const uint64_t q_at = q_desc + ((qbuf * L::kQBuf + (DUAL ? w * L::kQTile : 0)) >> 4), k_at = k_desc + ks * kStage + h * kPartRows;
 #pragma unroll
-        for (int kk = 0; kk < HD / 32; ++kk) mma_f8(tmem + buf * L::kPart, q_at + kk * 2, k_at + kk * 2, kIdescS, kk > 0 ? 1u : 0u);
+        for (int kk = 0; kk < HD / 32; ++kk) mma_f8(tmem + buf * L::kPart, q_at + kk * 2, k_at + kk * 2, kIdescH, kk > 0 ? 1u : 0u);
 #pragma unroll
-        for (int kk = 0; kk < HD / 32; ++kk) mma_f8(tmem + buf * L::kPart, q_at + kStage + kk * 2, k_at + kk * 2, kIdescS, 1u);
+        for (int kk = 0; kk < HD / 32; ++kk) mma_f8(tmem + buf * L::kPart, q_at + kStage + kk * 2, k_at + kk * 2, kIdescL, 1u);
         mma_commit(&sfull[buf]);
         if (h == L::kParts - 1) {
           mma_commit(&kempty[ks]);

@@ -605,8 +605,8 @@ int bm_paged_kv8_read(void* k_out, void* v_out, const bm_paged_kv8_t* cache, con
  * page sizes as there runs on the tensor cores where eight neighbouring slots of a tile of 128 share a
  * scale (blocks that are multiples of 8, in pages or equal parts of pages that are multiples of 8, or
  * a part inside one block); all others run on the CUDA cores. The tensor cores take a query
- * as two e4m3 parts (together its bf16 value down to 2^-9 of its head's largest, off by 2^-17 of that
- * below) and a weight as three e5m2 parts (off by 2^-11 of itself, or by 2^-29 of the sum's largest
+ * as an e4m3 and an e5m2 part (together its bf16 value down to 2^-13 of its head's largest, off by at most 2^-21
+ * of that below) and a weight as three e5m2 parts (off by 2^-11 of itself, or by 2^-29 of the sum's largest
  * weight times V's scale). */
 int bm_paged_kv8_tree_attention_workspace_size(int64_t total_q, int64_t batch, int32_t num_q_heads, int32_t num_kv_heads,
                                                int32_t head_dim, int32_t max_ctx, int32_t max_tree, size_t* bytes_out);

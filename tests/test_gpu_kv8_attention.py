@@ -480,3 +480,47 @@ def test_streams_at_once(cuda):
     for (args, kw), want in zip(calls, first):
         for k in kw:
             assert bits_equal(k["out"], want)
+
+
+class Parts(Batch):
+    """The tensor cores' own bounds, in place of bf16 weights and of the looser ones above:
+    * a query element's e4m3 part leaves at most 2^-4 of its power of two, in units of 2^-7 of it (bf16 has 8 bits): at
+      most 8 of them, a number of three bits, which the e5m2 part holds. Below 2^-6 (the row's largest is scaled to
+      128 at least) the first part leaves up to 2^-10, of which the second loses half a step, 2^-14: 2^-21 of 128;
+    * a weight is its fp16 value, off by 2^-11 of itself at most, in parts that hold all of it or end at 2^-16, off by
+      2^-17, where the largest weight times V's scale is 2^12 or more: 2^-29 of that."""
+
+    def want(self, scale=None, seqs=None):
+        assert self.tc and not self.tree and scale is None and seqs is None
+        k, v = (torch.from_numpy(np.nan_to_num(self.model.values(w))) for w in range(2))
+        seqs, scale = list(range(len(self.lens))), 1 / math.sqrt(self.hd)
+        mask = lambda row, i, j: j <= i  # noqa: E731
+        out, tol = ref.attention(self.q, k, v, self.table, seqs, [c for c, _ in self.lens], self.starts, mask, scale, self.dtype, False)
+        vs = 2.0 ** (np.clip(self.model.scales[1].astype(np.int64), 87, 167) - 127.0)
+        for b, (c, n) in enumerate(self.lens):
+            slots = np.arange(c + n)
+            ids, off = self.table[b].numpy()[slots // self.page], slots % self.page
+            seen = slots[None] <= c + np.arange(n)[:, None]
+            rows = slice(self.starts[b], self.starts[b + 1])
+            for h in range(self.q.shape[1]):
+                kv, x = h // self.group, self.q[rows, h].double().numpy()
+                kh, vh, ve = k[ids, kv, off].numpy(), np.abs(v[ids, kv, off].numpy()), vs[ids, kv, off // self.block]
+                s = np.where(seen, x @ kh.T * scale, -np.inf)
+                p = np.exp(s - s.max(-1, keepdims=True))
+                ds = 2.0 ** -21 * np.abs(x).max(-1) * np.where(seen, np.abs(kh).sum(-1), 0.0).max(-1) * scale
+                extra = (2 * ds + 2.0 ** -11)[:, None] * (p @ vh) + 2.0 ** -29 * (p * ve).max(-1)[:, None] * (seen @ (vh / ve[:, None]))
+                tol[rows, h] += 1.05 * extra / p.sum(-1, keepdims=True)
+        return out, tol
+
+
+@pytest.mark.parametrize("group,most", [(4, 8), (4, 16), (8, 16), (8, 40)])
+@pytest.mark.parametrize("hd", [48, 64, 128])
+@pytest.mark.parametrize("above", [0, 4, 8, 12])
+def test_queries_with_one_element_far_above_the_others(cuda, group, most, hd, above):
+    """2^above times as large, at a place where keys are zero: the others make the scores."""
+    b = Parts(cuda, [(700, most), (131, 1), (0, most)], 2 * group, 2, hd, 16, 16, BF16, seed=above + hd, tree=False)
+    codes = b.model.codes[0]
+    codes[..., 5] = np.where(codes[..., 5] == 127, 127, 0)
+    b.q[..., 5] = 2.0 ** above
+    b.upload()
+    b.check()
