@@ -142,13 +142,7 @@ __device__ __forceinline__ void mbar_arrive_n(uint64_t* bar, uint32_t count) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(count) : "memory");
 }
 
-// Two values as e4m3 (lo in the low byte); ends at +-448.
-__device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
-  uint16_t r;
-  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
-  return r;
-}
-// And as e5m2.
+// Two values as e5m2 (lo in the low byte), as kv8::to_codes makes e4m3.
 __device__ __forceinline__ uint32_t e5m2x2(float lo, float hi) {
   uint16_t r;
   asm("cvt.rn.satfinite.e5m2x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
@@ -220,7 +214,7 @@ __device__ __forceinline__ void convert_queries(const TreeArgs& a, const Seq& s,
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           float back[4];
-          hi[j] = e4m3x2(x[4 * j] * f, x[4 * j + 1] * f) | e4m3x2(x[4 * j + 2] * f, x[4 * j + 3] * f) << 16;
+          hi[j] = kv8::to_codes(x[4 * j] * f, x[4 * j + 1] * f) | kv8::to_codes(x[4 * j + 2] * f, x[4 * j + 3] * f) << 16;
           kv8::from_codes(hi[j], back);
 #pragma unroll
           for (int d = 0; d < 4; ++d) back[d] = fmaf(x[4 * j + d], f, -back[d]);
