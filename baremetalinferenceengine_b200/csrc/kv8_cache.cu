@@ -840,7 +840,8 @@ extern "C" int bm_paged_kv8_append(void* q_out, const void* q, const void* k, co
   a.batch = batch;
   a.max_tokens = max_tokens;
   a.blocks = static_cast<int>((static_cast<int64_t>(max_tokens) - 1 + c.block - 1) / c.block + 1);  // that max_tokens neighbouring slots can meet
-  a.parts = parts_for(std::min<int64_t>(rows, batch * static_cast<int64_t>(max_tokens)));
+  const int64_t most_rows = std::min<int64_t>(rows, batch * static_cast<int64_t>(max_tokens));
+  a.parts = parts_for(most_rows);
   return with_chunk(&a, dtype, [&](int n) {
     // A warp holds kUK passes of a block's rows in registers (of 128 elements in bf16: 8 rows); the widest blocks are
     // read twice.
@@ -850,10 +851,13 @@ extern "C" int bm_paged_kv8_append(void* q_out, const void* q, const void* k, co
     const int64_t per = kAppendWarps / a.warps_per_job;
     const double jobs = static_cast<double>(batch) * a.blocks * 2 * a.hkv, q_jobs = static_cast<double>(batch) * max_tokens * a.parts;
     if (jobs + q_jobs > INT32_MAX) return fail(BM_ERR_INVALID_ARGUMENT, "%s: batch * max_tokens too large", what);
-    // Few tokens go in one launch; where they fill the GPU, Q, K and V are better off in kernels of their own, since
-    // K's registers leave room for only 16 warps on an SM (32768 tokens of 64 + 8 heads, appended and read back: 512 us
-    // with all in one, 351 with K and V in one, 343).
-    const bool apart = a.parts == 1;
+    // Fewer than kApartRows rows go in one launch, more in one each for K, V and Q, since K's registers leave room for only 16
+    // warps on an SM; two launches more are 6 to 8 us. In one and apart, us: 1030 rows of 64 + 2 x 8 heads of 128 in bf16
+    // 21 and 28, 4096 48 and 55, 8192 90 and 89, 16384 167 and 159; of 32 + 2 x 8 4096 34 and 40, 8192 62 and 64, 12000 89
+    // and 89, 16384 118 and 113; of 32 + 2 x 4 of 64 8192 29 and 31, 16384 53 and 54; of 6 + 2 x 6 of 48 in fp32 4096 19
+    // and 23, 12000 50 and 50, 16384 67 and 64.
+    constexpr int64_t kApartRows = 12288;
+    const bool apart = most_rows >= kApartRows;
     a.kv_ctas = (batch * a.blocks * (apart ? 1 : 2) * a.hkv + per - 1) / per;
     const int64_t q_warps = num_q_heads ? batch * max_tokens * a.parts : 0;
     const int64_t q_ctas = apart ? 0 : (q_warps + kAppendWarps - 1) / kAppendWarps;

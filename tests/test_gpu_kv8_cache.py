@@ -385,3 +385,34 @@ def test_bounds_far_above_the_rows(cuda):
         got.append((q, k, v))
     for other in got[1:]:
         assert all(bits_equal(a, b) for a, b in zip(got[0], other))
+
+
+@pytest.mark.parametrize("dtype,hq,hkv,hd,rd,page,block,norm", [(BF16, 8, 2, 128, 128, 64, 64, True), (BF16, 3, 1, 48, 24, 24, 8, False),
+                                                                (F32, 4, 2, 64, 64, 100, 100, True), (BF16, 0, 2, 64, 0, 16, 1, False)])
+def test_large_calls_write_what_small_ones_do(cuda, dtype, hq, hkv, hd, rd, page, block, norm):
+    """Rows by the ten thousand, which Q, K and V have kernels of their own for, against one call a sequence."""
+    rng = np.random.RandomState(hd)
+    counts = [int(n) for n in rng.randint(0, 600, 50)] + [1, 1, 12287]
+    ctx = [int(c) for c in rng.randint(0, 300, 50)] + [5, 0, 77]
+    batch, rows, starts = len(counts), sum(counts), np.concatenate([[0], np.cumsum(counts)]).tolist()
+    x = randn((rows, hq + 2 * hkv, hd), dtype, gen(hd)).to(cuda)
+    got = []
+    for whole in (True, False):
+        s = State(cuda, batch, 12365, hkv, hd, page, block, dtype, seed=2, rd=rd, norm=norm)
+        for t in (s.cache.k_scales, s.cache.v_scales):
+            t.view(torch.uint8).fill_(118)
+        for t in (s.cache.k_pages, s.cache.v_pages):
+            t.view(torch.uint8).fill_(0x35)
+        st, q_out = ops.DeviceStatus(cuda), torch.zeros((rows, hq, hd), dtype=dtype, device=cuda)
+        for seqs in [range(batch)] if whole else [[b] for b in range(batch)]:
+            part = slice(starts[seqs[0]], starts[seqs[-1] + 1])
+            n = [counts[b] for b in seqs]
+            ops.paged_kv8_append(x[part, :hq] if hq else None, x[part, hq:hq + hkv], x[part, hq + hkv:], s.cache, i32([ctx[b] for b in seqs], cuda),
+                                 i32(np.concatenate([[0], np.cumsum(n)]).tolist(), cuda), max(n), table=s.rope, seq_ids=i32(list(seqs), cuda),
+                                 q_weight=s.wq.to(cuda) if norm and hq else None, k_weight=s.wk.to(cuda) if norm else None,
+                                 q_out=q_out[part] if hq else None, status=st)
+        assert st.read() == 0
+        got.append([t.view(torch.uint8) for t in (s.cache.k_pages, s.cache.v_pages, s.cache.k_scales, s.cache.v_scales)] + [q_out])
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
+    assert not bool((got[0][0] == 0x35).all())
