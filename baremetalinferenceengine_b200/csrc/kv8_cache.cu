@@ -12,7 +12,9 @@
 // by rows that a later call overwrites is at worst larger than needed, which costs a floating
 // code nothing above 2^-6.)
 //
-// Bound: memory; q, k and v are read once, and q and the codes written once.
+// Bound: memory; q, k and v are read once, and q and the codes written once. But where a block has more rows than its job
+// holds in registers (in bf16 more than 64 of 128 elements, or 32 of 256; in fp32 half of that; fewer where alignment
+// allows only narrower loads), its K and V are read twice.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
