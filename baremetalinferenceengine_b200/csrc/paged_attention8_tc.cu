@@ -20,11 +20,11 @@
 //
 // Bound: memory while group * tokens is below about 100 (a slot is half the bytes of a bf16 cache's, for the same
 // tensor time), above it the products. What it takes is neither: it is the chain scores, softmax, weights, mix of each
-// row tile, whose waits two groups of warps leave open (counters of 64 tokens at group 8: tensor pipe 20 % of its
-// cycles, conversions and exponentials 21 %, issue slots 35 %), and for few rows the ends of segments.
+// row tile, whose waits two groups of warps leave open (counters of 64 tokens at group 8: tensor pipe 24 % of its
+// cycles, conversions and exponentials 20 %, issue slots 38 %), and for few rows the ends of segments.
 // Measured, heads of 128, 8 kv heads: 1 sequence, 12 tokens at group 4 over 8000 slots 25 us; 64 ragged sequences of up
-// to 8192 slots, 8 tokens at group 4 188 us (2.7 TB/s of codes); 16 sequences of 4096 to 8192 slots, 64 tokens at group 8
-// 369 us (542 TFLOP/s of the formula's products). With weights of two parts 24, 171 and 337.
+// to 8192 slots, 8 tokens at group 4 188 to 193 us (2.7 TB/s of codes); 16 sequences of 4096 to 8192 slots, 64 tokens at group 8
+// 369 to 374 us (540 TFLOP/s of the formula's products). With weights of two parts 24, 171 and 337.
 //
 // Split and roles are paged_attention_tc.cu's, but for the queries, the scales and the MMAs. The warp that fetches V
 // converts a segment's queries into two operands in shared memory, some rows between two tiles, while the segment before
@@ -44,8 +44,10 @@ constexpr float kRescaleAt8 = 3.f;  // rise of the maximum (log2) that a row's s
 constexpr float kLift = 12.f;       // P is 2^12 at the running maximum, so at most 2^15: e5m2 ends at 1.75 * 2^15
 constexpr int kGroupSlots = 8;      // slots of a tile that share a scale
 constexpr int kGroups = kTile / kGroupSlots;
-// What beginning and ending an item costs a CTA, in tiles: of 0, 1, 2, 4, 6, 8 the cases above take 31, 24, 24, 24, 24, 23;
-// 213, 208, 196, 186, 179, 182 and 361, 356, 351, 347, 344, 343 us.
+// What beginning and ending an item costs a CTA, in tiles. 0, 1, 2, 4, 6, 8 take, us: the cases above 36, 27, 26, 26, 26,
+// 26; 227, 198, 191, 173, 166, 171; 383, 384, 370, 362, 358, 357; the same with heads of 64 33, 23, 23, 23, 23, 23; 214,
+// 188, 179, 163, 150, 152; 359, 355, 347, 336, 330, 327; one token for each of 64 sequences 219, 203, 188, 173, 170, 173;
+// 32 sequences of 500 to 3000, up to 12 tokens at group 8 150, 140, 131, 126, 115, 112.
 constexpr int kItemCost = 6;
 constexpr int kConvert = 8;         // pairs of rows of the next queries that are converted between two tiles
 constexpr int kQRing = 4;           // segments whose queries' factors are kept

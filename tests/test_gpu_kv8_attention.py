@@ -1,8 +1,9 @@
 """Tree attention over an 8-bit paged cache on the GPU against 64-bit softmax attention over the
 values that the cache stands for. On the CUDA cores the tolerance is serving_ref's. On the tensor
-cores a query is two e4m3 parts and a weight an e5m2 and an e4m3 part of its fp16 value, which
-adds (the kernel's own scaling puts a row's largest query in [128, 256), and its largest weight
-times V's scale at 2^6 or more):
+cores queries and weights are taken in 8-bit parts. Most tests allow for a query of two e4m3 parts and for a weight
+of an e5m2 and an e4m3 part of its fp16 value (a row's largest query scaled to [128, 256), its largest weight
+times V's scale to 2^6 or more); the kernel's parts are closer, and Parts and the long flat contexts hold it to that.
+What they add:
 * a query element off by at most 2^-10 of the 128 that its row's largest exceeds, 2^-17 of that;
 * a weight off by 2^-11 + 2^-8 of itself (the first part leaves at most 2^-3 of its power of two, of
   which the second loses at most 2^-5: its steps are 2^-7 up to 2^-3), or, where what is left is below the
